@@ -107,9 +107,10 @@ def _ints(values):
 
 
 class _Memory:
-    """Device memory of the library as a torch tensor sees it."""
+    """A storage's pool as a torch tensor sees it, which keeps the storage."""
 
-    def __init__(self, address, elements):
+    def __init__(self, storage, elements):
+        self.storage, address = storage, storage.page(0, 0)
         self.__cuda_array_interface__ = {"shape": (elements,), "typestr": "<f2", "data": (address, False), "version": 3}
 
 
@@ -161,7 +162,7 @@ def _prepare_append(case, seed):
     if own:
         device = _package()
         storage = device.Storage(1, kvh, dim, micro, extent)
-        pool = torch.as_tensor(_Memory(storage.page(0, 0), elements), device="cuda")
+        pool = torch.as_tensor(_Memory(storage, elements), device="cuda")
         pool.copy_(_normal(seed, 2, elements))
         table = np.zeros(len(jobs), dtype=device.APPEND_ROPE_JOB)
         for name, k in (("first_row", 0), ("token_count", 1), ("position", 2), ("dst_kind", 3), ("dst_slot", 4), ("dst_token", 5), ("cow_slot", 6),
