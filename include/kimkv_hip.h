@@ -237,6 +237,60 @@ kimkv_status kimkv_append_batch(const kimkv_storage* storage,
                                 const kimkv_append_job* device_jobs, uint32_t job_count,
                                 uint32_t max_layer_count, kimkv_stream_t stream);
 
+/* A rotation of query and key heads by position (rotary embedding): dims
+ * [0, rotary_dim) of a head turn in rotary_dim / 2 planes, plane i of a row at
+ * position p by the angle p * theta^(-2 i / rotary_dim); the other dims stay.
+ * Plane i is dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when
+ * adjacent_pairs != 0.  rotary_dim: even, at most the head dim and 512 (0: no
+ * rotation). */
+typedef struct kimkv_rope {
+    float theta;
+    uint32_t rotary_dim;
+    uint32_t adjacent_pairs;
+    uint32_t reserved;
+} kimkv_rope;
+
+/* One run of consecutive tokens of one page, from consecutive rows of a fused
+ * q | k | v projection: row first_row + i goes to page token dst_token + i at
+ * position + i.  cow_tokens as in kimkv_append_job (at most dst_token). */
+typedef struct kimkv_append_rope_job {
+    uint32_t first_row;
+    uint32_t token_count;
+    uint32_t position;
+    uint32_t dst_slot;
+    uint32_t cow_slot;
+    uint16_t dst_token;
+    uint16_t cow_tokens;
+    uint8_t dst_kind;
+    uint8_t cow_kind;
+    uint8_t reserved[2];
+} kimkv_append_rope_job;
+
+/* Batched append of one layer straight from the fused projection, rotated on
+ * the way: of each job's rows the keys are rotated into the page, the values
+ * copied into it, and the queries rotated to q_out, in one launch (the
+ * results of kimkv_model_rope_split followed by kimkv_append_batch, without
+ * the K and V rows in between).  A row of qkv is [query_heads | kv_heads |
+ * kv_heads][head_dim] fp16, rows are qkv_stride elements apart, rows of q_out
+ * ([query_heads][head_dim]) q_stride.  q_out may be NULL (only K and V are
+ * wanted), or qkv with q_stride = qkv_stride (queries rotated in place); it
+ * overlaps qkv in no other way.  Angles are reduced in 64 bits, so they are
+ * as exact at position 2^32 - 1 as at 1.  Jobs are in memory the device
+ * reads; max_token_count is the largest token_count among them.  No two jobs
+ * write the same page token or name the same row, and none copies from a page
+ * that another one writes.  Page tokens that no job names, and rows of q_out,
+ * stay as they are.  A job that names no page of the storage, tokens past the
+ * page, rows past `rows`, more than max_token_count tokens, positions past
+ * 2^32 - 1 or an invalid copy sets KIMKV_FAULT_APPEND_JOB and is skipped.
+ * Vector accesses where head_dim and the strides are multiples of 8, the
+ * rotary dim of 16 (8 for adjacent pairs) and the addresses 16-byte aligned;
+ * anything else goes element by element.  The storage's device is the current
+ * one. */
+kimkv_status kimkv_append_rope_batch(const kimkv_storage* storage, const kimkv_append_rope_job* device_jobs,
+                                     uint32_t job_count, uint32_t max_token_count, uint32_t layer, const uint16_t* qkv,
+                                     uint64_t qkv_stride, uint32_t rows, uint32_t query_heads, const kimkv_rope* rope,
+                                     uint16_t* q_out, uint64_t q_stride, kimkv_stream_t stream);
+
 /* Paged -> contiguous [layer][K/V][token][head][dim] copy of one table
  * (launchGather, kernels.cuh:67-75; gatherKernel page_kernels.cu:184-242).
  * Descriptors are in DEVICE memory, sorted and contiguous from token 0. */
@@ -521,6 +575,61 @@ kimkv_status kimkv_paged_decode_batch_noalloc(const kimkv_storage* storage,
                                               uint32_t chunk_tokens, uint32_t query_heads,
                                               kimkv_stream_t stream);
 
+/* A run of lanes of a decode batch whose first prefix_tokens tokens are the
+ * same pages' (requests forked from one prompt). */
+typedef struct kimkv_shared_group {
+    uint32_t first_lane;
+    uint32_t lane_count;
+    uint32_t prefix_tokens;
+} kimkv_shared_group;
+
+/* What kimkv_shared_decode_plan decided for a batch; kept with the entries it
+ * wrote and passed to kimkv_shared_decode_batch unchanged. */
+typedef struct kimkv_shared_plan {
+    uint64_t entry_bytes;       /* of the plan's entries, 16-byte aligned on the device */
+    uint64_t workspace_bytes;   /* of the launch's scratch, 16-byte aligned */
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t query_heads;
+    uint32_t lane_count;
+    uint32_t unit_count;
+    uint32_t slot_count;
+    uint32_t merge_lanes;
+    uint32_t column_blocks;
+} kimkv_shared_plan;
+
+/* Plans one layer's decode attention of a batch whose lanes share prefixes
+ * (pure host code, the same for every layer of a token step).  compute_units
+ * is the device's (the storage's kimkv_storage_info; 0: 256), token_counts
+ * each lane's tokens; the groups name disjoint runs of lanes, and lanes
+ * in none share nothing.  A group's prefix is read through its first lane's
+ * table, once for all its lanes; of it the plan takes whole blocks of 64
+ * tokens that all of its lanes hold, none where that would not pay, and the
+ * rest of each lane is read through the lane's own table.  Fills entries[0 ..
+ * plan->entry_bytes) for upload; KIMKV_INVALID_ARGUMENT when capacity is too
+ * small (plan->entry_bytes then holds the size needed; entries may be NULL
+ * with capacity 0), or for groups that overlap or leave the batch. */
+kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint32_t query_heads,
+                                      uint32_t compute_units, const uint32_t* token_counts, uint32_t lane_count,
+                                      const kimkv_shared_group* groups, uint32_t group_count, void* entries,
+                                      uint64_t capacity, kimkv_shared_plan* plan);
+
+/* kimkv_paged_decode_batch of the planned batch, with the shared prefixes
+ * read and multiplied once for all lanes of a group.  device_items: the lanes'
+ * items, whole tables and token counts as planned (their workspace is not
+ * used); device_entries: the plan's entries (made for the storage's heads and
+ * head dim); workspace: plan->workspace_bytes
+ * of device memory, contents ignored, not shared with a launch that may
+ * overlap this one.  Lanes of one group name the same layer.  A lane of no
+ * tokens is skipped (its output is not written); a lane whose item is invalid
+ * or not as planned, or whose group's first lane is, sets
+ * KIMKV_FAULT_DECODE_ITEM and is skipped.  Results as
+ * kimkv_paged_decode_batch's to the decode tolerance, the same for every run
+ * of one plan.  The storage's device is the current one. */
+kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv_decode_item* device_items,
+                                       const void* device_entries, const kimkv_shared_plan* plan, void* workspace,
+                                       kimkv_stream_t stream);
+
 /* New tokens handled by one prefill workgroup (per KV head) for this
  * storage's shape and query head count: items need
  * ceil(new_tokens / this) workgroups each.  0 for an invalid head count. */
@@ -645,6 +754,50 @@ kimkv_status kimkv_model_swiglu(const uint16_t* gate_up, uint32_t rows, uint32_t
 /* First index of each row's maximum (launchArgmaxBatch, kernels.cuh:111-117). */
 kimkv_status kimkv_model_argmax(const float* logits, uint32_t rows, uint32_t vocabulary, uint32_t* device_out,
                                 kimkv_stream_t stream);
+/* What is done to one row of logits before its token is picked.  With c(v) the
+ * times token v occurs in history[0 .. history_count) and x(v) its logit:
+ *   c(v) > 0:  x = x > 0 ? x / repetition_penalty : x * repetition_penalty,
+ *              then x -= frequency_penalty * c(v) + presence_penalty
+ *   x += the sum of the bias_values[i] with bias_tokens[i] == v, added up in
+ *        the list's order
+ *   v not in allowed:  x = -inf
+ * allowed: bit v % 32 of word v / 32 for every token of the vocabulary, NULL
+ * for all of them.  Listed tokens past the vocabulary are ignored. */
+typedef struct kimkv_logits_rule {
+    const uint32_t* history;
+    const uint32_t* bias_tokens;
+    const float* bias_values;
+    const uint32_t* allowed;
+    uint32_t history_count;
+    uint32_t bias_count;
+    float repetition_penalty;   /* > 0; 1 leaves the logits */
+    float presence_penalty;
+    float frequency_penalty;
+    uint32_t reserved;
+} kimkv_logits_rule;
+
+/* The token of a row that allows none or whose rule is invalid. */
+#define KIMKV_NO_TOKEN 0xFFFFFFFFu
+
+/* Workspace of kimkv_model_logits_adjust (0 for shapes that need none). */
+size_t kimkv_logits_workspace_bytes(uint32_t rows, uint32_t vocabulary);
+
+/* Applies device_rules[r] to row r of logits[rows][vocabulary]: the adjusted
+ * logits go to out (NULL: not wanted; may be logits itself, else apart from
+ * it), the greedy token of each row to device_tokens (NULL: not wanted), in
+ * one read of the logits.  The token is the first index of the adjusted row's
+ * maximum among the allowed ones (NaN never wins; an allowed -inf does where
+ * nothing is higher), KIMKV_NO_TOKEN where every allowed logit is NaN or none
+ * is allowed.  A rule with a list that is NULL but not empty or holds 2^31
+ * entries or more, or a repetition penalty that is not above 0 and finite,
+ * leaves its row of out alone and gives KIMKV_NO_TOKEN.  device_rules NULL: no row is adjusted.  workspace:
+ * kimkv_logits_workspace_bytes(rows, vocabulary) of device memory, 8-byte
+ * aligned, contents ignored, not shared with a call that may overlap this one
+ * (NULL where that is 0 or device_tokens is NULL).  No counterpart in the
+ * reference, whose runner picks the plain argmax. */
+kimkv_status kimkv_model_logits_adjust(const float* logits, uint32_t rows, uint32_t vocabulary,
+                                       const kimkv_logits_rule* device_rules, float* out, uint32_t* device_tokens,
+                                       void* workspace, kimkv_stream_t stream);
 /* Seeded weights: out[i] = fp16(float(synth(seed, row0 + i / cols, i % cols)) * scale). */
 kimkv_status kimkv_fill_rows_scaled(uint16_t* device_out, uint64_t count, uint64_t seed, uint64_t row0, uint32_t cols,
                                     float scale, kimkv_stream_t stream);

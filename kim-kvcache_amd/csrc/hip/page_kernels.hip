@@ -9,6 +9,8 @@
 //   gatherKernel                       src/cuda/kv/page_kernels.cu:184-242
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+#include <cstdint>
 #include <type_traits>
 
 #include "device_common.h"
@@ -314,6 +316,223 @@ __global__ __launch_bounds__(kBlock) void append_kernel(PoolView P, const kimkv_
         uint32_t const pt = job.dst_token + t;
         dst[dh + k_el(dcap, D, pt, d)] = job.src_key[so];
         dst[dh + v_el(dcap, D, pt, d)] = job.src_value[so];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Rotated append: block = (job, 8-token group of its page), q | k | v rows in,
+// rotated q rows, rotated page K and page V^T out.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kRopeGroup = 8;          // page tokens a block takes
+constexpr uint32_t kMaxRopePairs = 256;
+
+struct RopeArgs {
+    const kimkv_append_rope_job* jobs;
+    const uint16_t* qkv;
+    uint64_t qkv_stride;
+    uint16_t* q_out;
+    uint64_t q_stride;
+    uint32_t rows;
+    uint32_t max_tokens;
+    uint32_t layer;
+    uint32_t QH;
+    uint32_t rotary;
+    double log2_theta;
+    bool adjacent;
+    bool wide;          // 16-byte pieces: shapes, strides and addresses allow them
+    Divisor items;      // rotated pieces and kept pieces of a row's q and k heads
+    Divisor head_items;
+};
+
+// cos and sin of position * theta^(-2 i / R).  The angle is taken in turns and
+// reduced in 64 bits: a 32-bit angle is off by 2^-24 of itself, 0.008 radians
+// at position 131072.  What is left of a turn rounds to 32 bits.
+__device__ inline float2 rope_cos_sin(uint32_t position, uint32_t i, const RopeArgs& a)
+{
+    constexpr double kTurn = 0.15915494309189535;   // 1 / (2 pi)
+    double const turns = static_cast<double>(position) * (exp2(-2.0 * i / a.rotary * a.log2_theta) * kTurn);
+    float const left = static_cast<float>(turns - rint(turns));
+    return make_float2(cospif(2.0f * left), sinpif(2.0f * left));
+}
+
+__device__ inline float half_f(uint32_t w, bool high)
+{
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(high ? w >> 16 : w & 0xFFFFu)));
+}
+
+__device__ inline uint32_t half_pair(float a, float b)
+{
+    return static_cast<uint32_t>(__half_as_ushort(__float2half_rn(a)))
+        | static_cast<uint32_t>(__half_as_ushort(__float2half_rn(b))) << 16;
+}
+
+// Eight planes turned: (x, y) pairs are elements j of a and b.
+__device__ inline void turn_pieces(u32x4_t& a, u32x4_t& b, const float2* turn)
+{
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        float2 const t0 = turn[2 * j];
+        float2 const t1 = turn[2 * j + 1];
+        float const x0 = half_f(a[j], false), x1 = half_f(a[j], true);
+        float const y0 = half_f(b[j], false), y1 = half_f(b[j], true);
+        a[j] = half_pair(x0 * t0.x - y0 * t0.y, x1 * t1.x - y1 * t1.y);
+        b[j] = half_pair(y0 * t0.x + x0 * t0.y, y1 * t1.x + x1 * t1.y);
+    }
+}
+
+// Four planes of adjacent pairs turned.
+__device__ inline void turn_adjacent(u32x4_t& a, const float2* turn)
+{
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        float2 const t = turn[j];
+        float const x = half_f(a[j], false), y = half_f(a[j], true);
+        a[j] = half_pair(x * t.x - y * t.y, y * t.x + x * t.y);
+    }
+}
+
+template <bool kHuge>
+__global__ __launch_bounds__(kBlock) void append_rope_kernel(PoolView P, RopeArgs a, AppendDivisors dv)
+{
+    __shared__ float2 turn[kRopeGroup * kMaxRopePairs];
+    kimkv_append_rope_job const job = a.jobs[blockIdx.x];
+    uint32_t const tid = threadIdx.x;
+    uint32_t const H = P.heads;
+    uint32_t const D = P.dim;
+    uint32_t const dcap = pool_tokens(P, job.dst_kind);
+    uint16_t* dst = page_base(P, job.dst_kind, job.dst_slot, dcap);
+    uint32_t const scap = pool_tokens(P, job.cow_kind);
+    uint16_t const* src = job.cow_tokens != 0 ? page_base(P, job.cow_kind, job.cow_slot, scap) : nullptr;
+    uint32_t const n = job.token_count;
+    if (dst == nullptr || n > a.max_tokens || n > dcap || job.dst_token > dcap - n || n > a.rows
+        || job.first_row > a.rows - n || (n != 0 && job.position > 0xFFFFFFFFu - (n - 1))
+        || (job.cow_tokens != 0 && (src == nullptr || job.cow_tokens > scap || job.cow_tokens > job.dst_token))) {
+        if (blockIdx.y == 0) report_fault(P, KIMKV_FAULT_APPEND_JOB);
+        return;
+    }
+    uint32_t const layer = a.layer;
+    auto k_el = [](uint32_t cap, uint32_t dim, uint32_t t, uint32_t d) -> uint64_t {
+        return kHuge ? k_offset(cap, dim, t, d) : k_at(cap, dim, t, d);
+    };
+    auto v_el = [](uint32_t cap, uint32_t dim, uint32_t t, uint32_t d) -> uint64_t {
+        return kHuge ? v_offset(cap, dim, t, d) : v_at(cap, dim, t, d);
+    };
+
+    // The copied positions lie below the written ones: neither waits for the other.
+    if (blockIdx.y == 0 && job.cow_tokens != 0) {
+        uint32_t const m = job.cow_tokens;
+        if (!kHuge && ((D | scap | dcap) & 7u) == 0) {
+            copy_tokens_wide(dv, m, src + head_block(P, scap, layer, 0), scap, dst + head_block(P, dcap, layer, 0), dcap);
+        } else {
+            uint64_t const per_head = static_cast<uint64_t>(m) * D;
+            for (uint64_t i = tid; i < H * per_head; i += kBlock) {
+                auto const h = static_cast<uint32_t>(i / per_head);
+                uint64_t const rem = i - h * per_head;
+                auto const t = static_cast<uint32_t>(rem / D);
+                auto const d = static_cast<uint32_t>(rem - static_cast<uint64_t>(t) * D);
+                uint64_t const sh = head_block(P, scap, layer, h);
+                uint64_t const dh = head_block(P, dcap, layer, h);
+                dst[dh + k_el(dcap, D, t, d)] = src[sh + k_el(scap, D, t, d)];
+                dst[dh + v_el(dcap, D, t, d)] = src[sh + v_el(scap, D, t, d)];
+            }
+        }
+    }
+
+    // The group's tokens: page tokens [p0, p1) of the job's [dst_token, dst_token + n).
+    uint32_t const group = (job.dst_token / kRopeGroup + blockIdx.y) * kRopeGroup;
+    uint32_t const p0 = max(group, static_cast<uint32_t>(job.dst_token));
+    uint32_t const p1 = min(group + kRopeGroup, job.dst_token + n);
+    if (p0 >= p1) return;
+    uint32_t const tokens = p1 - p0;
+    uint32_t const first = p0 - job.dst_token;   // token of the job
+    uint32_t const pairs = a.rotary / 2;
+    for (uint32_t i = tid; i < tokens * pairs; i += kBlock) {
+        uint32_t const t = i / pairs;
+        turn[i] = rope_cos_sin(job.position + first + t, i - t * pairs, a);
+    }
+    __syncthreads();
+
+    const uint16_t* const rows = a.qkv + static_cast<uint64_t>(job.first_row + first) * a.qkv_stride;
+    uint16_t* const q_rows = a.q_out != nullptr ? a.q_out + static_cast<uint64_t>(job.first_row + first) * a.q_stride : nullptr;
+    uint32_t const QH = a.QH;
+    uint32_t const h0 = q_rows != nullptr ? 0 : QH;   // heads turned: q's, then k's
+    // Where dims of head `head` (q's, then k's) of token t go.
+    auto q_row = [&](uint32_t t, uint32_t head) { return q_rows + t * a.q_stride + static_cast<uint64_t>(head) * D; };
+    if (a.wide && !kHuge) {
+        uint32_t const turned = a.adjacent ? a.rotary / 8 : a.rotary / 16;
+        for (uint32_t i = tid; i < tokens * a.items.d; i += kBlock) {
+            uint32_t rem, c;
+            uint32_t const t = div_mod(i, a.items, &rem);
+            uint32_t const head = h0 + div_mod(rem, a.head_items, &c);
+            const uint16_t* const row = rows + t * a.qkv_stride + static_cast<uint64_t>(head) * D;
+            uint16_t* const kb = dst + head_block(P, dcap, layer, head - QH);   // read only for k's heads
+            auto put = [&](uint32_t d, u32x4_t v) {
+                uint16_t* const to = head < QH ? q_row(t, head) + d : kb + k_at(dcap, D, p0 + t, d);
+                *reinterpret_cast<u32x4_t*>(to) = v;
+            };
+            // A kept piece lies past the rotated dims.
+            uint32_t const d = c < turned ? 8 * c : a.rotary + 8 * (c - turned);
+            u32x4_t x = *reinterpret_cast<const u32x4_t*>(row + d);
+            if (c < turned && a.adjacent) {
+                turn_adjacent(x, turn + t * pairs + 4 * c);
+            } else if (c < turned) {
+                u32x4_t y = *reinterpret_cast<const u32x4_t*>(row + pairs + d);
+                turn_pieces(x, y, turn + t * pairs + 8 * c);
+                put(pairs + d, y);
+            }
+            put(d, x);
+        }
+    } else {
+        // Element by element: a plane, or a dim that stays.
+        uint32_t const per_head = D - pairs;
+        uint32_t const per_token = (QH + H - h0) * per_head;
+        for (uint32_t t = 0; t < tokens; ++t) {
+            for (uint32_t i = tid; i < per_token; i += kBlock) {
+                uint32_t const head = h0 + i / per_head;
+                uint32_t const c = i % per_head;
+                const uint16_t* const row = rows + t * a.qkv_stride + static_cast<uint64_t>(head) * D;
+                auto put = [&](uint32_t d, uint16_t v) {
+                    if (head < QH) q_row(t, head)[d] = v;
+                    else dst[head_block(P, dcap, layer, head - QH) + k_el(dcap, D, p0 + t, d)] = v;
+                };
+                if (c >= pairs) {
+                    put(c + pairs, row[c + pairs]);
+                    continue;
+                }
+                uint32_t const dx = a.adjacent ? 2 * c : c;
+                uint32_t const dy = a.adjacent ? 2 * c + 1 : c + pairs;
+                float2 const s = turn[t * pairs + c];
+                float const x = half_f(row[dx], false);
+                float const y = half_f(row[dy], false);
+                put(dx, __half_as_ushort(__float2half_rn(x * s.x - y * s.y)));
+                put(dy, __half_as_ushort(__float2half_rn(y * s.x + x * s.y)));
+            }
+        }
+    }
+
+    const uint16_t* const values = rows + static_cast<uint64_t>(QH + H) * D;
+    uint32_t const HD = H * D;
+    if (!kHuge && tokens == kRopeGroup && ((dcap | D) & 7u) == 0) {
+        // V^T: 16-byte pieces of the group's 8 tokens of one dim.
+        for (uint32_t i = tid; i < HD; i += kBlock) {
+            uint32_t d;
+            uint32_t const h = div_mod(i, dv.d, &d);
+            u32x4_t w;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                w[j] = static_cast<uint32_t>(values[2 * j * a.qkv_stride + i])
+                    | static_cast<uint32_t>(values[(2 * j + 1) * a.qkv_stride + i]) << 16;
+            }
+            *reinterpret_cast<u32x4_t*>(dst + head_block(P, dcap, layer, h) + v_at(dcap, D, p0, d)) = w;
+        }
+        return;
+    }
+    for (uint32_t t = 0; t < tokens; ++t) {
+        for (uint32_t i = tid; i < HD; i += kBlock) {
+            uint32_t d;
+            uint32_t const h = div_mod(i, dv.d, &d);
+            dst[head_block(P, dcap, layer, h) + v_el(dcap, D, p0 + t, d)] = values[t * a.qkv_stride + i];
+        }
     }
 }
 
@@ -706,6 +925,63 @@ kimkv_status kimkv_append_batch(const kimkv_storage* storage, const kimkv_append
     kimkv_status const status = launch_status();
     kernel_timing_end(TimedKernel::Append, native(stream), start);
     return status;
+}
+
+kimkv_status kimkv_append_rope_batch(const kimkv_storage* storage, const kimkv_append_rope_job* device_jobs,
+                                     uint32_t job_count, uint32_t max_token_count, uint32_t layer, const uint16_t* qkv,
+                                     uint64_t qkv_stride, uint32_t rows, uint32_t query_heads, const kimkv_rope* rope,
+                                     uint16_t* q_out, uint64_t q_stride, kimkv_stream_t stream)
+{
+    if (storage == nullptr || rope == nullptr || (job_count != 0 && (device_jobs == nullptr || qkv == nullptr))) {
+        return KIMKV_INVALID_ARGUMENT;
+    }
+    uint32_t const H = storage->layout.kv_heads;
+    uint32_t const D = storage->layout.head_dim;
+    uint64_t const heads = static_cast<uint64_t>(query_heads) + 2ull * H;
+    if (layer >= storage->layout.layers || !(rope->theta > 0.0f) || !std::isfinite(rope->theta) || rope->rotary_dim % 2 != 0
+        || rope->rotary_dim > D || rope->rotary_dim > 2 * kMaxRopePairs || job_count > 0x7FFFFFFFu
+        || heads * D > 0x7FFFFFFFull || qkv_stride < heads * D
+        || (q_out != nullptr && (query_heads == 0 || q_stride < static_cast<uint64_t>(query_heads) * D))) {
+        return KIMKV_INVALID_ARGUMENT;
+    }
+    // Rows are indexed in 64 bits: the last one's end must be too.
+    uint64_t const most = UINT64_MAX / 2 / (rows == 0 ? 1 : rows);
+    if (qkv_stride > most || (q_out != nullptr && q_stride > most) || !on_current_device(storage)) {
+        return KIMKV_INVALID_ARGUMENT;
+    }
+    if (job_count == 0) return KIMKV_OK;
+    // A job's tokens start anywhere in their first group of 8; more tokens
+    // than a page holds are refused by the kernel.
+    uint32_t const page = storage->micro_tokens > storage->extent_tokens ? storage->micro_tokens : storage->extent_tokens;
+    uint32_t const tokens = max_token_count < page ? max_token_count : page;
+    uint32_t const groups = (tokens + 2 * (kRopeGroup - 1)) / kRopeGroup;
+    PoolView const pv = pool_view(*storage);
+    RopeArgs a{};
+    a.jobs = device_jobs;
+    a.qkv = qkv;
+    a.qkv_stride = qkv_stride;
+    a.q_out = q_out;
+    a.q_stride = q_stride;
+    a.rows = rows;
+    a.max_tokens = max_token_count;
+    a.layer = layer;
+    a.QH = query_heads;
+    a.rotary = rope->rotary_dim;
+    a.log2_theta = std::log2(static_cast<double>(rope->theta));
+    a.adjacent = rope->adjacent_pairs != 0;
+    uint32_t const piece = a.adjacent ? 8 : 16;
+    a.wide = D % 8 == 0 && qkv_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(qkv) & 15u) == 0 && a.rotary % piece == 0
+        && (q_out == nullptr || (q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q_out) & 15u) == 0));
+    uint32_t const head_items = a.rotary / piece + (D - a.rotary) / 8;
+    a.head_items = divisor(head_items);
+    a.items = divisor((H + (q_out != nullptr ? query_heads : 0)) * head_items);
+    dim3 const grid(job_count, groups == 0 ? 1 : groups);
+    if (append_huge(pv)) {
+        append_rope_kernel<true><<<grid, kBlock, 0, native(stream)>>>(pv, a, append_divisors(*storage));
+    } else {
+        append_rope_kernel<false><<<grid, kBlock, 0, native(stream)>>>(pv, a, append_divisors(*storage));
+    }
+    return launch_status();
 }
 
 kimkv_status kimkv_gather(const kimkv_storage* storage, const kimkv_block_desc* device_descriptors,

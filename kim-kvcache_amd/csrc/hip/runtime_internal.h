@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include "device_common.h"
 #include "kimkv_hip.h"
 
 namespace kimkv {
@@ -14,6 +15,13 @@ kimkv_status record_error(hipError_t error, kimkv_status failure);
 inline kimkv_status launch_status()
 {
     return record_error(hipGetLastError(), KIMKV_SUBMISSION_FAILED);
+}
+
+// Whether a launch now would run on the storage's device.
+inline bool on_current_device(const kimkv_storage* storage)
+{
+    int device = -1;
+    return hipGetDevice(&device) == hipSuccess && device == storage->device;
 }
 
 inline hipStream_t native(kimkv_stream_t stream) { return static_cast<hipStream_t>(stream); }

@@ -46,6 +46,18 @@ APPEND_JOB = np.dtype({
     "offsets": [0, 8, 16, 24, 28, 32, 36, 40, 44, 48, 50, 52, 53],
     "itemsize": 56,
 })
+APPEND_ROPE_JOB = np.dtype([("first_row", "<u4"), ("token_count", "<u4"), ("position", "<u4"), ("dst_slot", "<u4"),
+                            ("cow_slot", "<u4"), ("dst_token", "<u2"), ("cow_tokens", "<u2"), ("dst_kind", "u1"),
+                            ("cow_kind", "u1"), ("reserved", "<u2")])
+# The reserved word at the end is left out, so that a rule can be given as a tuple of what it says.
+LOGITS_RULE = np.dtype({
+    "names": ["history", "bias_tokens", "bias_values", "allowed", "history_count", "bias_count", "repetition_penalty",
+              "presence_penalty", "frequency_penalty"],
+    "formats": ["<u8", "<u8", "<u8", "<u8", "<u4", "<u4", "<f4", "<f4", "<f4"],
+    "offsets": [0, 8, 16, 24, 32, 36, 40, 44, 48],
+    "itemsize": 56,
+})
+NO_TOKEN = 0xFFFFFFFF
 PREFILL_BLOCK = np.dtype([("item", "<u4"), ("head", "<u2"), ("block", "<u2")])
 DESCRIPTOR_PATCH = np.dtype({
     "names": ["table", "first", "count", "source"],
@@ -87,6 +99,24 @@ class DecodeLayerArgs(ctypes.Structure):
                 ("workspace", ctypes.c_uint64), ("workspace_stride", ctypes.c_uint64),
                 ("key", ctypes.c_uint64), ("key_stride", ctypes.c_uint64),
                 ("value", ctypes.c_uint64), ("value_stride", ctypes.c_uint64)]
+
+
+class Rope(ctypes.Structure):
+    """kimkv_rope: the rotation of query and key heads."""
+    _fields_ = [("theta", ctypes.c_float), ("rotary_dim", ctypes.c_uint32), ("adjacent_pairs", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
+class SharedGroup(ctypes.Structure):
+    _fields_ = [("first_lane", ctypes.c_uint32), ("lane_count", ctypes.c_uint32), ("prefix_tokens", ctypes.c_uint32)]
+
+
+class SharedPlan(ctypes.Structure):
+    """kimkv_shared_plan: what a shared decode's plan decided (entry and workspace sizes, counts)."""
+    _fields_ = [("entry_bytes", ctypes.c_uint64), ("workspace_bytes", ctypes.c_uint64), ("kv_heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("query_heads", ctypes.c_uint32), ("lane_count", ctypes.c_uint32),
+                ("unit_count", ctypes.c_uint32), ("slot_count", ctypes.c_uint32), ("merge_lanes", ctypes.c_uint32),
+                ("column_blocks", ctypes.c_uint32)]
 
 
 # kimkv_decode_lane (48 bytes): one chunk of a batched decode with its lane's step-constant part.
@@ -141,6 +171,18 @@ _SIGNATURES = {
     "kimkv_storage_faults": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
     "kimkv_append_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32,
                                           ctypes.c_void_p]),
+    "kimkv_append_rope_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32,
+                                               ctypes.c_uint32, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32,
+                                               ctypes.c_uint32, ctypes.POINTER(Rope), ctypes.c_void_p, ctypes.c_uint64,
+                                               ctypes.c_void_p]),
+    "kimkv_shared_decode_plan": (ctypes.c_int, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
+                                                ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_uint32,
+                                                ctypes.c_void_p, ctypes.c_uint64, ctypes.POINTER(SharedPlan)]),
+    "kimkv_shared_decode_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                                 ctypes.POINTER(SharedPlan), ctypes.c_void_p, ctypes.c_void_p]),
+    "kimkv_logits_workspace_bytes": (ctypes.c_size_t, [ctypes.c_uint32, ctypes.c_uint32]),
+    "kimkv_model_logits_adjust": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p,
+                                                 ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "kimkv_gather": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32,
                                     ctypes.c_void_p, ctypes.c_void_p]),
     "kimkv_promote_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p]),
@@ -402,6 +444,15 @@ class Storage:
                                        int(jobs["layer_count"].max()), _sh(stream)), "append_batch")
         sync(stream)
 
+    def append_rope_launch(self, jobs_ptr: int, job_count: int, max_tokens: int, layer: int, qkv_ptr: int,
+                           qkv_stride: int, rows: int, query_heads: int, rope: Rope, q_ptr: int, q_stride: int,
+                           stream: Optional[Stream] = None) -> None:
+        """kimkv_append_rope_batch: jobs (APPEND_ROPE_JOB, device memory) written from rows of a q | k | v projection,
+        q and k rotated; q_ptr 0 for no queries.  Strides in elements."""
+        check(lib().kimkv_append_rope_batch(self.handle, jobs_ptr, job_count, max_tokens, layer, qkv_ptr, qkv_stride, rows,
+                                            query_heads, rope, q_ptr, q_stride, stream.handle if stream else None),
+              "append_rope_batch")
+
     def gather(self, descs: np.ndarray, total_tokens: int, stream: Optional[Stream] = None) -> np.ndarray:
         descs = np.ascontiguousarray(descs, dtype=BLOCK_DESC)
         d = upload(descs, stream)
@@ -426,6 +477,16 @@ class Storage:
 
     def decode_plan(self, token_counts, query_heads: int):
         return decode_plan(self.handle, token_counts, query_heads)
+
+    def shared_decode_plan(self, token_counts, groups, query_heads: int) -> tuple[np.ndarray, SharedPlan]:
+        return shared_decode_plan(self.kv_heads, self.head_dim, query_heads, self.info().compute_units, token_counts,
+                                  groups)
+
+    def shared_decode_launch(self, items_ptr: int, entries_ptr: int, plan: SharedPlan, workspace_ptr: int,
+                             stream: Optional[Stream] = None) -> None:
+        """kimkv_shared_decode_batch: one layer of a planned batch (entries and workspace in device memory)."""
+        check(lib().kimkv_shared_decode_batch(self.handle, items_ptr, entries_ptr, plan, workspace_ptr,
+                                              stream.handle if stream else None), "shared_decode_batch")
 
     def decode_launch(self, items_ptr: int, prefix_ptr: int, lanes: int, total_chunks: int, chunk_tokens: int,
                       query_heads: int, stream: Optional[Stream] = None) -> None:
@@ -553,6 +614,24 @@ def decode_plan(storage_handle: int, token_counts, query_heads: int):
     return int(chunk.value), prefix, int(total.value)
 
 
+def shared_decode_plan(kv_heads: int, head_dim: int, query_heads: int, compute_units: int, token_counts,
+                       groups) -> tuple[np.ndarray, SharedPlan]:
+    """kimkv_shared_decode_plan: (entries to upload, plan) of a batch; groups are (first lane, lanes, prefix tokens) of
+    lanes whose first tokens are the same pages'."""
+    counts = np.ascontiguousarray(token_counts, dtype=np.uint32)
+    shared = (SharedGroup * len(groups))(*[SharedGroup(*map(int, g)) for g in groups])
+    plan = SharedPlan()
+    args = (kv_heads, head_dim, query_heads, compute_units, counts.ctypes.data_as(ctypes.c_void_p), len(counts), shared,
+            len(groups))
+    status = lib().kimkv_shared_decode_plan(*args, None, 0, ctypes.byref(plan))
+    if status != OK and not plan.entry_bytes:
+        check(status, "shared_decode_plan")
+    entries = np.zeros(plan.entry_bytes, dtype=np.uint8)
+    check(lib().kimkv_shared_decode_plan(*args, entries.ctypes.data_as(ctypes.c_void_p), plan.entry_bytes,
+                                         ctypes.byref(plan)), "shared_decode_plan")
+    return entries, plan
+
+
 def table_cache_bytes(total_chunks: int, chunk_tokens: int) -> int:
     """kimkv_decode_table_cache_bytes: the chunk table cache of a lane-record decode launch."""
     return int(lib().kimkv_decode_table_cache_bytes(total_chunks, chunk_tokens))
@@ -595,6 +674,18 @@ def linear_tune(x_ptr: int, rows: int, in_features: int, w_ptrs, out_features: i
     ws = (ctypes.c_void_p * len(w_ptrs))(*[ctypes.c_void_p(p) for p in w_ptrs])
     check(lib().kimkv_linear_tune(ctypes.c_void_p(x_ptr), rows, in_features, ws, len(w_ptrs), out_features,
                                   ctypes.c_void_p(y_ptr), 1 if y_f32 else 0, beta, _sh(stream)), "linear_tune")
+
+
+def logits_workspace_bytes(rows: int, vocabulary: int) -> int:
+    return int(lib().kimkv_logits_workspace_bytes(rows, vocabulary))
+
+
+def logits_adjust(logits_ptr: int, rows: int, vocabulary: int, rules_ptr: int, out_ptr: int, tokens_ptr: int,
+                  workspace_ptr: int = 0, stream: Optional[Stream] = None) -> None:
+    """kimkv_model_logits_adjust: a LOGITS_RULE for each row (device memory; 0: none) applied to fp32 logits; the
+    adjusted rows to out_ptr, their greedy tokens to tokens_ptr (0: not wanted)."""
+    check(lib().kimkv_model_logits_adjust(logits_ptr, rows, vocabulary, rules_ptr, out_ptr, tokens_ptr, workspace_ptr,
+                                          stream.handle if stream else None), "model_logits_adjust")
 
 
 def decode_timing(enable, every: int = 1):

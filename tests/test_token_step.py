@@ -1,0 +1,127 @@
+"""CPU checks of the token step's operators (rotated append, shared-prefix decode, adjusted logits): struct layouts,
+refusals that need no device, and the shared decode's plan, which is host code."""
+import ctypes
+
+import numpy as np
+import pytest
+
+UNIT = np.dtype([("table_lane", "<u4"), ("lane", "<u4"), ("lanes", "<u4"), ("begin", "<u4"), ("end", "<u4"), ("slot", "<u4"),
+                 ("head", "<u2"), ("heads", "<u2"), ("single", "<u4")])
+LANE = np.dtype([("table_lane", "<u4"), ("tokens", "<u4"), ("prefix_slot", "<u4"), ("prefix_stride", "<u4"),
+                 ("prefix_count", "<u4"), ("tail_slot", "<u4"), ("tail_count", "<u4"), ("merged", "<u4")])
+
+
+def split_entries(entries, plan):
+    units = entries[:plan.unit_count * UNIT.itemsize].view(UNIT)
+    return units[units["lanes"] != 0], entries[plan.unit_count * UNIT.itemsize:].view(LANE)
+
+
+def test_struct_layouts(kimkv):
+    d = kimkv.device
+    assert d.APPEND_ROPE_JOB.itemsize == 28
+    assert d.LOGITS_RULE.itemsize == 56
+    assert ctypes.sizeof(d.Rope) == 16
+    assert ctypes.sizeof(d.SharedGroup) == 12
+    assert ctypes.sizeof(d.SharedPlan) == 48
+
+
+@pytest.mark.parametrize("heads,dim,group", [(4, 64, 8), (8, 128, 4), (1, 64, 1), (3, 96, 5), (2, 12, 40), (16, 64, 1)])
+def test_plan_covers_every_key_once(kimkv, heads, dim, group):
+    """Every (lane, KV head, token) is in exactly one unit; parts sit in slots of their own that the lane's record lists;
+    a prefix is read through the group's first lane in blocks of 64 that every lane holds."""
+    d = kimkv.device
+    rng = np.random.default_rng(heads * dim + group)
+    cases = [([1], []), ([0], []), ([0, 5, 0], [(0, 3, 5)]), ([64] * 3, [(0, 3, 64)]), ([500, 700], [(0, 2, 450)]),
+             ([65, 63], [(0, 2, 64)]), ([3000] * 9 + [40], [(0, 9, 2999)]), ([9000, 100, 9000, 9000], [(2, 2, 8000)]),
+             ([40000] * 3, [(0, 3, 40000)]), ([1000] * 70, [(0, 70, 900)]), ([2000] * 6, [(0, 2, 1000), (3, 3, 1999)])]
+    for _ in range(6):
+        n = int(rng.integers(2, 40))
+        cut = int(rng.integers(1, n))
+        prefixes = rng.integers(1, 5000, 2)
+        counts = [int(prefixes[int(i >= cut)] + rng.integers(0, 900)) for i in range(n)]
+        cases.append((counts, [(0, cut, int(prefixes[0])), (cut, n - cut, int(prefixes[1]))]))
+    for counts, groups in cases:
+        entries, plan = d.shared_decode_plan(heads, dim, heads * group, 256, counts, groups)
+        assert plan.entry_bytes == len(entries) == plan.unit_count * 32 + len(counts) * 32
+        units, lanes = split_entries(entries, plan)
+        assert (plan.kv_heads, plan.head_dim, plan.query_heads, plan.lane_count) == (heads, dim, heads * group, len(counts))
+        seen = [np.zeros((heads, t), dtype=np.int32) for t in counts]
+        slots = {}
+        of_lane = {i: first for first, n, _ in groups for i in range(first, first + n)}
+        for u in units:
+            assert u["begin"] < u["end"] and u["heads"] > 0 and int(u["head"]) + int(u["heads"]) <= heads
+            for i in range(int(u["lanes"])):
+                lane = int(u["lane"]) + i
+                seen[lane][int(u["head"]):int(u["head"]) + int(u["heads"]), int(u["begin"]):int(u["end"])] += 1
+                if lane != u["table_lane"]:
+                    assert of_lane[lane] == u["table_lane"] and u["end"] <= groups[[g[0] for g in groups].index(of_lane[lane])][2]
+                    assert u["begin"] % 64 == 0 and u["end"] % 64 == 0
+                if not u["single"]:
+                    for h in range(int(u["head"]), int(u["head"]) + int(u["heads"])):
+                        assert (int(u["slot"]) + i, h) not in slots
+                        slots[int(u["slot"]) + i, h] = lane
+        for lane, marks in enumerate(seen):
+            assert np.all(marks == 1), (counts, groups, lane)
+        assert plan.merge_lanes == int(lanes["merged"].sum())
+        for lane, rec in enumerate(lanes):
+            assert rec["tokens"] == counts[lane]
+            mine = [int(rec["prefix_slot"]) + k * int(rec["prefix_stride"]) for k in range(int(rec["prefix_count"]))]
+            mine += [int(rec["tail_slot"]) + k for k in range(int(rec["tail_count"]))] if rec["merged"] else []
+            want = sorted(s for (s, h), at in slots.items() if at == lane and h == 0)
+            assert sorted(map(int, mine)) == want and all(s < plan.slot_count for s in want)
+            assert bool(rec["merged"]) == (len(want) > 0)
+        o = (plan.slot_count * heads * group * dim * 4 + 15) // 16 * 16
+        assert plan.workspace_bytes == o + plan.slot_count * heads * group * 8
+
+
+def test_plan_refusals(kimkv):
+    d = kimkv.device
+    lib = d.lib()
+    counts = np.array([100, 200, 300], dtype=np.uint32)
+    ptr = counts.ctypes.data_as(ctypes.c_void_p)
+    plan = d.SharedPlan()
+
+    def status(heads=4, dim=64, qh=32, lanes=3, groups=(), count_ptr=ptr, capacity=0, entries=None):
+        shared = (d.SharedGroup * len(groups))(*[d.SharedGroup(*g) for g in groups])
+        return lib.kimkv_shared_decode_plan(heads, dim, qh, 256, count_ptr, lanes, shared, len(groups), entries, capacity,
+                                            ctypes.byref(plan))
+
+    for bad in (dict(heads=0), dict(qh=0), dict(qh=30), dict(dim=0), dict(dim=257), dict(heads=1 << 16, qh=1 << 16), dict(count_ptr=None),
+                dict(groups=[(0, 4, 64)]), dict(groups=[(3, 1, 64)]), dict(groups=[(0, 2, 64), (1, 2, 64)]),
+                dict(groups=[(0xFFFFFFFF, 2, 64)]), dict(groups=[(1, 0xFFFFFFFF, 64)])):
+        assert status(**bad) == d.INVALID_ARGUMENT, bad
+        assert plan.entry_bytes == 0, bad
+    assert lib.kimkv_shared_decode_plan(4, 64, 32, 256, ptr, 3, None, 1, None, 0, ctypes.byref(plan)) == d.INVALID_ARGUMENT
+    assert lib.kimkv_shared_decode_plan(4, 64, 32, 256, ptr, 3, None, 0, None, 0, None) == d.INVALID_ARGUMENT
+    # Too small: the size comes back, and nothing is written past it.
+    assert status() == d.INVALID_ARGUMENT and plan.entry_bytes > 0
+    need = plan.entry_bytes
+    buf = np.full(need + 64, 0xAB, dtype=np.uint8)
+    assert status(capacity=need - 1, entries=buf.ctypes.data_as(ctypes.c_void_p)) == d.INVALID_ARGUMENT
+    assert np.all(buf == 0xAB) and plan.entry_bytes == need
+    assert status(capacity=need, entries=buf.ctypes.data_as(ctypes.c_void_p)) == d.OK and np.all(buf[need:] == 0xAB)
+    # No lanes: nothing to do, no error.
+    entries, empty = d.shared_decode_plan(4, 64, 32, 256, [], [])
+    assert len(entries) == 0 and empty.unit_count == 0 and empty.workspace_bytes == 0
+    # A group of lanes that do not all hold its prefix shares what they do hold.
+    entries, p = d.shared_decode_plan(4, 64, 32, 256, [5000, 700, 5000], [(0, 3, 4000)])
+    units, _ = split_entries(entries, p)
+    assert max(int(u["end"]) for u in units if u["lanes"] > 1) <= 700
+
+
+def test_entry_points_refuse_null(kimkv):
+    d = kimkv.device
+    lib = d.lib()
+    rope = d.Rope(10000.0, 64, 0)
+    assert lib.kimkv_append_rope_batch(None, None, 0, 0, 0, None, 0, 0, 32, rope, None, 0, None) == d.INVALID_ARGUMENT
+    assert lib.kimkv_shared_decode_batch(None, None, None, d.SharedPlan(), None, None) == d.INVALID_ARGUMENT
+    one = ctypes.c_void_p(16)
+    for args in ((None, 1, 8, None, one, one), (one, 1, 0, None, one, one), (one, 1, 8, None, None, None),
+                 (one, 1, 1 << 31, None, one, one)):
+        assert lib.kimkv_model_logits_adjust(*args, None, None) == d.INVALID_ARGUMENT
+    # Several slices of the vocabulary and no workspace, or one off its alignment.
+    assert lib.kimkv_logits_workspace_bytes(3, 1 << 20) > 0
+    assert lib.kimkv_model_logits_adjust(one, 3, 1 << 20, None, None, one, None, None) == d.INVALID_ARGUMENT
+    assert lib.kimkv_model_logits_adjust(one, 3, 1 << 20, None, None, one, ctypes.c_void_p(20), None) == d.INVALID_ARGUMENT
+    # No rows: nothing to do.
+    assert lib.kimkv_model_logits_adjust(one, 0, 1 << 20, None, None, one, None, None) == d.OK
