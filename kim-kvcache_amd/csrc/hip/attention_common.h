@@ -71,6 +71,20 @@ __device__ inline float wave_sum(float v)
     return v;
 }
 
+// Cross-row exchanges of a wave64 on the VALU (v_permlane16/32_swap): the
+// value of lane l ^ 16 and of lane l ^ 32.
+__device__ inline float xor16(float v)
+{
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 16u) ? r[0] : r[1]);
+}
+
+__device__ inline float xor32(float v)
+{
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 32u) ? r[0] : r[1]);
+}
+
 __device__ inline half8_t load_half8(const uint16_t* p)
 {
     return *reinterpret_cast<const half8_t*>(p);

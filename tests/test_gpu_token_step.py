@@ -559,15 +559,15 @@ def test_shared_decode_faults(dev):
 def test_shared_decode_bad_entries(dev):
     """Entries that name what is not there are reported, not run: every index is checked against the launch's buffers."""
     counts, groups = [700, 710, 720], [(0, 3, 690)]
-    for field, value in (("table_lane", 3), ("lane", 3), ("lanes", 4), ("lane", 0xFFFFFFFF), ("lanes", 0xFFFFFFFF), ("end", 1 << 20), ("begin", 1 << 20),
-                         ("slot", 1 << 20), ("slot", 0xFFFFFFFF), ("head", 2), ("heads", 3), ("heads", 0)):
+    for field, value in (("table_lane", 3), ("lane", 3), ("col0", 4), ("cols", 13), ("lane", 0xFFFFFFFF), ("col0", 0xFFFFFFFF), ("cols", 0xFFFFFFFF),
+                         ("end", 1 << 20), ("begin", 1 << 20), ("slot", 1 << 20), ("slot", 0xFFFFFFFF), ("head", 2), ("heads", 3), ("heads", 0)):
         print(f"shared entry {field}={value}", flush=True)
         b = _Batch(dev, 2, 64, 4, counts, groups)
         b.place()
         b.plan()
         entries = b.entries.copy()
         units = entries[:b.p.unit_count * UNIT.itemsize].view(UNIT)
-        at = [i for i in range(len(units)) if units[i]["lanes"] > 1][0]
+        at = [i for i in range(len(units)) if units[i]["cols"] > 4][0]   # 12 columns: three lanes
         units[at][field] = value
         b.entries_buf = dev.upload(entries)
         b.launch()

@@ -5,15 +5,16 @@ import ctypes
 import numpy as np
 import pytest
 
-UNIT = np.dtype([("table_lane", "<u4"), ("lane", "<u4"), ("lanes", "<u4"), ("begin", "<u4"), ("end", "<u4"), ("slot", "<u4"),
-                 ("head", "<u2"), ("heads", "<u2"), ("single", "<u4")])
+UNIT = np.dtype([("table_lane", "<u4"), ("lane", "<u4"), ("col0", "<u4"), ("cols", "<u4"), ("begin", "<u4"), ("end", "<u4"),
+                 ("slot", "<u4"), ("head", "<u2"), ("heads", "u1"), ("kind", "u1")])
+SINGLE = 0x80
 LANE = np.dtype([("table_lane", "<u4"), ("tokens", "<u4"), ("prefix_slot", "<u4"), ("prefix_stride", "<u4"),
                  ("prefix_count", "<u4"), ("tail_slot", "<u4"), ("tail_count", "<u4"), ("merged", "<u4")])
 
 
 def split_entries(entries, plan):
     units = entries[:plan.unit_count * UNIT.itemsize].view(UNIT)
-    return units[units["lanes"] != 0], entries[plan.unit_count * UNIT.itemsize:].view(LANE)
+    return units[units["cols"] != 0], entries[plan.unit_count * UNIT.itemsize:].view(LANE)
 
 
 def test_struct_layouts(kimkv):
@@ -27,7 +28,7 @@ def test_struct_layouts(kimkv):
 
 @pytest.mark.parametrize("heads,dim,group", [(4, 64, 8), (8, 128, 4), (1, 64, 1), (3, 96, 5), (2, 12, 40), (16, 64, 1)])
 def test_plan_covers_every_key_once(kimkv, heads, dim, group):
-    """Every (lane, KV head, token) is in exactly one unit; parts sit in slots of their own that the lane's record lists;
+    """Every (lane, query head, token) is in exactly one unit; parts sit in slots of their own that the lane's record lists;
     a prefix is read through the group's first lane in blocks of 64 that every lane holds."""
     d = kimkv.device
     rng = np.random.default_rng(heads * dim + group)
@@ -45,21 +46,24 @@ def test_plan_covers_every_key_once(kimkv, heads, dim, group):
         assert plan.entry_bytes == len(entries) == plan.unit_count * 32 + len(counts) * 32
         units, lanes = split_entries(entries, plan)
         assert (plan.kv_heads, plan.head_dim, plan.query_heads, plan.lane_count) == (heads, dim, heads * group, len(counts))
-        seen = [np.zeros((heads, t), dtype=np.int32) for t in counts]
+        seen = [np.zeros((heads, group, t), dtype=np.int8) for t in counts]
         slots = {}
         of_lane = {i: first for first, n, _ in groups for i in range(first, first + n)}
-        for u in units:
-            assert u["begin"] < u["end"] and u["heads"] > 0 and int(u["head"]) + int(u["heads"]) <= heads
-            for i in range(int(u["lanes"])):
-                lane = int(u["lane"]) + i
-                seen[lane][int(u["head"]):int(u["head"]) + int(u["heads"]), int(u["begin"]):int(u["end"])] += 1
-                if lane != u["table_lane"]:
-                    assert of_lane[lane] == u["table_lane"] and u["end"] <= groups[[g[0] for g in groups].index(of_lane[lane])][2]
-                    assert u["begin"] % 64 == 0 and u["end"] % 64 == 0
-                if not u["single"]:
-                    for h in range(int(u["head"]), int(u["head"]) + int(u["heads"])):
-                        assert (int(u["slot"]) + i, h) not in slots
-                        slots[int(u["slot"]) + i, h] = lane
+        assert plan.unit_count % 8 == 0
+        for u in units.tolist():
+            table_lane, lane0, col0, cols, begin, end, slot, head, of_heads, kind = u
+            assert begin < end and begin % 64 == 0 and end - begin <= 4096 and of_heads > 0 and head + of_heads <= heads
+            assert (cols <= 16) if kind & 0x7F == 0 else (cols <= 64 * (kind & 0x7F) and of_heads == 1 and end % 64 == 0)
+            for c in range(col0, col0 + cols):
+                lane = lane0 + c // group
+                seen[lane][head:head + of_heads, c % group, begin:end] += 1
+                if lane != table_lane:
+                    assert of_lane[lane] == table_lane and end <= groups[[g[0] for g in groups].index(of_lane[lane])][2]
+                if not kind & SINGLE:
+                    for h in range(head, head + of_heads):
+                        q = h * group + c % group
+                        assert (slot + c // group, q) not in slots
+                        slots[slot + c // group, q] = lane
         for lane, marks in enumerate(seen):
             assert np.all(marks == 1), (counts, groups, lane)
         assert plan.merge_lanes == int(lanes["merged"].sum())
@@ -68,6 +72,8 @@ def test_plan_covers_every_key_once(kimkv, heads, dim, group):
             mine = [int(rec["prefix_slot"]) + k * int(rec["prefix_stride"]) for k in range(int(rec["prefix_count"]))]
             mine += [int(rec["tail_slot"]) + k for k in range(int(rec["tail_count"]))] if rec["merged"] else []
             want = sorted(s for (s, h), at in slots.items() if at == lane and h == 0)
+            for q in range(heads * group):   # each part is whole
+                assert all(slots.get((s, q)) == lane for s in want)
             assert sorted(map(int, mine)) == want and all(s < plan.slot_count for s in want)
             assert bool(rec["merged"]) == (len(want) > 0)
         o = (plan.slot_count * heads * group * dim * 4 + 15) // 16 * 16
@@ -106,7 +112,7 @@ def test_plan_refusals(kimkv):
     # A group of lanes that do not all hold its prefix shares what they do hold.
     entries, p = d.shared_decode_plan(4, 64, 32, 256, [5000, 700, 5000], [(0, 3, 4000)])
     units, _ = split_entries(entries, p)
-    assert max(int(u["end"]) for u in units if u["lanes"] > 1) <= 700
+    assert max(u["end"] for u in units if u["lane"] == 0 and u["cols"] > 8) <= 700
 
 
 def test_entry_points_refuse_null(kimkv):
