@@ -130,4 +130,44 @@ __device__ inline void add_groups(const PoolView& P, kimkv_block_desc const& e, 
     }
 }
 
+// One 8-key group of a key range resolved for a layer and KV head (prefill and
+// shared-prefix decode): k points at the group's first key in K panel 0 (panel p, dims 32 p ..
+// 32 p + 31, is p * kpanel elements further), v at the group's first key in
+// V^T row 0 (dim d is d * vw elements further).
+struct HeadGroup {
+    const uint16_t* k;
+    const uint16_t* v;
+    uint32_t kpanel;
+    uint32_t vw;
+    uint64_t pad;
+};
+
+// Records the 8-key groups of [c0, c1) that entry `e` covers, for layer /
+// head.  An entry whose pages do not keep 8-token groups aligned (or that
+// names no page of the storage) switches the block to the generic path.
+template <uint32_t kDim>
+__device__ inline void add_head_groups(const PoolView& P, kimkv_block_desc const& e, uint32_t layer, uint32_t h,
+                                       uint32_t c0, uint32_t c1, uint32_t T, HeadGroup* groups, uint32_t* s_generic)
+{
+    uint32_t const b = e.logical_token_begin;
+    uint32_t const end = b + e.valid_tokens;
+    uint32_t const lo = max(b, c0);
+    uint32_t const hi = min(end, c1);
+    if (lo >= hi) return;
+    uint32_t const cap = e.page_token_capacity;
+    const uint16_t* page = page_base(P, e.kind, e.slot, cap);
+    bool const aligned = (b & 7u) == 0 && (cap & 7u) == 0 && e.valid_tokens <= cap
+        && ((end & 7u) == 0 || end >= T) && page != nullptr;
+    if (!aligned) {
+        *s_generic = 1;
+        return;
+    }
+    const uint16_t* hb = page + head_block(P, cap, layer, h);
+    uint32_t const vw = v_width(cap);
+    for (uint32_t g = (lo - c0) >> 3; g < (hi - c0 + 7) >> 3; ++g) {
+        uint32_t const pt0 = c0 + 8 * g - b;
+        groups[g] = HeadGroup{hb + k_offset(cap, kDim, pt0, 0), hb + v_offset(cap, kDim, pt0, 0), cap * 32u, vw, 0};
+    }
+}
+
 }  // namespace kimkv

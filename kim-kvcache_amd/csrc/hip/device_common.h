@@ -160,6 +160,28 @@ __host__ __device__ inline uint64_t v_offset(uint32_t cap, uint32_t D, uint32_t 
         + t % vw;
 }
 
+// x / d and x % d for a d that is uniform over the launch: the reciprocal is
+// computed on the host (floor((2^32 - 1) / d)), so the quotient is at most one
+// short and one compare corrects it.  Exact for every x < 2^32; an integer
+// division by a kernel argument is about 30 instructions, this is 7.
+struct Divisor {
+    uint32_t d;
+    uint32_t m;
+};
+inline Divisor divisor(uint32_t d) { return Divisor{d, 0xFFFFFFFFu / (d == 0 ? 1u : d)}; }
+
+__device__ inline uint32_t div_mod(uint32_t x, Divisor v, uint32_t* rem)
+{
+    uint32_t q = __umulhi(x, v.m);
+    uint32_t r = x - q * v.d;
+    if (r >= v.d) {
+        ++q;
+        r -= v.d;
+    }
+    *rem = r;
+    return q;
+}
+
 // ---- XCD-aware workgroup order ----------------------------------------------
 // MI355X dispatches the workgroups of a launch round-robin over its 8 XCDs
 // (workgroup w runs on XCD w % 8), each with its own L2.  This maps dispatch

@@ -30,28 +30,6 @@ struct TokEntry {
     uint32_t pt;
 };
 
-// x / d and x % d for a d that is uniform over the launch: the reciprocal is
-// computed on the host (floor((2^32 - 1) / d)), so the quotient is at most one
-// short and one compare corrects it.  Exact for every x < 2^32; an integer
-// division by a kernel argument is about 30 instructions, this is 7.
-struct Divisor {
-    uint32_t d;
-    uint32_t m;
-};
-inline Divisor divisor(uint32_t d) { return Divisor{d, 0xFFFFFFFFu / (d == 0 ? 1u : d)}; }
-
-__device__ inline uint32_t div_mod(uint32_t x, Divisor v, uint32_t* rem)
-{
-    uint32_t q = __umulhi(x, v.m);
-    uint32_t r = x - q * v.d;
-    if (r >= v.d) {
-        ++q;
-        r -= v.d;
-    }
-    *rem = r;
-    return q;
-}
-
 // k_offset and v_offset (device_common.h) without their divisions: d < D and
 // t < cap, so the column block is a shift or 0, which the compiler cannot
 // tell of a width that is 32 or the whole row.  A copy computes two such

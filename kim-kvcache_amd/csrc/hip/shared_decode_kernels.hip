@@ -25,7 +25,6 @@
 #include <vector>
 
 #include "attention_common.h"
-#include "attention_tiles.h"
 #include "device_common.h"
 #include "runtime_internal.h"
 
@@ -37,8 +36,7 @@ constexpr unsigned kWaves = kBlock / kWave;
 constexpr uint32_t kMaxDim = 256;
 
 // How a unit is computed.
-constexpr uint8_t kDirect = 0;      // few columns: the waves split heads and tokens; 1, 2, 4: staged tiles, that many
-constexpr uint8_t kSingle = 0x80;   // 16-column blocks a wave.  kSingle: the lane has no other part.
+constexpr uint8_t kSingle = 0x80;   // the lane has no other part; the rest: 1, 2 or 4 blocks of 16 columns a wave
 
 // Tokens [begin, end) of table_lane's table for KV heads [head, head + heads).
 // Of the score matrix of lanes lane, lane + 1, ... (G query heads of a KV head
@@ -90,6 +88,7 @@ struct SharedArgs {
     uint32_t lane_count;
     uint32_t slot_count;
     uint32_t QH;
+    Divisor group;   // query heads a KV head
 };
 
 // Whether a lane can be computed: an item as planned.
@@ -112,45 +111,71 @@ __device__ inline bool lane_ok(const PoolView& P, const SharedArgs& a, uint32_t 
     return lane_valid(P, first, a.lanes[rec.table_lane].tokens) && first.layer == item.layer;
 }
 
-// One column of a unit: query row, scale, and whether there is one (a lane
-// whose item is not as planned, or is of another layer than the table's, has
-// none).
+// Reports a column whose lane cannot be computed.
+__device__ inline void report_column(const PoolView& P, bool missing)
+{
+    if (missing && P.faults != nullptr) atomicOr(P.faults, KIMKV_FAULT_DECODE_ITEM);
+}
+
+// One column of a unit: its lane's item and query head in the group; !ok
+// where the lane's item is not as planned, or of another layer than the
+// table's.
 struct Column {
-    const uint16_t* query;
+    const uint16_t* query;   // row of KV head 0
+    uint16_t* output;
     float scale2;            // attention scale * log2 e
+    uint32_t lane;           // from u.lane on
+    uint32_t q;
     bool ok;
 };
 
-__device__ inline Column unit_column(const PoolView& P, const SharedArgs& a, const SharedUnit& u, uint32_t layer, uint32_t G,
-                                     uint32_t h, uint32_t c)
+__device__ inline Column unit_column(const PoolView& P, const SharedArgs& a, const SharedUnit& u, uint32_t layer, uint32_t c)
 {
-    if (c >= u.cols) return Column{nullptr, 0.0f, false};
-    uint32_t const lane = u.lane + (u.col0 + c) / G;
-    kimkv_decode_item const item = a.items[lane];
-    bool const ok = lane_valid(P, item, a.lanes[lane].tokens) && item.layer == layer;
-    return Column{item.query + (static_cast<uint64_t>(h) * G + (u.col0 + c) % G) * P.dim, item.attention_scale * kLog2e, ok};
+    Column out{};
+    out.lane = div_mod(u.col0 + min(c, u.cols - 1), a.group, &out.q);
+    kimkv_decode_item const item = a.items[u.lane + out.lane];
+    out.ok = c < u.cols && lane_valid(P, item, a.lanes[u.lane + out.lane].tokens) && item.layer == layer;
+    out.query = item.query + out.q * P.dim;
+    out.output = item.output + out.q * P.dim;
+    out.scale2 = item.attention_scale * kLog2e;
+    return out;
 }
 
-// Where column c's part of KV head h goes.
-struct PartOut {
-    float* o;
-    float2* ml;
-    uint16_t* output;   // instead, for a lane of one part
+// Where a column's parts go (KV head h: G h rows further), or its output
+// where the lane has one part.
+struct ColumnOut {
+    uint64_t row;
+    uint16_t* output;
+    uint32_t ok;
 };
 
-__device__ inline PartOut part_out(const SharedArgs& a, const SharedUnit& u, uint32_t D, uint32_t G, uint32_t h, uint32_t c)
+__device__ inline ColumnOut column_out(const SharedArgs& a, const SharedUnit& u, const Column& c)
 {
-    uint32_t const i = (u.col0 + c) / G;
-    uint32_t const q = h * G + (u.col0 + c) % G;
-    if ((u.kind & kSingle) != 0) return PartOut{nullptr, nullptr, a.items[u.lane + i].output + static_cast<uint64_t>(q) * D};
-    uint64_t const row = static_cast<uint64_t>(u.slot + i) * a.QH + q;
-    return PartOut{a.parts.o + row * D, a.parts.ml + row, nullptr};
+    return ColumnOut{static_cast<uint64_t>(u.slot + c.lane) * a.QH + c.q, (u.kind & kSingle) != 0 ? c.output : nullptr,
+                     c.ok ? 1u : 0u};
 }
 
 // o / l as an output: 0 for a row without any weight, l itself where it is not finite or NaN.
 __device__ inline uint16_t output_half(float o, float l)
 {
     return __half_as_ushort(__float2half_rn(l > 0.0f ? o / l : l == 0.0f ? 0.0f : l));
+}
+
+// kWidth outputs o / l, in one store where the address allows it.
+template <uint32_t kWidth, typename Vec>
+__device__ inline void store_outputs(uint16_t* to, const Vec& o, float l)
+{
+    float const inv = l > 0.0f ? 1.0f / l : 0.0f;
+    uint16_t v[kWidth];
+#pragma unroll
+    for (uint32_t j = 0; j < kWidth; ++j) v[j] = l >= 0.0f ? __half_as_ushort(__float2half_rn(o[j] * inv)) : output_half(o[j], l);
+    if (kWidth == 4 && (reinterpret_cast<uintptr_t>(to) & 7u) == 0) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(v[0] | static_cast<uint32_t>(v[1 % kWidth]) << 16,
+                                                   v[2 % kWidth] | static_cast<uint32_t>(v[3 % kWidth]) << 16);
+        return;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kWidth; ++j) to[j] = v[j];
 }
 
 // ---------------------------------------------------------------------------
@@ -172,7 +197,7 @@ struct RowParts {
     float l[kRows];
 };
 
-__device__ void attend_rows_generic(const PoolView& P, const kimkv_decode_item& table, uint32_t h, uint32_t c0,
+__device__ void attend_rows_generic(const PoolView& P, const kimkv_decode_item& table, uint32_t G, uint32_t h, uint32_t c0,
                                     uint32_t c1, Column const (&rows)[kRows], RowParts& out)
 {
     uint32_t const lane = threadIdx.x & (kWave - 1);
@@ -185,7 +210,7 @@ __device__ void attend_rows_generic(const PoolView& P, const kimkv_decode_item& 
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
             uint32_t const d = lane + 64 * k;
-            q[r][k] = rows[r].ok && d < D ? __half2float(__ushort_as_half(rows[r].query[d])) : 0.0f;
+            q[r][k] = rows[r].ok && d < D ? __half2float(__ushort_as_half(rows[r].query[h * G * D + d])) : 0.0f;
             out.o[r][k] = 0.0f;
         }
     }
@@ -290,9 +315,12 @@ __device__ void unit_generic(const PoolView& P, const SharedArgs& a, const Share
             uint32_t const c1 = min(c0 + piece, u.end);
             Column rows[kRows];
 #pragma unroll
-            for (uint32_t r = 0; r < kRows; ++r) rows[r] = unit_column(P, a, u, table.layer, G, h, col0 + r);
+            for (uint32_t r = 0; r < kRows; ++r) {
+                rows[r] = unit_column(P, a, u, table.layer, col0 + r);
+                report_column(P, !rows[r].ok && col0 + r < u.cols);
+            }
             RowParts part;
-            attend_rows_generic(P, table, h, c0, c1, rows, part);
+            attend_rows_generic(P, table, G, h, c0, c1, rows, part);
 #pragma unroll
             for (uint32_t r = 0; r < kRows; ++r) {
 #pragma unroll
@@ -310,7 +338,9 @@ __device__ void unit_generic(const PoolView& P, const SharedArgs& a, const Share
             uint32_t const w = i / D / kRows * split;
             uint32_t const mine = t0 + w / split;
             uint32_t const c = mine % batches * kRows + r;
-            if (mine >= tasks || !unit_column(P, a, u, table.layer, G, u.head + mine / batches, c).ok) continue;
+            if (mine >= tasks || c >= columns) continue;
+            Column const column = unit_column(P, a, u, table.layer, c);
+            if (!column.ok) continue;
             float M = -INFINITY;
             for (uint32_t s = 0; s < split; ++s) M = fmaxf(M, lds.m[w + s][r]);
             float o = 0.0f;
@@ -321,12 +351,13 @@ __device__ void unit_generic(const PoolView& P, const SharedArgs& a, const Share
                 o += f * lds.o[w + s][r][d];
                 l += f * lds.l[w + s][r];
             }
-            PartOut const to = part_out(a, u, D, G, u.head + mine / batches, c);
+            ColumnOut const to = column_out(a, u, column);
+            uint32_t const q = (u.head + mine / batches) * G;
             if (to.output != nullptr) {
-                to.output[d] = output_half(o, l);
+                to.output[q * D + d] = output_half(o, l);
             } else {
-                to.o[d] = o;
-                if (d == 0) *to.ml = make_float2(M, l);
+                a.parts.o[(to.row + q) * D + d] = o;
+                if (d == 0) a.parts.ml[to.row + q] = make_float2(M, l);
             }
         }
         __syncthreads();
@@ -342,7 +373,6 @@ __device__ void unit_generic(const PoolView& P, const SharedArgs& a, const Share
 // column l % 16.  Weights go to the matrix cores in two fp16 parts, p = hi +
 // lo, which keep what 32-bit weights do to 2^-22.
 // ---------------------------------------------------------------------------
-constexpr float kLazyRescaleLog2 = 8.0f;
 // Weights are 2^(s - m + kWeightShift), at most 2^15, so that lo stays a
 // normal fp16 number down to 2^-9 of the largest weight.
 constexpr float kWeightShift = 7.0f;
@@ -353,11 +383,17 @@ struct Columns {
     static constexpr uint32_t kDb = kDim / 16;
     half8_t q[kCB][kPanels];
     float scale2[kCB];
-    float m[kCB];   // reference point, -inf before the first finite score
+    float mref[kCB];   // weights are 2^(s - mref); inf (so 0) before the first finite score
     float l[kCB];   // of this lane's keys
     float4_t acc[kDb][kCB];   // O^T dims 16 db + 4 (l / 16) + i of column l % 16
     bool ok[kCB];
 };
+
+template <bool kStream>
+__device__ __attribute__((always_inline)) inline half8_t load_keys(const uint16_t* p)
+{
+    return kStream ? load_half8_stream(p) : *reinterpret_cast<const global_half8_t*>(reinterpret_cast<uintptr_t>(p));
+}
 
 // Eight halves of a caller's row, whose address carries no alignment promise.
 __device__ inline half8_t load_row8(const uint16_t* p)
@@ -369,45 +405,77 @@ __device__ inline half8_t load_row8(const uint16_t* p)
     return v;
 }
 
-// Column blocks from column c0 of the unit on.  Returns false when some
-// column's scale does not keep the order of the scores.
+// The unit's column blocks for KV head h, and where their parts go (outs, by
+// the first wave).  Returns false when some column's scale does not keep the
+// order of the scores.
 template <uint32_t kDim, uint32_t kCB>
 __device__ inline bool columns_init(Columns<kDim, kCB>& w, const PoolView& P, const SharedArgs& a, const SharedUnit& u,
-                                    uint32_t layer, uint32_t G, uint32_t h, uint32_t c0)
+                                    uint32_t layer, uint32_t h, ColumnOut* outs)
 {
+    // Lane i looks up column i of the wave's 16 kCB (a lane past them, one again) and hands it to the lanes that hold it.
     uint32_t const l = threadIdx.x & 63u;
+    uint32_t const mine = l % (16 * kCB);
+    Column const c = unit_column(P, a, u, layer, mine);
+    auto const at = reinterpret_cast<uintptr_t>(c.query + h * a.group.d * kDim);
+    auto const at_lo = static_cast<int>(at);
+    auto const at_hi = static_cast<int>(at >> 32);
+    if (threadIdx.x < 16 * kCB) outs[mine] = column_out(a, u, c);
     bool ordered = true;
 #pragma unroll
     for (uint32_t cb = 0; cb < kCB; ++cb) {
-        Column const c = unit_column(P, a, u, layer, G, h, c0 + 16 * cb + (l & 15u));
-        w.ok[cb] = c.ok;
-        w.scale2[cb] = c.ok ? c.scale2 : 1.0f;
-        ordered = ordered && w.scale2[cb] > 0.0f && w.scale2[cb] < INFINITY;
-        w.m[cb] = -INFINITY;
-        w.l[cb] = 0.0f;
+        auto const from = static_cast<int>(16 * cb + (l & 15u));
+        w.ok[cb] = __shfl(static_cast<int>(c.ok), from) != 0;
+        auto const lo = static_cast<uint32_t>(__shfl(at_lo, from));
+        auto const hi = static_cast<uint32_t>(__shfl(at_hi, from));
+        float const scale2 = __shfl(c.scale2, from);
+        const uint16_t* const row = reinterpret_cast<const uint16_t*>(static_cast<uint64_t>(hi) << 32 | lo);
 #pragma unroll
         for (uint32_t p = 0; p < kDim / 32; ++p) {
             w.q[cb][p] = half8_t{};
-            if (c.ok) w.q[cb][p] = load_row8(c.query + 32 * p + 8 * (l >> 4));
+            if (w.ok[cb]) w.q[cb][p] = load_row8(row + 32 * p + 8 * (l >> 4));
         }
+        w.scale2[cb] = w.ok[cb] ? scale2 : 1.0f;
+        ordered = ordered && w.scale2[cb] > 0.0f && w.scale2[cb] < INFINITY;
+        w.mref[cb] = INFINITY;
+        w.l[cb] = 0.0f;
 #pragma unroll
         for (uint32_t db = 0; db < kDim / 16; ++db) w.acc[db][cb] = float4_t{};
     }
+    bool const missing = !c.ok && mine < u.cols;
+    report_column(P, missing);
     return ordered;
 }
 
-// kMasked: only the first nvalid of the step's keys count (their V is finite).
-template <uint32_t kDim, uint32_t kCB, uint32_t kKB, bool kMasked>
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+
+// Both rounded toward zero: one instruction for two, and what it leaves of a
+// weight is taken up by the weight's second part.
+__device__ inline half2_t two_halves(float a, float b)
+{
+    return __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+
+// Only the first nvalid of the step's keys count (the others' V is finite).
+// Written so that there is one copy of it in a loop, whatever the step: its
+// instructions come from memory the first time, and a short unit runs them
+// once or twice.
+//
+// The weights are made against the reference point as it stands, and their
+// sum tells whether one of them passed 2^15: only then, and before the first
+// finite score, is the maximum taken, the reference moved and the step's
+// weights made anew.  (A maximum of every step's scores first costs half an
+// instruction a score and puts it in front of the exponentials.)
+template <uint32_t kDim, uint32_t kCB, uint32_t kKB>
 __device__ __attribute__((always_inline)) inline void attend_step(Columns<kDim, kCB>& w, half8_t const (&k)[kKB][2][kDim / 32],
                                                                   half8_t const (&v)[kKB][kDim / 16], uint32_t nvalid)
 {
-    uint32_t const a8 = (threadIdx.x & 48u) >> 1;   // 8 (l / 16)
+    constexpr float kMostWeight = 32768.0f;
+    // Not known to be -1, so that p - hi is one mixed-precision multiply-add.
+    float minus_one = -1.0f;
+    __asm__("" : "+s"(minus_one));
     float4_t s[kCB][kKB][2];
-    float mx[kCB];
-    bool over = false;
 #pragma unroll
     for (uint32_t cb = 0; cb < kCB; ++cb) {
-        mx[cb] = -INFINITY;
 #pragma unroll
         for (uint32_t kb = 0; kb < kKB; ++kb) {
 #pragma unroll
@@ -417,63 +485,114 @@ __device__ __attribute__((always_inline)) inline void attend_step(Columns<kDim, 
                 for (uint32_t p = 0; p < kDim / 32; ++p) {
                     z = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[kb][e][p], w.q[cb][p], z, 0, 0, 0);
                 }
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    if (kMasked && 32 * kb + a8 + 4 * e + i >= nvalid) z[i] = -INFINITY;
-                    mx[cb] = fmaxf(mx[cb], z[i]);
-                }
                 s[cb][kb][e] = z;
             }
         }
-        over = over || mx[cb] * w.scale2[cb] > w.m[cb] + kLazyRescaleLog2;
     }
-    // The reference point moves, and what was summed is rescaled, only when a
-    // score passes it by more than 2^8: a column's four lanes then agree on
-    // the maximum.
-    if (__builtin_expect(__any(over), 0)) {
-        __asm__ volatile("" ::: "memory");   // not speculated
+    if (__builtin_expect(nvalid < 32 * kKB, 0)) {
+        uint32_t a8 = (threadIdx.x & 48u) >> 1;   // 8 (l / 16)
+        __asm__ volatile("" : "+v"(a8));          // a branch, not a selection of every score
+#pragma unroll
+        for (uint32_t kb = 0; kb < kKB; ++kb) {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+                bool const gone = 32 * kb + a8 + j >= nvalid;
+#pragma unroll
+                for (uint32_t cb = 0; cb < kCB; ++cb) {
+                    if (gone) s[cb][kb][j / 4][j % 4] = -INFINITY;
+                }
+            }
+        }
+    }
+    half8_t hi[kCB][kKB], lo[kCB][kKB];
+    float sum[kCB];
+    bool over;
+    float alpha[kCB];
+#pragma unroll
+    for (uint32_t cb = 0; cb < kCB; ++cb) alpha[cb] = 1.0f;
+    uint32_t pass = 0;
+#pragma unroll 1
+    for (;;) {
+        over = false;
 #pragma unroll
         for (uint32_t cb = 0; cb < kCB; ++cb) {
-            float x = fmaxf(mx[cb], xor16(mx[cb]));
-            x = fmaxf(x, xor32(x)) * w.scale2[cb];
-            bool const grow = x > w.m[cb] + kLazyRescaleLog2;
-            float const alpha = grow ? __builtin_amdgcn_exp2f(w.m[cb] - x) : 1.0f;
-            if (grow) w.m[cb] = x;
-            w.l[cb] *= alpha;
+            sum[cb] = 0.0f;
 #pragma unroll
-            for (uint32_t db = 0; db < kDim / 16; ++db) w.acc[db][cb] *= alpha;
+            for (uint32_t kb = 0; kb < kKB; ++kb) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; j += 2) {
+                    float p[2];
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cb][kb][j / 4][j % 4 + i], w.scale2[cb], -w.mref[cb]));
+                    }
+                    sum[cb] += p[0] + p[1];
+                    half2_t const h = two_halves(p[0], p[1]);
+                    half2_t const rest = two_halves(__builtin_fmaf(static_cast<float>(h[0]), minus_one, p[0]),
+                                                    __builtin_fmaf(static_cast<float>(h[1]), minus_one, p[1]));
+                    hi[cb][kb][j] = h[0];
+                    hi[cb][kb][j + 1] = h[1];
+                    lo[cb][kb][j] = rest[0];
+                    lo[cb][kb][j + 1] = rest[1];
+                }
+            }
+            over = over || !(sum[cb] <= kMostWeight) || w.mref[cb] == INFINITY;
+        }
+        if (__builtin_expect(!__any(over), 1)) break;
+        // A column's four lanes agree on the maximum.  Once the reference
+        // stands there the sums are small, unless a score is infinite or NaN,
+        // which nothing helps.
+        if (pass != 0) break;
+        pass = 1;
+        __asm__ volatile("" : "+s"(pass));   // a loop of two passes would be made into two copies
+#pragma unroll
+        for (uint32_t cb = 0; cb < kCB; ++cb) {
+            float x = -INFINITY;
+#pragma unroll
+            for (uint32_t kb = 0; kb < kKB; ++kb) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    float score = s[cb][kb][j / 4][j % 4];
+                    __asm__ volatile("" : "+v"(score));   // taken here, not in front of the loop
+                    x = fmaxf(x, score);
+                }
+            }
+            x = fmaxf(x, xor16(x));
+            x = fmaxf(x, xor32(x)) * w.scale2[cb] - kWeightShift;
+            bool const first = w.mref[cb] == INFINITY && x > -INFINITY;
+            bool const grow = (first || x > w.mref[cb]) && x < INFINITY;
+            if (grow && !first) alpha[cb] = __builtin_amdgcn_exp2f(w.mref[cb] - x);
+            if (grow) w.mref[cb] = x;
+        }
+    }
+    if (__builtin_expect(pass != 0, 0)) {
+#pragma unroll
+        for (uint32_t cb = 0; cb < kCB; ++cb) {
+            w.l[cb] *= alpha[cb];
+#pragma unroll
+            for (uint32_t db = 0; db < kDim / 16; ++db) w.acc[db][cb] *= alpha[cb];
         }
     }
 #pragma unroll
     for (uint32_t cb = 0; cb < kCB; ++cb) {
-        // Without a finite score yet the reference is 0: the weights are 2^-inf.
-        float const mref = w.m[cb] == -INFINITY ? 0.0f : w.m[cb] - kWeightShift;
+        w.l[cb] += sum[cb];
 #pragma unroll
         for (uint32_t kb = 0; kb < kKB; ++kb) {
-            half8_t hi, lo;
 #pragma unroll
-            for (uint32_t e = 0; e < 2; ++e) {
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    float const p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cb][kb][e][i], w.scale2[cb], -mref));
-                    _Float16 const h = static_cast<_Float16>(p);
-                    w.l[cb] += p;
-                    hi[4 * e + i] = h;
-                    lo[4 * e + i] = static_cast<_Float16>(p - static_cast<float>(h));
-                }
+            for (uint32_t db = 0; db < kDim / 16; ++db) {
+                w.acc[db][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[kb][db], hi[cb][kb], w.acc[db][cb], 0, 0, 0);
             }
 #pragma unroll
             for (uint32_t db = 0; db < kDim / 16; ++db) {
-                w.acc[db][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[kb][db], hi, w.acc[db][cb], 0, 0, 0);
-                w.acc[db][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[kb][db], lo, w.acc[db][cb], 0, 0, 0);
+                w.acc[db][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[kb][db], lo[cb][kb], w.acc[db][cb], 0, 0, 0);
             }
         }
     }
 }
 
-// The state as a part: denominators summed over the column's lanes, m the
-// exponent's whole reference (-inf where there was no weight).  Returns
-// whether some value of a column that counts is not finite.
+// The state as a part: denominators summed over the column's lanes, mref -inf
+// where there was no finite score.  Returns whether some value of a column
+// that counts is not finite.
 template <uint32_t kDim, uint32_t kCB>
 __device__ inline bool columns_finish(Columns<kDim, kCB>& w)
 {
@@ -482,7 +601,7 @@ __device__ inline bool columns_finish(Columns<kDim, kCB>& w)
     for (uint32_t cb = 0; cb < kCB; ++cb) {
         w.l[cb] += xor16(w.l[cb]);
         w.l[cb] += xor32(w.l[cb]);
-        w.m[cb] -= kWeightShift;   // -inf stays
+        if (w.mref[cb] == INFINITY) w.mref[cb] = -INFINITY;
         float4_t f = {w.l[cb] * 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t db = 0; db < kDim / 16; ++db) f += w.acc[db][cb] * 0.0f;
@@ -493,52 +612,66 @@ __device__ inline bool columns_finish(Columns<kDim, kCB>& w)
 
 // ---- the unit's group table ---------------------------------------------------
 
-constexpr uint32_t kTableGroups = 512;   // 4096 keys: no longer units on the matrix cores
+constexpr uint32_t kTableGroups = 512;   // 4096 keys: a longer unit is taken in segments of that
+constexpr uint32_t kSegment = kTableGroups * 8;
 
 struct TableFlags {
-    uint32_t found;
     uint32_t generic;
     uint32_t first;
 };
 
-// Resolves the 8-key groups of [u.begin, u.end) for KV head u.head.  False
-// where the table does not keep them aligned and whole: the unit then goes the
-// generic path.  Called by every thread.
+// The entry that holds group threadIdx.x of keys begin.. in a table as promotion
+// leaves it: full extent pages of 64 tokens, then micro pages of 8.
+__device__ inline kimkv_block_desc guessed_entry(const kimkv_decode_item& table, uint32_t begin)
+{
+    uint32_t const t = begin + 8 * threadIdx.x;
+    uint32_t const extents = table.token_count / 64;
+    uint32_t const i = t / 64 < extents ? t / 64 : extents + (t - 64 * extents) / 8;
+    return table.descriptors[min(i, table.descriptor_count - 1)];
+}
+
+// Resolves the 8-key groups of [begin, end) for KV head `head`, group
+// threadIdx.x from `guess` (guessed_entry's) where every thread's is right,
+// else by searching.  False where the table does not keep the groups aligned
+// and whole: the unit then goes the generic path.  Called by every thread.
 template <uint32_t kDim>
-__device__ bool build_groups(const PoolView& P, const kimkv_decode_item& table, const SharedUnit& u, HeadGroup* groups,
-                             TableFlags& flags)
+__device__ bool build_groups(const PoolView& P, const kimkv_decode_item& table, uint32_t head, uint32_t begin,
+                             uint32_t end, kimkv_block_desc const& guess, HeadGroup* groups, TableFlags& flags)
 {
     uint32_t const tid = threadIdx.x;
-    uint32_t const ngroups = (u.end - u.begin + 7) / 8;
-    if (ngroups > kTableGroups || (u.begin & 7u) != 0) return false;
+    uint32_t const ngroups = (end - begin + 7) / 8;
+    static_assert(kTableGroups <= kBlock, "a thread a group");
+    bool right = true;
+    if (tid < ngroups) {
+        uint32_t const t = begin + 8 * tid;
+        uint32_t const cap = guess.page_token_capacity;
+        uint32_t const at = t - guess.logical_token_begin;
+        const uint16_t* const page = page_base(P, guess.kind, guess.slot, cap);
+        right = t >= guess.logical_token_begin && at < guess.valid_tokens && ((guess.logical_token_begin | cap) & 7u) == 0
+            && guess.valid_tokens <= cap && page != nullptr
+            && (guess.valid_tokens - at >= 8 || guess.logical_token_begin + guess.valid_tokens >= table.token_count);
+        if (right) {
+            const uint16_t* const block = page + head_block(P, cap, table.layer, head);
+            groups[tid] = HeadGroup{block + k_offset(cap, kDim, at, 0), block + v_offset(cap, kDim, at, 0), cap * 32u, v_width(cap), 0};
+        }
+    }
+    if (__syncthreads_and(right) != 0) return true;
     for (uint32_t g = tid; g < ngroups; g += kBlock) groups[g].k = nullptr;
-    if (tid == 0) flags = TableFlags{0, 0, 0};
-    __syncthreads();
-    // The first entry is guessed before it is searched for: when every entry
-    // before it is a full extent page of 64 tokens it is entry begin / 64.
-    auto add = [&](uint32_t first) {
-        for (uint32_t j = tid; j <= ngroups && first + j < table.descriptor_count; j += kBlock) {
-            kimkv_block_desc const e = table.descriptors[first + j];
-            if (j == 0 && e.logical_token_begin <= u.begin && u.begin - e.logical_token_begin < e.valid_tokens) flags.found = 1;
-            add_head_groups<kDim>(P, e, table.layer, u.head, u.begin, u.end, table.token_count, groups, &flags.generic);
-        }
-        __syncthreads();
-    };
-    add(min(u.begin / 64u, table.descriptor_count - 1));
-    if (flags.found == 0) {
-        for (uint32_t g = tid; g < ngroups; g += kBlock) groups[g].k = nullptr;
-        if (tid < kWave) {
-            uint32_t const first = find_descriptor_wave(table.descriptors, table.descriptor_count, u.begin);
-            if (tid == 0) flags.first = first;
-        }
-        __syncthreads();
-        add(flags.first);
-    }
-    for (uint32_t g = tid; g < ngroups; g += kBlock) {
-        if (groups[g].k == nullptr) flags.generic = 1;
+    if (tid == 0) flags.generic = 0;
+    if (tid < kWave) {
+        uint32_t const first = find_descriptor_wave(table.descriptors, table.descriptor_count, begin);
+        if (tid == 0) flags.first = first;
     }
     __syncthreads();
-    return flags.generic == 0;
+    // At most ngroups + 1 entries reach into the unit.
+    uint32_t const first = flags.first;
+    for (uint32_t j = tid; j <= ngroups && j < table.descriptor_count - first; j += kBlock) {
+        add_head_groups<kDim>(P, table.descriptors[first + j], table.layer, head, begin, end, table.token_count, groups,
+                              &flags.generic);
+    }
+    __syncthreads();
+    bool const hole = tid < ngroups && groups[tid].k == nullptr;
+    return __syncthreads_or(hole || flags.generic != 0) == 0;
 }
 
 // ---- direct units ---------------------------------------------------------------
@@ -547,18 +680,30 @@ __device__ bool build_groups(const PoolView& P, const kimkv_decode_item& table, 
 // work of lanes' own tokens and of groups too small to share a tile.  Bound by
 // the bytes and, for short units, by the chain of reads in front of them.
 
-template <uint32_t kDim>
+template <uint32_t kDim, uint32_t kCB>
 struct DirectRows {
     static constexpr uint32_t kRow = kDim + 4;   // o, m, l, pad
-    float row[kWaves][16][kRow];
-    uint32_t ok[16];
+    float row[kWaves][16 * kCB][kRow];
 };
 
+// Dims [d, d + 4) of the part o, m, l of query head out's + q.
 template <uint32_t kDim>
-__device__ bool unit_direct(const PoolView& P, const SharedArgs& a, const SharedUnit& u, const kimkv_decode_item& table,
-                            const HeadGroup* groups, DirectRows<kDim>& rows)
+__device__ inline void store_part(const SharedArgs& a, const ColumnOut& out, uint32_t q, uint32_t d, float4_t o, float m, float l)
 {
-    constexpr uint32_t kKB = kDim <= 64 ? 2 : 1;   // 32-key blocks a step
+    if (out.output == nullptr) {
+        *reinterpret_cast<float4_t*>(a.parts.o + (out.row + q) * kDim + d) = o;
+        if (d == 0) a.parts.ml[out.row + q] = make_float2(m, l);
+        return;
+    }
+    uint16_t* const to = out.output + q * kDim + d;
+    store_outputs<4>(to, o, l);
+}
+
+template <uint32_t kDim, uint32_t kCB>
+__device__ bool unit_direct(const PoolView& P, const SharedArgs& a, const SharedUnit& u, const kimkv_decode_item& table,
+                            HeadGroup* groups, TableFlags& flags, ColumnOut* outs, DirectRows<kDim, kCB>& rows)
+{
+    constexpr uint32_t kKB = kDim <= 64 && kCB == 1 ? 2 : 1;   // 32-key blocks a step
     constexpr uint32_t kStep = 32 * kKB;
     constexpr uint32_t kPanels = kDim / 32;
     constexpr uint32_t kDb = kDim / 16;
@@ -569,233 +714,158 @@ __device__ bool unit_direct(const PoolView& P, const SharedArgs& a, const Shared
     uint32_t const r = l & 15u;
     uint32_t const x = (l >> 2) & 3u;
     uint32_t const G = a.QH / P.heads;
-    uint32_t const hs = u.heads <= 1 ? 1 : u.heads <= 2 ? 2 : u.heads <= 4 ? 4 : 8;   // heads' share of the waves
+    uint32_t const hs = kCB > 1 || u.heads <= 1 ? 1 : u.heads <= 2 ? 2 : u.heads <= 4 ? 4 : 8;   // heads' share of the waves
     uint32_t const split = kWaves / hs;
     uint32_t const head = wave % hs;
-    uint32_t const piece = ((u.end - u.begin + split - 1) / split + 31) / 32 * 32;
-    uint32_t const c0 = min(wave / hs * piece, u.end - u.begin);   // relative to begin
-    uint32_t const c1 = min(c0 + piece, u.end - u.begin);
     bool const works = head < u.heads;
-    Columns<kDim, 1> w;
-    bool ordered = columns_init(w, P, a, u, table.layer, G, works ? u.head + head : u.head, 0);
-    if (wave == 0 && l < 16) rows.ok[l] = w.ok[0] ? 1 : 0;
-    struct Ops {
+    // The table's entries and the queries are on their way together.
+    kimkv_block_desc guess = guessed_entry(table, u.begin);
+    Columns<kDim, kCB> w;
+    bool const ordered = columns_init(w, P, a, u, table.layer, works ? u.head + head : u.head, outs);
+    // Two steps' keys in registers, and values of one where two do not fit.
+    constexpr uint32_t kValueSteps = kDim == 128 && kCB > 1 ? 1 : 2;
+    struct Keys {
         half8_t k[kKB][2][kPanels];
+    };
+    struct Values {
         half8_t v[kKB][kDb];
     };
-    auto load = [&](Ops& o, uint32_t t0, auto tail) {
-        constexpr bool kTail = decltype(tail)::value;
+    // Keys past the end are read at the last group's place.
+    uint32_t c0 = 0, c1 = 0;   // the wave's keys of the segment
+    auto load_k = [&](Keys& o, uint32_t t0) {
 #pragma unroll
         for (uint32_t kb = 0; kb < kKB; ++kb) {
-            uint32_t const tk = t0 + 32 * kb + 8 * x;
-            HeadGroup const gk = groups[(kTail ? min(tk, c1 - 1) : tk) / 8];
-            const uint16_t* const k0 = gk.k + head * (2u * kDim / 32u) * gk.kpanel;   // 2 cap D a head
+            HeadGroup const g = groups[min(t0 / 8 + 4 * kb + x, (c1 - 1) / 8)];
+            const uint16_t* const k0 = g.k + head * (2u * kDim / 32u) * g.kpanel + (l & 3u) * 32 + a4 * 8;   // 2 cap D a head
 #pragma unroll
             for (uint32_t e = 0; e < 2; ++e) {
-                const uint16_t* const row = k0 + (4 * e + (l & 3u)) * 32 + a4 * 8;
 #pragma unroll
-                for (uint32_t p = 0; p < kPanels; ++p) {
-                    o.k[kb][e][p] = half8_t{};
-                    if (!kTail || tk + 4 * e + (l & 3u) < c1) o.k[kb][e][p] = load_half8_stream(row + p * gk.kpanel);
+                for (uint32_t p = 0; p < kPanels; ++p) o.k[kb][e][p] = load_keys<kCB == 1>(k0 + 128 * e + p * g.kpanel);
+            }
+        }
+    };
+    auto load_v = [&](Values& o, uint32_t t0) {
+#pragma unroll
+        for (uint32_t kb = 0; kb < kKB; ++kb) {
+            HeadGroup const g = groups[min(t0 / 8 + 4 * kb + a4, (c1 - 1) / 8)];
+            const uint16_t* const v0 = g.v + head * (2u * kDim / 32u) * g.kpanel + r * g.vw;
+#pragma unroll
+            for (uint32_t db = 0; db < kDb; ++db) o.v[kb][db] = load_keys<kCB == 1>(v0 + 16 * db * g.vw);
+        }
+    };
+    auto step = [&](Keys const& k, Values& v, uint32_t t) {
+        uint32_t const nvalid = c1 - t;
+        if (__builtin_expect(nvalid < kStep, 0)) {   // V of keys past the end may hold anything
+            uint32_t first = 8 * a4;
+            __asm__ volatile("" : "+v"(first));      // a branch
+#pragma unroll
+            for (uint32_t kb = 0; kb < kKB; ++kb) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    if (32 * kb + first + j < nvalid) continue;
+#pragma unroll
+                    for (uint32_t db = 0; db < kDb; ++db) v.v[kb][db][j] = static_cast<_Float16>(0.0f);
                 }
             }
-            uint32_t const tv = t0 + 32 * kb + 8 * a4;
-            HeadGroup const gv = groups[(kTail ? min(tv, c1 - 1) : tv) / 8];
-            const uint16_t* const v0 = gv.v + head * (2u * kDim / 32u) * gv.kpanel + r * gv.vw;
+        }
+        attend_step(w, k.k, v.v, nvalid);
+    };
+    for (uint32_t s0 = u.begin; s0 < u.end; s0 += kSegment) {
+        uint32_t const s1 = min(u.end - s0, kSegment) + s0;
+        if (s0 != u.begin) {
+            guess = guessed_entry(table, s0);
+            __syncthreads();   // the last segment's groups have been read
+        }
+        if (!build_groups<kDim>(P, table, u.head, s0, s1, guess, groups, flags)) return false;
+        uint32_t const piece = ((s1 - s0 + split - 1) / split + 31) / 32 * 32;
+        c0 = min(wave / hs * piece, s1 - s0);
+        c1 = min(c0 + piece, s1 - s0);
+        if (works && c0 < c1) {
+            Keys k0, k1;
+            Values v0, v1;
+            load_k(k0, c0);
+            if (kValueSteps == 2) load_v(v0, c0);
+#pragma unroll 1
+            for (uint32_t t = c0;; t += 2 * kStep) {
+                bool const second = t + kStep < c1;
+                if (kValueSteps == 1) load_v(v0, t);
+                if (second) load_k(k1, t + kStep);
+                if (kValueSteps == 2 && second) load_v(v1, t + kStep);
+                step(k0, v0, t);
+                if (!second) break;
+                bool const third = t + 2 * kStep < c1;
+                if (kValueSteps == 1) load_v(v0, t + kStep);
+                if (third) load_k(k0, t + 2 * kStep);
+                if (kValueSteps == 2 && third) load_v(v0, t + 2 * kStep);
+                if (kValueSteps == 1) {
+                    step(k1, v0, t + kStep);
+                } else {
+                    step(k1, v1, t + kStep);
+                }
+                if (!third) break;
+            }
+        }
+    }
+    bool const again = columns_finish(w) || !ordered;
+    if (kCB == 1 && split == 1) {   // a wave's head is its own
+        if (__syncthreads_or(again) != 0) return false;
+        if (works && w.ok[0]) {
+            ColumnOut const out = outs[r];
 #pragma unroll
             for (uint32_t db = 0; db < kDb; ++db) {
-                o.v[kb][db] = half8_t{};
-                if (!kTail || tv < c1) o.v[kb][db] = load_half8_stream(v0 + 16 * db * gv.vw);
-            }
-            if (kTail && tv < c1 && tv + 8 > c1) {   // keys past the end may hold anything
-#pragma unroll
-                for (uint32_t db = 0; db < kDb; ++db) {
-#pragma unroll
-                    for (uint32_t j = 0; j < 8; ++j) {
-                        if (tv + j >= c1) o.v[kb][db][j] = static_cast<_Float16>(0.0f);
-                    }
-                }
+                store_part<kDim>(a, out, (u.head + head) * G, 16 * db + 4 * a4, w.acc[db][0], w.mref[0], w.l[0]);
             }
         }
-    };
-    auto full = [&](Ops const& o) { attend_step<kDim, 1, kKB, false>(w, o.k, o.v, kStep); };
-    std::false_type const whole{};
-    if (works && c0 < c1) {
-        Ops buf_a, buf_b;
-        uint32_t const steps = (c1 - c0) / kStep;
-        uint32_t t = c0;
-        if (steps > 0) {
-            load(buf_a, t, whole);
-            uint32_t i = 1;
-            for (; i + 1 < steps; i += 2) {
-                load(buf_b, t + kStep, whole);
-                full(buf_a);
-                load(buf_a, t + 2 * kStep, whole);
-                full(buf_b);
-                t += 2 * kStep;
-            }
-            if (i < steps) {
-                load(buf_b, t + kStep, whole);
-                full(buf_a);
-                full(buf_b);
-                t += 2 * kStep;
-            } else {
-                full(buf_a);
-                t += kStep;
-            }
-        }
-        if (t < c1) {
-            load(buf_a, t, std::true_type{});
-            attend_step<kDim, 1, kKB, true>(w, buf_a.k, buf_a.v, c1 - t);
-        }
+        return true;
     }
-    bool const again = columns_finish(w) || !ordered;
-    float* const mine = rows.row[wave][r];
-#pragma unroll
-    for (uint32_t db = 0; db < kDb; ++db) *reinterpret_cast<float4_t*>(mine + 16 * db + 4 * a4) = w.acc[db][0];
-    if (l < 16) {
-        mine[kDim] = w.m[0];
-        mine[kDim + 1] = w.l[0];
-    }
-    if (__syncthreads_or(again) != 0) return false;
-    for (uint32_t i = tid; i < u.heads * 16 * (kDim / 4); i += kBlock) {
-        uint32_t const d = i % (kDim / 4) * 4;
-        uint32_t const c = i / (kDim / 4) % 16;
-        uint32_t const hd = i / (kDim / 4) / 16;
-        if (c >= u.cols || rows.ok[c] == 0) continue;
-        float M = -INFINITY;
-        for (uint32_t s = 0; s < split; ++s) M = fmaxf(M, rows.row[s * hs + hd][c][kDim]);
-        float4_t o = {};
-        float den = 0.0f;
-        for (uint32_t s = 0; s < split; ++s) {
-            const float* const part = rows.row[s * hs + hd][c];
-            float const f = part[kDim] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part[kDim] - M);
-            o += f * *reinterpret_cast<const float4_t*>(part + d);
-            den += f * part[kDim + 1];
-        }
-        PartOut const to = part_out(a, u, kDim, G, u.head + hd, c);
-        if (to.output != nullptr) {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) to.output[d + j] = output_half(o[j], den);
-        } else {
-            *reinterpret_cast<float4_t*>(to.o + d) = o;
-            if (d == 0) *to.ml = make_float2(M, den);
-        }
-    }
-    return true;
-}
-
-// ---- staged units ---------------------------------------------------------------
-// Whole 64-key blocks of one KV head and up to 64 kCB columns.  Each half of
-// the workgroup takes every other tile: its 256 threads stage it in LDS, and
-// its four waves compute kCB blocks of 16 columns each from it.  The halves'
-// states are merged in LDS, so that a unit leaves one part.
-
-template <uint32_t kDim>
-struct StagedLds {
-    union {
-        KvTile<kDim> tile[2][2];                // [half][buffer]
-        struct {
-            float4_t acc[4][16][64];            // [column wave][register][lane]
-            float2 ml[4][4][64];
-        } part;
-    };
-};
-
-template <uint32_t kDim, uint32_t kCB>
-__device__ bool unit_staged(const PoolView& P, const SharedArgs& a, const SharedUnit& u, const kimkv_decode_item& table,
-                            const HeadGroup* groups, StagedLds<kDim>& lds)
-{
-    using Dims = TileDims<kDim>;
-    constexpr uint32_t kPanels = kDim / 32;
-    constexpr uint32_t kDb = kDim / 16;
-    constexpr uint32_t kGroups = Dims::kTileKeys / 8;
-    static_assert(kDb * kCB <= 16 && kCB <= 4, "a wave's state fits its part");
-    uint32_t const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t const half = wave >> 2;
-    uint32_t const cw = wave & 3u;
-    uint32_t const tid = threadIdx.x & (kTileThreads - 1);
-    uint32_t const l = tid & 63u;
-    uint32_t const a4 = l >> 4;
-    uint32_t const r = l & 15u;
-    uint32_t const x = (l >> 2) & 3u;
-    uint32_t const G = a.QH / P.heads;
-    uint32_t const tiles = (u.end - u.begin) / Dims::kTileKeys;
-    uint32_t const rounds = (tiles + 1) / 2;
-    TileLoad ld;
-    if (half < tiles) {
-        tile_fetch<kDim, true>(ld, groups, half * kGroups, Dims::kTileKeys, tid);
-        tile_store(lds.tile[half][0], ld, tid);
-    }
-    if (half + 2 < tiles) tile_fetch<kDim, true>(ld, groups, (half + 2) * kGroups, Dims::kTileKeys, tid);
-    Columns<kDim, kCB> w;
-    bool const ordered = columns_init(w, P, a, u, table.layer, G, u.head, cw * 16 * kCB);
-    bool const works = cw * 16 * kCB < u.cols;
-    __syncthreads();
-    for (uint32_t i = 0; i < rounds; ++i) {
-        uint32_t const j = 2 * i + half;
-        KvTile<kDim> const& tile = lds.tile[half][i & 1u];
-        if (works && j < tiles) {
-#pragma unroll
-            for (uint32_t kb = 0; kb < Dims::kKB; ++kb) {
-                half8_t k[1][2][kPanels];
-                half8_t v[1][kDb];
-#pragma unroll
-                for (uint32_t e = 0; e < 2; ++e) {
-#pragma unroll
-                    for (uint32_t p = 0; p < kPanels; ++p) {
-                        k[0][e][p] = tile.k[k_unit<kDim>(32 * kb + 8 * x + 4 * e + (l & 3u), 4 * p + a4)];
-                    }
-                }
-#pragma unroll
-                for (uint32_t db = 0; db < kDb; ++db) v[0][db] = tile.v[v_unit<kDim>(16 * db + r, 4 * kb + a4)];
-                attend_step<kDim, kCB, 1, false>(w, k, v, 32);
-            }
-        }
-        if (j + 2 < tiles) tile_store(lds.tile[half][(i + 1) & 1u], ld, tid);
-        if (j + 4 < tiles) tile_fetch<kDim, true>(ld, groups, (j + 4) * kGroups, Dims::kTileKeys, tid);
-        __syncthreads();
-    }
-    bool const again = columns_finish(w) || !ordered;
-    if (half == 1) {
-#pragma unroll
-        for (uint32_t cb = 0; cb < kCB; ++cb) {
-#pragma unroll
-            for (uint32_t db = 0; db < kDb; ++db) lds.part.acc[cw][db * kCB + cb][l] = w.acc[db][cb];
-            lds.part.ml[cw][cb][l] = make_float2(w.m[cb], w.l[cb]);
-        }
-    }
-    if (__syncthreads_or(again) != 0) return false;
-    if (half == 1 || !works) return true;
 #pragma unroll
     for (uint32_t cb = 0; cb < kCB; ++cb) {
-        uint32_t const c = (cw * kCB + cb) * 16 + r;
-        if (!w.ok[cb]) continue;
-        float2 const other = lds.part.ml[cw][cb][l];
-        float const M = fmaxf(w.m[cb], other.x);
-        float const f0 = w.m[cb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.m[cb] - M);
-        float const f1 = other.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(other.x - M);
-        float const den = f0 * w.l[cb] + f1 * other.y;
-        PartOut const to = part_out(a, u, kDim, G, u.head, c);
+        float* const mine = rows.row[wave][16 * cb + r];
 #pragma unroll
-        for (uint32_t db = 0; db < kDb; ++db) {
-            float4_t const o = f0 * w.acc[db][cb] + f1 * lds.part.acc[cw][db * kCB + cb][l];
-            uint32_t const d = 16 * db + 4 * a4;
-            if (to.output != nullptr) {
+        for (uint32_t db = 0; db < kDb; ++db) *reinterpret_cast<float4_t*>(mine + 16 * db + 4 * a4) = w.acc[db][cb];
+        if (l < 16) {
+            mine[kDim] = w.mref[cb];
+            mine[kDim + 1] = w.l[cb];
+        }
+    }
+    if (__syncthreads_or(again) != 0) return false;
+    // Four dims of a column of a head at a time.
+    constexpr uint32_t kQuads = kDim / 4;
+    for (uint32_t i = tid; i < u.heads * u.cols * kQuads; i += kBlock) {
+        uint32_t const d = i % kQuads * 4;
+        uint32_t const c = i / kQuads % u.cols;
+        uint32_t const hd = i / kQuads / u.cols;
+        ColumnOut const out = outs[c];
+        if (out.ok == 0) continue;
+        // All eight waves' rows are read at once; those of another head count for nothing.
+        float m[kWaves];
+        float M = -INFINITY;
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) to.output[d + j] = output_half(o[j], den);
-            } else {
-                *reinterpret_cast<float4_t*>(to.o + d) = o;
+        for (uint32_t v = 0; v < kWaves; ++v) {
+            m[v] = v % hs == hd ? rows.row[v][c][kDim] : -INFINITY;
+            M = fmaxf(M, m[v]);
+        }
+        float4_t o = {};
+        float den = 0.0f;
+#pragma unroll
+        for (uint32_t v = 0; v < kWaves; ++v) {
+            const float* const part = rows.row[v][c];
+            float const f = m[v] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[v] - M);
+            if (f != 0.0f) {
+                o += f * *reinterpret_cast<const float4_t*>(part + d);
+                den += f * part[kDim + 1];
             }
         }
-        if (to.output == nullptr && a4 == 0) *to.ml = make_float2(M, den);
+        uint32_t const q = (u.head + hd) * G;   // past the column's query head of KV head 0
+        store_part<kDim>(a, out, q, d, o, M, den);
     }
     return true;
 }
 
-// Dims with a matrix-core path, and with tiles.
+// Head dims with a matrix-core path, and the most 16-column blocks a wave's
+// registers hold at one.
 constexpr bool direct_dim(uint32_t D) { return D == 64 || D == 96 || D == 128; }
-constexpr bool staged_dim(uint32_t D) { return D == 64 || D == 128; }
+constexpr uint32_t most_blocks(uint32_t D) { return D == 64 ? 4 : direct_dim(D) ? 2 : 1; }
 
 struct NoLds {};
 
@@ -807,20 +877,20 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     // One workgroup a compute unit (its registers see to that), so the paths' memory may be large.
     union Paths {
         GenericLds generic;
-        std::conditional_t<direct_dim(kDim), DirectRows<kDim == 0 ? 64 : kDim>, NoLds> direct;
-        std::conditional_t<staged_dim(kDim), StagedLds<staged_dim(kDim) ? kDim : 64>, NoLds> staged;
+        std::conditional_t<kDim != 0, DirectRows<kDim == 0 ? 64 : kDim, most_blocks(kDim)>, NoLds> direct;
     };
     __shared__ __attribute__((aligned(16))) unsigned char path_lds[sizeof(Paths)];
+    __shared__ ColumnOut outs[64];
     __shared__ HeadGroup groups[kDim != 0 ? kTableGroups : 1];
     __shared__ TableFlags flags;
     Paths& lds = *reinterpret_cast<Paths*>(path_lds);
     SharedUnit const u = a.units[xcd_logical_index(blockIdx.x, gridDim.x)];
     if (u.cols == 0) return;
-    uint32_t const G = a.QH / P.heads;
     // The entries lie in the caller's memory: nothing outside the launch's buffers is touched, whatever they hold.
-    uint64_t const last = (static_cast<uint64_t>(u.col0) + u.cols - 1) / G;   // lane of the last column, from u.lane
-    if (u.table_lane >= a.lane_count || u.lane + last >= a.lane_count || u.heads == 0 || u.head + u.heads > P.heads
-        || u.begin >= u.end || ((u.kind & kSingle) == 0 && u.slot + last >= a.slot_count)) {
+    uint32_t rest;
+    uint64_t const last = div_mod(u.col0 + (u.cols - 1), a.group, &rest);   // lane of the last column, from u.lane
+    if (u.cols - 1 > 0xFFFFFFFFu - u.col0 || u.table_lane >= a.lane_count || u.lane + last >= a.lane_count || u.heads == 0
+        || u.head + u.heads > P.heads || u.begin >= u.end || ((u.kind & kSingle) == 0 && u.slot + last >= a.slot_count)) {
         report_fault(P, KIMKV_FAULT_DECODE_ITEM);
         return;
     }
@@ -830,23 +900,19 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         report_fault(P, KIMKV_FAULT_DECODE_ITEM);
         return;
     }
-    bool bad = false;
-    for (uint32_t c = threadIdx.x; c < u.cols; c += kBlock) bad |= !unit_column(P, a, u, table.layer, G, u.head, c).ok;
-    if (bad && P.faults != nullptr) atomicOr(P.faults, KIMKV_FAULT_DECODE_ITEM);
     if constexpr (kDim != 0) {
         bool done = false;
         uint32_t const kind = u.kind & ~kSingle;
-        if (build_groups<kDim>(P, table, u, groups, flags)) {
-            if (kind == kDirect) {
-                if (u.cols <= 16 && u.heads <= kWaves) done = unit_direct<kDim>(P, a, u, table, groups, lds.direct);
-            } else if constexpr (staged_dim(kDim)) {
-                bool const whole = u.heads == 1 && (u.begin & 63u) == 0 && (u.end & 63u) == 0 && u.cols <= 64 * kind;
-                if (whole && kind == 1) done = unit_staged<kDim, 1>(P, a, u, table, groups, lds.staged);
-                if (whole && kind == 2) done = unit_staged<kDim, 2>(P, a, u, table, groups, lds.staged);
-                if constexpr (kDim == 64) {
-                    if (whole && kind == 4) done = unit_staged<kDim, 4>(P, a, u, table, groups, lds.staged);
-                }
-            }
+        auto direct = [&](auto blocks) {
+            constexpr uint32_t kCB = decltype(blocks)::value;
+            if (u.cols > 16 * kCB || (u.begin & 7u) != 0 || (kCB == 1 ? u.heads > kWaves : u.heads != 1)) return;
+            done = unit_direct<kDim, kCB>(P, a, u, table, groups, flags, outs,
+                                          *reinterpret_cast<DirectRows<kDim, kCB>*>(path_lds));
+        };
+        if (kind == 1) direct(std::integral_constant<uint32_t, 1>{});
+        else if (kind == 2) direct(std::integral_constant<uint32_t, 2>{});
+        if constexpr (most_blocks(kDim) == 4) {
+            if (kind == 4) direct(std::integral_constant<uint32_t, 4>{});
         }
         if (done) return;
         __syncthreads();   // the generic path's rows take the same memory
@@ -866,7 +932,7 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
     typedef float vec_t __attribute__((ext_vector_type(kWidth)));
     uint32_t const lane = blockIdx.x;
     SharedLane const rec = a.lanes[lane];
-    if (rec.merged == 0 || !lane_ok(P, a, lane)) return;   // a unit reported it
+    if (rec.merged == 0) return;
     uint64_t const last_prefix = rec.prefix_slot + static_cast<uint64_t>(rec.prefix_stride) * (rec.prefix_count - 1ull);
     if (rec.prefix_count > a.slot_count || rec.tail_count > a.slot_count
         || (rec.prefix_count != 0 && last_prefix >= a.slot_count)
@@ -875,6 +941,7 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
     }
     uint32_t const D = P.dim;
     uint32_t const parts = rec.prefix_count + rec.tail_count;
+    bool const ok = lane_ok(P, a, lane);   // a unit reported it; not waited for before the parts are read
     uint16_t* const output = a.items[lane].output;
     uint32_t const per_row = D / kWidth;
     for (uint32_t x = blockIdx.y * kMergeBlock + threadIdx.x; x < a.QH * per_row; x += gridDim.y * kMergeBlock) {
@@ -911,23 +978,36 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
                 l += f * ml[j].y;
             }
         }
-        uint16_t* const to = output + static_cast<uint64_t>(q) * D + d;
-#pragma unroll
-        for (uint32_t j = 0; j < kWidth; ++j) to[j] = output_half(o[j], l);
+        if (!ok) return;
+        store_outputs<kWidth>(output + static_cast<uint64_t>(q) * D + d, o, l);
     }
 }
 
 // ---- planning -----------------------------------------------------------------
 
 constexpr uint32_t kShareBlock = 64;     // tokens: a shared prefix is cut to whole blocks
-constexpr uint32_t kMaxUnit = kTableGroups * 8;
 
-// What a unit costs its compute unit, in nanoseconds.
+// What a unit costs its compute unit, in nanoseconds, as measured: the chain of
+// reads in front of a unit and the merge and stores behind it; the bytes that
+// a compute unit streams (45 a nanosecond when not all of them do); the steps
+// of a wave when the loads' latency is all there is; the arithmetic of many
+// columns.  And what the bytes of all units take, whoever reads them.
 struct UnitCost {
     uint32_t D;
-    static constexpr double kStart = 3000;   // the chain of reads in front, the merge and the stores behind
-    double direct(uint32_t heads, uint32_t tokens) const { return kStart + 10.0 * D / 64 * heads * tokens; }
-    double staged(uint32_t blocks, uint32_t tokens) const { return kStart + 700.0 * blocks + 4.5 * D / 64 * blocks * tokens; }
+    static constexpr double kStart = 5500;
+    static constexpr double kMergeLaunch = 5000;
+    static constexpr double kBytes = 5500;   // HBM's, a nanosecond
+    // `split` waves share a head's tokens.
+    double own(uint32_t heads, uint32_t split, uint32_t tokens) const
+    {
+        double const steps = std::ceil(std::ceil(tokens / static_cast<double>(split)) * D / 64 / 64);
+        return kStart + std::max(5.5 * D / 64 * heads * tokens, 700.0 * steps);
+    }
+    double prefix(uint32_t blocks, uint32_t tokens) const
+    {
+        return kStart + 600.0 * blocks + std::max(4.5, 1.8 * blocks) * D / 64 * tokens;
+    }
+    double bytes(uint32_t heads, uint32_t tokens) const { return 4.0 * D * heads * tokens; }
 };
 
 struct Planned {
@@ -942,10 +1022,11 @@ uint64_t align16(uint64_t n) { return (n + 15) / 16 * 16; }
 
 // Spreads the units over the XCDs (workgroup w runs on XCD w % 8): units of
 // one range of keys and head together, whose K and V then stay in one L2, the
-// costliest first onto the XCD with least to do, and each XCD's costliest
-// first.  Short lists end in idle entries.
-void place_units(Planned& p)
+// costliest first onto the XCD with least to do that still has a compute unit
+// for each, and each XCD's costliest first.  Short lists end in idle entries.
+void place_units(Planned& p, uint32_t compute_units)
 {
+    size_t const per_xcd = std::max(1u, compute_units / kXcds);
     size_t const n = p.units.size();
     struct Bundle {
         size_t first, count;
@@ -968,9 +1049,10 @@ void place_units(Planned& p)
     std::vector<size_t> xcd[kXcds];
     double load[kXcds] = {};
     for (Bundle const& b : bundles) {
+        auto const key = [&](uint32_t x) { return std::make_pair(xcd[x].size() + b.count > per_xcd, load[x]); };
         uint32_t best = 0;
         for (uint32_t x = 1; x < kXcds; ++x) {
-            if (load[x] < load[best] || (load[x] == load[best] && xcd[x].size() < xcd[best].size())) best = x;
+            if (key(x) < key(best)) best = x;
         }
         load[best] += b.cost;
         for (size_t i = 0; i < b.count; ++i) xcd[best].push_back(b.first + i);
@@ -987,29 +1069,134 @@ void place_units(Planned& p)
     p.units = std::move(placed);
 }
 
-// Tokens of each of the pieces of [0, tokens), in blocks of 64.
-uint32_t piece_tokens(uint64_t tokens, double pieces)
+// Tokens of each of the pieces of [0, tokens), in blocks of 64, when they are
+// to be about n.
+uint32_t piece_tokens(uint64_t tokens, double n)
 {
-    uint64_t const n = std::max<uint64_t>(1, std::max<uint64_t>(static_cast<uint64_t>(pieces + 0.5), (tokens + kMaxUnit - 1) / kMaxUnit));
-    return static_cast<uint32_t>(std::max<uint64_t>(64, ((tokens + n - 1) / n + 63) / 64 * 64));
+    auto const each = static_cast<uint64_t>(std::ceil(static_cast<double>(tokens) / std::max(1.0, std::floor(n + 0.5))));
+    return static_cast<uint32_t>(std::max<uint64_t>(64, (each + 63) / 64 * 64));
+}
+
+// The lanes' work before it is cut into pieces.
+struct Work {
+    struct Prefix {
+        uint32_t lane, lanes, tokens, blocks;   // blocks: of 16 columns a wave
+        uint64_t tiles;                         // units that take all its columns
+    };
+    std::vector<Prefix> prefixes;
+    std::vector<uint32_t> shared;   // tokens of each lane that a prefix takes
+};
+
+struct Shape {
+    uint32_t H, G, D, compute_units;
+    const uint32_t* tokens;
+    uint32_t lane_count;
+};
+
+// How a batch is cut: KV heads of a unit of a lane's own tokens, the cost that
+// no unit's pieces go far past, and what that comes to.
+struct Cut {
+    uint32_t heads{1};
+    double share{0};
+    double time{0};
+};
+
+template <typename PrefixFn, typename OwnFn>
+void each_piece(Shape const& s, Work const& work, Cut const& cut, PrefixFn&& prefix_piece, OwnFn&& own_piece)
+{
+    UnitCost const cost{s.D};
+    for (Work::Prefix const& p : work.prefixes) {
+        double const whole = cost.prefix(p.blocks, p.tokens) - UnitCost::kStart;
+        prefix_piece(p, piece_tokens(p.tokens, whole / std::max(1.0, cut.share - UnitCost::kStart)));
+    }
+    uint32_t const split = kWaves / cut.heads;
+    for (uint32_t i = 0; i < s.lane_count; ++i) {
+        uint32_t const own = s.tokens[i] - work.shared[i];
+        if (own == 0) continue;
+        double const whole = cost.own(std::min(cut.heads, s.H), split, own) - UnitCost::kStart;
+        own_piece(i, own, piece_tokens(own, whole / std::max(1.0, cut.share - UnitCost::kStart)));
+    }
+}
+
+// The time of a cut: of its longest unit, or of all of them where there are
+// more than compute units, whose gaps the smallest fill; and of the merge
+// where a lane has several parts.
+double cut_time(Shape const& s, Work const& work, Cut const& cut)
+{
+    UnitCost const cost{s.D};
+    double total = 0;
+    double longest = 0;
+    double shortest = 1e30;
+    double bytes = 0;
+    uint64_t units = 0;
+    bool merged = !work.prefixes.empty();
+    auto add = [&](double each, uint64_t n) {
+        units += n;
+        total += each * static_cast<double>(n);
+        longest = std::max(longest, each);
+        shortest = std::min(shortest, each);
+    };
+    each_piece(
+        s, work, cut,
+        [&](Work::Prefix const& p, uint32_t piece) {
+            add(cost.prefix(p.blocks, std::min(piece, p.tokens)), (p.tokens + piece - 1ull) / piece * s.H * p.tiles);
+            bytes += cost.bytes(s.H, p.tokens);
+        },
+        [&](uint32_t, uint32_t own, uint32_t piece) {
+            uint64_t const pieces = (own + piece - 1ull) / piece;
+            add(cost.own(std::min(cut.heads, s.H), kWaves / cut.heads, std::min(piece, own)),
+                pieces * ((s.H + cut.heads - 1) / cut.heads) * ((s.G + 15) / 16));
+            merged = merged || pieces > 1;
+            bytes += cost.bytes(s.H, own);
+        });
+    double const units_time = units <= s.compute_units ? longest : std::max(longest, total / s.compute_units) + shortest;
+    double const time = std::max(units_time, UnitCost::kStart + bytes / UnitCost::kBytes);
+    return time + (merged ? UnitCost::kMergeLaunch : 0.0);
+}
+
+// The best of a few cuts: pieces of a few sizes around an equal share for each
+// compute unit, and whole ones.
+Cut best_cut(Shape const& s, Work const& work)
+{
+    UnitCost const cost{s.D};
+    // KV heads of a unit of a lane's own tokens: all that eight waves take,
+    // fewer, with more waves for each, while the units are few.
+    uint32_t heads = 1;
+    while (heads < kWaves && heads < s.H) heads *= 2;
+    uint64_t own_units = 0;
+    double total = 0;
+    for (uint32_t i = 0; i < s.lane_count; ++i) {
+        uint32_t const own = s.tokens[i] - work.shared[i];
+        if (own == 0) continue;
+        own_units += static_cast<uint64_t>((s.H + heads - 1) / heads) * ((s.G + 15) / 16);
+        total += cost.own(s.H, kWaves, own) * ((s.G + 15) / 16);
+    }
+    while (heads > 1 && own_units * 4 <= s.compute_units) {
+        heads /= 2;
+        own_units *= 2;
+    }
+    for (Work::Prefix const& p : work.prefixes) {
+        total += cost.prefix(p.blocks, p.tokens) * static_cast<double>(p.tiles) * s.H;
+    }
+    double const even = total / s.compute_units + UnitCost::kStart;
+    Cut best;
+    for (double const share : {1e12, 0.7 * even, 0.85 * even, even, 1.15 * even, 1.35 * even, 1.7 * even, 2.2 * even}) {
+        Cut c{heads, std::max(share, UnitCost::kStart + 1500), 0};
+        c.time = cut_time(s, work, c);
+        if (best.share == 0 || c.time < best.time) best = c;
+    }
+    return best;
 }
 
 bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, const uint32_t* tokens, uint32_t lane_count,
                 const kimkv_shared_group* groups, uint32_t group_count, Planned& out)
 {
-    uint32_t const G = QH / H;
-    UnitCost const unit_cost{D};
-    uint32_t const max_blocks = D == 64 ? 4 : staged_dim(D) ? 2 : 0;
-    out.lanes.resize(lane_count);
-    for (uint32_t i = 0; i < lane_count; ++i) out.lanes[i] = SharedLane{i, tokens[i], 0, 0, 0, 0, 0, 0};
+    Shape const shape{H, QH / H, D, compute_units, tokens, lane_count};
+    UnitCost const cost{D};
     std::vector<uint8_t> grouped(lane_count, 0);
-    std::vector<uint32_t> shared(lane_count, 0);   // tokens of the lane that a group's units take
-    struct Shared {
-        uint32_t lane, lanes, prefix, blocks;   // blocks: of 16 columns a wave, 0 for direct units
-        uint64_t tiles;                         // column tiles
-    };
-    std::vector<Shared> prefixes;
-    double total = 0;
+    Work apart;
+    apart.shared.assign(lane_count, 0);
+    Work work = apart;
     for (uint32_t g = 0; g < group_count; ++g) {
         kimkv_shared_group const& group = groups[g];
         if (group.first_lane > lane_count || group.lane_count > lane_count - group.first_lane) return false;
@@ -1021,97 +1208,89 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
         }
         prefix = prefix / kShareBlock * kShareBlock;
         if (group.lane_count < 2 || prefix == 0) continue;
-        uint64_t const columns = static_cast<uint64_t>(group.lane_count) * G;
+        uint64_t const columns = static_cast<uint64_t>(group.lane_count) * shape.G;
         if (columns > 0x7FFFFFFFu) return false;
-        Shared s{group.first_lane, group.lane_count, prefix, 0, (columns + 15) / 16};
-        if (columns > 32 && max_blocks != 0) {
-            s.blocks = columns <= 64 ? 1 : columns <= 128 || max_blocks == 2 ? 2 : 4;
-            s.tiles = (columns + 64 * s.blocks - 1) / (64 * s.blocks);
+        Work::Prefix p{group.first_lane, group.lane_count, prefix, 1, 0};
+        while (p.blocks < most_blocks(D) && 16 * p.blocks < columns) p.blocks *= 2;
+        p.tiles = (columns + 16 * p.blocks - 1) / (16 * p.blocks);
+        work.prefixes.push_back(p);
+        for (uint32_t i = 0; i < group.lane_count; ++i) work.shared[group.first_lane + i] = prefix;
+    }
+    // Short prefixes of few lanes are read faster lane by lane, without a merge.
+    Cut cut = best_cut(shape, work);
+    if (!work.prefixes.empty()) {
+        Cut const other = best_cut(shape, apart);
+        if (other.time <= cut.time) {
+            cut = other;
+            work = apart;
         }
-        prefixes.push_back(s);
-        for (uint32_t i = 0; i < group.lane_count; ++i) shared[group.first_lane + i] = prefix;
-        double const whole = s.blocks != 0 ? unit_cost.staged(s.blocks, prefix) : unit_cost.direct(1, prefix);
-        total += whole * static_cast<double>(s.tiles) * H;
     }
-    uint32_t heads = 1;   // KV heads of a unit of a lane's own tokens
-    while (heads < 8 && heads < H) heads *= 2;
-    uint64_t own_units = 0;
-    for (uint32_t i = 0; i < lane_count; ++i) {
-        if (tokens[i] == shared[i]) continue;
-        own_units += static_cast<uint64_t>((H + heads - 1) / heads) * ((G + 15) / 16);
-        total += unit_cost.direct(H, tokens[i] - shared[i]) * ((G + 15) / 16);
-    }
-    // Fewer heads a unit, and more waves for each, while the units are few.
-    while (heads > 1 && own_units * 4 <= compute_units) {
-        heads /= 2;
-        own_units *= 2;
-    }
-    // Each compute unit is to take about the same: pieces of that cost, but
-    // none so short that starting it costs more than its work.
-    double const share = std::max(total / compute_units, 3 * UnitCost::kStart);
-    auto push = [&](SharedUnit u, double cost) {
+    out.lanes.resize(lane_count);
+    for (uint32_t i = 0; i < lane_count; ++i) out.lanes[i] = SharedLane{i, tokens[i], 0, 0, 0, 0, 0, 0};
+    bool fits = true;
+    auto push = [&](SharedUnit const& u, double c) {
         out.units.push_back(u);
-        out.cost.push_back(cost);
+        out.cost.push_back(c);
     };
-    for (Shared const& s : prefixes) {
-        double const whole = s.blocks != 0 ? unit_cost.staged(s.blocks, s.prefix) : unit_cost.direct(1, s.prefix);
-        uint32_t const piece = piece_tokens(s.prefix, whole / share);
-        uint32_t const pieces = (s.prefix + piece - 1) / piece;
-        uint32_t const width = s.blocks != 0 ? 64 * s.blocks : 16;
-        uint32_t const columns = s.lanes * G;
-        if (out.slots + static_cast<uint64_t>(s.lanes) * pieces > 0x7FFFFFFFu) return false;
-        for (uint32_t i = 0; i < s.lanes; ++i) {
-            SharedLane& lane = out.lanes[s.lane + i];
-            lane.table_lane = s.lane;
-            lane.prefix_slot = static_cast<uint32_t>(out.slots + i);
-            lane.prefix_stride = s.lanes;
-            lane.prefix_count = pieces;
-        }
-        for (uint64_t at = 0; at < s.prefix; at += piece) {
-            auto const b = static_cast<uint32_t>(at);
-            auto const end = static_cast<uint32_t>(std::min<uint64_t>(s.prefix, at + piece));
-            for (uint32_t h = 0; h < H; ++h) {
-                for (uint32_t c = 0; c < columns; c += width) {
-                    push(SharedUnit{s.lane, s.lane, c, std::min(width, columns - c), b, end, static_cast<uint32_t>(out.slots),
-                                    static_cast<uint16_t>(h), 1, static_cast<uint8_t>(s.blocks)},
-                         s.blocks != 0 ? unit_cost.staged(s.blocks, end - b) : unit_cost.direct(1, end - b));
-                }
+    auto take_slots = [&](uint64_t n) {
+        fits = fits && out.slots + n <= 0x7FFFFFFFu;
+        return fits;
+    };
+    each_piece(
+        shape, work, cut,
+        [&](Work::Prefix const& p, uint32_t piece) {
+            uint32_t const pieces = (p.tokens + piece - 1) / piece;
+            if (!take_slots(static_cast<uint64_t>(p.lanes) * pieces)) return;
+            for (uint32_t i = 0; i < p.lanes; ++i) {
+                SharedLane& lane = out.lanes[p.lane + i];
+                lane.table_lane = p.lane;
+                lane.prefix_slot = static_cast<uint32_t>(out.slots + i);
+                lane.prefix_stride = p.lanes;
+                lane.prefix_count = pieces;
             }
-            out.slots += s.lanes;
-        }
-    }
-    for (uint32_t i = 0; i < lane_count; ++i) {
-        SharedLane& lane = out.lanes[i];
-        uint32_t const own = tokens[i] - shared[i];
-        if (own == 0) {
-            lane.merged = lane.prefix_count != 0 ? 1 : 0;
-            out.merge_lanes += lane.merged;
-            continue;
-        }
-        uint32_t const piece = piece_tokens(own, unit_cost.direct(heads, own) / share);
-        uint32_t const pieces = (own + piece - 1) / piece;
-        bool const single = pieces == 1 && lane.prefix_count == 0;
-        if (out.slots + pieces > 0x7FFFFFFFu) return false;
-        lane.tail_slot = static_cast<uint32_t>(out.slots);
-        lane.tail_count = single ? 0 : pieces;
-        lane.merged = single ? 0 : 1;
+            uint32_t const columns = p.lanes * shape.G;
+            for (uint64_t at = 0; at < p.tokens; at += piece) {
+                auto const end = static_cast<uint32_t>(std::min<uint64_t>(p.tokens, at + piece));
+                double const c = cost.prefix(p.blocks, end - static_cast<uint32_t>(at));
+                for (uint32_t h = 0; h < H; ++h) {
+                    for (uint32_t col = 0; col < columns; col += 16 * p.blocks) {
+                        push(SharedUnit{p.lane, p.lane, col, std::min(16 * p.blocks, columns - col), static_cast<uint32_t>(at), end,
+                                        static_cast<uint32_t>(out.slots), static_cast<uint16_t>(h), 1, static_cast<uint8_t>(p.blocks)},
+                             c);
+                    }
+                }
+                out.slots += p.lanes;
+            }
+        },
+        [&](uint32_t i, uint32_t own, uint32_t piece) {
+            SharedLane& lane = out.lanes[i];
+            uint32_t const pieces = static_cast<uint32_t>((own + piece - 1ull) / piece);
+            bool const single = pieces == 1 && lane.prefix_count == 0;
+            if (!take_slots(single ? 0 : pieces)) return;
+            lane.tail_slot = static_cast<uint32_t>(out.slots);
+            lane.tail_count = single ? 0 : pieces;
+            for (uint64_t at = work.shared[i]; at < tokens[i]; at += piece) {
+                auto const end = static_cast<uint32_t>(std::min<uint64_t>(tokens[i], at + piece));
+                for (uint32_t h = 0; h < H; h += cut.heads) {
+                    uint32_t const n = std::min(cut.heads, H - h);
+                    double const c = cost.own(n, kWaves / cut.heads, end - static_cast<uint32_t>(at));
+                    for (uint32_t col = 0; col < shape.G; col += 16) {
+                        push(SharedUnit{i, i, col, std::min(16u, shape.G - col), static_cast<uint32_t>(at), end,
+                                        static_cast<uint32_t>(out.slots), static_cast<uint16_t>(h), static_cast<uint8_t>(n),
+                                        static_cast<uint8_t>(1 | (single ? kSingle : 0))},
+                             c);
+                    }
+                }
+                if (!single) out.slots += 1;
+            }
+        });
+    if (!fits || out.units.size() > 0x7FFFFFF0u) return false;
+    for (SharedLane& lane : out.lanes) {
+        lane.merged = lane.prefix_count + lane.tail_count != 0 ? 1 : 0;
         out.merge_lanes += lane.merged;
-        for (uint64_t b = shared[i]; b < tokens[i]; b += piece) {
-            auto const end = static_cast<uint32_t>(std::min<uint64_t>(tokens[i], b + piece));
-            for (uint32_t h = 0; h < H; h += heads) {
-                uint32_t const n = std::min(heads, H - h);
-                for (uint32_t c = 0; c < G; c += 16) {
-                    push(SharedUnit{i, i, c, std::min(16u, G - c), static_cast<uint32_t>(b), end, static_cast<uint32_t>(out.slots),
-                                    static_cast<uint16_t>(h), static_cast<uint8_t>(n),
-                                    static_cast<uint8_t>(kDirect | (single ? kSingle : 0))},
-                         unit_cost.direct(n, end - static_cast<uint32_t>(b)));
-                }
-            }
-            if (!single) out.slots += 1;
-        }
     }
-    place_units(out);
-    return out.slots <= 0x7FFFFFFFu && out.units.size() <= 0x7FFFFFFFu;
+    place_units(out, compute_units);
+    return true;
 }
 
 }  // namespace
@@ -1190,6 +1369,7 @@ kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv
     a.lane_count = plan->lane_count;
     a.slot_count = plan->slot_count;
     a.QH = plan->query_heads;
+    a.group = divisor(plan->query_heads / H);
     PoolView const pv = pool_view(*storage);
     void* start = nullptr;
     kernel_timing_begin(TimedKernel::Decode, s, &start);

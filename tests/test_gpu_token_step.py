@@ -250,9 +250,10 @@ class _Batch:
         rng = np.random.default_rng(seed)
         total = sum(counts) + sum(p for _, _, p in groups)
         unit = min(micro_tokens, extent_tokens)
-        self.storage = dev.Storage(layers, heads, dim, total // micro_tokens + 4 * len(counts) + 16, total // unit + len(counts) + 8, micro_tokens,
-                                   extent_tokens)
-        alloc = helpers.SlotAllocator(total // micro_tokens + 4 * len(counts) + 16, total // unit + len(counts) + 8, seed=seed)
+        short = micro_tokens if pages != "ragged" else max(1, micro_tokens - 2)
+        slots = total // short + 4 * len(counts) + 16, total // unit + len(counts) + 8
+        self.storage = dev.Storage(layers, heads, dim, *slots, micro_tokens, extent_tokens)
+        alloc = helpers.SlotAllocator(*slots, seed=seed)
         self.k, self.v, self.tables, keep = [], [], [], []
         shared = {}
         for first, n, prefix in groups:
@@ -308,8 +309,9 @@ class _Batch:
             change(items)
         self.items = dev.upload(items)
 
-    def plan(self, counts=None):
-        self.entries, self.p = self.storage.shared_decode_plan(counts or self.counts, self.groups, self.heads * self.group)
+    def plan(self, units=4):
+        """A plan for a device of `units` compute units: on a small one every shared prefix pays, however short."""
+        self.entries, self.p = self.dev.shared_decode_plan(self.heads, self.dim, self.heads * self.group, units, self.counts, self.groups)
         self.entries_buf = self.dev.upload(self.entries)
         # Bytes around the workspace are looked at afterwards.
         self.work = self.dev.upload(np.full(self.p.workspace_bytes + 4096, 0x5A, np.uint8))
@@ -373,18 +375,40 @@ BATCHES = {
 }
 
 
+def _kinds(b):
+    """How the plan's units are computed: (blocks of columns and flags, whether they hold several lanes' columns)."""
+    units = b.entries[:b.p.unit_count * UNIT.itemsize].view(UNIT)
+    return {(int(u["kind"]) & 0x7F, bool(u["cols"] > b.group)) for u in units if u["cols"]}
+
+
 @pytest.mark.parametrize("name", list(BATCHES))
 @pytest.mark.parametrize("heads,dim,group", [(4, 64, 8), (8, 128, 4), (2, 64, 16)])
-def test_shared_decode(dev, name, heads, dim, group):
-    print(f"shared {name} H={heads} D={dim} G={group}", flush=True)
+@pytest.mark.parametrize("units", [4, 256])
+def test_shared_decode(dev, name, heads, dim, group, units):
+    print(f"shared {name} H={heads} D={dim} G={group} units={units}", flush=True)
     b = _Batch(dev, heads, dim, group, *BATCHES[name])
     b.place()
-    b.plan()
+    b.plan(units)
     b.launch()
     first = b.outputs()
     b.check(first)
     b.launch()
     assert np.array_equal(first, b.outputs()), "the same plan gives the same bits"
+    assert b.storage.faults() == (0, 0)
+
+
+@pytest.mark.parametrize("heads,dim,lanes,kind", [(2, 64, 2, 1), (2, 64, 4, 2), (2, 64, 8, 4), (1, 64, 25, 4), (1, 64, 70, 4), (2, 96, 2, 1),
+                                                  (2, 96, 9, 2), (2, 128, 2, 1), (2, 128, 5, 2), (1, 128, 17, 2), (1, 128, 40, 2)])
+@pytest.mark.parametrize("prefix", [64, 130, 2000, 9000])
+def test_shared_decode_every_kind(dev, heads, dim, lanes, kind, prefix):
+    """Groups of few and of many columns, which are computed differently, on prefixes of one block of 64 to several pieces."""
+    print(f"shared kind {kind} H={heads} D={dim} lanes={lanes} prefix={prefix}", flush=True)
+    b = _Batch(dev, heads, dim, 8, [prefix + 1 + 3 * i for i in range(lanes)], [(0, lanes, prefix)])
+    b.place()
+    b.plan(1)
+    assert (kind, True) in _kinds(b) or prefix < 2000   # short ones may not pay
+    b.launch()
+    b.check(b.outputs())
     assert b.storage.faults() == (0, 0)
 
 
@@ -400,12 +424,14 @@ def test_shared_decode_other_shapes(dev, heads, dim, group):
     assert b.storage.faults() == (0, 0)
 
 
-@pytest.mark.parametrize("pages,micro,extent", [("ragged", 8, 64), ("micro", 6, 48), ("hetero", 16, 128), ("extents", 8, 96), ("micro", 1, 8)])
+@pytest.mark.parametrize("pages,micro,extent", [("ragged", 8, 64), ("micro", 6, 48), ("micro", 8, 64), ("hetero", 16, 128), ("extents", 8, 96),
+                                                ("micro", 1, 8)])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_shared_decode_other_pages(dev, pages, micro, extent, dim):
+@pytest.mark.parametrize("lanes", [3, 50])
+def test_shared_decode_other_pages(dev, pages, micro, extent, dim, lanes):
     """Tables off the 8-token grid, pages that end inside a tile, pages of other sizes."""
-    print(f"shared pages {pages} {micro} {extent} D={dim}", flush=True)
-    b = _Batch(dev, 2, dim, 4, [600, 640, 613, 77], [(0, 3, 590)], pages=pages, micro_tokens=micro, extent_tokens=extent)
+    print(f"shared pages {pages} {micro} {extent} D={dim} lanes={lanes}", flush=True)
+    b = _Batch(dev, 2, dim, 4, [600 + 7 * i for i in range(lanes)] + [77], [(0, lanes, 590)], pages=pages, micro_tokens=micro, extent_tokens=extent)
     b.place()
     b.plan()
     b.launch()
@@ -522,7 +548,7 @@ def test_shared_decode_without_groups(dev):
     """The same batch with its groups and without them."""
     b = _Batch(dev, 4, 64, 8, *BATCHES["two groups and alone"])
     b.place()
-    b.plan()
+    b.plan(1)
     b.launch()
     with_groups = b.outputs()
     b.check(with_groups)
@@ -535,7 +561,7 @@ def test_shared_decode_without_groups(dev):
 def test_shared_decode_faults(dev):
     """A lane that is not as planned is reported and left alone, with its group where it is the group's first; the others
     come out as they should."""
-    counts, groups = [700, 710, 720, 730, 300, 5], [(0, 2, 690), (2, 2, 690)]
+    counts, groups = [2700, 2710, 2720, 2730, 300, 5], [(0, 2, 2690), (2, 2, 2690)]
 
     def spoil(lane, field, value):
         def change(items):
@@ -548,6 +574,7 @@ def test_shared_decode_faults(dev):
         b = _Batch(dev, 2, 64, 4, counts, groups, layers=2)
         b.place(change=spoil(lane, field, value))
         b.plan()
+        assert (1, True) in _kinds(b)
         b.launch()
         got = b.outputs()
         gone = [lane] if lane else [0, 1]
@@ -564,7 +591,7 @@ def test_shared_decode_bad_entries(dev):
         print(f"shared entry {field}={value}", flush=True)
         b = _Batch(dev, 2, 64, 4, counts, groups)
         b.place()
-        b.plan()
+        b.plan(1)
         entries = b.entries.copy()
         units = entries[:b.p.unit_count * UNIT.itemsize].view(UNIT)
         at = [i for i in range(len(units)) if units[i]["cols"] > 4][0]   # 12 columns: three lanes
@@ -578,7 +605,7 @@ def test_shared_decode_bad_entries(dev):
         print(f"shared record {field}={value}", flush=True)
         b = _Batch(dev, 2, 64, 4, counts, groups)
         b.place()
-        b.plan()
+        b.plan(1)
         entries = b.entries.copy()
         entries[b.p.unit_count * UNIT.itemsize:].view(LANE)[1][field] = value
         b.entries_buf = dev.upload(entries)
@@ -592,7 +619,7 @@ def test_shared_decode_bad_entries(dev):
 def test_shared_decode_refusals(dev):
     b = _Batch(dev, 2, 64, 4, [700, 710, 720], [(0, 3, 690)])
     b.place()
-    b.plan()
+    b.plan(1)
     lib = dev.lib()
 
     def status(storage=b.storage.h, items=b.items.ptr, entries=b.entries_buf.ptr, work=b.work.ptr + 2048, **fields):
