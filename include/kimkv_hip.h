@@ -758,8 +758,7 @@ kimkv_status kimkv_model_argmax(const float* logits, uint32_t rows, uint32_t voc
  * times token v occurs in history[0 .. history_count) and x(v) its logit:
  *   c(v) > 0:  x = x > 0 ? x / repetition_penalty : x * repetition_penalty,
  *              then x -= frequency_penalty * c(v) + presence_penalty
- *   x += the sum of the bias_values[i] with bias_tokens[i] == v, added up in
- *        the list's order
+ *   x += bias_values[i] for each i with bias_tokens[i] == v, in the list's order
  *   v not in allowed:  x = -inf
  * allowed: bit v % 32 of word v / 32 for every token of the vocabulary, NULL
  * for all of them.  Listed tokens past the vocabulary are ignored. */

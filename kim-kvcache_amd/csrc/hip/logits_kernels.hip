@@ -1,12 +1,16 @@
 // logits_kernels.hip -- penalties, biases and allowed-token masks on rows of
 // fp32 logits, and the greedy token of each adjusted row, in one read.
 //
-// The work follows the vocabulary: block = (slice of kSlice tokens, row).  A
-// block counts the history's tokens of its slice and adds up its biases in
-// LDS, then takes the slice's logits once: adjusted, stored if wanted, and
-// folded into the slice's maximum.  A second, small launch picks the first of
-// the slices' maxima.  The reference picks the plain argmax
-// (src/cuda/model/kernels.cuh:111-117).
+// The work follows the vocabulary: block = (slice of the vocabulary, row).  A
+// slice's logits are on their way to registers, 16 bytes a lane, while the
+// block counts the history's tokens of its slice in LDS, a word a token.  Then
+// one thread for each token that occurs, and one for each bias, replaces the
+// word by the changed logit: a few hundred of a slice's thousands, where the
+// penalties' arithmetic on every logit would cost half as much again as its
+// bytes.  So each logit is read once: exchanged where its word says so, stored
+// if wanted and folded into the slice's maximum.  Where a row takes several
+// blocks a second, small launch picks the first of the slices' maxima.  The
+// reference picks the plain argmax (src/cuda/model/kernels.cuh:111-117).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -18,9 +22,6 @@
 namespace kimkv {
 namespace {
 
-constexpr unsigned kBlock = 256;
-constexpr unsigned kWaves = kBlock / kWave;
-constexpr uint32_t kSlice = 8192;      // tokens of the vocabulary a block takes
 constexpr uint32_t kOwners = 1024;
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -71,35 +72,104 @@ __device__ inline RowRule load_rule(const kimkv_logits_rule* rules, uint32_t row
     return rule;
 }
 
-// The tokens [s0, s1) of a row as the rule changes them.
-struct SliceLds {
-    uint32_t seen[kSlice];    // times a token occurs in the history
-    float bias[kSlice];
-    uint32_t owner[kOwners];
-    Best best[kWaves];
+// A slice of a row: positions [first, first + count) of its tokens, which
+// stand `shift` positions further so that every fourth position is a 16-byte
+// address of the row's logits.
+struct Slice {
+    uint32_t first;
+    uint32_t count;
+    uint32_t shift;
+    uint32_t V;
+    // The token's place in the slice; count or more: it is not in it.
+    __device__ uint32_t place(uint32_t token) const { return token < V ? token + shift - first : 0xFFFFFFFFu; }
 };
 
-// Adds the biases of the slice's tokens, those of one token in the list's
-// order: of the 256 entries a round looks at, each thread holds one, and of
-// the entries of one token (of one owner word: tokens that share it wait for
+// A changed logit as its token's word: never 0, which stands for one that is as it was.
+__device__ inline uint32_t word_of(float x) { return x == x ? ~__float_as_uint(x) : ~0x7FC00000u; }
+__device__ inline float value_of(uint32_t word, float unchanged) { return word != 0 ? __uint_as_float(~word) : unchanged; }
+
+// A logit whose token occurs `seen` times, as the penalties leave it.  Each operation rounds by itself.
+__device__ inline float penalized(float x, uint32_t seen, const kimkv_logits_rule& r)
+{
+#pragma clang fp contract(off)
+    x = x > 0.0f ? x / r.repetition_penalty : x * r.repetition_penalty;
+    return x - (r.frequency_penalty * static_cast<float>(seen) + r.presence_penalty);
+}
+
+// Slices are `per` positions, a multiple of 4 kBlock up to 4 kBlock kVecs.
+template <unsigned kBlock, uint32_t kVecs>
+struct SliceLds {
+    uint4 words[kBlock * kVecs];
+    uint32_t taken[kBlock * kVecs / 8];   // a bit a token: some thread has it in hand
+    uint32_t owners[kOwners];
+    Best best[kBlock / kWave];
+};
+
+// The words of the tokens in the history: how often each occurs, then the
+// penalized logit.  The words are 0 before.
+template <unsigned kBlock, typename Lds>
+__device__ void apply_history(Lds& lds, const float* from, const kimkv_logits_rule& r, const Slice& slice)
+{
+    constexpr uint32_t kAhead = 8;   // entries of a thread in flight
+    constexpr uint32_t kStep = kAhead * kBlock;
+    uint32_t* const words = reinterpret_cast<uint32_t*>(lds.words);
+    uint32_t place[kAhead];
+    auto const fetch = [&](uint32_t at) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            uint32_t const n = at + i * kBlock + threadIdx.x;
+            place[i] = n < r.history_count ? slice.place(r.history[n]) : 0xFFFFFFFFu;
+        }
+    };
+    uint32_t at = 0;
+    for (;; at += kStep) {
+        fetch(at);
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            if (place[i] < slice.count) atomicAdd(words + place[i], 1u);
+        }
+        if (r.history_count - at <= kStep) break;
+    }
+    __syncthreads();
+    // The last entries are still at hand; the others are read again.
+    for (;; fetch(at)) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            if (place[i] >= slice.count) continue;
+            uint32_t const bit = 1u << (place[i] & 31u);
+            if ((atomicOr(lds.taken + (place[i] >> 5), bit) & bit) != 0) continue;
+            float const x = from[slice.first + place[i] - slice.shift];
+            words[place[i]] = word_of(penalized(x, words[place[i]], r));
+        }
+        if (at == 0) break;
+        at -= kStep;
+    }
+}
+
+// Adds the biases of the slice's tokens to their logits, those of one token in
+// the list's order: of the entries a round looks at, each thread holds one, and
+// of the entries of one token (of one owner word: tokens that share it wait for
 // each other) the first left goes.
-__device__ void add_biases(SliceLds& lds, const kimkv_logits_rule& r, uint32_t s0, uint32_t s1)
+template <unsigned kBlock, typename Lds>
+__device__ void apply_biases(Lds& lds, const float* from, const kimkv_logits_rule& r, const Slice& slice)
 {
     uint32_t const tid = threadIdx.x;
+    uint32_t* const words = reinterpret_cast<uint32_t*>(lds.words);
     for (uint32_t at = 0; at < r.bias_count; at += kBlock) {
-        uint32_t token = KIMKV_NO_TOKEN;
-        float value = 0.0f;
+        uint32_t place = 0xFFFFFFFFu;
+        float bias = 0.0f;
         if (r.bias_count - at > tid) {
-            token = r.bias_tokens[at + tid];
-            value = r.bias_values[at + tid];
+            place = slice.place(r.bias_tokens[at + tid]);
+            bias = r.bias_values[at + tid];
         }
-        bool waits = token >= s0 && token < s1;
+        bool waits = place < slice.count;
+        float const x = waits ? from[slice.first + place - slice.shift] : 0.0f;
         while (__syncthreads_or(waits) != 0) {
-            uint32_t* const owner = lds.owner + (token & (kOwners - 1));
+            uint32_t* const owner = lds.owners + (place & (kOwners - 1));
             if (waits) atomicMin(owner, tid);
             __syncthreads();
             if (waits && *owner == tid) {
-                lds.bias[token - s0] += value;
+                words[place] = word_of(value_of(words[place], x) + bias);
                 *owner = 0xFFFFFFFFu;
                 waits = false;
             }
@@ -107,57 +177,101 @@ __device__ void add_biases(SliceLds& lds, const kimkv_logits_rule& r, uint32_t s
     }
 }
 
-// One logit as the rule leaves it.  Each operation rounds by itself.
-__device__ inline float adjusted(float x, uint32_t seen, float bias, const kimkv_logits_rule& r)
-{
-#pragma clang fp contract(off)
-    if (seen != 0) {
-        x = x > 0.0f ? x / r.repetition_penalty : x * r.repetition_penalty;
-        x -= r.frequency_penalty * static_cast<float>(seen) + r.presence_penalty;
-    }
-    return x + bias;
-}
-
+template <unsigned kBlock, uint32_t kVecs>
 __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uint32_t V, uint32_t per,
                                                         const kimkv_logits_rule* rules, float* out, uint32_t* tokens,
                                                         Best* partial)
 {
-    __shared__ SliceLds lds;
+    __shared__ SliceLds<kBlock, kVecs> lds;
     uint32_t const tid = threadIdx.x;
     uint32_t const row = blockIdx.y;
-    uint32_t const s0 = blockIdx.x * per;
-    uint32_t const s1 = min(s0 + per, V);
+    const float* const from = logits + static_cast<uint64_t>(row) * V;
+    Slice const slice{blockIdx.x * per, per, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from) >> 2) & 3u, V};
+    uint32_t const vecs = per / (4 * kBlock);
+    // Vector j of this thread holds tokens token(j) + 0 .. 3, those below V (a token in front of the row is a huge one).
+    auto const token = [&](uint32_t j) { return slice.first + 4 * (j * kBlock + tid) - slice.shift; };
+    auto const whole = [&](uint32_t v) { return v < V && V - v > 3; };
+    f32x4_t x[kVecs];
+#pragma unroll
+    for (uint32_t j = 0; j < kVecs; ++j) {
+        x[j] = f32x4_t{};
+        uint32_t const v = token(j);
+        if (j < vecs && whole(v)) {
+            x[j] = *reinterpret_cast<const f32x4_t*>(from + v);
+        } else if (j < vecs) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                if (v + i < V) x[j][i] = from[v + i];
+            }
+        }
+    }
     RowRule const rule = load_rule(rules, row);
     kimkv_logits_rule const& r = rule.r;
     Best best{-INFINITY, KIMKV_NO_TOKEN};
     if (rule.valid) {
-        for (uint32_t i = tid; i < s1 - s0; i += kBlock) {
-            lds.seen[i] = 0;
-            lds.bias[i] = -0.0f;   // the sum of no biases: x + -0 is x
+        bool const changes = (r.history_count | r.bias_count) != 0;
+        if (changes) {
+            for (uint32_t i = tid; i < vecs * kBlock; i += kBlock) lds.words[i] = uint4{0, 0, 0, 0};
+            for (uint32_t i = tid; i < vecs * kBlock / 8; i += kBlock) lds.taken[i] = 0;
+            for (uint32_t i = tid; i < kOwners; i += kBlock) lds.owners[i] = 0xFFFFFFFFu;
+            __syncthreads();
+            if (r.history_count != 0) {
+                apply_history<kBlock>(lds, from, r, slice);
+                __syncthreads();
+            }
+            apply_biases<kBlock>(lds, from, r, slice);
+            __syncthreads();
         }
-        for (uint32_t i = tid; i < kOwners; i += kBlock) lds.owner[i] = 0xFFFFFFFFu;
-        __syncthreads();
-        for (uint32_t i = tid; i < r.history_count; i += kBlock) {
-            uint32_t const token = r.history[i];
-            if (token >= s0 && token < s1) atomicAdd(&lds.seen[token - s0], 1u);
-        }
-        add_biases(lds, r, s0, s1);
-        __syncthreads();
-        uint64_t const at = static_cast<uint64_t>(row) * V;
-        for (uint32_t v = s0 + tid; v < s1; v += kBlock) {
-            float x = adjusted(logits[at + v], lds.seen[v - s0], lds.bias[v - s0], r);
-            bool const allowed = r.allowed == nullptr || ((r.allowed[v >> 5] >> (v & 31u)) & 1u) != 0;
-            if (!allowed) x = -INFINITY;
-            if (out != nullptr) out[at + v] = x;
-            if (allowed && x == x) take_best(best, x, v);
+        float* const to = out + static_cast<uint64_t>(row) * V;
+        bool const aligned = ((reinterpret_cast<uintptr_t>(to) >> 2) & 3u) == slice.shift;
+#pragma unroll
+        for (uint32_t j = 0; j < kVecs; ++j) {
+            if (j >= vecs) break;
+            uint32_t const v = token(j);
+            bool const all = whole(v);
+            uint32_t allowed = 15;
+            if (r.allowed != nullptr && all) {
+                uint64_t const two = r.allowed[v >> 5] | static_cast<uint64_t>(r.allowed[(v + 3) >> 5]) << 32;
+                allowed = static_cast<uint32_t>(two >> (v & 31u));
+            }
+            if (!all) {
+                uint32_t there = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    if (v + i >= V) continue;
+                    there |= (r.allowed == nullptr ? 1u : r.allowed[(v + i) >> 5] >> ((v + i) & 31u) & 1u) << i;
+                }
+                allowed = there;
+            }
+            uint4 word{0, 0, 0, 0};
+            if (changes) word = lds.words[j * kBlock + tid];
+            uint32_t const w[4] = {word.x, word.y, word.z, word.w};
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                float const value = value_of(w[i], x[j][i]);
+                bool const may = (allowed >> i & 1u) != 0;
+                x[j][i] = may ? value : -INFINITY;
+                // A thread's tokens ascend, so an equal value is no better.
+                if (may && (value > best.value || (best.token == KIMKV_NO_TOKEN && value == value))) best = Best{value, v + i};
+            }
+            if (out == nullptr) continue;
+            if (all && aligned) {
+                *reinterpret_cast<f32x4_t*>(to + v) = x[j];
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    if (v + i < V) to[v + i] = x[j][i];
+                }
+            }
         }
     }
     if (tokens == nullptr) return;
     best = wave_best(best);
     if ((tid & (kWave - 1)) == 0) lds.best[tid / kWave] = best;
     __syncthreads();
+    if (tid >= kWave) return;
+    best = wave_best(lds.best[tid < kBlock / kWave ? tid : 0]);
     if (tid != 0) return;
-    for (uint32_t w = 1; w < kWaves; ++w) take_best(best, lds.best[w].value, lds.best[w].token);
     if (gridDim.x == 1) {
         tokens[row] = best.token;
     } else {
@@ -165,11 +279,13 @@ __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uin
     }
 }
 
+constexpr unsigned kPickBlock = 256;
+
 // One wave a row: the first of the slices' maxima.
-__global__ __launch_bounds__(kBlock) void logits_pick_kernel(const Best* partial, uint32_t rows, uint32_t slices,
+__global__ __launch_bounds__(kPickBlock) void logits_pick_kernel(const Best* partial, uint32_t rows, uint32_t slices,
                                                              uint32_t* tokens)
 {
-    uint32_t const row = blockIdx.x * kWaves + threadIdx.x / kWave;
+    uint32_t const row = blockIdx.x * (kPickBlock / kWave) + threadIdx.x / kWave;
     if (row >= rows) return;
     Best best{-INFINITY, KIMKV_NO_TOKEN};
     for (uint32_t i = threadIdx.x & (kWave - 1); i < slices; i += kWave) {
@@ -180,7 +296,32 @@ __global__ __launch_bounds__(kBlock) void logits_pick_kernel(const Best* partial
     if ((threadIdx.x & (kWave - 1)) == 0) tokens[row] = best.token;
 }
 
-uint32_t logits_slices(uint32_t vocabulary) { return ceil_div(vocabulary, kSlice); }
+// How rows are cut.  A row up to kRowMost goes to one block of 1024 threads
+// while there is a compute unit for each, which saves the second launch.
+// Else slices of 2048 positions up to 8192, as large as leaves kBlocksWanted:
+// every block reads its row's whole history.
+constexpr uint32_t kRowMost = 32768 - 3;      // 3: a row's shift
+constexpr uint32_t kRowBlock = 1024;
+constexpr uint32_t kRowVecs = 8;
+constexpr uint32_t kSliceBlock = 512;
+constexpr uint32_t kSliceVecs = 4;
+constexpr uint32_t kBlocksWanted = 512;
+
+struct RowCut {
+    bool one_block;
+    uint32_t per;
+    uint32_t slices;
+};
+
+RowCut row_cut(uint32_t rows, uint32_t vocabulary)
+{
+    if (vocabulary <= kRowMost && rows <= 256) return RowCut{true, ceil_div(vocabulary + 3, 4 * kRowBlock) * 4 * kRowBlock, 1};
+    uint64_t const even = static_cast<uint64_t>(rows) * vocabulary / kBlocksWanted;
+    uint32_t const step = 4 * kSliceBlock;
+    uint32_t const most = step * kSliceVecs;
+    uint32_t const per = even >= most ? most : even <= step ? step : ceil_div(even, step) * step;
+    return RowCut{false, per, ceil_div(static_cast<uint64_t>(vocabulary) + 3, per)};
+}
 
 }  // namespace
 }  // namespace kimkv
@@ -191,7 +332,7 @@ extern "C" {
 
 size_t kimkv_logits_workspace_bytes(uint32_t rows, uint32_t vocabulary)
 {
-    uint32_t const slices = logits_slices(vocabulary);
+    uint32_t const slices = row_cut(rows, vocabulary).slices;
     return slices <= 1 ? 0 : static_cast<size_t>(rows) * slices * sizeof(Best);
 }
 
@@ -202,27 +343,31 @@ kimkv_status kimkv_model_logits_adjust(const float* logits, uint32_t rows, uint3
     if (logits == nullptr || vocabulary == 0 || vocabulary > 0x7FFFFFFFu || (out == nullptr && device_tokens == nullptr)) {
         return KIMKV_INVALID_ARGUMENT;
     }
-    uint32_t const slices = logits_slices(vocabulary);
-    bool const split = slices > 1 && device_tokens != nullptr;
+    RowCut const cut = row_cut(rows, vocabulary);
+    bool const split = cut.slices > 1 && device_tokens != nullptr;
     if (split && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 7u) != 0) && rows != 0) {
         return KIMKV_INVALID_ARGUMENT;
     }
-    uint32_t const per = ceil_div(vocabulary, slices);
     auto* const partial = static_cast<Best*>(workspace);
     // A launch takes 65535 rows of a grid.
     for (uint32_t first = 0; first < rows;) {
         uint32_t const n = rows - first < 65535u ? rows - first : 65535u;
         uint64_t const at = static_cast<uint64_t>(first) * vocabulary;
-        Best* const part = split ? partial + static_cast<uint64_t>(first) * slices : nullptr;
-        logits_kernel<<<dim3(slices, n), kBlock, 0, native(stream)>>>(
-            logits + at, vocabulary, per, device_rules != nullptr ? device_rules + first : nullptr,
-            out != nullptr ? out + at : nullptr, device_tokens != nullptr ? device_tokens + first : nullptr, part);
+        Best* const part = split ? partial + static_cast<uint64_t>(first) * cut.slices : nullptr;
+        auto const launch = [&](auto kernel, unsigned block) {
+            kernel<<<dim3(cut.slices, n), block, 0, native(stream)>>>(
+                logits + at, vocabulary, cut.per, device_rules != nullptr ? device_rules + first : nullptr,
+                out != nullptr ? out + at : nullptr, device_tokens != nullptr ? device_tokens + first : nullptr, part);
+        };
+        if (cut.one_block) launch(logits_kernel<kRowBlock, kRowVecs>, kRowBlock);
+        else launch(logits_kernel<kSliceBlock, kSliceVecs>, kSliceBlock);
         kimkv_status const status = launch_status();
         if (status != KIMKV_OK) return status;
         first += n;
     }
     if (!split || rows == 0) return KIMKV_OK;
-    logits_pick_kernel<<<ceil_div(rows, kWaves), kBlock, 0, native(stream)>>>(partial, rows, slices, device_tokens);
+    logits_pick_kernel<<<ceil_div(rows, kPickBlock / kWave), kPickBlock, 0, native(stream)>>>(partial, rows, cut.slices,
+                                                                                             device_tokens);
     return launch_status();
 }
 

@@ -660,7 +660,7 @@ def _adjust_reference(row, rule):
         for token, value in rule["biases"]:
             if token < len(x):
                 y[token] += float(np.float32(value))
-                # The sums are of the biases first, then the logit.
+                # Each sum rounds by 2^-24 of it.
                 bound[token] += half * 2 * (abs(float(np.float32(value))) * len(rule["biases"]) + abs(y[token]))
     top = float(np.finfo(np.float32).max)
     y[np.abs(y) > top] *= np.inf
