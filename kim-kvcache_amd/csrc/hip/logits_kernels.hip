@@ -22,6 +22,8 @@
 namespace kimkv {
 namespace {
 
+constexpr unsigned kBlock = 512;
+constexpr uint32_t kVecs = 4;          // 16-byte vectors of a row's logits a thread holds
 constexpr uint32_t kOwners = 1024;
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -97,7 +99,6 @@ __device__ inline float penalized(float x, uint32_t seen, const kimkv_logits_rul
 }
 
 // Slices are `per` positions, a multiple of 4 kBlock up to 4 kBlock kVecs.
-template <unsigned kBlock, uint32_t kVecs>
 struct SliceLds {
     uint4 words[kBlock * kVecs];
     uint32_t taken[kBlock * kVecs / 8];   // a bit a token: some thread has it in hand
@@ -107,8 +108,7 @@ struct SliceLds {
 
 // The words of the tokens in the history: how often each occurs, then the
 // penalized logit.  The words are 0 before.
-template <unsigned kBlock, typename Lds>
-__device__ void apply_history(Lds& lds, const float* from, const kimkv_logits_rule& r, const Slice& slice)
+__device__ void apply_history(SliceLds& lds, const float* from, const kimkv_logits_rule& r, const Slice& slice)
 {
     constexpr uint32_t kAhead = 8;   // entries of a thread in flight
     constexpr uint32_t kStep = kAhead * kBlock;
@@ -150,8 +150,7 @@ __device__ void apply_history(Lds& lds, const float* from, const kimkv_logits_ru
 // the list's order: of the entries a round looks at, each thread holds one, and
 // of the entries of one token (of one owner word: tokens that share it wait for
 // each other) the first left goes.
-template <unsigned kBlock, typename Lds>
-__device__ void apply_biases(Lds& lds, const float* from, const kimkv_logits_rule& r, const Slice& slice)
+__device__ void apply_biases(SliceLds& lds, const float* from, const kimkv_logits_rule& r, const Slice& slice)
 {
     uint32_t const tid = threadIdx.x;
     uint32_t* const words = reinterpret_cast<uint32_t*>(lds.words);
@@ -177,12 +176,11 @@ __device__ void apply_biases(Lds& lds, const float* from, const kimkv_logits_rul
     }
 }
 
-template <unsigned kBlock, uint32_t kVecs>
 __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uint32_t V, uint32_t per,
                                                         const kimkv_logits_rule* rules, float* out, uint32_t* tokens,
                                                         Best* partial)
 {
-    __shared__ SliceLds<kBlock, kVecs> lds;
+    __shared__ SliceLds lds;
     uint32_t const tid = threadIdx.x;
     uint32_t const row = blockIdx.y;
     const float* const from = logits + static_cast<uint64_t>(row) * V;
@@ -216,10 +214,10 @@ __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uin
             for (uint32_t i = tid; i < kOwners; i += kBlock) lds.owners[i] = 0xFFFFFFFFu;
             __syncthreads();
             if (r.history_count != 0) {
-                apply_history<kBlock>(lds, from, r, slice);
+                apply_history(lds, from, r, slice);
                 __syncthreads();
             }
-            apply_biases<kBlock>(lds, from, r, slice);
+            apply_biases(lds, from, r, slice);
             __syncthreads();
         }
         float* const to = out + static_cast<uint64_t>(row) * V;
@@ -296,31 +294,24 @@ __global__ __launch_bounds__(kPickBlock) void logits_pick_kernel(const Best* par
     if ((threadIdx.x & (kWave - 1)) == 0) tokens[row] = best.token;
 }
 
-// How rows are cut.  A row up to kRowMost goes to one block of 1024 threads
-// while there is a compute unit for each, which saves the second launch.
-// Else slices of 2048 positions up to 8192, as large as leaves kBlocksWanted:
-// every block reads its row's whole history.
-constexpr uint32_t kRowMost = 32768 - 3;      // 3: a row's shift
-constexpr uint32_t kRowBlock = 1024;
-constexpr uint32_t kRowVecs = 8;
-constexpr uint32_t kSliceBlock = 512;
-constexpr uint32_t kSliceVecs = 4;
+// How rows are cut: slices of 2048 positions up to 8192, as large as leaves
+// kBlocksWanted, since every block reads its row's whole history.  (A block of
+// 1024 threads for a row of 32000 saves the second launch and loses more: 12.6
+// us for 4 rows and 16.2 for 72, where slices take 9.2 and 13.4.)
 constexpr uint32_t kBlocksWanted = 512;
 
 struct RowCut {
-    bool one_block;
     uint32_t per;
     uint32_t slices;
 };
 
 RowCut row_cut(uint32_t rows, uint32_t vocabulary)
 {
-    if (vocabulary <= kRowMost && rows <= 256) return RowCut{true, ceil_div(vocabulary + 3, 4 * kRowBlock) * 4 * kRowBlock, 1};
+    constexpr uint32_t kStep = 4 * kBlock;
+    constexpr uint32_t kMost = kStep * kVecs;
     uint64_t const even = static_cast<uint64_t>(rows) * vocabulary / kBlocksWanted;
-    uint32_t const step = 4 * kSliceBlock;
-    uint32_t const most = step * kSliceVecs;
-    uint32_t const per = even >= most ? most : even <= step ? step : ceil_div(even, step) * step;
-    return RowCut{false, per, ceil_div(static_cast<uint64_t>(vocabulary) + 3, per)};
+    uint32_t const per = even >= kMost ? kMost : even <= kStep ? kStep : ceil_div(even, kStep) * kStep;
+    return RowCut{per, ceil_div(vocabulary + 3ull, per)};   // 3: a row's shift
 }
 
 }  // namespace
@@ -354,13 +345,9 @@ kimkv_status kimkv_model_logits_adjust(const float* logits, uint32_t rows, uint3
         uint32_t const n = rows - first < 65535u ? rows - first : 65535u;
         uint64_t const at = static_cast<uint64_t>(first) * vocabulary;
         Best* const part = split ? partial + static_cast<uint64_t>(first) * cut.slices : nullptr;
-        auto const launch = [&](auto kernel, unsigned block) {
-            kernel<<<dim3(cut.slices, n), block, 0, native(stream)>>>(
-                logits + at, vocabulary, cut.per, device_rules != nullptr ? device_rules + first : nullptr,
-                out != nullptr ? out + at : nullptr, device_tokens != nullptr ? device_tokens + first : nullptr, part);
-        };
-        if (cut.one_block) launch(logits_kernel<kRowBlock, kRowVecs>, kRowBlock);
-        else launch(logits_kernel<kSliceBlock, kSliceVecs>, kSliceBlock);
+        logits_kernel<<<dim3(cut.slices, n), kBlock, 0, native(stream)>>>(
+            logits + at, vocabulary, cut.per, device_rules != nullptr ? device_rules + first : nullptr,
+            out != nullptr ? out + at : nullptr, device_tokens != nullptr ? device_tokens + first : nullptr, part);
         kimkv_status const status = launch_status();
         if (status != KIMKV_OK) return status;
         first += n;
