@@ -16,13 +16,14 @@
 #include <cmath>
 #include <cstdint>
 
+#include "attention_common.h"
 #include "device_common.h"
 #include "runtime_internal.h"
 
 namespace kimkv {
 namespace {
 
-constexpr unsigned kBlock = 512;
+constexpr unsigned kBlock = 1024;
 constexpr uint32_t kVecs = 4;          // 16-byte vectors of a row's logits a thread holds
 constexpr uint32_t kOwners = 1024;
 
@@ -43,15 +44,14 @@ __device__ inline void take_best(Best& best, float value, uint32_t token)
     }
 }
 
+// The wave's: the first token of the highest value.  (No token, the highest number, has the lowest value.)
 __device__ inline Best wave_best(Best best)
 {
+    float const value = wave_max(best.value);
+    uint32_t token = best.value == value ? best.token : KIMKV_NO_TOKEN;
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        float const v = __shfl_xor(best.value, m);
-        uint32_t const t = __shfl_xor(best.token, m);
-        take_best(best, v, t);
-    }
-    return best;
+    for (int m = 32; m >= 1; m >>= 1) token = min(token, static_cast<uint32_t>(__shfl_xor(static_cast<int>(token), m)));
+    return Best{value, token};
 }
 
 struct RowRule {
@@ -106,33 +106,38 @@ struct SliceLds {
     Best best[kBlock / kWave];
 };
 
-// The words of the tokens in the history: how often each occurs, then the
-// penalized logit.  The words are 0 before.
-__device__ void apply_history(SliceLds& lds, const float* from, const kimkv_logits_rule& r, const Slice& slice)
+constexpr uint32_t kAhead = 4;   // history entries of a thread in flight
+constexpr uint32_t kHistoryStep = kAhead * kBlock;
+
+// The places of kAhead entries from entry `at` on.
+__device__ inline void history_places(uint32_t (&place)[kAhead], const kimkv_logits_rule& r, const Slice& slice, uint32_t at)
 {
-    constexpr uint32_t kAhead = 8;   // entries of a thread in flight
-    constexpr uint32_t kStep = kAhead * kBlock;
-    uint32_t* const words = reinterpret_cast<uint32_t*>(lds.words);
-    uint32_t place[kAhead];
-    auto const fetch = [&](uint32_t at) {
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            uint32_t const n = at + i * kBlock + threadIdx.x;
-            place[i] = n < r.history_count ? slice.place(r.history[n]) : 0xFFFFFFFFu;
-        }
-    };
+    for (uint32_t i = 0; i < kAhead; ++i) {
+        uint32_t const n = at + i * kBlock + threadIdx.x;
+        place[i] = n < r.history_count ? slice.place(r.history[n]) : 0xFFFFFFFFu;
+    }
+}
+
+// The words of the tokens in the history: how often each occurs, then the
+// penalized logit.  The words are 0 before, `place` those of entry 0 on.
+__device__ void apply_history(SliceLds& lds, uint32_t (&place)[kAhead], const float* from, const kimkv_logits_rule& r,
+                              const Slice& slice)
+{
+    uint32_t* const words = reinterpret_cast<uint32_t*>(lds.words);
     uint32_t at = 0;
-    for (;; at += kStep) {
-        fetch(at);
+    for (;;) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i) {
             if (place[i] < slice.count) atomicAdd(words + place[i], 1u);
         }
-        if (r.history_count - at <= kStep) break;
+        if (r.history_count - at <= kHistoryStep) break;
+        at += kHistoryStep;
+        history_places(place, r, slice, at);
     }
     __syncthreads();
     // The last entries are still at hand; the others are read again.
-    for (;; fetch(at)) {
+    for (;;) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i) {
             if (place[i] >= slice.count) continue;
@@ -142,33 +147,41 @@ __device__ void apply_history(SliceLds& lds, const float* from, const kimkv_logi
             words[place[i]] = word_of(penalized(x, words[place[i]], r));
         }
         if (at == 0) break;
-        at -= kStep;
+        at -= kHistoryStep;
+        history_places(place, r, slice, at);
     }
+}
+
+// A bias of the list.
+struct Bias {
+    uint32_t place;
+    float value;
+};
+
+__device__ inline Bias bias_at(const kimkv_logits_rule& r, const Slice& slice, uint32_t i)
+{
+    if (i >= r.bias_count) return Bias{0xFFFFFFFFu, 0.0f};
+    return Bias{slice.place(r.bias_tokens[i]), r.bias_values[i]};
 }
 
 // Adds the biases of the slice's tokens to their logits, those of one token in
 // the list's order: of the entries a round looks at, each thread holds one, and
 // of the entries of one token (of one owner word: tokens that share it wait for
-// each other) the first left goes.
-__device__ void apply_biases(SliceLds& lds, const float* from, const kimkv_logits_rule& r, const Slice& slice)
+// each other) the first left goes.  `bias` is the first round's.
+__device__ void apply_biases(SliceLds& lds, Bias bias, const float* from, const kimkv_logits_rule& r, const Slice& slice)
 {
     uint32_t const tid = threadIdx.x;
     uint32_t* const words = reinterpret_cast<uint32_t*>(lds.words);
     for (uint32_t at = 0; at < r.bias_count; at += kBlock) {
-        uint32_t place = 0xFFFFFFFFu;
-        float bias = 0.0f;
-        if (r.bias_count - at > tid) {
-            place = slice.place(r.bias_tokens[at + tid]);
-            bias = r.bias_values[at + tid];
-        }
-        bool waits = place < slice.count;
-        float const x = waits ? from[slice.first + place - slice.shift] : 0.0f;
+        if (at != 0) bias = bias_at(r, slice, at + tid);
+        bool waits = bias.place < slice.count;
+        float const x = waits ? from[slice.first + bias.place - slice.shift] : 0.0f;
         while (__syncthreads_or(waits) != 0) {
-            uint32_t* const owner = lds.owners + (place & (kOwners - 1));
+            uint32_t* const owner = lds.owners + (bias.place & (kOwners - 1));
             if (waits) atomicMin(owner, tid);
             __syncthreads();
             if (waits && *owner == tid) {
-                words[place] = word_of(value_of(words[place], x) + bias);
+                words[bias.place] = word_of(value_of(words[bias.place], x) + bias.value);
                 *owner = 0xFFFFFFFFu;
                 waits = false;
             }
@@ -189,6 +202,15 @@ __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uin
     // Vector j of this thread holds tokens token(j) + 0 .. 3, those below V (a token in front of the row is a huge one).
     auto const token = [&](uint32_t j) { return slice.first + 4 * (j * kBlock + tid) - slice.shift; };
     auto const whole = [&](uint32_t v) { return v < V && V - v > 3; };
+    // The lists are asked for first: loads come back in order.
+    RowRule const rule = load_rule(rules, row);
+    kimkv_logits_rule const& r = rule.r;
+    uint32_t place[kAhead];
+    Bias bias{};
+    if (rule.valid) {
+        history_places(place, r, slice, 0);
+        bias = bias_at(r, slice, tid);
+    }
     f32x4_t x[kVecs];
 #pragma unroll
     for (uint32_t j = 0; j < kVecs; ++j) {
@@ -203,8 +225,6 @@ __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uin
             }
         }
     }
-    RowRule const rule = load_rule(rules, row);
-    kimkv_logits_rule const& r = rule.r;
     Best best{-INFINITY, KIMKV_NO_TOKEN};
     if (rule.valid) {
         bool const changes = (r.history_count | r.bias_count) != 0;
@@ -214,10 +234,10 @@ __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uin
             for (uint32_t i = tid; i < kOwners; i += kBlock) lds.owners[i] = 0xFFFFFFFFu;
             __syncthreads();
             if (r.history_count != 0) {
-                apply_history(lds, from, r, slice);
+                apply_history(lds, place, from, r, slice);
                 __syncthreads();
             }
-            apply_biases(lds, from, r, slice);
+            apply_biases(lds, bias, from, r, slice);
             __syncthreads();
         }
         float* const to = out + static_cast<uint64_t>(row) * V;
@@ -294,7 +314,7 @@ __global__ __launch_bounds__(kPickBlock) void logits_pick_kernel(const Best* par
     if ((threadIdx.x & (kWave - 1)) == 0) tokens[row] = best.token;
 }
 
-// How rows are cut: slices of 2048 positions up to 8192, as large as leaves
+// How rows are cut: slices of 4096 positions up to 16384, as large as leaves
 // kBlocksWanted, since every block reads its row's whole history.  (A block of
 // 1024 threads for a row of 32000 saves the second launch and loses more: 12.6
 // us for 4 rows and 16.2 for 72, where slices take 9.2 and 13.4.)
