@@ -84,6 +84,7 @@ struct Slice {
     uint32_t V;
     // The token's place in the slice; count or more: it is not in it.
     __device__ uint32_t place(uint32_t token) const { return token < V ? token + shift - first : 0xFFFFFFFFu; }
+    __device__ float logit(const float* row, uint32_t place) const { return place < count ? row[first + place - shift] : 0.0f; }
 };
 
 // A changed logit as its token's word: never 0, which stands for one that is as it was.
@@ -109,19 +110,28 @@ struct SliceLds {
 constexpr uint32_t kAhead = 4;   // history entries of a thread in flight
 constexpr uint32_t kHistoryStep = kAhead * kBlock;
 
-// The places of kAhead entries from entry `at` on.
-__device__ inline void history_places(uint32_t (&place)[kAhead], const kimkv_logits_rule& r, const Slice& slice, uint32_t at)
-{
+// kAhead entries from entry `at` on: their places and logits.
+struct Entries {
+    uint32_t place[kAhead];
+    float logit[kAhead];
+    __device__ void find(const kimkv_logits_rule& r, const Slice& slice, uint32_t at)
+    {
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i) {
-        uint32_t const n = at + i * kBlock + threadIdx.x;
-        place[i] = n < r.history_count ? slice.place(r.history[n]) : 0xFFFFFFFFu;
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            uint32_t const n = at + i * kBlock + threadIdx.x;
+            place[i] = n < r.history_count ? slice.place(r.history[n]) : 0xFFFFFFFFu;
+        }
     }
-}
+    __device__ void read(const float* from, const Slice& slice)
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) logit[i] = slice.logit(from, place[i]);
+    }
+};
 
 // The words of the tokens in the history: how often each occurs, then the
-// penalized logit.  The words are 0 before, `place` those of entry 0 on.
-__device__ void apply_history(SliceLds& lds, uint32_t (&place)[kAhead], const float* from, const kimkv_logits_rule& r,
+// penalized logit.  The words are 0 before, `e` those of entry 0 on.
+__device__ void apply_history(SliceLds& lds, Entries& e, const float* from, const kimkv_logits_rule& r,
                               const Slice& slice)
 {
     uint32_t* const words = reinterpret_cast<uint32_t*>(lds.words);
@@ -129,26 +139,27 @@ __device__ void apply_history(SliceLds& lds, uint32_t (&place)[kAhead], const fl
     for (;;) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i) {
-            if (place[i] < slice.count) atomicAdd(words + place[i], 1u);
+            if (e.place[i] < slice.count) atomicAdd(words + e.place[i], 1u);
         }
         if (r.history_count - at <= kHistoryStep) break;
         at += kHistoryStep;
-        history_places(place, r, slice, at);
+        e.find(r, slice, at);
+        e.read(from, slice);
     }
     __syncthreads();
     // The last entries are still at hand; the others are read again.
     for (;;) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i) {
-            if (place[i] >= slice.count) continue;
-            uint32_t const bit = 1u << (place[i] & 31u);
-            if ((atomicOr(lds.taken + (place[i] >> 5), bit) & bit) != 0) continue;
-            float const x = from[slice.first + place[i] - slice.shift];
-            words[place[i]] = word_of(penalized(x, words[place[i]], r));
+            if (e.place[i] >= slice.count) continue;
+            uint32_t const bit = 1u << (e.place[i] & 31u);
+            if ((atomicOr(lds.taken + (e.place[i] >> 5), bit) & bit) != 0) continue;
+            words[e.place[i]] = word_of(penalized(e.logit[i], words[e.place[i]], r));
         }
         if (at == 0) break;
         at -= kHistoryStep;
-        history_places(place, r, slice, at);
+        e.find(r, slice, at);
+        e.read(from, slice);
     }
 }
 
@@ -156,12 +167,13 @@ __device__ void apply_history(SliceLds& lds, uint32_t (&place)[kAhead], const fl
 struct Bias {
     uint32_t place;
     float value;
+    float logit;   // its token's, unchanged
 };
 
 __device__ inline Bias bias_at(const kimkv_logits_rule& r, const Slice& slice, uint32_t i)
 {
-    if (i >= r.bias_count) return Bias{0xFFFFFFFFu, 0.0f};
-    return Bias{slice.place(r.bias_tokens[i]), r.bias_values[i]};
+    if (i >= r.bias_count) return Bias{0xFFFFFFFFu, 0.0f, 0.0f};
+    return Bias{slice.place(r.bias_tokens[i]), r.bias_values[i], 0.0f};
 }
 
 // Adds the biases of the slice's tokens to their logits, those of one token in
@@ -173,19 +185,21 @@ __device__ void apply_biases(SliceLds& lds, Bias bias, const float* from, const 
     uint32_t const tid = threadIdx.x;
     uint32_t* const words = reinterpret_cast<uint32_t*>(lds.words);
     for (uint32_t at = 0; at < r.bias_count; at += kBlock) {
-        if (at != 0) bias = bias_at(r, slice, at + tid);
+        if (at != 0) {
+            bias = bias_at(r, slice, at + tid);
+            bias.logit = slice.logit(from, bias.place);
+        }
         bool waits = bias.place < slice.count;
-        float const x = waits ? from[slice.first + bias.place - slice.shift] : 0.0f;
-        while (__syncthreads_or(waits) != 0) {
+        do {
             uint32_t* const owner = lds.owners + (bias.place & (kOwners - 1));
             if (waits) atomicMin(owner, tid);
             __syncthreads();
             if (waits && *owner == tid) {
-                words[bias.place] = word_of(value_of(words[bias.place], x) + bias.value);
+                words[bias.place] = word_of(value_of(words[bias.place], bias.logit) + bias.value);
                 *owner = 0xFFFFFFFFu;
                 waits = false;
             }
-        }
+        } while (__syncthreads_or(waits) != 0);
     }
 }
 
@@ -205,10 +219,10 @@ __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uin
     // The lists are asked for first: loads come back in order.
     RowRule const rule = load_rule(rules, row);
     kimkv_logits_rule const& r = rule.r;
-    uint32_t place[kAhead];
+    Entries entries{};
     Bias bias{};
     if (rule.valid) {
-        history_places(place, r, slice, 0);
+        entries.find(r, slice, 0);
         bias = bias_at(r, slice, tid);
     }
     f32x4_t x[kVecs];
@@ -225,6 +239,10 @@ __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uin
             }
         }
     }
+    if (rule.valid) {
+        entries.read(from, slice);
+        bias.logit = slice.logit(from, bias.place);
+    }
     Best best{-INFINITY, KIMKV_NO_TOKEN};
     if (rule.valid) {
         bool const changes = (r.history_count | r.bias_count) != 0;
@@ -234,7 +252,7 @@ __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uin
             for (uint32_t i = tid; i < kOwners; i += kBlock) lds.owners[i] = 0xFFFFFFFFu;
             __syncthreads();
             if (r.history_count != 0) {
-                apply_history(lds, place, from, r, slice);
+                apply_history(lds, entries, from, r, slice);
                 __syncthreads();
             }
             apply_biases(lds, bias, from, r, slice);
@@ -274,7 +292,7 @@ __global__ __launch_bounds__(kBlock) void logits_kernel(const float* logits, uin
             }
             if (out == nullptr) continue;
             if (all && aligned) {
-                *reinterpret_cast<f32x4_t*>(to + v) = x[j];
+                __builtin_nontemporal_store(x[j], reinterpret_cast<f32x4_t*>(to + v));
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
