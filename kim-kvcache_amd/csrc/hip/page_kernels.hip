@@ -299,7 +299,9 @@ __global__ __launch_bounds__(kBlock) void append_kernel(PoolView P, const kimkv_
 
 // ---------------------------------------------------------------------------
 // Rotated append: block = (job, 8-token group of its page), q | k | v rows in,
-// rotated q rows, rotated page K and page V^T out.
+// rotated q rows, rotated page K and page V^T out.  The groups of a page are
+// neighbours on one XCD: four of them write the 16-byte quarters of V^T's
+// 64-byte runs, which meet in its L2.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kRopeGroup = 8;          // page tokens a block takes
 constexpr uint32_t kMaxRopePairs = 256;
@@ -311,13 +313,16 @@ struct RopeArgs {
     uint16_t* q_out;
     uint64_t q_stride;
     uint32_t rows;
+    uint32_t job_count;
     uint32_t max_tokens;
     uint32_t layer;
     uint32_t QH;
     uint32_t rotary;
     double log2_theta;
     bool adjacent;
-    bool wide;          // 16-byte pieces: shapes, strides and addresses allow them
+    bool aligned;       // D is a multiple of 8 and every head of qkv lies at a 16-byte address
+    bool wide;          // 16-byte pieces: q_out and the rotated dims allow them too
+    Divisor groups;     // of a job
     Divisor items;      // rotated pieces and kept pieces of a row's q and k heads
     Divisor head_items;
 };
@@ -373,7 +378,10 @@ template <bool kHuge>
 __global__ __launch_bounds__(kBlock) void append_rope_kernel(PoolView P, RopeArgs a, AppendDivisors dv)
 {
     __shared__ float2 turn[kRopeGroup * kMaxRopePairs];
-    kimkv_append_rope_job const job = a.jobs[blockIdx.x];
+    uint32_t my_group;
+    uint32_t const my_job = div_mod(blockIdx.x / kXcds, a.groups, &my_group) * kXcds + blockIdx.x % kXcds;
+    if (my_job >= a.job_count) return;
+    kimkv_append_rope_job const job = a.jobs[my_job];
     uint32_t const tid = threadIdx.x;
     uint32_t const H = P.heads;
     uint32_t const D = P.dim;
@@ -385,7 +393,7 @@ __global__ __launch_bounds__(kBlock) void append_rope_kernel(PoolView P, RopeArg
     if (dst == nullptr || n > a.max_tokens || n > dcap || job.dst_token > dcap - n || n > a.rows
         || job.first_row > a.rows - n || (n != 0 && job.position > 0xFFFFFFFFu - (n - 1))
         || (job.cow_tokens != 0 && (src == nullptr || job.cow_tokens > scap || job.cow_tokens > job.dst_token))) {
-        if (blockIdx.y == 0) report_fault(P, KIMKV_FAULT_APPEND_JOB);
+        if (my_group == 0) report_fault(P, KIMKV_FAULT_APPEND_JOB);
         return;
     }
     uint32_t const layer = a.layer;
@@ -397,7 +405,7 @@ __global__ __launch_bounds__(kBlock) void append_rope_kernel(PoolView P, RopeArg
     };
 
     // The copied positions lie below the written ones: neither waits for the other.
-    if (blockIdx.y == 0 && job.cow_tokens != 0) {
+    if (my_group == 0 && job.cow_tokens != 0) {
         uint32_t const m = job.cow_tokens;
         if (!kHuge && ((D | scap | dcap) & 7u) == 0) {
             copy_tokens_wide(dv, m, src + head_block(P, scap, layer, 0), scap, dst + head_block(P, dcap, layer, 0), dcap);
@@ -417,12 +425,47 @@ __global__ __launch_bounds__(kBlock) void append_rope_kernel(PoolView P, RopeArg
     }
 
     // The group's tokens: page tokens [p0, p1) of the job's [dst_token, dst_token + n).
-    uint32_t const group = (job.dst_token / kRopeGroup + blockIdx.y) * kRopeGroup;
+    uint32_t const group = (job.dst_token / kRopeGroup + my_group) * kRopeGroup;
     uint32_t const p0 = max(group, static_cast<uint32_t>(job.dst_token));
     uint32_t const p1 = min(group + kRopeGroup, job.dst_token + n);
     if (p0 >= p1) return;
     uint32_t const tokens = p1 - p0;
     uint32_t const first = p0 - job.dst_token;   // token of the job
+    const uint16_t* const rows = a.qkv + static_cast<uint64_t>(job.first_row + first) * a.qkv_stride;
+    uint32_t const QH = a.QH;
+    const uint16_t* const values = rows + static_cast<uint64_t>(QH + H) * D;
+    uint32_t const HD = H * D;
+    if (!kHuge && a.aligned && tokens == kRopeGroup && (dcap & 7u) == 0) {
+        // V^T: the group's 8 tokens of four dims in, 16-byte pieces of 8 tokens of one dim out.
+        for (uint32_t i = 4 * tid; i < HD; i += 4 * kBlock) {
+            uint32_t d;
+            uint32_t const h = div_mod(i, dv.d, &d);
+            uint2 v[kRopeGroup];
+#pragma unroll
+            for (uint32_t j = 0; j < kRopeGroup; ++j) v[j] = *reinterpret_cast<const uint2*>(values + j * a.qkv_stride + i);
+            uint16_t* const to = dst + head_block(P, dcap, layer, h);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                u32x4_t w;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    uint32_t const even = k < 2 ? v[2 * j].x : v[2 * j].y;
+                    uint32_t const odd = k < 2 ? v[2 * j + 1].x : v[2 * j + 1].y;
+                    w[j] = __builtin_amdgcn_perm(odd, even, k % 2 == 0 ? 0x05040100u : 0x07060302u);
+                }
+                *reinterpret_cast<u32x4_t*>(to + v_at(dcap, D, p0, d + k)) = w;
+            }
+        }
+    } else {
+        for (uint32_t t = 0; t < tokens; ++t) {
+            for (uint32_t i = tid; i < HD; i += kBlock) {
+                uint32_t d;
+                uint32_t const h = div_mod(i, dv.d, &d);
+                dst[head_block(P, dcap, layer, h) + v_el(dcap, D, p0 + t, d)] = values[t * a.qkv_stride + i];
+            }
+        }
+    }
+
     uint32_t const pairs = a.rotary / 2;
     for (uint32_t i = tid; i < tokens * pairs; i += kBlock) {
         uint32_t const t = i / pairs;
@@ -430,9 +473,7 @@ __global__ __launch_bounds__(kBlock) void append_rope_kernel(PoolView P, RopeArg
     }
     __syncthreads();
 
-    const uint16_t* const rows = a.qkv + static_cast<uint64_t>(job.first_row + first) * a.qkv_stride;
     uint16_t* const q_rows = a.q_out != nullptr ? a.q_out + static_cast<uint64_t>(job.first_row + first) * a.q_stride : nullptr;
-    uint32_t const QH = a.QH;
     uint32_t const h0 = q_rows != nullptr ? 0 : QH;   // heads turned: q's, then k's
     // Where dims of head `head` (q's, then k's) of token t go.
     auto q_row = [&](uint32_t t, uint32_t head) { return q_rows + t * a.q_stride + static_cast<uint64_t>(head) * D; };
@@ -446,7 +487,7 @@ __global__ __launch_bounds__(kBlock) void append_rope_kernel(PoolView P, RopeArg
             uint16_t* const kb = dst + head_block(P, dcap, layer, head - QH);   // read only for k's heads
             auto put = [&](uint32_t d, u32x4_t v) {
                 uint16_t* const to = head < QH ? q_row(t, head) + d : kb + k_at(dcap, D, p0 + t, d);
-                *reinterpret_cast<u32x4_t*>(to) = v;
+                __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(to));
             };
             // A kept piece lies past the rotated dims.
             uint32_t const d = c < turned ? 8 * c : a.rotary + 8 * (c - turned);
@@ -485,31 +526,6 @@ __global__ __launch_bounds__(kBlock) void append_rope_kernel(PoolView P, RopeArg
                 put(dx, __half_as_ushort(__float2half_rn(x * s.x - y * s.y)));
                 put(dy, __half_as_ushort(__float2half_rn(y * s.x + x * s.y)));
             }
-        }
-    }
-
-    const uint16_t* const values = rows + static_cast<uint64_t>(QH + H) * D;
-    uint32_t const HD = H * D;
-    if (!kHuge && tokens == kRopeGroup && ((dcap | D) & 7u) == 0) {
-        // V^T: 16-byte pieces of the group's 8 tokens of one dim.
-        for (uint32_t i = tid; i < HD; i += kBlock) {
-            uint32_t d;
-            uint32_t const h = div_mod(i, dv.d, &d);
-            u32x4_t w;
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                w[j] = static_cast<uint32_t>(values[2 * j * a.qkv_stride + i])
-                    | static_cast<uint32_t>(values[(2 * j + 1) * a.qkv_stride + i]) << 16;
-            }
-            *reinterpret_cast<u32x4_t*>(dst + head_block(P, dcap, layer, h) + v_at(dcap, D, p0, d)) = w;
-        }
-        return;
-    }
-    for (uint32_t t = 0; t < tokens; ++t) {
-        for (uint32_t i = tid; i < HD; i += kBlock) {
-            uint32_t d;
-            uint32_t const h = div_mod(i, dv.d, &d);
-            dst[head_block(P, dcap, layer, h) + v_el(dcap, D, p0 + t, d)] = values[t * a.qkv_stride + i];
         }
     }
 }
@@ -932,10 +948,11 @@ kimkv_status kimkv_append_rope_batch(const kimkv_storage* storage, const kimkv_a
     // than a page holds are refused by the kernel.
     uint32_t const page = storage->micro_tokens > storage->extent_tokens ? storage->micro_tokens : storage->extent_tokens;
     uint32_t const tokens = max_token_count < page ? max_token_count : page;
-    uint32_t const groups = (tokens + 2 * (kRopeGroup - 1)) / kRopeGroup;
+    uint32_t const spanned = (tokens + 2 * (kRopeGroup - 1)) / kRopeGroup;
+    uint32_t const whole = ceil_div(page, kRopeGroup);
+    uint32_t const groups = spanned == 0 ? 1 : spanned < whole ? spanned : whole;
     PoolView const pv = pool_view(*storage);
     RopeArgs a{};
-    a.jobs = device_jobs;
     a.qkv = qkv;
     a.qkv_stride = qkv_stride;
     a.q_out = q_out;
@@ -948,18 +965,26 @@ kimkv_status kimkv_append_rope_batch(const kimkv_storage* storage, const kimkv_a
     a.log2_theta = std::log2(static_cast<double>(rope->theta));
     a.adjacent = rope->adjacent_pairs != 0;
     uint32_t const piece = a.adjacent ? 8 : 16;
-    a.wide = D % 8 == 0 && qkv_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(qkv) & 15u) == 0 && a.rotary % piece == 0
+    a.aligned = D % 8 == 0 && qkv_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(qkv) & 15u) == 0;
+    a.wide = a.aligned && a.rotary % piece == 0
         && (q_out == nullptr || (q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q_out) & 15u) == 0));
     uint32_t const head_items = a.rotary / piece + (D - a.rotary) / 8;
     a.head_items = divisor(head_items);
     a.items = divisor((H + (q_out != nullptr ? query_heads : 0)) * head_items);
-    dim3 const grid(job_count, groups == 0 ? 1 : groups);
-    if (append_huge(pv)) {
-        append_rope_kernel<true><<<grid, kBlock, 0, native(stream)>>>(pv, a, append_divisors(*storage));
-    } else {
-        append_rope_kernel<false><<<grid, kBlock, 0, native(stream)>>>(pv, a, append_divisors(*storage));
+    a.groups = divisor(groups);
+    // A launch takes fewer than 2^32 threads.
+    uint32_t const most_jobs = 0xFFFFFFu / groups;
+    for (uint32_t first = 0; first < job_count;) {
+        uint32_t const jobs = job_count - first < most_jobs ? job_count - first : most_jobs;
+        a.jobs = device_jobs + first;
+        auto const kernel = append_huge(pv) ? append_rope_kernel<true> : append_rope_kernel<false>;
+        a.job_count = jobs;
+        kernel<<<(jobs + kXcds - 1) / kXcds * kXcds * groups, kBlock, 0, native(stream)>>>(pv, a, append_divisors(*storage));
+        kimkv_status const status = launch_status();
+        if (status != KIMKV_OK) return status;
+        first += jobs;
     }
-    return launch_status();
+    return KIMKV_OK;
 }
 
 kimkv_status kimkv_gather(const kimkv_storage* storage, const kimkv_block_desc* device_descriptors,

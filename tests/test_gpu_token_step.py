@@ -809,6 +809,16 @@ def test_logits_repeated_biases_add_up_in_order(dev):
         assert np.array_equal(got.out[i], want)
 
 
+def test_logits_long_lists_and_wide_rows(dev):
+    """Histories and bias lists longer than a block holds at once, rows in slices of every size."""
+    for n, vocab, history, biases in ((3, 4093, 4096, 1024), (3, 4094, 4097, 1025), (2, 9001, 13000, 2500), (70, 130001, 5000, 1100)):
+        print(f"logits lists {n} {vocab} {history} {biases}", flush=True)
+        rng = np.random.default_rng(vocab)
+        rows = (3 * rng.standard_normal((n, vocab), dtype=np.float32)).astype(np.float32)
+        rules = [_rule(rng, vocab, history - i, biases - i if i < 3 else i, i % 2 == 1, 1.0 + 0.01 * i, 0.1, 0.05) for i in range(n)]
+        _check_logits(rows, rules, _Logits(dev, rows, rules))
+
+
 def test_logits_listed_tokens_past_the_vocabulary(dev):
     vocab = 100
     rng = np.random.default_rng(1)
