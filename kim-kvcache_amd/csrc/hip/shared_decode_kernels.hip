@@ -620,12 +620,14 @@ struct TableFlags {
     uint32_t first;
 };
 
-// The entry that holds group threadIdx.x of keys begin.. in a table as promotion
-// leaves it: full extent pages of 64 tokens, then micro pages of 8.
+// The entry that holds group threadIdx.x of keys begin.. in a table of full
+// extent pages of 64 tokens, then micro pages of 8; its length tells how many
+// there are of each.
 __device__ inline kimkv_block_desc guessed_entry(const kimkv_decode_item& table, uint32_t begin)
 {
     uint32_t const t = begin + 8 * threadIdx.x;
-    uint32_t const extents = table.token_count / 64;
+    uint32_t const micro = (table.token_count + 7) / 8;   // entries without an extent page, which saves seven
+    uint32_t const extents = micro > table.descriptor_count ? (micro - table.descriptor_count) / 7 : 0;
     uint32_t const i = t / 64 < extents ? t / 64 : extents + (t - 64 * extents) / 8;
     return table.descriptors[min(i, table.descriptor_count - 1)];
 }
@@ -988,24 +990,26 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
 constexpr uint32_t kShareBlock = 64;     // tokens: a shared prefix is cut to whole blocks
 
 // What a unit costs its compute unit, in nanoseconds, as measured: the chain of
-// reads in front of a unit and the merge and stores behind it; the bytes that
-// a compute unit streams (45 a nanosecond when not all of them do); the steps
-// of a wave when the loads' latency is all there is; the arithmetic of many
-// columns.  And what the bytes of all units take, whoever reads them.
+// reads in front of a unit and the merge and stores behind it (6.2 to 7.0 us
+// for a few tokens); the bytes that a compute unit streams (40 a nanosecond);
+// the steps of a wave when the loads' latency is all there is; the arithmetic
+// of many columns (25.7 and 71.7 us for 2048 and 8192 tokens of 64 columns at
+// D = 64, 17.2 and 21.0 for 1024 and 1408 of 32 at D = 128).  And what the
+// bytes of all units take, whoever reads them.
 struct UnitCost {
     uint32_t D;
-    static constexpr double kStart = 5500;
+    static constexpr double kStart = 6500;
     static constexpr double kMergeLaunch = 5000;
     static constexpr double kBytes = 5500;   // HBM's, a nanosecond
     // `split` waves share a head's tokens.
     double own(uint32_t heads, uint32_t split, uint32_t tokens) const
     {
         double const steps = std::ceil(std::ceil(tokens / static_cast<double>(split)) * D / 64 / 64);
-        return kStart + std::max(5.5 * D / 64 * heads * tokens, 700.0 * steps);
+        return kStart + std::max(6.0 * D / 64 * heads * tokens, 700.0 * steps);
     }
     double prefix(uint32_t blocks, uint32_t tokens) const
     {
-        return kStart + 600.0 * blocks + std::max(4.5, 1.8 * blocks) * D / 64 * tokens;
+        return kStart + 600.0 * blocks + std::max(4.9, 1.87 * blocks) * D / 64 * tokens;
     }
     double bytes(uint32_t heads, uint32_t tokens) const { return 4.0 * D * heads * tokens; }
 };
@@ -1093,11 +1097,13 @@ struct Shape {
     uint32_t lane_count;
 };
 
-// How a batch is cut: KV heads of a unit of a lane's own tokens, the cost that
-// no unit's pieces go far past, and what that comes to.
+// How a batch is cut: KV heads of a unit of a lane's own tokens, the costs
+// that pieces of prefixes and of lanes' own tokens do not go far past, and what
+// that comes to.
 struct Cut {
     uint32_t heads{1};
     double share{0};
+    double own_share{0};
     double time{0};
 };
 
@@ -1114,27 +1120,35 @@ void each_piece(Shape const& s, Work const& work, Cut const& cut, PrefixFn&& pre
         uint32_t const own = s.tokens[i] - work.shared[i];
         if (own == 0) continue;
         double const whole = cost.own(std::min(cut.heads, s.H), split, own) - UnitCost::kStart;
-        own_piece(i, own, piece_tokens(own, whole / std::max(1.0, cut.share - UnitCost::kStart)));
+        own_piece(i, own, piece_tokens(own, whole / std::max(1.0, cut.own_share - UnitCost::kStart)));
     }
 }
 
-// The time of a cut: of its longest unit, or of all of them where there are
-// more than compute units, whose gaps the smallest fill; and of the merge
-// where a lane has several parts.
+// The time of a cut: units go to compute units as these come free, the costliest
+// first, so one starts no later than when the costlier ones' work, spread
+// evenly, is done (costs within an eighth of each other count as equal); no less
+// than what their bytes take; and the merge where a lane has several parts.
 double cut_time(Shape const& s, Work const& work, Cut const& cut)
 {
     UnitCost const cost{s.D};
-    double total = 0;
-    double longest = 0;
-    double shortest = 1e30;
+    constexpr int kLevels = 64;   // 8 an octave from kStart on
+    struct Level {
+        double total{0};
+        double longest{0};
+        uint64_t units{0};
+    };
+    Level levels[kLevels];
     double bytes = 0;
-    uint64_t units = 0;
     bool merged = !work.prefixes.empty();
     auto add = [&](double each, uint64_t n) {
-        units += n;
-        total += each * static_cast<double>(n);
-        longest = std::max(longest, each);
-        shortest = std::min(shortest, each);
+        // The exponent and the first three bits behind the leading one.
+        auto const ratio = static_cast<float>(each / UnitCost::kStart);
+        uint32_t bits;
+        std::memcpy(&bits, &ratio, sizeof bits);
+        Level& level = levels[std::min(kLevels - 1, std::max(0, static_cast<int>(bits >> 20) - (127 << 3)))];
+        level.total += each * static_cast<double>(n);
+        level.longest = std::max(level.longest, each);
+        level.units += n;
     };
     each_piece(
         s, work, cut,
@@ -1149,13 +1163,23 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
             merged = merged || pieces > 1;
             bytes += cost.bytes(s.H, own);
         });
-    double const units_time = units <= s.compute_units ? longest : std::max(longest, total / s.compute_units) + shortest;
-    double const time = std::max(units_time, UnitCost::kStart + bytes / UnitCost::kBytes);
+    double time = UnitCost::kStart + bytes / UnitCost::kBytes;
+    double before = 0;
+    uint64_t units = 0;
+    for (int i = kLevels - 1; i >= 0; --i) {
+        Level const& level = levels[i];
+        if (level.units == 0) continue;
+        units += level.units;
+        before += level.total;
+        double const start = units <= s.compute_units ? 0.0 : (before - level.longest) / s.compute_units;
+        time = std::max(time, start + level.longest);
+    }
     return time + (merged ? UnitCost::kMergeLaunch : 0.0);
 }
 
 // The best of a few cuts: pieces of a few sizes around an equal share for each
-// compute unit, and whole ones.
+// compute unit, and whole ones; lanes' own tokens in pieces alike, or smaller
+// ones, which fill the end behind long pieces of prefixes.
 Cut best_cut(Shape const& s, Work const& work)
 {
     UnitCost const cost{s.D};
@@ -1165,9 +1189,11 @@ Cut best_cut(Shape const& s, Work const& work)
     while (heads < kWaves && heads < s.H) heads *= 2;
     uint64_t own_units = 0;
     double total = 0;
+    uint32_t longest_own = 0;
     for (uint32_t i = 0; i < s.lane_count; ++i) {
         uint32_t const own = s.tokens[i] - work.shared[i];
         if (own == 0) continue;
+        longest_own = std::max(longest_own, own);
         own_units += static_cast<uint64_t>((s.H + heads - 1) / heads) * ((s.G + 15) / 16);
         total += cost.own(s.H, kWaves, own) * ((s.G + 15) / 16);
     }
@@ -1180,10 +1206,16 @@ Cut best_cut(Shape const& s, Work const& work)
     }
     double const even = total / s.compute_units + UnitCost::kStart;
     Cut best;
-    for (double const share : {1e12, 0.7 * even, 0.85 * even, even, 1.15 * even, 1.35 * even, 1.7 * even, 2.2 * even}) {
-        Cut c{heads, std::max(share, UnitCost::kStart + 1500), 0};
-        c.time = cut_time(s, work, c);
-        if (best.share == 0 || c.time < best.time) best = c;
+    double const longest = cost.own(std::min(heads, s.H), kWaves / heads, longest_own);
+    for (double const part : {1.0, 0.35, 0.15}) {
+        for (double const share : {1e12, 0.7 * even, 0.85 * even, even, 1.15 * even, 1.35 * even, 1.7 * even, 2.2 * even}) {
+            double const own_share = share < 1e12 ? part * share : part < 1.0 ? part * even : share;
+            if (part < 1.0 && longest <= own_share) continue;   // cuts nothing more
+            Cut c{heads, std::max(share, UnitCost::kStart + 1500), std::max(own_share, UnitCost::kStart + 1500), 0};
+            c.time = cut_time(s, work, c);
+            if (best.share == 0 || c.time < best.time) best = c;
+        }
+        if (work.prefixes.empty()) break;   // own tokens alone: the shares say it all
     }
     return best;
 }

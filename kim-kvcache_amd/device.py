@@ -623,13 +623,14 @@ def shared_decode_plan(kv_heads: int, head_dim: int, query_heads: int, compute_u
     plan = SharedPlan()
     args = (kv_heads, head_dim, query_heads, compute_units, counts.ctypes.data_as(ctypes.c_void_p), len(counts), shared,
             len(groups))
-    status = lib().kimkv_shared_decode_plan(*args, None, 0, ctypes.byref(plan))
-    if status != OK and not plan.entry_bytes:
-        check(status, "shared_decode_plan")
-    entries = np.zeros(plan.entry_bytes, dtype=np.uint8)
-    check(lib().kimkv_shared_decode_plan(*args, entries.ctypes.data_as(ctypes.c_void_p), plan.entry_bytes,
-                                         ctypes.byref(plan)), "shared_decode_plan")
-    return entries, plan
+    # Room for the usual plan: a record a lane, a few units each and a few for each compute unit.
+    entries = np.empty(32 * (4 * len(counts) + 4 * (compute_units or 256)), dtype=np.uint8)
+    status = lib().kimkv_shared_decode_plan(*args, entries.ctypes.data_as(ctypes.c_void_p), len(entries), ctypes.byref(plan))
+    if status != OK and plan.entry_bytes > len(entries):
+        entries = np.empty(plan.entry_bytes, dtype=np.uint8)
+        status = lib().kimkv_shared_decode_plan(*args, entries.ctypes.data_as(ctypes.c_void_p), len(entries), ctypes.byref(plan))
+    check(status, "shared_decode_plan")
+    return entries[:plan.entry_bytes], plan
 
 
 def table_cache_bytes(total_chunks: int, chunk_tokens: int) -> int:

@@ -371,6 +371,8 @@ BATCHES = {
     "many": ([1030 + 7 * i for i in range(33)], [(0, 33, 1030)]),
     "more": ([400 + i % 50 for i in range(70)], [(0, 70, 390)]),
     "two groups and alone": ([700, 701, 800, 2100, 2070, 2300, 90, 2111], [(0, 3, 690), (3, 3, 2065)]),
+    "long prefix is all": ([2048, 2048, 2500, 40, 0], [(0, 3, 2048), (3, 2, 40)]),
+    "shorter lane in a long group": ([5000, 3001, 5003], [(0, 3, 4990)]),
     "long": ([5200, 5000, 4990, 9000], [(0, 3, 4985)]),
 }
 
@@ -585,7 +587,7 @@ def test_shared_decode_faults(dev):
 
 def test_shared_decode_bad_entries(dev):
     """Entries that name what is not there are reported, not run: every index is checked against the launch's buffers."""
-    counts, groups = [700, 710, 720], [(0, 3, 690)]
+    counts, groups = [2700, 2710, 2720], [(0, 3, 2690)]
     for field, value in (("table_lane", 3), ("lane", 3), ("col0", 4), ("cols", 13), ("lane", 0xFFFFFFFF), ("col0", 0xFFFFFFFF), ("cols", 0xFFFFFFFF),
                          ("end", 1 << 20), ("begin", 1 << 20), ("slot", 1 << 20), ("slot", 0xFFFFFFFF), ("head", 2), ("heads", 3), ("heads", 0)):
         print(f"shared entry {field}={value}", flush=True)
@@ -617,7 +619,7 @@ def test_shared_decode_bad_entries(dev):
 
 
 def test_shared_decode_refusals(dev):
-    b = _Batch(dev, 2, 64, 4, [700, 710, 720], [(0, 3, 690)])
+    b = _Batch(dev, 2, 64, 4, [2700, 2710, 2720], [(0, 3, 2690)])
     b.place()
     b.plan(1)
     lib = dev.lib()
