@@ -608,7 +608,8 @@ typedef struct kimkv_shared_plan {
  * rest of each lane is read through the lane's own table.  Fills entries[0 ..
  * plan->entry_bytes) for upload; KIMKV_INVALID_ARGUMENT when capacity is too
  * small (plan->entry_bytes then holds the size needed; entries may be NULL
- * with capacity 0), or for groups that overlap or leave the batch. */
+ * with capacity 0), for groups that overlap or leave the batch, or for lanes of
+ * 2^31 tokens or more. */
 kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint32_t query_heads,
                                       uint32_t compute_units, const uint32_t* token_counts, uint32_t lane_count,
                                       const kimkv_shared_group* groups, uint32_t group_count, void* entries,
@@ -622,7 +623,7 @@ kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint
  * of device memory, contents ignored, not shared with a launch that may
  * overlap this one.  Lanes of one group name the same layer.  A lane of no
  * tokens is skipped (its output is not written); a lane whose item is invalid
- * or not as planned, or whose group's first lane is, sets
+ * or not as planned, or whose prefix is read through such a lane's table, sets
  * KIMKV_FAULT_DECODE_ITEM and is skipped.  Results as
  * kimkv_paged_decode_batch's to the decode tolerance, the same for every run
  * of one plan.  The storage's device is the current one. */

@@ -299,9 +299,19 @@ __global__ __launch_bounds__(kBlock) void append_kernel(PoolView P, const kimkv_
 
 // ---------------------------------------------------------------------------
 // Rotated append: block = (job, 8-token group of its page), q | k | v rows in,
-// rotated q rows, rotated page K and page V^T out.  The groups of a page are
-// neighbours on one XCD: four of them write the 16-byte quarters of V^T's
-// 64-byte runs, which meet in its L2.
+// rotated q rows, rotated page K and page V^T out: every byte once, where the
+// split, the copy into pages and the rotation apart move K and V twice.
+//
+// Page p's groups are neighbours on XCD p % 8: four of them write the 16-byte
+// quarters of V^T's 64-byte runs, which meet in its L2 (in the order of the
+// grid's dimensions, which spreads them, four prompts of 4096 tokens and 48
+// heads of 128 took 113 us, so 104; contiguous runs of pages for an XCD leave
+// the XCDs of a mixed batch unlike loads, 9.7 for 8.2 us).  Rows of q and K
+// are whole lines and are stored past the caches (95 us); V^T is not (152 us
+// when its quarters go to memory one by one).  Bound by HBM for prompts: 94 us
+// for 369 MB, 3.9 TB/s, where a large copy reaches 4.8; by the launch and the
+// chain of job, angle, row and store for a token step, 4.8 us for 4 or 128
+// lanes.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kRopeGroup = 8;          // page tokens a block takes
 constexpr uint32_t kMaxRopePairs = 256;
@@ -972,8 +982,8 @@ kimkv_status kimkv_append_rope_batch(const kimkv_storage* storage, const kimkv_a
     a.head_items = divisor(head_items);
     a.items = divisor((H + (q_out != nullptr ? query_heads : 0)) * head_items);
     a.groups = divisor(groups);
-    // A launch takes fewer than 2^32 threads.
-    uint32_t const most_jobs = 0xFFFFFFu / groups;
+    // A launch takes fewer than 2^32 threads, and a block for each of eight jobs or none.
+    uint32_t const most_jobs = 0xFFFFFFu / groups / kXcds * kXcds;
     for (uint32_t first = 0; first < job_count;) {
         uint32_t const jobs = job_count - first < most_jobs ? job_count - first : most_jobs;
         a.jobs = device_jobs + first;

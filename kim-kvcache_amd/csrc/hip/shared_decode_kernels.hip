@@ -677,11 +677,21 @@ __device__ bool build_groups(const PoolView& P, const kimkv_decode_item& table, 
 }
 
 // ---- direct units ---------------------------------------------------------------
-// At most 16 columns.  The waves split the unit's heads, then its tokens, and
-// read K and V^T straight into operand registers, two steps in flight: the
-// work of lanes' own tokens and of groups too small to share a tile.  Bound by
-// the bytes and, for short units, by the chain of reads in front of them.
-
+// The waves split the unit's heads, then its tokens, and read K and V^T
+// straight into operand registers, two steps in flight; at the end they merge
+// their parts through LDS.  Each wave holds all of the unit's columns (up to
+// 64 of 64 dims, 32 of 128), so every byte enters the compute unit once and
+// nothing is staged.
+//
+// Times of a unit, alone on its compute unit: about 1.1 us until its table is
+// known, 1.2 for queries, 0.7 for the pages, 2.4 for the merge and its stores
+// (instructions that come from memory once a launch).  Between them 1 us a
+// 64-token step of one block of columns is the loads' latency; many columns
+// are bound by the weights: 57 cycles for 64 scores a SIMD, of which 44 remain
+// without loads (8192 tokens x 64 columns x 64 dims in 71 us, 0.48 PFLOP/s over
+// 256 units).  Tiles of 64 keys staged in LDS for 256 columns of 8 waves
+// measured 153 us where this took 173 (128 lanes x 65536 tokens), and 62 where
+// this took 53 (16384): the barriers cost what the fewer loads save.
 template <uint32_t kDim, uint32_t kCB>
 struct DirectRows {
     static constexpr uint32_t kRow = kDim + 4;   // o, m, l, pad
@@ -891,7 +901,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     // The entries lie in the caller's memory: nothing outside the launch's buffers is touched, whatever they hold.
     uint32_t rest;
     uint64_t const last = div_mod(u.col0 + (u.cols - 1), a.group, &rest);   // lane of the last column, from u.lane
-    if (u.cols - 1 > 0xFFFFFFFFu - u.col0 || u.table_lane >= a.lane_count || u.lane + last >= a.lane_count || u.heads == 0
+    if (((u.col0 | (u.cols - 1)) >> 30) != 0 || u.table_lane >= a.lane_count || u.lane + last >= a.lane_count || u.heads == 0
         || u.head + u.heads > P.heads || u.begin >= u.end || ((u.kind & kSingle) == 0 && u.slot + last >= a.slot_count)) {
         report_fault(P, KIMKV_FAULT_DECODE_ITEM);
         return;
@@ -1126,7 +1136,8 @@ void each_piece(Shape const& s, Work const& work, Cut const& cut, PrefixFn&& pre
 
 // The time of a cut: units go to compute units as these come free, the costliest
 // first, so one starts no later than when the costlier ones' work, spread
-// evenly, is done (costs within an eighth of each other count as equal); no less
+// evenly, is done, and the whole takes no longer than rounds of one unit on each
+// compute unit (costs within an eighth of each other count as equal); no less
 // than what their bytes take; and the merge where a lane has several parts.
 double cut_time(Shape const& s, Work const& work, Cut const& cut)
 {
@@ -1163,17 +1174,21 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
             merged = merged || pieces > 1;
             bytes += cost.bytes(s.H, own);
         });
-    double time = UnitCost::kStart + bytes / UnitCost::kBytes;
+    double spread = 0;
+    double rounds = 0;
     double before = 0;
     uint64_t units = 0;
+    auto const rounds_of = [&](uint64_t n) { return (n + s.compute_units - 1) / s.compute_units; };
     for (int i = kLevels - 1; i >= 0; --i) {
         Level const& level = levels[i];
         if (level.units == 0) continue;
+        rounds += static_cast<double>(rounds_of(units + level.units) - rounds_of(units)) * level.longest;
         units += level.units;
         before += level.total;
         double const start = units <= s.compute_units ? 0.0 : (before - level.longest) / s.compute_units;
-        time = std::max(time, start + level.longest);
+        spread = std::max(spread, start + level.longest);
     }
+    double const time = std::max(std::min(spread, rounds), UnitCost::kStart + bytes / UnitCost::kBytes);
     return time + (merged ? UnitCost::kMergeLaunch : 0.0);
 }
 
@@ -1225,6 +1240,9 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
 {
     Shape const shape{H, QH / H, D, compute_units, tokens, lane_count};
     UnitCost const cost{D};
+    for (uint32_t i = 0; i < lane_count; ++i) {
+        if (tokens[i] >> 31 != 0) return false;
+    }
     std::vector<uint8_t> grouped(lane_count, 0);
     Work apart;
     apart.shared.assign(lane_count, 0);
@@ -1241,7 +1259,7 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
         prefix = prefix / kShareBlock * kShareBlock;
         if (group.lane_count < 2 || prefix == 0) continue;
         uint64_t const columns = static_cast<uint64_t>(group.lane_count) * shape.G;
-        if (columns > 0x7FFFFFFFu) return false;
+        if (columns >> 30 != 0) return false;
         Work::Prefix p{group.first_lane, group.lane_count, prefix, 1, 0};
         while (p.blocks < most_blocks(D) && 16 * p.blocks < columns) p.blocks *= 2;
         p.tiles = (columns + 16 * p.blocks - 1) / (16 * p.blocks);

@@ -41,8 +41,8 @@ def test_plan_covers_every_key_once(kimkv, heads, dim, group):
         prefixes = rng.integers(1, 5000, 2)
         counts = [int(prefixes[int(i >= cut)] + rng.integers(0, 900)) for i in range(n)]
         cases.append((counts, [(0, cut, int(prefixes[0])), (cut, n - cut, int(prefixes[1]))]))
-    for counts, groups in cases:
-        entries, plan = d.shared_decode_plan(heads, dim, heads * group, 256, counts, groups)
+    for compute_units, (counts, groups) in [(n, c) for n in (256, 3) for c in cases]:
+        entries, plan = d.shared_decode_plan(heads, dim, heads * group, compute_units, counts, groups)
         assert plan.entry_bytes == len(entries) == plan.unit_count * 32 + len(counts) * 32
         units, lanes = split_entries(entries, plan)
         assert (plan.kv_heads, plan.head_dim, plan.query_heads, plan.lane_count) == (heads, dim, heads * group, len(counts))
@@ -100,6 +100,10 @@ def test_plan_refusals(kimkv):
         assert plan.entry_bytes == 0, bad
     assert lib.kimkv_shared_decode_plan(4, 64, 32, 256, ptr, 3, None, 1, None, 0, ctypes.byref(plan)) == d.INVALID_ARGUMENT
     assert lib.kimkv_shared_decode_plan(4, 64, 32, 256, ptr, 3, None, 0, None, 0, None) == d.INVALID_ARGUMENT
+    for tokens in (1 << 31, 0xFFFFFFFF):
+        counts[1] = tokens
+        assert status() == d.INVALID_ARGUMENT and plan.entry_bytes == 0
+    counts[1] = 200
     # Too small: the size comes back, and nothing is written past it.
     assert status() == d.INVALID_ARGUMENT and plan.entry_bytes > 0
     need = plan.entry_bytes
