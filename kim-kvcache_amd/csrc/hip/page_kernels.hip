@@ -302,16 +302,15 @@ __global__ __launch_bounds__(kBlock) void append_kernel(PoolView P, const kimkv_
 // rotated q rows, rotated page K and page V^T out: every byte once, where the
 // split, the copy into pages and the rotation apart move K and V twice.
 //
-// Page p's groups are neighbours on XCD p % 8: four of them write the 16-byte
-// quarters of V^T's 64-byte runs, which meet in its L2 (in the order of the
-// grid's dimensions, which spreads them, four prompts of 4096 tokens and 48
-// heads of 128 took 113 us, so 104; contiguous runs of pages for an XCD leave
-// the XCDs of a mixed batch unlike loads, 9.7 for 8.2 us).  Rows of q and K
-// are whole lines and are stored past the caches (95 us); V^T is not (152 us
-// when its quarters go to memory one by one).  Bound by HBM for prompts: 94 us
-// for 369 MB, 3.9 TB/s, where a large copy reaches 4.8; by the launch and the
-// chain of job, angle, row and store for a token step, 4.8 us for 4 or 128
-// lanes.
+// A job's groups are neighbours on one XCD, and jobs go round the XCDs: four
+// groups write the 16-byte quarters of V^T's 64-byte runs, which meet in that
+// L2.  15000 rows of 48 heads of 128 took 113 us in the order of the grid's
+// dimensions and 104 so; contiguous runs of jobs for an XCD leave the XCDs of a
+// mixed batch unlike loads (9.7 for 8.2 us).  Rows of q and K are whole lines
+// and are stored past the caches (95 us); V^T is not (152 us when its quarters
+// go to memory one by one).  Bound by HBM for prompts, 94 us for those 369 MB,
+// 3.9 TB/s where a large copy reaches 4.8; by the launch and the chain of job,
+// angle, row and store for a token step, 4.8 us for 4 or 128 lanes.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kRopeGroup = 8;          // page tokens a block takes
 constexpr uint32_t kMaxRopePairs = 256;
