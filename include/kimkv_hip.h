@@ -595,7 +595,7 @@ typedef struct kimkv_shared_plan {
     uint32_t unit_count;
     uint32_t slot_count;
     uint32_t merge_lanes;
-    uint32_t reserved;
+    uint32_t merge_split;
 } kimkv_shared_plan;
 
 /* Plans one layer's decode attention of a batch whose lanes share prefixes

@@ -849,7 +849,7 @@ __device__ bool unit_direct(const PoolView& P, const SharedArgs& a, const Shared
         uint32_t const hd = i / kQuads / u.cols;
         ColumnOut const out = outs[c];
         if (out.ok == 0) continue;
-        // All eight waves' rows are read at once; those of another head count for nothing.
+        // All the waves' rows are read at once; those of another head count for nothing.
         float m[kWaves];
         float M = -INFINITY;
 #pragma unroll
@@ -933,14 +933,17 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 }
 
 // Merges the lanes' parts, four dims a thread (one where the head dim is no
-// multiple of 4).  Bound by the parts' bytes, which the launch before has just
-// written; kBatch parts are in flight together.
+// multiple of 4), the parts of a row over `split` neighbouring threads where
+// they are many.  Bound by the parts' bytes, which the launch before has just
+// written, and for many by the rounds of reads (8 lanes of 8192 tokens in 32
+// pieces: 23.4 us a pass with a thread a row, 19.5 so); kMergeBatch parts of a
+// thread are in flight together.
 constexpr unsigned kMergeBlock = 256;
+constexpr uint32_t kMergeBatch = 8;
 
 template <uint32_t kWidth>
-__global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, SharedArgs a)
+__global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, SharedArgs a, uint32_t split)
 {
-    constexpr uint32_t kBatch = 8;
     typedef float vec_t __attribute__((ext_vector_type(kWidth)));
     uint32_t const lane = blockIdx.x;
     SharedLane const rec = a.lanes[lane];
@@ -956,42 +959,61 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
     bool const ok = lane_ok(P, a, lane);   // a unit reported it; not waited for before the parts are read
     uint16_t* const output = a.items[lane].output;
     uint32_t const per_row = D / kWidth;
-    for (uint32_t x = blockIdx.y * kMergeBlock + threadIdx.x; x < a.QH * per_row; x += gridDim.y * kMergeBlock) {
+    uint32_t const mine = threadIdx.x & (split - 1);
+    uint32_t const at_once = kMergeBlock / split;
+    for (uint32_t x0 = blockIdx.y * at_once; x0 < a.QH * per_row; x0 += gridDim.y * at_once) {
+        uint32_t const x = min(x0 + threadIdx.x / split, a.QH * per_row - 1);   // past the end: once again
         uint32_t const q = x / per_row;
         uint32_t const d = (x - q * per_row) * kWidth;
         float M = -INFINITY;
         float l = 0.0f;
         vec_t o = {};
-        for (uint32_t i0 = 0; i0 < parts; i0 += kBatch) {
-            float2 ml[kBatch];
-            vec_t row[kBatch];
+        for (uint32_t i0 = 0; i0 < parts; i0 += kMergeBatch * split) {
+            float2 ml[kMergeBatch];
+            vec_t row[kMergeBatch];
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) {
-                uint32_t const i = min(i0 + j, parts - 1);
+            for (uint32_t j = 0; j < kMergeBatch; ++j) {
+                uint32_t const n = i0 + j * split + mine;
+                uint32_t const i = min(n, parts - 1);
                 uint32_t const slot = i < rec.prefix_count ? rec.prefix_slot + i * rec.prefix_stride
                                                            : rec.tail_slot + (i - rec.prefix_count);
                 uint64_t const at = static_cast<uint64_t>(slot) * a.QH + q;
                 ml[j] = a.parts.ml[at];
                 row[j] = *reinterpret_cast<const vec_t*>(a.parts.o + at * D + d);
-                if (i0 + j >= parts) ml[j].x = -INFINITY;
+                if (n >= parts) ml[j].x = -INFINITY;
             }
             float m_new = M;
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) m_new = fmaxf(m_new, ml[j].x);
+            for (uint32_t j = 0; j < kMergeBatch; ++j) m_new = fmaxf(m_new, ml[j].x);
             float const c = M == -INFINITY ? 0.0f : exp2f(M - m_new);
             M = m_new;
             o *= c;
             l *= c;
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) {
+            for (uint32_t j = 0; j < kMergeBatch; ++j) {
                 float const f = ml[j].x == -INFINITY ? 0.0f : exp2f(ml[j].x - M);
                 if (f == 0.0f) continue;   // whatever V made of it, as for a key of weight 0
                 o += f * row[j];
                 l += f * ml[j].y;
             }
         }
-        if (!ok) return;
-        store_outputs<kWidth>(output + static_cast<uint64_t>(q) * D + d, o, l);
+        for (uint32_t step = 1; step < split; step *= 2) {
+            float const other = __shfl_xor(M, static_cast<int>(step));
+            float const m_new = fmaxf(M, other);
+            float const f = M == -INFINITY ? 0.0f : exp2f(M - m_new);
+            M = m_new;
+            // A side of no weight hands over nothing, whatever it holds.
+            l = f == 0.0f ? 0.0f : f * l;
+            l += __shfl_xor(l, static_cast<int>(step));
+#pragma unroll
+            for (uint32_t k = 0; k < kWidth; ++k) {
+                float const v = f == 0.0f ? 0.0f : f * o[k];
+                o[k] = v + __shfl_xor(v, static_cast<int>(step));
+            }
+        }
+        if (ok && mine == 0 && x0 + threadIdx.x / split < a.QH * per_row) {
+            store_outputs<kWidth>(output + static_cast<uint64_t>(q) * D + d, o, l);
+        }
     }
 }
 
@@ -1004,13 +1026,16 @@ constexpr uint32_t kShareBlock = 64;     // tokens: a shared prefix is cut to wh
 // for a few tokens); the bytes that a compute unit streams (40 a nanosecond);
 // the steps of a wave when the loads' latency is all there is; the arithmetic
 // of many columns (25.7 and 71.7 us for 2048 and 8192 tokens of 64 columns at
-// D = 64, 17.2 and 21.0 for 1024 and 1408 of 32 at D = 128).  And what the
-// bytes of all units take, whoever reads them.
+// D = 64, 17.2 and 21.0 for 1024 and 1408 of 32 at D = 128).  What the bytes of
+// all units take, whoever reads them; and the merge: its launch, a round of
+// reads, and what the parts take to write and read.
 struct UnitCost {
     uint32_t D;
     static constexpr double kStart = 6500;
-    static constexpr double kMergeLaunch = 5000;
-    static constexpr double kBytes = 5500;   // HBM's, a nanosecond
+    static constexpr double kBytes = 5500;        // HBM's, a nanosecond
+    static constexpr double kMergeLaunch = 4000;
+    static constexpr double kMergeRound = 1000;
+    static constexpr double kPartBytes = 4000;    // a nanosecond
     // `split` waves share a head's tokens.
     double own(uint32_t heads, uint32_t split, uint32_t tokens) const
     {
@@ -1024,12 +1049,21 @@ struct UnitCost {
     double bytes(uint32_t heads, uint32_t tokens) const { return 4.0 * D * heads * tokens; }
 };
 
+// Threads that share the merge of a row of so many parts.
+uint32_t merge_split(uint64_t parts)
+{
+    uint32_t split = 1;
+    while (split < 8 && parts > kMergeBatch * split) split *= 2;
+    return split;
+}
+
 struct Planned {
     std::vector<SharedUnit> units;
     std::vector<double> cost;
     std::vector<SharedLane> lanes;
     uint64_t slots{0};
     uint32_t merge_lanes{0};
+    uint32_t merge_parts{0};   // of the lane that has most
 };
 
 uint64_t align16(uint64_t n) { return (n + 15) / 16 * 16; }
@@ -1150,7 +1184,9 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
     };
     Level levels[kLevels];
     double bytes = 0;
-    bool merged = !work.prefixes.empty();
+    uint64_t parts = 0;        // of all lanes
+    uint64_t prefix_most = 0;  // of a lane
+    uint64_t own_most = 0;
     auto add = [&](double each, uint64_t n) {
         // The exponent and the first three bits behind the leading one.
         auto const ratio = static_cast<float>(each / UnitCost::kStart);
@@ -1166,12 +1202,16 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
         [&](Work::Prefix const& p, uint32_t piece) {
             add(cost.prefix(p.blocks, std::min(piece, p.tokens)), (p.tokens + piece - 1ull) / piece * s.H * p.tiles);
             bytes += cost.bytes(s.H, p.tokens);
+            uint64_t const pieces = (p.tokens + piece - 1ull) / piece;
+            parts += pieces * p.lanes;
+            prefix_most = std::max(prefix_most, pieces);
         },
         [&](uint32_t, uint32_t own, uint32_t piece) {
             uint64_t const pieces = (own + piece - 1ull) / piece;
             add(cost.own(std::min(cut.heads, s.H), kWaves / cut.heads, std::min(piece, own)),
                 pieces * ((s.H + cut.heads - 1) / cut.heads) * ((s.G + 15) / 16));
-            merged = merged || pieces > 1;
+            parts += pieces;
+            own_most = std::max(own_most, pieces);
             bytes += cost.bytes(s.H, own);
         });
     double spread = 0;
@@ -1189,7 +1229,11 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
         spread = std::max(spread, start + level.longest);
     }
     double const time = std::max(std::min(spread, rounds), UnitCost::kStart + bytes / UnitCost::kBytes);
-    return time + (merged ? UnitCost::kMergeLaunch : 0.0);
+    if (prefix_most == 0 && own_most <= 1) return time;
+    uint64_t const most = prefix_most + own_most;
+    double const merge_rounds = std::ceil(static_cast<double>(most) / (kMergeBatch * merge_split(most)));
+    return time + UnitCost::kMergeLaunch + UnitCost::kMergeRound * merge_rounds
+        + 4.0 * static_cast<double>(parts) * s.H * s.G * s.D / UnitCost::kPartBytes;
 }
 
 // The best of a few cuts: pieces of a few sizes around an equal share for each
@@ -1198,8 +1242,8 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
 Cut best_cut(Shape const& s, Work const& work)
 {
     UnitCost const cost{s.D};
-    // KV heads of a unit of a lane's own tokens: all that eight waves take,
-    // fewer, with more waves for each, while the units are few.
+    // KV heads of a unit of a lane's own tokens: one for each wave, fewer, with
+    // more waves for each, while the units are few.
     uint32_t heads = 1;
     while (heads < kWaves && heads < s.H) heads *= 2;
     uint64_t own_units = 0;
@@ -1338,6 +1382,7 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
     for (SharedLane& lane : out.lanes) {
         lane.merged = lane.prefix_count + lane.tail_count != 0 ? 1 : 0;
         out.merge_lanes += lane.merged;
+        out.merge_parts = std::max(out.merge_parts, lane.prefix_count + lane.tail_count);
     }
     place_units(out, compute_units);
     return true;
@@ -1380,6 +1425,7 @@ kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint
         plan->unit_count = static_cast<uint32_t>(p.units.size());
         plan->slot_count = static_cast<uint32_t>(p.slots);
         plan->merge_lanes = p.merge_lanes;
+        plan->merge_split = merge_split(p.merge_parts);
         if (capacity < plan->entry_bytes || (plan->entry_bytes != 0 && entries == nullptr)) return KIMKV_INVALID_ARGUMENT;
         if (unit_bytes != 0) std::memcpy(entries, p.units.data(), unit_bytes);
         if (lane_bytes != 0) std::memcpy(static_cast<unsigned char*>(entries) + unit_bytes, p.lanes.data(), lane_bytes);
@@ -1402,7 +1448,8 @@ kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv
     if (plan->unit_count == 0) return KIMKV_OK;
     uint64_t const o_bytes = align16(parts_o_floats(plan->slot_count, plan->query_heads, D) * sizeof(float));
     if (device_items == nullptr || device_entries == nullptr || plan->lane_count == 0 || plan->query_heads == 0 || H == 0
-        || plan->query_heads % H != 0 || D > kMaxDim || plan->unit_count > 0x7FFFFFFFu
+        || plan->query_heads % H != 0 || D > kMaxDim || plan->merge_split == 0 || plan->merge_split > 8
+        || (plan->merge_split & (plan->merge_split - 1)) != 0 || plan->unit_count > 0x7FFFFFFFu
         || (reinterpret_cast<uintptr_t>(device_entries) & 15u) != 0
         || plan->entry_bytes != plan->unit_count * sizeof(SharedUnit) + plan->lane_count * sizeof(SharedLane)
         || plan->workspace_bytes != o_bytes + static_cast<uint64_t>(plan->slot_count) * plan->query_heads * sizeof(float2)
@@ -1432,10 +1479,10 @@ kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv
     kimkv_status const status = launch_status();
     if (status != KIMKV_OK || plan->merge_lanes == 0) return status;
     uint32_t const width = D % 4 == 0 ? 4 : 1;
-    uint32_t const blocks = ceil_div(static_cast<uint64_t>(plan->query_heads) * D / width, kMergeBlock);
+    uint32_t const blocks = ceil_div(static_cast<uint64_t>(plan->query_heads) * D / width * plan->merge_split, kMergeBlock);
     dim3 const grid(plan->lane_count, blocks < 65535u ? blocks : 65535u);
-    if (width == 4) shared_merge_kernel<4><<<grid, kMergeBlock, 0, s>>>(pv, a);
-    else shared_merge_kernel<1><<<grid, kMergeBlock, 0, s>>>(pv, a);
+    if (width == 4) shared_merge_kernel<4><<<grid, kMergeBlock, 0, s>>>(pv, a, plan->merge_split);
+    else shared_merge_kernel<1><<<grid, kMergeBlock, 0, s>>>(pv, a, plan->merge_split);
     return launch_status();
 }
 

@@ -414,6 +414,20 @@ def test_shared_decode_every_kind(dev, heads, dim, lanes, kind, prefix):
     assert b.storage.faults() == (0, 0)
 
 
+@pytest.mark.parametrize("heads,dim,group", [(1, 64, 8), (2, 128, 3), (1, 30, 2), (1, 96, 16)])
+@pytest.mark.parametrize("units,split", [(24, 2), (36, 2), (64, 4), (512, 8), (2000, 8)])
+def test_shared_decode_many_parts(dev, heads, dim, group, units, split):
+    """Lanes cut into many parts, beside short ones, on a plan for a device with more compute units than this one."""
+    print(f"shared parts H={heads} D={dim} units={units}", flush=True)
+    b = _Batch(dev, heads, dim, group, [13000, 12500, 12460, 70, 5], [(0, 3, 12400)])
+    b.place()
+    b.plan(units)
+    assert b.p.merge_split >= split or dim == 30
+    b.launch()
+    b.check(b.outputs())
+    assert b.storage.faults() == (0, 0)
+
+
 @pytest.mark.parametrize("heads,dim,group", [(1, 64, 1), (3, 64, 5), (2, 96, 3), (1, 128, 40), (5, 64, 2), (2, 32, 4), (1, 8, 2), (2, 200, 1),
                                              (1, 256, 7), (2, 12, 3), (1, 64, 33)])
 def test_shared_decode_other_shapes(dev, heads, dim, group):
@@ -633,7 +647,7 @@ def test_shared_decode_refusals(dev):
     for bad in (dict(items=None), dict(entries=None), dict(work=None), dict(entries=b.entries_buf.ptr + 4), dict(work=b.work.ptr + 2052),
                 dict(kv_heads=4), dict(head_dim=128), dict(query_heads=16), dict(query_heads=7), dict(query_heads=0), dict(lane_count=2),
                 dict(lane_count=0), dict(unit_count=b.p.unit_count + 1), dict(slot_count=b.p.slot_count + 1), dict(entry_bytes=0),
-                dict(workspace_bytes=0)):
+                dict(workspace_bytes=0), dict(merge_split=0), dict(merge_split=3), dict(merge_split=16)):
         assert status(**bad) == dev.INVALID_ARGUMENT, bad
     assert lib.kimkv_shared_decode_batch(b.storage.h, None, None, None, None, None) == dev.INVALID_ARGUMENT
     other = dev.Storage(1, 4, 64, 8, 2)
