@@ -596,6 +596,8 @@ typedef struct kimkv_shared_plan {
     uint32_t slot_count;
     uint32_t merge_lanes;
     uint32_t merge_split;
+    uint32_t waves;
+    uint32_t reserved;
 } kimkv_shared_plan;
 
 /* Plans one layer's decode attention of a batch whose lanes share prefixes

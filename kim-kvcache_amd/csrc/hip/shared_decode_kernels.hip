@@ -31,8 +31,15 @@
 namespace kimkv {
 namespace {
 
-constexpr unsigned kBlock = 512;   // 8 waves
-constexpr unsigned kWaves = kBlock / kWave;
+// Workgroups of 8 waves, one a compute unit, or of 4, two a compute unit (256
+// registers a lane either way): the plan says which.  Two hide one's start and
+// end behind the other's keys, which short units gain by (lanes' own tokens;
+// 4 lanes of 500 tokens 10.4 and 9.2 us, eight groups of four 21.8 and 20.1);
+// one starts half as many units for the same keys, which long ones on many
+// columns gain by (64 lanes of 128 dims on 4100 tokens 35.2 and 38.9 us, 128
+// lanes on 16384 54.7 and 58.5).
+constexpr uint32_t kManyWaves = 8;
+constexpr uint32_t kFewWaves = 4;
 constexpr uint32_t kMaxDim = 256;
 
 // How a unit is computed.
@@ -284,6 +291,7 @@ __device__ void attend_rows_generic(const PoolView& P, const kimkv_decode_item& 
 }
 
 // Rows as the waves leave them in LDS for the workgroup's own merge.
+template <uint32_t kWaves>
 struct GenericLds {
     float o[kWaves][kRows][kMaxDim];
     float m[kWaves][kRows];
@@ -293,7 +301,8 @@ struct GenericLds {
 // The whole unit by the generic path.  A task is kRows columns of one KV head;
 // where there are fewer tasks than waves, the waves of a task take a part of
 // the tokens each.
-__device__ void unit_generic(const PoolView& P, const SharedArgs& a, const SharedUnit& u, GenericLds& lds)
+template <uint32_t kWaves>
+__device__ void unit_generic(const PoolView& P, const SharedArgs& a, const SharedUnit& u, GenericLds<kWaves>& lds)
 {
     uint32_t const tid = threadIdx.x;
     uint32_t const wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -332,7 +341,7 @@ __device__ void unit_generic(const PoolView& P, const SharedArgs& a, const Share
             }
         }
         __syncthreads();
-        for (uint32_t i = tid; i < at_once * kRows * D; i += kBlock) {
+        for (uint32_t i = tid; i < at_once * kRows * D; i += kWaves * kWave) {
             uint32_t const d = i % D;
             uint32_t const r = i / D % kRows;
             uint32_t const w = i / D / kRows * split;
@@ -612,8 +621,10 @@ __device__ inline bool columns_finish(Columns<kDim, kCB>& w)
 
 // ---- the unit's group table ---------------------------------------------------
 
-constexpr uint32_t kTableGroups = 512;   // 4096 keys: a longer unit is taken in segments of that
-constexpr uint32_t kSegment = kTableGroups * 8;
+// Groups of 8 keys that a workgroup resolves at once, one a thread: a longer
+// unit is taken in segments of that.
+template <uint32_t kWaves>
+constexpr uint32_t kTableGroups = kWaves * kWave;
 
 struct TableFlags {
     uint32_t generic;
@@ -636,13 +647,12 @@ __device__ inline kimkv_block_desc guessed_entry(const kimkv_decode_item& table,
 // threadIdx.x from `guess` (guessed_entry's) where every thread's is right,
 // else by searching.  False where the table does not keep the groups aligned
 // and whole: the unit then goes the generic path.  Called by every thread.
-template <uint32_t kDim>
+template <uint32_t kDim, uint32_t kWaves>
 __device__ bool build_groups(const PoolView& P, const kimkv_decode_item& table, uint32_t head, uint32_t begin,
                              uint32_t end, kimkv_block_desc const& guess, HeadGroup* groups, TableFlags& flags)
 {
     uint32_t const tid = threadIdx.x;
     uint32_t const ngroups = (end - begin + 7) / 8;
-    static_assert(kTableGroups <= kBlock, "a thread a group");
     bool right = true;
     if (tid < ngroups) {
         uint32_t const t = begin + 8 * tid;
@@ -658,7 +668,7 @@ __device__ bool build_groups(const PoolView& P, const kimkv_decode_item& table, 
         }
     }
     if (__syncthreads_and(right) != 0) return true;
-    for (uint32_t g = tid; g < ngroups; g += kBlock) groups[g].k = nullptr;
+    if (tid < ngroups) groups[tid].k = nullptr;
     if (tid == 0) flags.generic = 0;
     if (tid < kWave) {
         uint32_t const first = find_descriptor_wave(table.descriptors, table.descriptor_count, begin);
@@ -667,7 +677,7 @@ __device__ bool build_groups(const PoolView& P, const kimkv_decode_item& table, 
     __syncthreads();
     // At most ngroups + 1 entries reach into the unit.
     uint32_t const first = flags.first;
-    for (uint32_t j = tid; j <= ngroups && j < table.descriptor_count - first; j += kBlock) {
+    for (uint32_t j = tid; j <= ngroups && j < table.descriptor_count - first; j += kWaves * kWave) {
         add_head_groups<kDim>(P, table.descriptors[first + j], table.layer, head, begin, end, table.token_count, groups,
                               &flags.generic);
     }
@@ -692,7 +702,7 @@ __device__ bool build_groups(const PoolView& P, const kimkv_decode_item& table, 
 // 256 units).  Tiles of 64 keys staged in LDS for 256 columns of 8 waves
 // measured 153 us where this took 173 (128 lanes x 65536 tokens), and 62 where
 // this took 53 (16384): the barriers cost what the fewer loads save.
-template <uint32_t kDim, uint32_t kCB>
+template <uint32_t kDim, uint32_t kCB, uint32_t kWaves>
 struct DirectRows {
     static constexpr uint32_t kRow = kDim + 4;   // o, m, l, pad
     float row[kWaves][16 * kCB][kRow];
@@ -711,10 +721,11 @@ __device__ inline void store_part(const SharedArgs& a, const ColumnOut& out, uin
     store_outputs<4>(to, o, l);
 }
 
-template <uint32_t kDim, uint32_t kCB>
+template <uint32_t kDim, uint32_t kCB, uint32_t kWaves>
 __device__ bool unit_direct(const PoolView& P, const SharedArgs& a, const SharedUnit& u, const kimkv_decode_item& table,
-                            HeadGroup* groups, TableFlags& flags, ColumnOut* outs, DirectRows<kDim, kCB>& rows)
+                            HeadGroup* groups, TableFlags& flags, ColumnOut* outs, DirectRows<kDim, kCB, kWaves>& rows)
 {
+    constexpr uint32_t kSegment = 8 * kTableGroups<kWaves>;
     constexpr uint32_t kKB = kDim <= 64 && kCB == 1 ? 2 : 1;   // 32-key blocks a step
     constexpr uint32_t kStep = 32 * kKB;
     constexpr uint32_t kPanels = kDim / 32;
@@ -726,7 +737,7 @@ __device__ bool unit_direct(const PoolView& P, const SharedArgs& a, const Shared
     uint32_t const r = l & 15u;
     uint32_t const x = (l >> 2) & 3u;
     uint32_t const G = a.QH / P.heads;
-    uint32_t const hs = kCB > 1 || u.heads <= 1 ? 1 : u.heads <= 2 ? 2 : u.heads <= 4 ? 4 : 8;   // heads' share of the waves
+    uint32_t const hs = kCB > 1 || u.heads <= 1 ? 1 : u.heads <= 2 ? 2 : u.heads <= 4 ? 4 : kWaves;   // heads' share of the waves
     uint32_t const split = kWaves / hs;
     uint32_t const head = wave % hs;
     bool const works = head < u.heads;
@@ -788,7 +799,7 @@ __device__ bool unit_direct(const PoolView& P, const SharedArgs& a, const Shared
             guess = guessed_entry(table, s0);
             __syncthreads();   // the last segment's groups have been read
         }
-        if (!build_groups<kDim>(P, table, u.head, s0, s1, guess, groups, flags)) return false;
+        if (!build_groups<kDim, kWaves>(P, table, u.head, s0, s1, guess, groups, flags)) return false;
         uint32_t const piece = ((s1 - s0 + split - 1) / split + 31) / 32 * 32;
         c0 = min(wave / hs * piece, s1 - s0);
         c1 = min(c0 + piece, s1 - s0);
@@ -843,7 +854,7 @@ __device__ bool unit_direct(const PoolView& P, const SharedArgs& a, const Shared
     if (__syncthreads_or(again) != 0) return false;
     // Four dims of a column of a head at a time.
     constexpr uint32_t kQuads = kDim / 4;
-    for (uint32_t i = tid; i < u.heads * u.cols * kQuads; i += kBlock) {
+    for (uint32_t i = tid; i < u.heads * u.cols * kQuads; i += kWaves * kWave) {
         uint32_t const d = i % kQuads * 4;
         uint32_t const c = i / kQuads % u.cols;
         uint32_t const hd = i / kQuads / u.cols;
@@ -881,20 +892,23 @@ constexpr uint32_t most_blocks(uint32_t D) { return D == 64 ? 4 : direct_dim(D) 
 
 struct NoLds {};
 
+constexpr size_t kMostLds = 160 * 1024;   // of a compute unit
+
 // kDim: the head dim, or 0 for one that has only the generic path.
-template <uint32_t kDim>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2))) void shared_decode_kernel(PoolView P,
-                                                                                                         SharedArgs a)
+template <uint32_t kDim, uint32_t kWaves>
+__global__ __launch_bounds__(kWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) void shared_decode_kernel(PoolView P,
+                                                                                                                 SharedArgs a)
 {
-    // One workgroup a compute unit (its registers see to that), so the paths' memory may be large.
+    // Registers allow 8 waves a compute unit, so a workgroup's memory may take its share of the unit's: all or nearly half.
     union Paths {
-        GenericLds generic;
-        std::conditional_t<kDim != 0, DirectRows<kDim == 0 ? 64 : kDim, most_blocks(kDim)>, NoLds> direct;
+        GenericLds<kWaves> generic;
+        std::conditional_t<kDim != 0, DirectRows<kDim == 0 ? 64 : kDim, most_blocks(kDim), kWaves>, NoLds> direct;
     };
     __shared__ __attribute__((aligned(16))) unsigned char path_lds[sizeof(Paths)];
     __shared__ ColumnOut outs[64];
-    __shared__ HeadGroup groups[kDim != 0 ? kTableGroups : 1];
+    __shared__ HeadGroup groups[kDim != 0 ? kTableGroups<kWaves> : 1];
     __shared__ TableFlags flags;
+    static_assert(kMostLds / (kManyWaves / kWaves) >= sizeof path_lds + sizeof outs + sizeof groups + sizeof flags + 64);
     Paths& lds = *reinterpret_cast<Paths*>(path_lds);
     SharedUnit const u = a.units[xcd_logical_index(blockIdx.x, gridDim.x)];
     if (u.cols == 0) return;
@@ -918,8 +932,8 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         auto direct = [&](auto blocks) {
             constexpr uint32_t kCB = decltype(blocks)::value;
             if (u.cols > 16 * kCB || (u.begin & 7u) != 0 || (kCB == 1 ? u.heads > kWaves : u.heads != 1)) return;
-            done = unit_direct<kDim, kCB>(P, a, u, table, groups, flags, outs,
-                                          *reinterpret_cast<DirectRows<kDim, kCB>*>(path_lds));
+            done = unit_direct<kDim, kCB, kWaves>(P, a, u, table, groups, flags, outs,
+                                                  *reinterpret_cast<DirectRows<kDim, kCB, kWaves>*>(path_lds));
         };
         if (kind == 1) direct(std::integral_constant<uint32_t, 1>{});
         else if (kind == 2) direct(std::integral_constant<uint32_t, 2>{});
@@ -929,7 +943,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         if (done) return;
         __syncthreads();   // the generic path's rows take the same memory
     }
-    unit_generic(P, a, u, lds.generic);
+    unit_generic<kWaves>(P, a, u, lds.generic);
 }
 
 // Merges the lanes' parts, four dims a thread (one where the head dim is no
@@ -1021,30 +1035,34 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
 
 constexpr uint32_t kShareBlock = 64;     // tokens: a shared prefix is cut to whole blocks
 
-// What a unit costs its compute unit, in nanoseconds, as measured: the chain of
-// reads in front of a unit and the merge and stores behind it (6.2 to 7.0 us
-// for a few tokens); the bytes that a compute unit streams (40 a nanosecond);
-// the steps of a wave when the loads' latency is all there is; the arithmetic
-// of many columns (25.7 and 71.7 us for 2048 and 8192 tokens of 64 columns at
-// D = 64, 17.2 and 21.0 for 1024 and 1408 of 32 at D = 128).  What the bytes of
-// all units take, whoever reads them; and the merge: its launch, a round of
-// reads, and what the parts take to write and read.
+// What a unit costs, in nanoseconds, as measured on a full device: the chain of
+// reads in front of it and the merge and stores behind it (6.2 to 7.0 us for a
+// few tokens, 6.7 to 8.5 with another beside it); the bytes that a workgroup
+// streams; the steps of a wave when the loads' latency is all there is; the
+// arithmetic of many columns (at D = 64, 64 columns: 25.7 and 71.7 us for 2048
+// and 8192 tokens by 8 waves, 28.4 and 77 for 1024 and 4096 by 4).  What the
+// bytes of all units take, whoever reads them; and the merge: its launch, a
+// round of reads, and what the parts take to write and read.
 struct UnitCost {
     uint32_t D;
-    static constexpr double kStart = 6500;
+    uint32_t waves;
     static constexpr double kBytes = 5500;        // HBM's, a nanosecond
     static constexpr double kMergeLaunch = 4000;
     static constexpr double kMergeRound = 1000;
     static constexpr double kPartBytes = 4000;    // a nanosecond
+    static constexpr double kLeast = 6500;        // of any unit
+    double own_start() const { return waves == kManyWaves ? 6500 : 8000; }
+    double prefix_start(uint32_t blocks) const { return 6500.0 + (waves == kManyWaves ? 600 : 800) * blocks; }
     // `split` waves share a head's tokens.
     double own(uint32_t heads, uint32_t split, uint32_t tokens) const
     {
         double const steps = std::ceil(std::ceil(tokens / static_cast<double>(split)) * D / 64 / 64);
-        return kStart + std::max(6.0 * D / 64 * heads * tokens, 700.0 * steps);
+        return own_start() + std::max((waves == kManyWaves ? 6.0 : 11.5) * D / 64 * heads * tokens, 700.0 * steps);
     }
     double prefix(uint32_t blocks, uint32_t tokens) const
     {
-        return kStart + 600.0 * blocks + std::max(4.9, 1.87 * blocks) * D / 64 * tokens;
+        double const token = waves == kManyWaves ? std::max(4.9, 1.87 * blocks) : std::max(10.9, 3.9 * blocks);
+        return prefix_start(blocks) + token * D / 64 * tokens;
     }
     double bytes(uint32_t heads, uint32_t tokens) const { return 4.0 * D * heads * tokens; }
 };
@@ -1064,6 +1082,7 @@ struct Planned {
     uint64_t slots{0};
     uint32_t merge_lanes{0};
     uint32_t merge_parts{0};   // of the lane that has most
+    uint32_t waves{0};         // of a workgroup
 };
 
 uint64_t align16(uint64_t n) { return (n + 15) / 16 * 16; }
@@ -1072,9 +1091,9 @@ uint64_t align16(uint64_t n) { return (n + 15) / 16 * 16; }
 // one range of keys and head together, whose K and V then stay in one L2, the
 // costliest first onto the XCD with least to do that still has a compute unit
 // for each, and each XCD's costliest first.  Short lists end in idle entries.
-void place_units(Planned& p, uint32_t compute_units)
+void place_units(Planned& p, uint32_t at_once)
 {
-    size_t const per_xcd = std::max(1u, compute_units / kXcds);
+    size_t const per_xcd = std::max(1u, at_once / kXcds);
     size_t const n = p.units.size();
     struct Bundle {
         size_t first, count;
@@ -1121,7 +1140,7 @@ void place_units(Planned& p, uint32_t compute_units)
 // to be about n.
 uint32_t piece_tokens(uint64_t tokens, double n)
 {
-    auto const each = static_cast<uint64_t>(std::ceil(static_cast<double>(tokens) / std::max(1.0, std::floor(n + 0.5))));
+    auto const each = static_cast<uint64_t>(std::ceil(static_cast<double>(tokens) / std::max(1.0, std::ceil(n - 0.25))));
     return static_cast<uint32_t>(std::max<uint64_t>(64, (each + 63) / 64 * 64));
 }
 
@@ -1136,7 +1155,9 @@ struct Work {
 };
 
 struct Shape {
-    uint32_t H, G, D, compute_units;
+    uint32_t H, G, D;
+    uint32_t waves;     // of a workgroup
+    uint32_t at_once;   // workgroups that run at the same time
     const uint32_t* tokens;
     uint32_t lane_count;
 };
@@ -1154,17 +1175,18 @@ struct Cut {
 template <typename PrefixFn, typename OwnFn>
 void each_piece(Shape const& s, Work const& work, Cut const& cut, PrefixFn&& prefix_piece, OwnFn&& own_piece)
 {
-    UnitCost const cost{s.D};
+    UnitCost const cost{s.D, s.waves};
     for (Work::Prefix const& p : work.prefixes) {
-        double const whole = cost.prefix(p.blocks, p.tokens) - UnitCost::kStart;
-        prefix_piece(p, piece_tokens(p.tokens, whole / std::max(1.0, cut.share - UnitCost::kStart)));
+        double const start = cost.prefix_start(p.blocks);
+        double const whole = cost.prefix(p.blocks, p.tokens) - start;
+        prefix_piece(p, piece_tokens(p.tokens, whole / std::max(1.0, cut.share - start)));
     }
-    uint32_t const split = kWaves / cut.heads;
+    uint32_t const split = s.waves / cut.heads;
     for (uint32_t i = 0; i < s.lane_count; ++i) {
         uint32_t const own = s.tokens[i] - work.shared[i];
         if (own == 0) continue;
-        double const whole = cost.own(std::min(cut.heads, s.H), split, own) - UnitCost::kStart;
-        own_piece(i, own, piece_tokens(own, whole / std::max(1.0, cut.own_share - UnitCost::kStart)));
+        double const whole = cost.own(std::min(cut.heads, s.H), split, own) - cost.own_start();
+        own_piece(i, own, piece_tokens(own, whole / std::max(1.0, cut.own_share - cost.own_start())));
     }
 }
 
@@ -1175,8 +1197,8 @@ void each_piece(Shape const& s, Work const& work, Cut const& cut, PrefixFn&& pre
 // than what their bytes take; and the merge where a lane has several parts.
 double cut_time(Shape const& s, Work const& work, Cut const& cut)
 {
-    UnitCost const cost{s.D};
-    constexpr int kLevels = 64;   // 8 an octave from kStart on
+    UnitCost const cost{s.D, s.waves};
+    constexpr int kLevels = 64;   // 8 an octave from the least cost on
     struct Level {
         double total{0};
         double longest{0};
@@ -1189,7 +1211,7 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
     uint64_t own_most = 0;
     auto add = [&](double each, uint64_t n) {
         // The exponent and the first three bits behind the leading one.
-        auto const ratio = static_cast<float>(each / UnitCost::kStart);
+        auto const ratio = static_cast<float>(each / UnitCost::kLeast);
         uint32_t bits;
         std::memcpy(&bits, &ratio, sizeof bits);
         Level& level = levels[std::min(kLevels - 1, std::max(0, static_cast<int>(bits >> 20) - (127 << 3)))];
@@ -1208,7 +1230,7 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
         },
         [&](uint32_t, uint32_t own, uint32_t piece) {
             uint64_t const pieces = (own + piece - 1ull) / piece;
-            add(cost.own(std::min(cut.heads, s.H), kWaves / cut.heads, std::min(piece, own)),
+            add(cost.own(std::min(cut.heads, s.H), s.waves / cut.heads, std::min(piece, own)),
                 pieces * ((s.H + cut.heads - 1) / cut.heads) * ((s.G + 15) / 16));
             parts += pieces;
             own_most = std::max(own_most, pieces);
@@ -1218,17 +1240,17 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
     double rounds = 0;
     double before = 0;
     uint64_t units = 0;
-    auto const rounds_of = [&](uint64_t n) { return (n + s.compute_units - 1) / s.compute_units; };
+    auto const rounds_of = [&](uint64_t n) { return (n + s.at_once - 1) / s.at_once; };
     for (int i = kLevels - 1; i >= 0; --i) {
         Level const& level = levels[i];
         if (level.units == 0) continue;
         rounds += static_cast<double>(rounds_of(units + level.units) - rounds_of(units)) * level.longest;
         units += level.units;
         before += level.total;
-        double const start = units <= s.compute_units ? 0.0 : (before - level.longest) / s.compute_units;
+        double const start = units <= s.at_once ? 0.0 : (before - level.longest) / s.at_once;
         spread = std::max(spread, start + level.longest);
     }
-    double const time = std::max(std::min(spread, rounds), UnitCost::kStart + bytes / UnitCost::kBytes);
+    double const time = std::max(std::min(spread, rounds), UnitCost::kLeast + bytes / UnitCost::kBytes);
     if (prefix_most == 0 && own_most <= 1) return time;
     uint64_t const most = prefix_most + own_most;
     double const merge_rounds = std::ceil(static_cast<double>(most) / (kMergeBatch * merge_split(most)));
@@ -1241,11 +1263,11 @@ double cut_time(Shape const& s, Work const& work, Cut const& cut)
 // ones, which fill the end behind long pieces of prefixes.
 Cut best_cut(Shape const& s, Work const& work)
 {
-    UnitCost const cost{s.D};
+    UnitCost const cost{s.D, s.waves};
     // KV heads of a unit of a lane's own tokens: one for each wave, fewer, with
     // more waves for each, while the units are few.
     uint32_t heads = 1;
-    while (heads < kWaves && heads < s.H) heads *= 2;
+    while (heads < s.waves && heads < s.H) heads *= 2;
     uint64_t own_units = 0;
     double total = 0;
     uint32_t longest_own = 0;
@@ -1254,23 +1276,23 @@ Cut best_cut(Shape const& s, Work const& work)
         if (own == 0) continue;
         longest_own = std::max(longest_own, own);
         own_units += static_cast<uint64_t>((s.H + heads - 1) / heads) * ((s.G + 15) / 16);
-        total += cost.own(s.H, kWaves, own) * ((s.G + 15) / 16);
+        total += cost.own(s.H, s.waves, own) * ((s.G + 15) / 16);
     }
-    while (heads > 1 && own_units * 4 <= s.compute_units) {
+    while (heads > 1 && own_units * 4 <= s.at_once) {
         heads /= 2;
         own_units *= 2;
     }
     for (Work::Prefix const& p : work.prefixes) {
         total += cost.prefix(p.blocks, p.tokens) * static_cast<double>(p.tiles) * s.H;
     }
-    double const even = total / s.compute_units + UnitCost::kStart;
+    double const even = total / s.at_once + UnitCost::kLeast;
     Cut best;
-    double const longest = cost.own(std::min(heads, s.H), kWaves / heads, longest_own);
+    double const longest = cost.own(std::min(heads, s.H), s.waves / heads, longest_own);
     for (double const part : {1.0, 0.35, 0.15}) {
-        for (double const share : {1e12, 0.7 * even, 0.85 * even, even, 1.15 * even, 1.35 * even, 1.7 * even, 2.2 * even}) {
+        for (double const share : {1e12, 0.7 * even, 0.8 * even, 0.9 * even, even, 1.1 * even, 1.25 * even, 1.45 * even, 1.8 * even}) {
             double const own_share = share < 1e12 ? part * share : part < 1.0 ? part * even : share;
             if (part < 1.0 && longest <= own_share) continue;   // cuts nothing more
-            Cut c{heads, std::max(share, UnitCost::kStart + 1500), std::max(own_share, UnitCost::kStart + 1500), 0};
+            Cut c{heads, std::max(share, UnitCost::kLeast + 4000), std::max(own_share, cost.own_start() + 1500), 0};
             c.time = cut_time(s, work, c);
             if (best.share == 0 || c.time < best.time) best = c;
         }
@@ -1282,8 +1304,7 @@ Cut best_cut(Shape const& s, Work const& work)
 bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, const uint32_t* tokens, uint32_t lane_count,
                 const kimkv_shared_group* groups, uint32_t group_count, Planned& out)
 {
-    Shape const shape{H, QH / H, D, compute_units, tokens, lane_count};
-    UnitCost const cost{D};
+    uint32_t const G = QH / H;
     for (uint32_t i = 0; i < lane_count; ++i) {
         if (tokens[i] >> 31 != 0) return false;
     }
@@ -1302,7 +1323,7 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
         }
         prefix = prefix / kShareBlock * kShareBlock;
         if (group.lane_count < 2 || prefix == 0) continue;
-        uint64_t const columns = static_cast<uint64_t>(group.lane_count) * shape.G;
+        uint64_t const columns = static_cast<uint64_t>(group.lane_count) * G;
         if (columns >> 30 != 0) return false;
         Work::Prefix p{group.first_lane, group.lane_count, prefix, 1, 0};
         while (p.blocks < most_blocks(D) && 16 * p.blocks < columns) p.blocks *= 2;
@@ -1310,15 +1331,33 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
         work.prefixes.push_back(p);
         for (uint32_t i = 0; i < group.lane_count; ++i) work.shared[group.first_lane + i] = prefix;
     }
-    // Short prefixes of few lanes are read faster lane by lane, without a merge.
+    // Many waves a workgroup where the prefixes are most of the work.
+    auto const shape_of = [&](uint32_t waves) {
+        return Shape{H, G, D, waves, std::min(compute_units, 1u << 20) * (kManyWaves / waves), tokens, lane_count};
+    };
+    UnitCost const rough{D, kManyWaves};
+    double prefix_work = 0;
+    double own_work = 0;
+    for (Work::Prefix const& p : work.prefixes) {
+        prefix_work += (rough.prefix(p.blocks, p.tokens) - rough.prefix_start(p.blocks)) * static_cast<double>(p.tiles) * H;
+    }
+    for (uint32_t i = 0; i < lane_count; ++i) {
+        if (tokens[i] != work.shared[i]) own_work += rough.own(H, kManyWaves, tokens[i] - work.shared[i]);
+    }
+    Shape shape = shape_of(prefix_work > own_work ? kManyWaves : kFewWaves);
     Cut cut = best_cut(shape, work);
+    // Short prefixes of few lanes are read faster lane by lane, without a merge.
     if (!work.prefixes.empty()) {
-        Cut const other = best_cut(shape, apart);
+        Shape const other_shape = shape_of(kFewWaves);
+        Cut const other = best_cut(other_shape, apart);
         if (other.time <= cut.time) {
+            shape = other_shape;
             cut = other;
             work = apart;
         }
     }
+    UnitCost const cost{D, shape.waves};
+    out.waves = shape.waves;
     out.lanes.resize(lane_count);
     for (uint32_t i = 0; i < lane_count; ++i) out.lanes[i] = SharedLane{i, tokens[i], 0, 0, 0, 0, 0, 0};
     bool fits = true;
@@ -1367,7 +1406,7 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
                 auto const end = static_cast<uint32_t>(std::min<uint64_t>(tokens[i], at + piece));
                 for (uint32_t h = 0; h < H; h += cut.heads) {
                     uint32_t const n = std::min(cut.heads, H - h);
-                    double const c = cost.own(n, kWaves / cut.heads, end - static_cast<uint32_t>(at));
+                    double const c = cost.own(n, shape.waves / cut.heads, end - static_cast<uint32_t>(at));
                     for (uint32_t col = 0; col < shape.G; col += 16) {
                         push(SharedUnit{i, i, col, std::min(16u, shape.G - col), static_cast<uint32_t>(at), end,
                                         static_cast<uint32_t>(out.slots), static_cast<uint16_t>(h), static_cast<uint8_t>(n),
@@ -1384,7 +1423,7 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
         out.merge_lanes += lane.merged;
         out.merge_parts = std::max(out.merge_parts, lane.prefix_count + lane.tail_count);
     }
-    place_units(out, compute_units);
+    place_units(out, shape.at_once);
     return true;
 }
 
@@ -1426,6 +1465,7 @@ kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint
         plan->slot_count = static_cast<uint32_t>(p.slots);
         plan->merge_lanes = p.merge_lanes;
         plan->merge_split = merge_split(p.merge_parts);
+        plan->waves = p.waves;
         if (capacity < plan->entry_bytes || (plan->entry_bytes != 0 && entries == nullptr)) return KIMKV_INVALID_ARGUMENT;
         if (unit_bytes != 0) std::memcpy(entries, p.units.data(), unit_bytes);
         if (lane_bytes != 0) std::memcpy(static_cast<unsigned char*>(entries) + unit_bytes, p.lanes.data(), lane_bytes);
@@ -1448,7 +1488,7 @@ kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv
     if (plan->unit_count == 0) return KIMKV_OK;
     uint64_t const o_bytes = align16(parts_o_floats(plan->slot_count, plan->query_heads, D) * sizeof(float));
     if (device_items == nullptr || device_entries == nullptr || plan->lane_count == 0 || plan->query_heads == 0 || H == 0
-        || plan->query_heads % H != 0 || D > kMaxDim || plan->merge_split == 0 || plan->merge_split > 8
+        || plan->query_heads % H != 0 || D > kMaxDim || (plan->waves != kManyWaves && plan->waves != kFewWaves) || plan->merge_split == 0 || plan->merge_split > 8
         || (plan->merge_split & (plan->merge_split - 1)) != 0 || plan->unit_count > 0x7FFFFFFFu
         || (reinterpret_cast<uintptr_t>(device_entries) & 15u) != 0
         || plan->entry_bytes != plan->unit_count * sizeof(SharedUnit) + plan->lane_count * sizeof(SharedLane)
@@ -1470,7 +1510,13 @@ kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv
     PoolView const pv = pool_view(*storage);
     void* start = nullptr;
     kernel_timing_begin(TimedKernel::Decode, s, &start);
-    auto attend = [&](auto dim) { shared_decode_kernel<decltype(dim)::value><<<plan->unit_count, kBlock, 0, s>>>(pv, a); };
+    auto launch = [&](auto dim, auto waves) {
+        shared_decode_kernel<decltype(dim)::value, decltype(waves)::value><<<plan->unit_count, plan->waves * kWave, 0, s>>>(pv, a);
+    };
+    auto attend = [&](auto dim) {
+        if (plan->waves == kManyWaves) launch(dim, std::integral_constant<uint32_t, kManyWaves>{});
+        else launch(dim, std::integral_constant<uint32_t, kFewWaves>{});
+    };
     if (D == 64) attend(std::integral_constant<uint32_t, 64>{});
     else if (D == 96) attend(std::integral_constant<uint32_t, 96>{});
     else if (D == 128) attend(std::integral_constant<uint32_t, 128>{});

@@ -116,7 +116,7 @@ class SharedPlan(ctypes.Structure):
     _fields_ = [("entry_bytes", ctypes.c_uint64), ("workspace_bytes", ctypes.c_uint64), ("kv_heads", ctypes.c_uint32),
                 ("head_dim", ctypes.c_uint32), ("query_heads", ctypes.c_uint32), ("lane_count", ctypes.c_uint32),
                 ("unit_count", ctypes.c_uint32), ("slot_count", ctypes.c_uint32), ("merge_lanes", ctypes.c_uint32),
-                ("merge_split", ctypes.c_uint32)]
+                ("merge_split", ctypes.c_uint32), ("waves", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
 
 
 # kimkv_decode_lane (48 bytes): one chunk of a batched decode with its lane's step-constant part.

@@ -414,8 +414,24 @@ def test_shared_decode_every_kind(dev, heads, dim, lanes, kind, prefix):
     assert b.storage.faults() == (0, 0)
 
 
+@pytest.mark.parametrize("heads,dim,lanes,kind", [(2, 64, 2, 1), (2, 64, 4, 2), (4, 64, 8, 4), (3, 96, 4, 2), (2, 128, 5, 2), (1, 128, 2, 1)])
+@pytest.mark.parametrize("own", [40, 4500])
+def test_shared_decode_workgroups(dev, heads, dim, lanes, kind, own):
+    """Workgroups of many waves where prefixes are most of the work, of few where the lanes' own tokens are; units of
+    several segments in both."""
+    print(f"shared workgroups H={heads} D={dim} lanes={lanes} own={own}", flush=True)
+    b = _Batch(dev, heads, dim, 8, [4200 + own + 30 * i for i in range(lanes)], [(0, lanes, 4200)])
+    b.place()
+    b.plan(1)
+    assert (kind, True) in _kinds(b)
+    assert b.p.waves == (8 if own == 40 else 4)
+    b.launch()
+    b.check(b.outputs())
+    assert b.storage.faults() == (0, 0)
+
+
 @pytest.mark.parametrize("heads,dim,group", [(1, 64, 8), (2, 128, 3), (1, 30, 2), (1, 96, 16)])
-@pytest.mark.parametrize("units,split", [(24, 2), (36, 2), (64, 4), (512, 8), (2000, 8)])
+@pytest.mark.parametrize("units,split", [(12, 1), (40, 2), (64, 4), (2000, 4)])
 def test_shared_decode_many_parts(dev, heads, dim, group, units, split):
     """Lanes cut into many parts, beside short ones, on a plan for a device with more compute units than this one."""
     print(f"shared parts H={heads} D={dim} units={units}", flush=True)
@@ -647,7 +663,7 @@ def test_shared_decode_refusals(dev):
     for bad in (dict(items=None), dict(entries=None), dict(work=None), dict(entries=b.entries_buf.ptr + 4), dict(work=b.work.ptr + 2052),
                 dict(kv_heads=4), dict(head_dim=128), dict(query_heads=16), dict(query_heads=7), dict(query_heads=0), dict(lane_count=2),
                 dict(lane_count=0), dict(unit_count=b.p.unit_count + 1), dict(slot_count=b.p.slot_count + 1), dict(entry_bytes=0),
-                dict(workspace_bytes=0), dict(merge_split=0), dict(merge_split=3), dict(merge_split=16)):
+                dict(workspace_bytes=0), dict(merge_split=0), dict(merge_split=3), dict(merge_split=16), dict(waves=0), dict(waves=6)):
         assert status(**bad) == dev.INVALID_ARGUMENT, bad
     assert lib.kimkv_shared_decode_batch(b.storage.h, None, None, None, None, None) == dev.INVALID_ARGUMENT
     other = dev.Storage(1, 4, 64, 8, 2)

@@ -23,7 +23,7 @@ def test_struct_layouts(kimkv):
     assert d.LOGITS_RULE.itemsize == 56
     assert ctypes.sizeof(d.Rope) == 16
     assert ctypes.sizeof(d.SharedGroup) == 12
-    assert ctypes.sizeof(d.SharedPlan) == 48
+    assert ctypes.sizeof(d.SharedPlan) == 56
 
 
 @pytest.mark.parametrize("heads,dim,group", [(4, 64, 8), (8, 128, 4), (1, 64, 1), (3, 96, 5), (2, 12, 40), (16, 64, 1)])
