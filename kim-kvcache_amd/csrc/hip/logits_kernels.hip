@@ -339,11 +339,15 @@ __global__ __launch_bounds__(kPickBlock) void logits_pick_kernel(const Best* par
     if ((threadIdx.x & (kWave - 1)) == 0) tokens[row] = best.token;
 }
 
-// How rows are cut: slices of 4096 positions up to 16384, as large as leaves
-// kBlocksWanted, since every block reads its row's whole history.  (A block of
-// 1024 threads for a row of 32000 saves the second launch and loses more: 12.6
-// us for 4 rows and 16.2 for 72, where slices take 9.2 and 13.4.)
-constexpr uint32_t kBlocksWanted = 512;
+// How rows are cut: slices of 4096 positions up to 16384, those whose rounds
+// of the blocks that run at once, and the second launch where a row takes
+// several, come to least.  A round takes about 3.5 us and 1.2 for each 4096
+// positions, the second launch 2.5.  (Slices as large as leave 512 blocks took
+// 11.2 us for 101 rows of 20562, 10.7 for 242 of 6793, 11.1 for 153 of 10726
+// and 19.0 for 85 of 99226, these 9.9, 7.7, 9.2 and 17.4.  A block of 1024
+// threads for a row of 32000 saves the second launch too and loses more: 12.6
+// us for 4 rows and 16.2 for 72, where slices took 9.2 and 13.4.)
+constexpr uint32_t kBlocksAtOnce = 512;
 
 struct RowCut {
     uint32_t per;
@@ -352,11 +356,19 @@ struct RowCut {
 
 RowCut row_cut(uint32_t rows, uint32_t vocabulary)
 {
-    constexpr uint32_t kStep = 4 * kBlock;
-    constexpr uint32_t kMost = kStep * kVecs;
-    uint64_t const even = static_cast<uint64_t>(rows) * vocabulary / kBlocksWanted;
-    uint32_t const per = even >= kMost ? kMost : even <= kStep ? kStep : ceil_div(even, kStep) * kStep;
-    return RowCut{per, ceil_div(vocabulary + 3ull, per)};   // 3: a row's shift
+    RowCut cut{};
+    double best = 0.0;
+    for (uint32_t vecs = 1; vecs <= kVecs; ++vecs) {
+        uint32_t const per = 4 * kBlock * vecs;
+        uint32_t const slices = ceil_div(vocabulary + 3ull, per);   // 3: a row's shift
+        uint32_t const rounds = ceil_div(static_cast<uint64_t>(rows) * slices, kBlocksAtOnce);
+        double const cost = rounds * (3.5 + 1.2 * vecs) + (slices > 1 ? 2.5 : 0.0);
+        if (cut.per == 0 || cost < best) {
+            best = cost;
+            cut = RowCut{per, slices};
+        }
+    }
+    return cut;
 }
 
 }  // namespace
