@@ -446,11 +446,12 @@ def test_shared_decode_many_parts(dev, heads, dim, group, units, split):
 
 @pytest.mark.parametrize("heads,dim,group", [(1, 64, 1), (3, 64, 5), (2, 96, 3), (1, 128, 40), (5, 64, 2), (2, 32, 4), (1, 8, 2), (2, 200, 1),
                                              (1, 256, 7), (2, 12, 3), (1, 64, 33)])
-def test_shared_decode_other_shapes(dev, heads, dim, group):
-    print(f"shared H={heads} D={dim} G={group}", flush=True)
-    b = _Batch(dev, heads, dim, group, [330, 400, 345, 12], [(0, 3, 321)], layers=2, layer=1)
+@pytest.mark.parametrize("more", [0, 2000])
+def test_shared_decode_other_shapes(dev, heads, dim, group, more):
+    print(f"shared H={heads} D={dim} G={group} more={more}", flush=True)
+    b = _Batch(dev, heads, dim, group, [330 + more, 400 + more, 345 + more, 12], [(0, 3, 321 + more)], layers=2, layer=1)
     b.place()
-    b.plan()
+    b.plan(1 if more else 4)
     b.launch()
     b.check(b.outputs())
     assert b.storage.faults() == (0, 0)
@@ -496,11 +497,12 @@ def test_shared_decode_hole(dev, lanes, dim):
 def test_shared_decode_scales_and_addresses(dev, dim):
     """Lanes of one group with scales of their own (one negative, one zero), and queries off the vectors' alignment."""
     for off in (0, 1):
-        b = _Batch(dev, 2, dim, 8, [300 + i for i in range(20)], [(0, 20, 290)])
+        b = _Batch(dev, 2, dim, 8, [1500 + i for i in range(20)], [(0, 20, 1490)])
         b.scale = np.array([0.01 * (i + 1) for i in range(20)], dtype=np.float32)
         b.scale[3], b.scale[7] = -0.1, 0.0
         b.place(q_off=off)
         b.plan()
+        assert ({64: 4, 128: 2}[dim], True) in _kinds(b)
         b.launch()
         b.check(b.outputs())
 
@@ -574,6 +576,24 @@ def test_shared_decode_all_scores_minus_infinity(dev):
         for i in range(3):
             want, bound = reference(b.query[i, 4:], b.k[i][320:, 1:], b.v[i][320:, 1:], float(b.scale[i]))
             assert np.all(np.abs(got[i, 4:].astype(np.float64) - want) <= bound)
+
+
+def test_shared_decode_two_at_once(dev):
+    """Two launches of one plan on two streams, each with a workspace and outputs of its own, and one on the first's
+    stream again."""
+    streams = [dev.Stream(), dev.Stream()]
+    batches = [_Batch(dev, 4, 64, 8, [6000 + i for i in range(12)], [(0, 12, 5990)], seed=3 + i) for i in range(2)]
+    for b in batches:
+        b.place()
+        b.plan(256)
+        assert b.p.merge_lanes == 12
+    for k in (0, 1, 0, 1):
+        b = batches[k]
+        b.storage.shared_decode_launch(b.items.ptr, b.entries_buf.ptr, b.p, b.work.ptr + 2048, streams[k])
+    for stream, b in zip(streams, batches):
+        stream.synchronize()
+        b.check(b.outputs())
+        stream.destroy()
 
 
 def test_shared_decode_without_groups(dev):
