@@ -781,7 +781,9 @@ typedef struct kimkv_logits_rule {
 /* The token of a row that allows none or whose rule is invalid. */
 #define KIMKV_NO_TOKEN 0xFFFFFFFFu
 
-/* Workspace of kimkv_model_logits_adjust (0 for shapes that need none). */
+/* Workspace of kimkv_model_logits_adjust for up to `rows` rows of up to
+ * `vocabulary` tokens (0 for shapes that need none): what is enough for a
+ * batch is enough for every smaller one. */
 size_t kimkv_logits_workspace_bytes(uint32_t rows, uint32_t vocabulary);
 
 /* Applies device_rules[r] to row r of logits[rows][vocabulary]: the adjusted
@@ -792,11 +794,12 @@ size_t kimkv_logits_workspace_bytes(uint32_t rows, uint32_t vocabulary);
  * nothing is higher), KIMKV_NO_TOKEN where every allowed logit is NaN or none
  * is allowed.  A rule with a list that is NULL but not empty or holds 2^31
  * entries or more, or a repetition penalty that is not above 0 and finite,
- * leaves its row of out alone and gives KIMKV_NO_TOKEN.  device_rules NULL: no row is adjusted.  workspace:
- * kimkv_logits_workspace_bytes(rows, vocabulary) of device memory, 8-byte
- * aligned, contents ignored, not shared with a call that may overlap this one
- * (NULL where that is 0 or device_tokens is NULL).  No counterpart in the
- * reference, whose runner picks the plain argmax. */
+ * leaves its row of out alone and gives KIMKV_NO_TOKEN.  device_rules NULL: no
+ * row is adjusted.  workspace: kimkv_logits_workspace_bytes of at least these
+ * rows and this vocabulary, in device memory, 8-byte aligned, contents ignored,
+ * not shared with a call that may overlap this one (NULL where that is 0 or
+ * device_tokens is NULL).  No counterpart in the reference, whose runner picks
+ * the plain argmax. */
 kimkv_status kimkv_model_logits_adjust(const float* logits, uint32_t rows, uint32_t vocabulary,
                                        const kimkv_logits_rule* device_rules, float* out, uint32_t* device_tokens,
                                        void* workspace, kimkv_stream_t stream);

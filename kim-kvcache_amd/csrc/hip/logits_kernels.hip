@@ -378,9 +378,11 @@ using namespace kimkv;
 
 extern "C" {
 
+// A row is cut into more slices in a small batch than in a large one, so the
+// size is that of the smallest slices, whatever the batch: enough for fewer rows too.
 size_t kimkv_logits_workspace_bytes(uint32_t rows, uint32_t vocabulary)
 {
-    uint32_t const slices = row_cut(rows, vocabulary).slices;
+    uint32_t const slices = ceil_div(vocabulary + 3ull, 4 * kBlock);
     return slices <= 1 ? 0 : static_cast<size_t>(rows) * slices * sizeof(Best);
 }
 

@@ -905,6 +905,22 @@ def test_logits_invalid_rules(dev):
     _check_logits(rows[8:], rules[8:], got)
 
 
+@pytest.mark.parametrize("vocab,most,rows", [(16000, 256, (128, 3)), (32000, 65, (64, 1)), (128000, 17, (16, 5))])
+def test_logits_scratch_of_a_larger_batch(dev, vocab, most, rows):
+    """Scratch made once for the largest batch serves the smaller ones that come after it; the bytes behind it stay."""
+    rng = np.random.default_rng(most)
+    need = dev.logits_workspace_bytes(most, vocab)
+    for n in (most, *rows):
+        print(f"logits scratch V={vocab} for {most}: {n} rows", flush=True)
+        assert dev.logits_workspace_bytes(n, vocab) <= need   # else the call would write past it
+        x = rng.standard_normal((n, vocab)).astype(np.float32)
+        logits, tokens, work = dev.upload(x), dev.upload(np.zeros(n, np.uint32)), dev.upload(np.full(need + 65536, 0x5A, np.uint8))
+        dev.logits_adjust(logits.ptr, n, vocab, 0, 0, tokens.ptr, work.ptr)
+        dev.sync()
+        assert np.array_equal(dev.download(tokens.ptr, (n,), np.uint32), x.argmax(1))
+        assert np.all(dev.download(work.ptr, (need + 65536,), np.uint8)[need:] == 0x5A)
+
+
 def test_logits_many_rows(dev):
     """More rows than a grid's y takes."""
     rng = np.random.default_rng(9)

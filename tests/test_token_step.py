@@ -136,3 +136,16 @@ def test_entry_points_refuse_null(kimkv):
     assert lib.kimkv_model_logits_adjust(one, 3, 1 << 20, None, None, one, ctypes.c_void_p(20), None) == d.INVALID_ARGUMENT
     # No rows: nothing to do.
     assert lib.kimkv_model_logits_adjust(one, 0, 1 << 20, None, None, one, None, None) == d.OK
+
+
+def test_logits_workspace_never_falls(kimkv):
+    """Scratch for a batch is enough for any smaller one, of rows as of vocabulary."""
+    size = kimkv.device.logits_workspace_bytes
+    vocabularies = [1, 5, 4093, 4094, 8189, 8190, 16000, 16381, 16382, 32000, 50257, 128000, 1 << 20]
+    for vocabulary in vocabularies:
+        of_rows = [size(rows, vocabulary) for rows in range(300)]
+        assert of_rows == sorted(of_rows), vocabulary
+        assert of_rows[0] == 0 and size(1 << 20, vocabulary) >= of_rows[-1]
+    for rows in (1, 16, 17, 64, 65, 128, 129, 256):
+        of_vocabulary = [size(rows, v) for v in vocabularies]
+        assert of_vocabulary == sorted(of_vocabulary), rows
