@@ -1090,7 +1090,11 @@ uint64_t align16(uint64_t n) { return (n + 15) / 16 * 16; }
 // Spreads the units over the XCDs (workgroup w runs on XCD w % 8): units of
 // one range of keys and head together, whose K and V then stay in one L2, the
 // costliest first onto the XCD with least to do that still has a compute unit
-// for each, and each XCD's costliest first.  Short lists end in idle entries.
+// for each, and each XCD's costliest first.  Where these are more than an XCD
+// runs at once (many lanes' columns on few heads), they are cut every so many
+// units, or every eighth of all such units where that is more (256 lanes of 16
+// query heads on 8192 tokens, 2 KV heads: 128 units on each of two XCDs and
+// none on the others, so 32 on each).  Short lists end in idle entries.
 void place_units(Planned& p, uint32_t at_once)
 {
     size_t const per_xcd = std::max(1u, at_once / kXcds);
@@ -1111,6 +1115,32 @@ void place_units(Planned& p, uint32_t at_once)
             }
         }
         bundles.push_back(Bundle{i, 1, p.cost[i]});
+    }
+    size_t wide = 0;
+    for (Bundle const& b : bundles) wide += b.count > per_xcd ? b.count : 0;
+    if (wide != 0) {
+        size_t const most = std::max<size_t>(per_xcd, (wide + kXcds - 1) / kXcds);
+        std::vector<Bundle> cut;
+        bool open = false;   // the last one takes more units
+        for (Bundle b : bundles) {
+            if (b.count <= per_xcd) {
+                cut.push_back(b);
+                open = false;
+                continue;
+            }
+            double const each = b.cost / static_cast<double>(b.count);
+            while (b.count != 0) {
+                if (!open) cut.push_back(Bundle{b.first, 0, 0.0});
+                Bundle& last = cut.back();
+                size_t const n = std::min(b.count, most - last.count);
+                last.count += n;
+                last.cost += each * static_cast<double>(n);
+                b.first += n;
+                b.count -= n;
+                open = last.count < most;
+            }
+        }
+        bundles = std::move(cut);
     }
     std::stable_sort(bundles.begin(), bundles.end(), [](Bundle const& x, Bundle const& y) { return x.cost > y.cost; });
     std::vector<size_t> xcd[kXcds];

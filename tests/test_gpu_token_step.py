@@ -414,6 +414,20 @@ def test_shared_decode_every_kind(dev, heads, dim, lanes, kind, prefix):
     assert b.storage.faults() == (0, 0)
 
 
+@pytest.mark.parametrize("heads,dim", [(1, 64), (2, 128), (3, 96)])
+@pytest.mark.parametrize("units", [24, 256])
+def test_shared_decode_wide_group(dev, heads, dim, units):
+    """Columns of one head and key range that are more than an XCD computes at once, on several of them."""
+    print(f"shared wide H={heads} D={dim} units={units}", flush=True)
+    b = _Batch(dev, heads, dim, 8, [640 + i % 40 for i in range(270)], [(0, 270, 640)])
+    b.place()
+    b.plan(units)
+    assert units == 256 or any(wide for _, wide in _kinds(b))   # a large device may read so little lane by lane
+    b.launch()
+    b.check(b.outputs())
+    assert b.storage.faults() == (0, 0)
+
+
 @pytest.mark.parametrize("heads,dim,lanes,kind", [(2, 64, 2, 1), (2, 64, 4, 2), (4, 64, 8, 4), (3, 96, 4, 2), (2, 128, 5, 2), (1, 128, 2, 1)])
 @pytest.mark.parametrize("own", [40, 4500])
 def test_shared_decode_workgroups(dev, heads, dim, lanes, kind, own):

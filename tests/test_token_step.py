@@ -81,6 +81,25 @@ def test_plan_covers_every_key_once(kimkv, heads, dim, group):
         assert plan.workspace_bytes == o + plan.slot_count * heads * group * 8
 
 
+@pytest.mark.parametrize("heads,dim,group,lanes,prefix,own", [
+    (1, 64, 8, 512, 8192, 100), (1, 128, 8, 256, 8192, 100), (2, 128, 16, 256, 8192, 100), (2, 64, 8, 600, 4096, 1),
+    (4, 64, 8, 512, 16384, 100), (4, 128, 4, 500, 2048, 30), (3, 96, 5, 300, 8192, 700), (1, 64, 64, 512, 4096, 100)])
+@pytest.mark.parametrize("compute_units", [256, 64])
+def test_plan_spreads_wide_groups(kimkv, heads, dim, group, lanes, prefix, own, compute_units):
+    """More columns of one head and key range than an XCD has compute units go to several XCDs: none has more of them
+    than run there at once, or much more than its share."""
+    entries, plan = kimkv.device.shared_decode_plan(heads, dim, heads * group, compute_units, [prefix + own] * lanes, [(0, lanes, prefix)])
+    units = entries[:plan.unit_count * UNIT.itemsize].view(UNIT).reshape(8, -1)   # a row an XCD
+    shared = (units["end"] <= prefix) & (units["cols"] != 0)
+    columns = {(int(u["head"]), int(u["begin"])) for u in units[shared]}
+    assert shared.sum() > len(columns) * compute_units // 8   # wide indeed
+    on_xcd = shared.sum(1)
+    at_once = compute_units // 8 * (8 // plan.waves)
+    assert on_xcd.max() <= max(at_once, 1.25 * on_xcd.mean()), on_xcd
+    work = np.where(shared, (units["end"] - units["begin"]).astype(np.int64), 0).sum(1)
+    assert work.max() <= max(1.25 * work.mean(), at_once * (units["end"] - units["begin"])[shared].max()), work
+
+
 def test_plan_refusals(kimkv):
     d = kimkv.device
     lib = d.lib()
