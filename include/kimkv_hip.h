@@ -604,10 +604,11 @@ typedef struct kimkv_shared_plan {
  * (pure host code, the same for every layer of a token step).  compute_units
  * is the device's (the storage's kimkv_storage_info; 0: 256), token_counts
  * each lane's tokens; the groups name disjoint runs of lanes, and lanes
- * in none share nothing.  A group's prefix is read through its first lane's
- * table, once for all its lanes; of it the plan takes whole blocks of 64
- * tokens that all of its lanes hold, none where that would not pay, and the
- * rest of each lane is read through the lane's own table.  Fills entries[0 ..
+ * in none share nothing.  Lanes of no tokens may stand anywhere in the batch
+ * and in its groups.  A group's prefix is read through the table of its first
+ * lane that has tokens, once for all of these; of it the plan takes whole
+ * blocks of 64 tokens that all of them hold, none where that would not pay,
+ * and the rest of each lane is read through the lane's own table.  Fills entries[0 ..
  * plan->entry_bytes) for upload; KIMKV_INVALID_ARGUMENT when capacity is too
  * small (plan->entry_bytes then holds the size needed; entries may be NULL
  * with capacity 0), for groups that overlap or leave the batch, or for lanes of
@@ -623,8 +624,9 @@ kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint
  * used); device_entries: the plan's entries (made for the storage's heads and
  * head dim); workspace: plan->workspace_bytes
  * of device memory, contents ignored, not shared with a launch that may
- * overlap this one.  Lanes of one group name the same layer.  A lane of no
- * tokens is skipped (its output is not written); a lane whose item is invalid
+ * overlap this one.  Lanes of one group name the same layer.  A lane planned
+ * with no tokens is skipped, whatever its item holds (its output is not
+ * written); a lane whose item is invalid
  * or not as planned, or whose prefix is read through such a lane's table, sets
  * KIMKV_FAULT_DECODE_ITEM and is skipped.  Results as
  * kimkv_paged_decode_batch's to the decode tolerance, the same for every run

@@ -125,8 +125,8 @@ __device__ inline void report_column(const PoolView& P, bool missing)
 }
 
 // One column of a unit: its lane's item and query head in the group; !ok
-// where the lane's item is not as planned, or of another layer than the
-// table's.
+// where the lane is planned with no tokens, or `missing`: its item is not as
+// planned, or of another layer than the table's.
 struct Column {
     const uint16_t* query;   // row of KV head 0
     uint16_t* output;
@@ -134,6 +134,7 @@ struct Column {
     uint32_t lane;           // from u.lane on
     uint32_t q;
     bool ok;
+    bool missing;
 };
 
 __device__ inline Column unit_column(const PoolView& P, const SharedArgs& a, const SharedUnit& u, uint32_t layer, uint32_t c)
@@ -141,7 +142,9 @@ __device__ inline Column unit_column(const PoolView& P, const SharedArgs& a, con
     Column out{};
     out.lane = div_mod(u.col0 + min(c, u.cols - 1), a.group, &out.q);
     kimkv_decode_item const item = a.items[u.lane + out.lane];
-    out.ok = c < u.cols && lane_valid(P, item, a.lanes[u.lane + out.lane].tokens) && item.layer == layer;
+    uint32_t const planned = a.lanes[u.lane + out.lane].tokens;
+    out.ok = c < u.cols && lane_valid(P, item, planned) && item.layer == layer;
+    out.missing = c < u.cols && planned != 0 && !out.ok;
     out.query = item.query + out.q * P.dim;
     out.output = item.output + out.q * P.dim;
     out.scale2 = item.attention_scale * kLog2e;
@@ -326,7 +329,7 @@ __device__ void unit_generic(const PoolView& P, const SharedArgs& a, const Share
 #pragma unroll
             for (uint32_t r = 0; r < kRows; ++r) {
                 rows[r] = unit_column(P, a, u, table.layer, col0 + r);
-                report_column(P, !rows[r].ok && col0 + r < u.cols);
+                report_column(P, rows[r].missing);
             }
             RowParts part;
             attend_rows_generic(P, table, G, h, c0, c1, rows, part);
@@ -450,8 +453,7 @@ __device__ inline bool columns_init(Columns<kDim, kCB>& w, const PoolView& P, co
 #pragma unroll
         for (uint32_t db = 0; db < kDim / 16; ++db) w.acc[db][cb] = float4_t{};
     }
-    bool const missing = !c.ok && mine < u.cols;
-    report_column(P, missing);
+    report_column(P, c.missing);
     return ordered;
 }
 
@@ -1178,7 +1180,7 @@ uint32_t piece_tokens(uint64_t tokens, double n)
 struct Work {
     struct Prefix {
         uint32_t lane, lanes, tokens, blocks;   // blocks: of 16 columns a wave
-        uint64_t tiles;                         // units that take all its columns
+        uint64_t tiles;                         // units that take all its columns, but those of empty lanes alone
     };
     std::vector<Prefix> prefixes;
     std::vector<uint32_t> shared;   // tokens of each lane that a prefix takes
@@ -1331,6 +1333,16 @@ Cut best_cut(Shape const& s, Work const& work)
     return best;
 }
 
+// Whether columns [col, col + 16 p.blocks) of a prefix belong to lanes with tokens, some of them.
+bool any_tokens(const uint32_t* tokens, Work::Prefix const& p, uint32_t G, uint32_t col)
+{
+    uint32_t const end = std::min(p.lanes, (col + 16 * p.blocks - 1) / G + 1);
+    for (uint32_t i = col / G; i < end; ++i) {
+        if (tokens[p.lane + i] != 0) return true;
+    }
+    return false;
+}
+
 bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, const uint32_t* tokens, uint32_t lane_count,
                 const kimkv_shared_group* groups, uint32_t group_count, Planned& out)
 {
@@ -1346,20 +1358,28 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
         kimkv_shared_group const& group = groups[g];
         if (group.first_lane > lane_count || group.lane_count > lane_count - group.first_lane) return false;
         uint32_t prefix = group.prefix_tokens;
+        // Lanes of no tokens (requests that ended, padding) share nothing and hold nobody up: the prefix is the
+        // others', read through the first of them.
+        uint32_t live = 0, first = 0, last = 0;
         for (uint32_t i = group.first_lane; i < group.first_lane + group.lane_count; ++i) {
             if (grouped[i] != 0) return false;
             grouped[i] = 1;
+            if (tokens[i] == 0) continue;
+            if (live == 0) first = i;
+            last = i;
+            ++live;
             prefix = std::min(prefix, tokens[i]);
         }
         prefix = prefix / kShareBlock * kShareBlock;
-        if (group.lane_count < 2 || prefix == 0) continue;
-        uint64_t const columns = static_cast<uint64_t>(group.lane_count) * G;
+        if (live < 2 || prefix == 0) continue;
+        uint32_t const run = last - first + 1;
+        uint64_t const columns = static_cast<uint64_t>(run) * G;
         if (columns >> 30 != 0) return false;
-        Work::Prefix p{group.first_lane, group.lane_count, prefix, 1, 0};
+        Work::Prefix p{first, run, prefix, 1, 0};
         while (p.blocks < most_blocks(D) && 16 * p.blocks < columns) p.blocks *= 2;
-        p.tiles = (columns + 16 * p.blocks - 1) / (16 * p.blocks);
+        for (uint32_t col = 0; col < columns; col += 16 * p.blocks) p.tiles += any_tokens(tokens, p, G, col) ? 1 : 0;
         work.prefixes.push_back(p);
-        for (uint32_t i = 0; i < group.lane_count; ++i) work.shared[group.first_lane + i] = prefix;
+        for (uint32_t i = first; i <= last; ++i) work.shared[i] = std::min(prefix, tokens[i]);
     }
     // Many waves a workgroup where the prefixes are most of the work.
     auto const shape_of = [&](uint32_t waves) {
@@ -1406,6 +1426,7 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
             if (!take_slots(static_cast<uint64_t>(p.lanes) * pieces)) return;
             for (uint32_t i = 0; i < p.lanes; ++i) {
                 SharedLane& lane = out.lanes[p.lane + i];
+                if (lane.tokens == 0) continue;   // its columns' parts are nobody's
                 lane.table_lane = p.lane;
                 lane.prefix_slot = static_cast<uint32_t>(out.slots + i);
                 lane.prefix_stride = p.lanes;
@@ -1417,6 +1438,7 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
                 double const c = cost.prefix(p.blocks, end - static_cast<uint32_t>(at));
                 for (uint32_t h = 0; h < H; ++h) {
                     for (uint32_t col = 0; col < columns; col += 16 * p.blocks) {
+                        if (!any_tokens(tokens, p, shape.G, col)) continue;
                         push(SharedUnit{p.lane, p.lane, col, std::min(16 * p.blocks, columns - col), static_cast<uint32_t>(at), end,
                                         static_cast<uint32_t>(out.slots), static_cast<uint16_t>(h), 1, static_cast<uint8_t>(p.blocks)},
                              c);

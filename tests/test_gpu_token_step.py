@@ -414,6 +414,29 @@ def test_shared_decode_every_kind(dev, heads, dim, lanes, kind, prefix):
     assert b.storage.faults() == (0, 0)
 
 
+@pytest.mark.parametrize("heads,dim,group", [(4, 64, 8), (2, 128, 4), (2, 80, 3)])
+@pytest.mark.parametrize("empty", [[0], [6], [11], [0, 1, 4, 5, 10, 11], [2, 3, 4, 5]])
+def test_shared_decode_empty_lanes_in_a_group(dev, heads, dim, group, empty):
+    """Ended requests and padding in a group: the others share its prefix, and nothing is written or reported for these,
+    whatever their items hold."""
+    print(f"shared empty {empty} H={heads} D={dim}", flush=True)
+    prefix = 2000
+
+    def spoil(items):
+        items["layer"][empty] = 7
+        items["token_count"][empty[-1]] = 5
+
+    first = min(set(range(12)) - set(empty))
+    b = _Batch(dev, heads, dim, group, [0 if i in empty else prefix + 3 * i for i in range(12)], [(first, 12 - first, prefix)])
+    b.groups = [(0, 12, prefix)]
+    b.place(change=spoil)
+    b.plan(1)
+    assert any(wide for _, wide in _kinds(b))
+    b.launch()
+    b.check(b.outputs())
+    assert b.storage.faults() == (0, 0)
+
+
 @pytest.mark.parametrize("heads,dim", [(1, 64), (2, 128), (3, 96)])
 @pytest.mark.parametrize("units", [24, 256])
 def test_shared_decode_wide_group(dev, heads, dim, units):

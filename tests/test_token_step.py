@@ -81,6 +81,33 @@ def test_plan_covers_every_key_once(kimkv, heads, dim, group):
         assert plan.workspace_bytes == o + plan.slot_count * heads * group * 8
 
 
+@pytest.mark.parametrize("empty", [[0], [5], [39], [0, 1, 2, 20, 38, 39], list(range(9, 33))])
+def test_plan_shares_beside_empty_lanes(kimkv, empty):
+    """Lanes of no tokens in a group (requests that ended, padding) do not end the others' sharing."""
+    lanes, prefix = 40, 8192
+    counts = [0 if i in empty else prefix + 1 + i for i in range(lanes)]
+    live = [i for i in range(lanes) if counts[i]]
+    entries, plan = kimkv.device.shared_decode_plan(4, 64, 32, 8, counts, [(0, lanes, prefix)])
+    units, records = split_entries(entries, plan)
+    shared = units[units["cols"] > 8]
+    assert len(shared) and np.all(shared["table_lane"] == live[0])
+    for u in shared:   # none computes columns of empty lanes alone
+        assert any(counts[int(u["lane"]) + c // 8] for c in range(int(u["col0"]), int(u["col0"] + u["cols"])))
+    for head in range(4):   # every live lane's columns on every block of the prefix, once; of nobody past the last live lane
+        seen = np.zeros((lanes, 8, prefix // 64), dtype=np.int8)
+        for u in shared[shared["head"] == head]:
+            for c in range(int(u["col0"]), int(u["col0"] + u["cols"])):
+                seen[int(u["lane"]) + c // 8, c % 8, int(u["begin"]) // 64:int(u["end"]) // 64] += 1
+        assert np.all(seen[live] == 1) and np.all(seen[:live[0]] == 0) and np.all(seen[live[-1] + 1:] == 0)
+    used = set()
+    for i, rec in enumerate(records):
+        assert rec["tokens"] == counts[i] and bool(rec["merged"]) == (i in live) and (i in live or rec["prefix_count"] == rec["tail_count"] == 0)
+        mine = [int(rec["prefix_slot"]) + k * int(rec["prefix_stride"]) for k in range(int(rec["prefix_count"]))]
+        mine += [int(rec["tail_slot"]) + k for k in range(int(rec["tail_count"]))]
+        assert not used.intersection(mine) and all(m < plan.slot_count for m in mine)
+        used.update(mine)
+
+
 @pytest.mark.parametrize("heads,dim,group,lanes,prefix,own", [
     (1, 64, 8, 512, 8192, 100), (1, 128, 8, 256, 8192, 100), (2, 128, 16, 256, 8192, 100), (2, 64, 8, 600, 4096, 1),
     (4, 64, 8, 512, 16384, 100), (4, 128, 4, 500, 2048, 30), (3, 96, 5, 300, 8192, 700), (1, 64, 64, 512, 4096, 100)])
