@@ -630,7 +630,7 @@ kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint
  * or not as planned, or whose prefix is read through such a lane's table, sets
  * KIMKV_FAULT_DECODE_ITEM and is skipped.  Results as
  * kimkv_paged_decode_batch's to the decode tolerance, the same for every run
- * of one plan.  The storage's device is the current one. */
+ * of one plan; a NaN score makes its row NaN.  The storage's device is the current one. */
 kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv_decode_item* device_items,
                                        const void* device_entries, const kimkv_shared_plan* plan, void* workspace,
                                        kimkv_stream_t stream);

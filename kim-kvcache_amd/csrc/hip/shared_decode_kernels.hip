@@ -200,6 +200,9 @@ __device__ inline float read_lane(float v, uint32_t lane)
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), static_cast<int>(lane)));
 }
 
+// Whether a part of denominator l that weighs `factor` is left out: where it weighs nothing, unless a score was NaN.
+__device__ inline bool left_out(float factor, float l) { return factor == 0.0f && l == l; }
+
 // Parts of kRows rows: lane i holds o[r][k] of dim i + 64 k, every lane m and l.
 struct RowParts {
     float o[kRows][4];
@@ -256,9 +259,11 @@ __device__ void attend_rows_generic(const PoolView& P, const kimkv_decode_item& 
 #pragma unroll
         for (uint32_t r = 0; r < kRows; ++r) {
             s[r] = hb != nullptr ? s[r] * rows[r].scale2 : -INFINITY;
+            // The maximum passes over NaN scores; their weights carry them into the sum.
             float const m_new = fmaxf(out.m[r], wave_max(s[r]));
+            float const m_top = m_new == -INFINITY ? 0.0f : m_new;
             float const alpha = m_new == -INFINITY ? 1.0f : exp2f(out.m[r] - m_new);
-            p[r] = hb != nullptr && m_new != -INFINITY ? exp2f(s[r] - m_new) : 0.0f;
+            p[r] = hb != nullptr ? exp2f(s[r] - m_top) : 0.0f;
             out.l[r] = out.l[r] * alpha + wave_sum(p[r]);
             out.m[r] = m_new;
 #pragma unroll
@@ -359,7 +364,7 @@ __device__ void unit_generic(const PoolView& P, const SharedArgs& a, const Share
             float l = 0.0f;
             for (uint32_t s = 0; s < split; ++s) {
                 float const f = lds.m[w + s][r] == -INFINITY ? 0.0f : exp2f(lds.m[w + s][r] - M);
-                if (f == 0.0f) continue;   // whatever V made of it, as for a key of weight 0
+                if (left_out(f, lds.l[w + s][r])) continue;
                 o += f * lds.o[w + s][r][d];
                 l += f * lds.l[w + s][r];
             }
@@ -1008,7 +1013,7 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
 #pragma unroll
             for (uint32_t j = 0; j < kMergeBatch; ++j) {
                 float const f = ml[j].x == -INFINITY ? 0.0f : exp2f(ml[j].x - M);
-                if (f == 0.0f) continue;   // whatever V made of it, as for a key of weight 0
+                if (left_out(f, ml[j].y)) continue;
                 o += f * row[j];
                 l += f * ml[j].y;
             }
@@ -1018,8 +1023,7 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
             float const m_new = fmaxf(M, other);
             float const f = M == -INFINITY ? 0.0f : exp2f(M - m_new);
             M = m_new;
-            // A side of no weight hands over nothing, whatever it holds.
-            l = f == 0.0f ? 0.0f : f * l;
+            l = left_out(f, l) ? 0.0f : f * l;
             l += __shfl_xor(l, static_cast<int>(step));
 #pragma unroll
             for (uint32_t k = 0; k < kWidth; ++k) {

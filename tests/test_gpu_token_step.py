@@ -615,6 +615,37 @@ def test_shared_decode_all_scores_minus_infinity(dev):
             assert np.all(np.abs(got[i, 4:].astype(np.float64) - want) <= bound)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("lanes,prefix,units", [(3, 960, 4), (24, 960, 4), (2, 13000, 2000)])
+@pytest.mark.parametrize("where", ["query", "one key", "first keys", "prefix", "own key"])
+def test_shared_decode_nan_scores(dev, dim, lanes, prefix, units, where):
+    """A score that is NaN makes its row NaN wherever its key lies, also where a step, a unit or a whole part has no other
+    score; rows without one are as they should be."""
+    print(f"shared NaN {where} D={dim} lanes={lanes} prefix={prefix}", flush=True)
+    keys = {"query": (0, 0), "one key": (70, 71), "first keys": (0, 64), "prefix": (0, prefix), "own key": (prefix, prefix + 1)}[where]
+
+    def spread(rng, i, k, v):
+        k[keys[0]:keys[1], 1, 3] = np.nan
+
+    b = _Batch(dev, 2, dim, 4, [prefix + 1 + i for i in range(lanes)], [(0, lanes, prefix)], spread=spread, q_scale=1.0)
+    bad = np.zeros((lanes, 8), dtype=bool)
+    if where == "query":
+        b.query[1, 2, 5] = np.nan
+        bad[1, 2] = True
+    else:
+        bad[:, 4:] = True
+    b.place()
+    b.plan(units)
+    b.launch()
+    got = b.outputs().view(np.float16)
+    assert np.all(np.isnan(got[bad]))
+    for i in range(lanes):
+        query, k = np.nan_to_num(b.query[i]), np.nan_to_num(b.k[i])
+        want, bound = reference(query, k, b.v[i], float(b.scale[i]))
+        ok = np.abs(got[i].astype(np.float64) - want) <= bound
+        assert np.all(ok[~bad[i]]), i
+
+
 def test_shared_decode_two_at_once(dev):
     """Two launches of one plan on two streams, each with a workspace and outputs of its own, and one on the first's
     stream again."""
