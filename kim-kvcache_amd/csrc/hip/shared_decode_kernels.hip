@@ -200,6 +200,9 @@ __device__ inline float read_lane(float v, uint32_t lane)
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), static_cast<int>(lane)));
 }
 
+// A sum of weighted values under a new reference: 0 where it weighs nothing, whatever V made of it.
+__device__ inline float carried(float o, float factor) { return factor == 0.0f ? 0.0f : o * factor; }
+
 // Whether a part of denominator l that weighs `factor` is left out: where it weighs nothing, unless a score was NaN.
 __device__ inline bool left_out(float factor, float l) { return factor == 0.0f && l == l; }
 
@@ -267,7 +270,7 @@ __device__ void attend_rows_generic(const PoolView& P, const kimkv_decode_item& 
             out.l[r] = out.l[r] * alpha + wave_sum(p[r]);
             out.m[r] = m_new;
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) out.o[r][k] *= alpha;
+            for (uint32_t k = 0; k < 4; ++k) out.o[r][k] = carried(out.o[r][k], alpha);
         }
         const uint16_t* const vb = hb != nullptr ? hb + v_offset(cap, D, pt, 0) : nullptr;
         auto const vb_lo = static_cast<int>(reinterpret_cast<uintptr_t>(vb));
@@ -1008,7 +1011,8 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
             for (uint32_t j = 0; j < kMergeBatch; ++j) m_new = fmaxf(m_new, ml[j].x);
             float const c = M == -INFINITY ? 0.0f : exp2f(M - m_new);
             M = m_new;
-            o *= c;
+#pragma unroll
+            for (uint32_t k = 0; k < kWidth; ++k) o[k] = carried(o[k], c);
             l *= c;
 #pragma unroll
             for (uint32_t j = 0; j < kMergeBatch; ++j) {
@@ -1027,7 +1031,7 @@ __global__ __launch_bounds__(kMergeBlock) void shared_merge_kernel(PoolView P, S
             l += __shfl_xor(l, static_cast<int>(step));
 #pragma unroll
             for (uint32_t k = 0; k < kWidth; ++k) {
-                float const v = f == 0.0f ? 0.0f : f * o[k];
+                float const v = carried(o[k], f);
                 o[k] = v + __shfl_xor(v, static_cast<int>(step));
             }
         }

@@ -646,6 +646,27 @@ def test_shared_decode_nan_scores(dev, dim, lanes, prefix, units, where):
         assert np.all(ok[~bad[i]]), i
 
 
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("low,prefix,units", [(64, 960, 4), (960, 960, 4), (500, 30000, 2000), (30000, 30000, 2000)])
+def test_shared_decode_infinite_value_overtaken(dev, dim, low, prefix, units):
+    """An infinite V of a key that outweighs all keys before it and weighs nothing beside those behind it is left out, as
+    where it weighs nothing from the start."""
+    print(f"shared overtaken D={dim} low={low} prefix={prefix}", flush=True)
+
+    def spread(rng, i, k, v):
+        k[:low, :, 0] = -60000.0
+        v[3, 0, 5], v[40, 1, 7] = np.inf, -np.inf
+
+    b = _Batch(dev, 2, dim, 4, [prefix + 50, prefix + 9], [(0, 2, prefix)], spread=spread, q_scale=1.0)
+    b.query[:, :, 0] = 4.0
+    b.place()
+    b.plan(units)
+    b.launch()
+    for v in b.v:
+        v[3, 0, 5] = v[40, 1, 7] = 0
+    b.check(b.outputs())
+
+
 def test_shared_decode_two_at_once(dev):
     """Two launches of one plan on two streams, each with a workspace and outputs of its own, and one on the first's
     stream again."""
