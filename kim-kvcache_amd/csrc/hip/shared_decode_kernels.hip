@@ -1095,6 +1095,10 @@ struct Planned {
     uint32_t waves{0};         // of a workgroup
 };
 
+// A launch takes fewer than 2^32 threads.
+constexpr uint32_t most_units(uint32_t waves) { return 0xFFFFFFFFu / (waves * kWave); }
+constexpr uint32_t kMostLanes = 0xFFFFFFFFu / kMergeBlock;
+
 uint64_t align16(uint64_t n) { return (n + 15) / 16 * 16; }
 
 // Spreads the units over the XCDs (workgroup w runs on XCD w % 8): units of
@@ -1415,6 +1419,14 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
         }
     }
     UnitCost const cost{D, shape.waves};
+    uint64_t units = 0;
+    each_piece(
+        shape, work, cut,
+        [&](Work::Prefix const& p, uint32_t piece) { units += (p.tokens + piece - 1ull) / piece * H * p.tiles; },
+        [&](uint32_t, uint32_t own, uint32_t piece) {
+            units += (own + piece - 1ull) / piece * ((H + cut.heads - 1) / cut.heads) * ((G + 15ull) / 16);
+        });
+    if (units > most_units(shape.waves)) return false;
     out.waves = shape.waves;
     out.lanes.resize(lane_count);
     for (uint32_t i = 0; i < lane_count; ++i) out.lanes[i] = SharedLane{i, tokens[i], 0, 0, 0, 0, 0, 0};
@@ -1477,14 +1489,14 @@ bool plan_batch(uint32_t H, uint32_t D, uint32_t QH, uint32_t compute_units, con
                 if (!single) out.slots += 1;
             }
         });
-    if (!fits || out.units.size() > 0x7FFFFFF0u) return false;
+    if (!fits) return false;
     for (SharedLane& lane : out.lanes) {
         lane.merged = lane.prefix_count + lane.tail_count != 0 ? 1 : 0;
         out.merge_lanes += lane.merged;
         out.merge_parts = std::max(out.merge_parts, lane.prefix_count + lane.tail_count);
     }
     place_units(out, shape.at_once);
-    return true;
+    return out.units.size() <= most_units(shape.waves);
 }
 
 }  // namespace
@@ -1503,7 +1515,7 @@ kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint
     *plan = kimkv_shared_plan{};
     if ((lane_count != 0 && token_counts == nullptr) || (group_count != 0 && groups == nullptr) || query_heads == 0
         || kv_heads == 0 || query_heads % kv_heads != 0 || kv_heads > 0xFFFFu || head_dim == 0 || head_dim > kMaxDim
-        || lane_count > 0x7FFFFFFFu) {
+        || lane_count > kMostLanes) {
         return KIMKV_INVALID_ARGUMENT;
     }
     try {
@@ -1548,8 +1560,9 @@ kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv
     if (plan->unit_count == 0) return KIMKV_OK;
     uint64_t const o_bytes = align16(parts_o_floats(plan->slot_count, plan->query_heads, D) * sizeof(float));
     if (device_items == nullptr || device_entries == nullptr || plan->lane_count == 0 || plan->query_heads == 0 || H == 0
-        || plan->query_heads % H != 0 || D > kMaxDim || (plan->waves != kManyWaves && plan->waves != kFewWaves) || plan->merge_split == 0 || plan->merge_split > 8
-        || (plan->merge_split & (plan->merge_split - 1)) != 0 || plan->unit_count > 0x7FFFFFFFu
+        || plan->query_heads % H != 0 || D > kMaxDim || (plan->waves != kManyWaves && plan->waves != kFewWaves)
+        || plan->merge_split == 0 || plan->merge_split > 8 || (plan->merge_split & (plan->merge_split - 1)) != 0
+        || plan->unit_count > most_units(plan->waves) || plan->lane_count > kMostLanes
         || (reinterpret_cast<uintptr_t>(device_entries) & 15u) != 0
         || plan->entry_bytes != plan->unit_count * sizeof(SharedUnit) + plan->lane_count * sizeof(SharedLane)
         || plan->workspace_bytes != o_bytes + static_cast<uint64_t>(plan->slot_count) * plan->query_heads * sizeof(float2)

@@ -166,6 +166,18 @@ def test_plan_refusals(kimkv):
     assert max(u["end"] for u in units if u["cols"] > 8) == 4000 // 64 * 64
 
 
+@pytest.mark.parametrize("heads,dim,query_heads,lanes", [(1, 64, 1 << 28, 1), (65535, 8, 65535, 4200), (1, 64, 0xFFFFFFFF, 1), (1, 64, 8, 1 << 24)])
+def test_plan_refuses_what_no_launch_takes(kimkv, heads, dim, query_heads, lanes):
+    """A plan of more units than a launch has workgroups for is refused before it is made, and so is one of more lanes."""
+    d = kimkv.device
+    counts = np.zeros(lanes, dtype=np.uint32)
+    counts[:4200] = 64
+    plan = d.SharedPlan()
+    assert d.lib().kimkv_shared_decode_plan(heads, dim, query_heads, 256, counts.ctypes.data_as(ctypes.c_void_p), lanes, None, 0, None, 0,
+                                            ctypes.byref(plan)) == d.INVALID_ARGUMENT
+    assert plan.entry_bytes == 0 and plan.unit_count == 0
+
+
 def test_entry_points_refuse_null(kimkv):
     d = kimkv.device
     lib = d.lib()
