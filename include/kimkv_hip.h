@@ -277,8 +277,9 @@ typedef struct kimkv_append_rope_job {
  * overlaps qkv in no other way.  Angles are reduced in 64 bits, so they are
  * as exact at position 2^32 - 1 as at 1.  Jobs are in memory the device
  * reads; max_token_count is the largest token_count among them.  No two jobs
- * write the same page token or name the same row, and none copies from a page
- * that another one writes.  Page tokens that no job names, and rows of q_out,
+ * write the same page token or name the same row, and none copies page tokens
+ * that another one writes; any number may copy from one page, while another
+ * writes on behind what they copy.  Page tokens that no job names, and rows of q_out,
  * stay as they are.  A job that names no page of the storage, tokens past the
  * page, rows past `rows`, more than max_token_count tokens, positions past
  * 2^32 - 1 or an invalid copy sets KIMKV_FAULT_APPEND_JOB and is skipped.

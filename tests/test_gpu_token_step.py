@@ -187,6 +187,19 @@ def test_append_rope_other_pages(dev, tokens):
     assert t.storage.faults() == (0, 0)
 
 
+@pytest.mark.parametrize("heads,dim,group", [(4, 64, 8), (8, 128, 4), (2, 12, 2)])
+def test_append_rope_fork_from_one_page(dev, heads, dim, group):
+    """Requests leave one shared partial page, each with a copy of its own, while its last holder writes on behind what they
+    copy; a micro page and an extent page, of which one goes on by a whole group of 8."""
+    print(f"append_rope fork H={heads} D={dim}", flush=True)
+    t = _Append(dev, heads, dim)
+    jobs = [_job(i, 1, 5, 0, 1 + i, 5, (0, 0, 5)) for i in range(12)] + [_job(12, 1, 5, 0, 0, 5)]
+    jobs += [_job(13, 1, 3, 0, 14, 3, (0, 0, 3)), _job(14, 2, 4, 0, 15, 4, (0, 0, 4))]
+    jobs += [_job(16 + i, 1, 40, 1, 1 + i, 40, (1, 0, 40)) for i in range(3)] + [_job(19, 12, 40, 1, 0, 40), _job(31, 3, 37, 1, 4, 37, (1, 0, 37))]
+    _run_append(t, jobs, 34, group, dev.Rope(10000.0, dim, 0), layer=1)
+    assert t.storage.faults() == (0, 0)
+
+
 def test_append_rope_equals_split_and_append_at_near_positions(dev):
     """What the rotation and the append do in two calls, to the angles' last bits."""
     heads, dim, group, rows = 4, 64, 8, 40
