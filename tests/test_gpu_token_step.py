@@ -218,6 +218,37 @@ def test_append_rope_equals_split_and_append_at_near_positions(dev):
     assert np.all(np.abs(got - two) <= 2 * FP16 * np.abs(two) + 1e-3)
 
 
+@pytest.mark.parametrize("heads,dim,rotary", [(258, 128, 128), (1, 33024, 512)])
+@pytest.mark.parametrize("adjacent", [0, 1])
+def test_append_rope_past_32_bit_offsets(dev, heads, dim, rotary, adjacent):
+    """Pages of 65528 tokens whose last heads' blocks, or last dims' V rows, begin more than 2^32 elements into the page: a
+    prompt's rows, then a copied tail and the token after it."""
+    print(f"append_rope huge H={heads} D={dim}", flush=True)
+    storage = dev.Storage(1, heads, dim, 1, 2, 8, 65528)
+    rng = np.random.default_rng(heads)
+    qkv = _fp16(rng, 9, 3 * heads, dim)
+    width = 3 * heads * dim
+    src, q = dev.upload(_bits(qkv)), dev.upload(np.full((9, heads * dim), 0x1234, np.uint16))
+    rope = dev.Rope(500000.0, rotary, adjacent)
+    for job in [(0, 8, 70000, 0, 0, 0, 0, 1, 0, 0), (8, 1, 3, 1, 0, 5, 5, 1, 1, 0)]:
+        table = dev.upload(np.array([job], dtype=dev.APPEND_ROPE_JOB))
+        storage.append_rope_launch(table.ptr, 1, job[1], 0, src.ptr, width, 9, heads, rope, q.ptr, heads * dim)
+        dev.sync()
+    positions = np.array([*range(70000, 70008), 3], dtype=np.uint64)
+    want, size = _rotate(qkv[:, :2 * heads], positions, 500000.0, rotary, adjacent)
+    desc = lambda slot, n: np.array([(slot, 1, 0, n, 65528, 1)], dtype=helpers.DESC)  # noqa: E731
+    held = storage.gather(desc(0, 8), 8).view(np.float16).reshape(2, 8, heads, dim)
+    _near(held[0], want[:8, heads:], size[:8, heads:], positions[:8])
+    assert np.array_equal(_bits(held[1]), _bits(qkv[:8, 2 * heads:]))
+    fork = storage.gather(desc(1, 6), 6).view(np.float16).reshape(2, 6, heads, dim)
+    assert np.array_equal(_bits(fork[:, :5]), _bits(held[:, :5]))
+    _near(fork[0, 5:], want[8:, heads:], size[8:, heads:], positions[8:])
+    assert np.array_equal(_bits(fork[1, 5]), _bits(qkv[8, 2 * heads:]))
+    got = dev.download(q.ptr, (9, heads, dim), np.uint16).view(np.float16)
+    _near(got, want[:, :heads], size[:, :heads], positions)
+    assert storage.faults() == (0, 0)
+
+
 def test_append_rope_faults(dev):
     """Jobs that name what is not there are reported and change nothing; the good one beside them runs."""
     t = _Append(dev, 4, 64)
