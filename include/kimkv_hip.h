@@ -274,8 +274,9 @@ typedef struct kimkv_append_rope_job {
  * kv_heads][head_dim] fp16, rows are qkv_stride elements apart, rows of q_out
  * ([query_heads][head_dim]) q_stride.  q_out may be NULL (only K and V are
  * wanted), or qkv with q_stride = qkv_stride (queries rotated in place); it
- * overlaps qkv in no other way.  Angles are reduced in 64 bits, so they are
- * as exact at position 2^32 - 1 as at 1.  Jobs are in memory the device
+ * overlaps qkv in no other way.  Angles are formed and reduced in 64 bits:
+ * off by at most 6 * 2^-53 radians a position (3e-6 at position 2^32 - 1)
+ * before the 32-bit sines and products.  Jobs are in memory the device
  * reads; max_token_count is the largest token_count among them.  No two jobs
  * write the same page token or name the same row, and none copies page tokens
  * that another one writes; any number may copy from one page, while another
@@ -695,7 +696,9 @@ kimkv_status kimkv_reference_attention(const kimkv_storage* storage,
 /* Summed duration (ms) and count of the decode kernels timed since the last
  * call, measured with events on the launch stream; for the benchmark's
  * roofline.  `enable` > 0 times every enable-th launch from now on (the events
- * around a launch cost the stream a few microseconds), 0 stops timing. */
+ * around a launch cost the stream a few microseconds), 0 stops timing.  Of
+ * kimkv_paged_decode_batch and kimkv_shared_decode_batch that is the launch
+ * that reads keys and values, not the merge behind it. */
 kimkv_status kimkv_decode_timing(int enable, double* total_ms, uint64_t* launches);
 /* The same for the chunked-prefill attention kernel (same `enable`). */
 kimkv_status kimkv_prefill_timing(int enable, double* total_ms, uint64_t* launches);

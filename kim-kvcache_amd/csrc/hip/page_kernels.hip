@@ -308,10 +308,10 @@ __global__ __launch_bounds__(kBlock) void append_kernel(PoolView P, const kimkv_
 // dimensions and 104 so; contiguous runs of jobs for an XCD leave the XCDs of a
 // mixed batch unlike loads (9.7 for 8.2 us).  Rows of q and K are whole lines
 // and are stored past the caches (95 us); V^T is not (152 us when its quarters
-// go to memory one by one).  Bound by HBM for prompts, 87 to 94 us for those
-// 369 MB where a large copy's rate (4.8 TB/s) makes 77; by the launch and the
-// chain of job, angle, row and store for a token step, 4.8 us for 4 or 128
-// lanes.
+// go to memory one by one).  Bound by HBM for prompts, 87 to 95 us for those
+// 369 MB where the best copy's rate (6.03 TB/s) makes 61; by the launch and the
+// chain of job, angle, row and store for a token step, 4.3 to 5.1 us for 4 or
+// 128 lanes.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kRopeGroup = 8;          // page tokens a block takes
 constexpr uint32_t kMaxRopePairs = 256;

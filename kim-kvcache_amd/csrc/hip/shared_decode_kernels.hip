@@ -37,7 +37,9 @@ namespace {
 // 4 lanes of 500 tokens 10.4 and 9.2 us, eight groups of four 21.8 and 20.1);
 // one starts half as many units for the same keys, which long ones on many
 // columns gain by (64 lanes of 128 dims on 4100 tokens 35.2 and 38.9 us, 128
-// lanes on 16384 54.7 and 58.5).
+// lanes on 16384 54.7 and 58.5).  (Passes over one set of inputs, which the
+// caches hold in part; the first two take 9.0 and 22.0, the third 36.1 with
+// inputs from memory.)
 constexpr uint32_t kManyWaves = 8;
 constexpr uint32_t kFewWaves = 4;
 constexpr uint32_t kMaxDim = 256;
@@ -391,7 +393,7 @@ __device__ void unit_generic(const PoolView& P, const SharedArgs& a, const Share
 // 32-key block are permuted (HeadGroup readers below) so that the layout S^T
 // leaves is the operand layout of P^T: lane l holds keys 8 (l / 16) .. + 7 of
 // column l % 16.  Weights go to the matrix cores in two fp16 parts, p = hi +
-// lo, which keep what 32-bit weights do to 2^-22.
+// lo, each cut off behind its bits, so a weight is kept to 2^-20 of itself.
 // ---------------------------------------------------------------------------
 // Weights are 2^(s - m + kWeightShift), at most 2^15, so that lo stays a
 // normal fp16 number down to 2^-9 of the largest weight.
