@@ -249,6 +249,57 @@ def test_append_rope_past_32_bit_offsets(dev, heads, dim, rotary, adjacent):
     assert storage.faults() == (0, 0)
 
 
+def test_append_rope_rows_and_pages_far_away(dev):
+    """Rows, queries and pages more than 2^32 elements from the start of their buffers, then attention to those pages."""
+    heads, dim, group, stride, pages = 8, 128, 4, (1 << 30) + 8, 40000
+    qh = heads * group
+    storage = dev.Storage(1, heads, dim, 8, pages)   # 131072 elements a page
+    rng = np.random.default_rng(31)
+    # Row 5 is a token, rows 0..4 are not named.  The pages' other tokens come from plain rows, unrotated.
+    far, q = dev.DeviceBuffer(6 * stride * 2), dev.DeviceBuffer(6 * stride * 2)
+    row = _fp16(rng, qh + 2 * heads, dim)
+    dev.copy_to_device(far.ptr + 2 * 5 * stride, _bits(row))
+    lanes, prefix, slots = 2, 128, [[pages - 1, pages - 5, pages - 2], [pages - 1, pages - 5, pages - 3]]
+    known = {slot: _fp16(rng, 64, qh + 2 * heads, dim) for slot in sorted({s for t in slots for s in t})}
+    jobs = np.zeros(1, dtype=dev.APPEND_ROPE_JOB)
+    for slot, x in known.items():
+        src = dev.upload(_bits(x))
+        jobs[0] = (0, 64, 0, slot, 0, 0, 0, 1, 0, 0)
+        table = dev.upload(jobs)
+        storage.append_rope_launch(table.ptr, 1, 64, 0, src.ptr, (qh + 2 * heads) * dim, 64, qh, dev.Rope(10000.0, 0, 0), 0, 0)
+        dev.sync()
+    rope, tokens = dev.Rope(10000.0, dim, 0), prefix + 40
+    jobs[0] = (5, 1, tokens - 1, slots[1][2], 0, (tokens - 1) % 64, 0, 1, 0, 0)
+    table = dev.upload(jobs)
+    storage.append_rope_launch(table.ptr, 1, 1, 0, far.ptr, stride, 6, qh, rope, q.ptr, stride)
+    dev.sync()
+    want, size = _rotate(row[None, :qh + heads], np.array([tokens - 1], np.uint64), 10000.0, dim, 0)
+    query = dev.download(q.ptr + 2 * 5 * stride, (qh, dim), np.uint16).view(np.float16)
+    _near(query[None], want[:, :qh], size[:, :qh], np.array([tokens - 1], np.uint64))
+    tables = [np.array([(s, 1, 64 * i, min(64, tokens - 64 * i), 64, 1) for i, s in enumerate(t)], dtype=dev.BLOCK_DESC) for t in slots]
+    held = [storage.gather(t, tokens).view(np.float16).reshape(2, tokens, heads, dim) for t in tables]
+    _near(held[1][0, -1:], want[:, qh:], size[:, qh:], np.array([tokens - 1], np.uint64))
+    assert np.array_equal(_bits(held[1][1, -1]), _bits(row[qh + heads:]))
+    for i in range(lanes):   # everything but the far token is as it was written
+        for part in range(2):
+            plain = np.concatenate([known[s][:, qh + part * heads:qh + (part + 1) * heads] for s in slots[i]])[:tokens - i]
+            assert np.array_equal(_bits(held[i][part, :tokens - i]), _bits(plain))
+    out = dev.upload(np.full((lanes, qh, dim), 0x1234, np.uint16))
+    on_gpu = [dev.upload(t) for t in tables]
+    items = np.zeros(lanes, dtype=dev.DECODE_ITEM)
+    for i in range(lanes):
+        items[i] = (on_gpu[i].ptr, len(tables[i]), tokens, 0, q.ptr + 2 * 5 * stride, 0, out.ptr + 2 * i * qh * dim, 1.0 / math.sqrt(dim))
+    entries, plan = dev.shared_decode_plan(heads, dim, qh, 1, [tokens] * lanes, [(0, lanes, prefix)])
+    buf, entries_buf, work = dev.upload(items), dev.upload(entries), dev.DeviceBuffer(max(16, plan.workspace_bytes))
+    storage.shared_decode_launch(buf.ptr, entries_buf.ptr, plan, work.ptr)
+    dev.sync()
+    got = dev.download(out.ptr, (lanes, qh, dim), np.uint16).view(np.float16)
+    for i in range(lanes):
+        want, bound = reference(query, held[i][0], held[i][1], 1.0 / math.sqrt(dim))
+        assert np.all(np.abs(got[i].astype(np.float64) - want) <= bound)
+    assert storage.faults() == (0, 0)
+
+
 def test_append_rope_faults(dev):
     """Jobs that name what is not there are reported and change nothing; the good one beside them runs."""
     t = _Append(dev, 4, 64)
@@ -1052,6 +1103,33 @@ def test_logits_scratch_of_a_larger_batch(dev, vocab, most, rows):
         dev.sync()
         assert np.array_equal(dev.download(tokens.ptr, (n,), np.uint32), x.argmax(1))
         assert np.all(dev.download(work.ptr, (need + 65536,), np.uint8)[need:] == 0x5A)
+
+
+def test_logits_rows_far_away(dev):
+    """Rows of more than 2^30 tokens, the last of them more than 2^32 logits from the first, in place."""
+    rows, vocab = 4, (1 << 30) + 400_000_001
+    buf = dev.DeviceBuffer(4 * rows * vocab)
+    dev.fill_rows(buf.ptr, 2 * rows * vocab, 3, 0, 256)   # pairs of fp16 numbers below 4 are fp32 numbers below 512
+    at = lambda r, t: buf.ptr + 4 * (r * vocab + t)   # noqa: E731
+    for r in range(rows):
+        for t, x in ((vocab - 2, 5000.0), (7 + r, 6000.0), (vocab // 2, 5050.0)):
+            dev.copy_to_device(at(r, t), np.array([x], np.float32))
+    tokens, work = dev.DeviceBuffer(4 * rows), dev.DeviceBuffer(dev.logits_workspace_bytes(rows, vocab))
+    history = dev.upload(np.array([8, 8, vocab // 2, 0xFFFFFFFF], np.uint32))
+    bias_tokens, bias_values = dev.upload(np.array([9, vocab - 1, 10], np.uint32)), dev.upload(np.array([-2000.0, 10000.0, -3000.0], np.float32))
+    table = np.zeros(rows, dtype=dev.LOGITS_RULE)
+    table["repetition_penalty"] = 1.0
+    table[1] = (history.ptr, 0, 0, 0, 4, 0, 4.0, 0.0, 0.0)   # tokens 8 and vocab / 2 fall to a quarter
+    table[2] = (0, bias_tokens.ptr, bias_values.ptr, 0, 0, 3, 1.0, 0.0, 0.0)
+    table[3] = (0, bias_tokens.ptr, bias_values.ptr, 0, 0, 3, 1.0, 0.0, 0.0)
+    rules = dev.upload(table)
+    dev.logits_adjust(buf.ptr, rows, vocab, rules.ptr, buf.ptr, tokens.ptr, work.ptr)
+    dev.sync()
+    picked = dev.download(tokens.ptr, (rows,), np.uint32)
+    read = lambda r, t: float(dev.download(at(r, t), (1,), np.float32)[0])   # noqa: E731
+    assert list(picked) == [7, vocab - 2, vocab - 1, vocab - 1]
+    assert (read(0, 7), read(1, 8), read(1, vocab // 2), read(1, vocab - 2)) == (6000.0, 1500.0, 1262.5, 5000.0)
+    assert (read(2, 9), read(3, 10), read(3, vocab // 2)) == (4000.0, 3000.0, 5050.0) and 9488.0 < read(3, vocab - 1) < 10512.0
 
 
 def test_logits_many_rows(dev):
