@@ -614,8 +614,8 @@ typedef struct kimkv_shared_plan {
  * plan->entry_bytes) for upload; KIMKV_INVALID_ARGUMENT when capacity is too
  * small (plan->entry_bytes then holds the size needed; entries may be NULL
  * with capacity 0), for groups that overlap or leave the batch, for lanes of 2^31
- * tokens or more, 2^24 lanes or more, or a batch of more work than one launch
- * takes (2^32 threads). */
+ * tokens or more, query rows of 2^31 elements or more, 2^24 lanes or more, or a
+ * batch of more work than one launch takes (2^32 threads). */
 kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint32_t query_heads,
                                       uint32_t compute_units, const uint32_t* token_counts, uint32_t lane_count,
                                       const kimkv_shared_group* groups, uint32_t group_count, void* entries,

@@ -1100,6 +1100,7 @@ struct Planned {
 // A launch takes fewer than 2^32 threads.
 constexpr uint32_t most_units(uint32_t waves) { return 0xFFFFFFFFu / (waves * kWave); }
 constexpr uint32_t kMostLanes = 0xFFFFFFFFu / kMergeBlock;
+constexpr uint32_t kMostRow = 0x7FFFFFFFu;   // elements of a lane's query, indexed in 32 bits
 
 uint64_t align16(uint64_t n) { return (n + 15) / 16 * 16; }
 
@@ -1517,7 +1518,7 @@ kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint
     *plan = kimkv_shared_plan{};
     if ((lane_count != 0 && token_counts == nullptr) || (group_count != 0 && groups == nullptr) || query_heads == 0
         || kv_heads == 0 || query_heads % kv_heads != 0 || kv_heads > 0xFFFFu || head_dim == 0 || head_dim > kMaxDim
-        || lane_count > kMostLanes) {
+        || static_cast<uint64_t>(query_heads) * head_dim > kMostRow || lane_count > kMostLanes) {
         return KIMKV_INVALID_ARGUMENT;
     }
     try {
@@ -1562,7 +1563,8 @@ kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv
     if (plan->unit_count == 0) return KIMKV_OK;
     uint64_t const o_bytes = align16(parts_o_floats(plan->slot_count, plan->query_heads, D) * sizeof(float));
     if (device_items == nullptr || device_entries == nullptr || plan->lane_count == 0 || plan->query_heads == 0 || H == 0
-        || plan->query_heads % H != 0 || D > kMaxDim || (plan->waves != kManyWaves && plan->waves != kFewWaves)
+        || plan->query_heads % H != 0 || static_cast<uint64_t>(plan->query_heads) * D > kMostRow || D > kMaxDim
+        || (plan->waves != kManyWaves && plan->waves != kFewWaves)
         || plan->merge_split == 0 || plan->merge_split > 8 || (plan->merge_split & (plan->merge_split - 1)) != 0
         || plan->unit_count > most_units(plan->waves) || plan->lane_count > kMostLanes
         || (reinterpret_cast<uintptr_t>(device_entries) & 15u) != 0

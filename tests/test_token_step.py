@@ -178,6 +178,18 @@ def test_plan_refuses_what_no_launch_takes(kimkv, heads, dim, query_heads, lanes
     assert plan.entry_bytes == 0 and plan.unit_count == 0
 
 
+def test_plan_refuses_rows_past_32_bit_offsets(kimkv):
+    """A lane's query row is indexed in 32 bits: one of 2^31 elements or more is refused, one just below is planned."""
+    d = kimkv.device
+    counts = np.array([64], dtype=np.uint32)
+    for query_heads, dim, want in ((1 << 25, 64, d.INVALID_ARGUMENT), (1 << 24, 128, d.INVALID_ARGUMENT), (1 << 23, 256, d.INVALID_ARGUMENT),
+                                   ((1 << 23) - 16, 255, d.OK)):
+        plan = d.SharedPlan()
+        entries = np.empty(1 << 26, dtype=np.uint8)
+        assert d.lib().kimkv_shared_decode_plan(1, dim, query_heads, 256, counts.ctypes.data_as(ctypes.c_void_p), 1, None, 0,
+                                                entries.ctypes.data_as(ctypes.c_void_p), len(entries), ctypes.byref(plan)) == want, (query_heads, dim)
+
+
 def test_entry_points_refuse_null(kimkv):
     d = kimkv.device
     lib = d.lib()
