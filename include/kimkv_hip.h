@@ -268,20 +268,20 @@ typedef struct kimkv_append_rope_job {
 
 /* Batched append of one layer straight from the fused projection, rotated on
  * the way: of each job's rows the keys are rotated into the page, the values
- * copied into it, and the queries rotated to q_out, in one launch (the
- * results of kimkv_model_rope_split followed by kimkv_append_batch, without
- * the K and V rows in between).  A row of qkv is [query_heads | kv_heads |
+ * copied into it, and the queries rotated to q_out, in one launch (the results
+ * of kimkv_model_rope_split followed by kimkv_append_batch, without the K and
+ * V rows in between).  A row of qkv is [query_heads | kv_heads |
  * kv_heads][head_dim] fp16, rows are qkv_stride elements apart, rows of q_out
  * ([query_heads][head_dim]) q_stride.  q_out may be NULL (only K and V are
  * wanted), or qkv with q_stride = qkv_stride (queries rotated in place); it
- * overlaps qkv in no other way.  Angles are formed and reduced in 64 bits:
- * off by at most 6 * 2^-53 radians a position (3e-6 at position 2^32 - 1)
- * before the 32-bit sines and products.  Jobs are in memory the device
- * reads; max_token_count is the largest token_count among them.  No two jobs
- * write the same page token or name the same row, and none copies page tokens
- * that another one writes; any number may copy from one page, while another
- * writes on behind what they copy.  Page tokens that no job names, and rows of q_out,
- * stay as they are.  A job that names no page of the storage, tokens past the
+ * overlaps qkv in no other way.  Angles are formed and reduced in 64 bits: off
+ * by at most 6 * 2^-53 radians a position for theta of 1 or more (3e-6 at
+ * position 2^32 - 1) before the 32-bit sines and products.  Jobs are in memory
+ * the device reads; max_token_count is the largest token_count among them.  No
+ * two jobs write the same page token or name the same row, and none copies
+ * page tokens that another one writes; any number may copy from one page,
+ * while another writes on behind what they copy.  Page tokens and rows of
+ * q_out that no job names stay as they are.  A job that names no page of the storage, tokens past the
  * page, rows past `rows`, more than max_token_count tokens, positions past
  * 2^32 - 1 or an invalid copy sets KIMKV_FAULT_APPEND_JOB and is skipped.
  * Vector accesses where head_dim and the strides are multiples of 8, the
@@ -605,35 +605,35 @@ typedef struct kimkv_shared_plan {
 /* Plans one layer's decode attention of a batch whose lanes share prefixes
  * (pure host code, the same for every layer of a token step).  compute_units
  * is the device's (the storage's kimkv_storage_info; 0: 256), token_counts
- * each lane's tokens; the groups name disjoint runs of lanes, and lanes
- * in none share nothing.  Lanes of no tokens may stand anywhere in the batch
- * and in its groups.  A group's prefix is read through the table of its first
- * lane that has tokens, once for all of these; of it the plan takes whole
- * blocks of 64 tokens that all of them hold, none where that would not pay,
- * and the rest of each lane is read through the lane's own table.  Fills entries[0 ..
+ * each lane's tokens; the groups name disjoint runs of lanes, and lanes in
+ * none share nothing.  Lanes of no tokens may stand anywhere in the batch and
+ * in its groups.  A group's prefix is read through the table of its first lane
+ * that has tokens, once for all of these; of it the plan takes whole blocks of
+ * 64 tokens that all of them hold, none where that would not pay, and the rest
+ * of each lane is read through the lane's own table.  Fills entries[0 ..
  * plan->entry_bytes) for upload; KIMKV_INVALID_ARGUMENT when capacity is too
  * small (plan->entry_bytes then holds the size needed; entries may be NULL
- * with capacity 0), for groups that overlap or leave the batch, for lanes of 2^31
- * tokens or more, query rows of 2^31 elements or more, 2^24 lanes or more, or a
- * batch of more work than one launch takes (2^32 threads). */
+ * with capacity 0), for groups that overlap or leave the batch, for lanes of
+ * 2^31 tokens or more, query rows of 2^31 elements or more, 2^24 lanes or
+ * more, or a batch of more work than one launch takes (2^32 threads). */
 kimkv_status kimkv_shared_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint32_t query_heads,
                                       uint32_t compute_units, const uint32_t* token_counts, uint32_t lane_count,
                                       const kimkv_shared_group* groups, uint32_t group_count, void* entries,
                                       uint64_t capacity, kimkv_shared_plan* plan);
 
-/* kimkv_paged_decode_batch of the planned batch, with the shared prefixes
- * read and multiplied once for all lanes of a group.  device_items: the lanes'
+/* kimkv_paged_decode_batch of the planned batch, with the shared prefixes read
+ * and multiplied once for all lanes of a group.  device_items: the lanes'
  * items, whole tables and token counts as planned (their workspace is not
  * used); device_entries: the plan's entries (made for the storage's heads and
- * head dim); workspace: plan->workspace_bytes
- * of device memory, contents ignored, not shared with a launch that may
- * overlap this one.  Lanes of one group name the same layer.  A lane planned
- * with no tokens is skipped, whatever its item holds (its output is not
- * written); a lane whose item is invalid
- * or not as planned, or whose prefix is read through such a lane's table, sets
- * KIMKV_FAULT_DECODE_ITEM and is skipped.  Results as
+ * head dim); workspace: plan->workspace_bytes of device memory, contents
+ * ignored, not shared with a launch that may overlap this one.  Lanes of one
+ * group name the same layer.  A lane planned with no tokens is skipped,
+ * whatever its item holds (its output is not written); a lane whose item is
+ * invalid or not as planned, or whose prefix is read through such a lane's
+ * table, sets KIMKV_FAULT_DECODE_ITEM and is skipped.  Results as
  * kimkv_paged_decode_batch's to the decode tolerance, the same for every run
- * of one plan; a NaN score makes its row NaN.  The storage's device is the current one. */
+ * of one plan; a NaN score makes its row NaN.  The storage's device is the
+ * current one. */
 kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv_decode_item* device_items,
                                        const void* device_entries, const kimkv_shared_plan* plan, void* workspace,
                                        kimkv_stream_t stream);
