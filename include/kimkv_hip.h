@@ -281,9 +281,10 @@ typedef struct kimkv_append_rope_job {
  * two jobs write the same page token or name the same row, and none copies
  * page tokens that another one writes; any number may copy from one page,
  * while another writes on behind what they copy.  Page tokens and rows of
- * q_out that no job names stay as they are.  A job that names no page of the storage, tokens past the
- * page, rows past `rows`, more than max_token_count tokens, positions past
- * 2^32 - 1 or an invalid copy sets KIMKV_FAULT_APPEND_JOB and is skipped.
+ * q_out that no job names stay as they are.  A job that names no page of the
+ * storage, tokens past the page, rows past `rows`, more than max_token_count
+ * tokens, positions past 2^32 - 1 or an invalid copy sets
+ * KIMKV_FAULT_APPEND_JOB and is skipped.
  * Vector accesses where head_dim and the strides are multiples of 8, the
  * rotary dim of 16 (8 for adjacent pairs) and the addresses 16-byte aligned;
  * anything else goes element by element.  The storage's device is the current
