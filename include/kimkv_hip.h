@@ -639,6 +639,131 @@ kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv
                                        const void* device_entries, const kimkv_shared_plan* plan, void* workspace,
                                        kimkv_stream_t stream);
 
+/* ---- cache in 8 bits -------------------------------------------------------
+ * The same micro and extent pages, tables and jobs over a storage that holds K
+ * and V in 8 bits: about half the bytes of kimkv_storage, and half the time of
+ * what reads them.  No counterpart in the reference.
+ *
+ * A row is the D values of one token's K or V of one head.  It is held as D
+ * codes and one scale s: with a the largest |x| of the row, s is the smallest
+ * number of 8 significant bits that is at least a / 127 (whole numbers) or a /
+ * 448 (e4m3), and each code is x / s rounded to nearest, ties to even.  A row
+ * of zeros holds zeros; a row with an infinity or a NaN reads as NaN
+ * throughout. */
+#define KIMKV_QUANT_INT8 1u   /* whole numbers -127 .. 127 */
+#define KIMKV_QUANT_E4M3 2u   /* 4 bits of exponent, 3 of mantissa, largest 448 */
+
+typedef struct kimkv_quant_storage kimkv_quant_storage;
+
+typedef struct kimkv_quant_storage_info {
+    kimkv_layout layout;
+    uint32_t format;
+    uint32_t micro_capacity;
+    uint32_t extent_capacity;
+    uint16_t micro_page_tokens;
+    uint16_t extent_page_tokens;
+    uint32_t reserved;
+    uint64_t micro_page_bytes;    /* one page, every layer */
+    uint64_t extent_page_bytes;
+    uint64_t reserved_bytes;      /* both pools */
+    int device;
+    int compute_units;
+} kimkv_quant_storage_info;
+
+/* As kimkv_storage_create, on the current device, zero-filled.  Pages are of a
+ * multiple of 8 tokens, at most 64; head_dim is at most 256. */
+kimkv_status kimkv_quant_storage_create(kimkv_quant_storage** out, kimkv_layout layout, uint32_t format,
+                                        uint32_t micro_capacity, uint32_t extent_capacity,
+                                        uint16_t micro_page_tokens, uint16_t extent_page_tokens);
+kimkv_status kimkv_quant_storage_destroy(kimkv_quant_storage* storage);
+kimkv_status kimkv_quant_storage_query(const kimkv_quant_storage* storage, kimkv_quant_storage_info* info);
+/* As kimkv_storage_faults.  The storage's device is the current one, here and
+ * in every launch below (else KIMKV_INVALID_ARGUMENT). */
+kimkv_status kimkv_quant_storage_faults(kimkv_quant_storage* storage, kimkv_stream_t stream, uint32_t* faults);
+
+/* kimkv_append_batch into a quantised storage: each row of the jobs' fp16
+ * sources is quantised into its page, the copied tokens of a copy-on-write
+ * keep their codes and scales.  No two jobs write the same page token, and none
+ * copies page tokens that another one writes; any number may copy from one
+ * page, while another writes on behind what they copy.  Page tokens that no
+ * job names stay as they are.  A job that names no page of the storage, tokens
+ * past the page, layers past the storage's, no source, or copies more tokens
+ * than the page has or than lie below dst_token sets KIMKV_FAULT_APPEND_JOB and
+ * is skipped.  Vector accesses where head_dim and the token stride are
+ * multiples of 8 and the sources 16-byte aligned in every layer; anything else
+ * goes element by element. */
+kimkv_status kimkv_quant_append_batch(const kimkv_quant_storage* storage, const kimkv_append_job* device_jobs,
+                                      uint32_t job_count, uint32_t max_layer_count, kimkv_stream_t stream);
+
+/* Reads tokens [first_token, first_token + token_count) of a table back as
+ * fp16 rows, output [layer_count][K/V][token_count][head][dim] for layers
+ * [layer_begin, layer_begin + layer_count): each code times its scale, rounded
+ * once, kept to +-65504.  The table is sorted and may hold more tokens than are
+ * read (each entry costs a workgroup, so pass the part that is needed).  Tokens
+ * that it does not cover stay as they are in the output; an entry that names no
+ * page of the storage sets KIMKV_FAULT_GATHER_ENTRY and is left out.  Rows of
+ * one layer go into the sources of kimkv_append_batch as they are, for a
+ * prefill over pages of fp16. */
+#define KIMKV_FAULT_GATHER_ENTRY 0x10u
+kimkv_status kimkv_quant_gather(const kimkv_quant_storage* storage, const kimkv_block_desc* device_descriptors,
+                                uint32_t descriptor_count, uint32_t first_token, uint32_t token_count,
+                                uint32_t layer_begin, uint32_t layer_count, uint16_t* device_output,
+                                kimkv_stream_t stream);
+
+/* kimkv_promote_batch of quantised pages (of 8 and 64 tokens), codes and
+ * scales as they are.  A job that names no page of the storage sets
+ * KIMKV_FAULT_PROMOTION_JOB and is skipped. */
+kimkv_status kimkv_quant_promote_batch(const kimkv_quant_storage* storage, const kimkv_promotion_job* device_jobs,
+                                       uint32_t job_count, kimkv_stream_t stream);
+
+/* What kimkv_quant_decode_plan decided for a batch; kept with the entries it
+ * wrote and passed to kimkv_quant_decode_batch unchanged. */
+typedef struct kimkv_quant_plan {
+    uint64_t entry_bytes;       /* of the plan's entries, 16-byte aligned on the device */
+    uint64_t workspace_bytes;   /* of the launch's scratch, 16-byte aligned */
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t query_heads;
+    uint32_t lane_count;
+    uint32_t unit_count;
+    uint32_t slot_count;
+    uint32_t merge_lanes;
+    uint32_t reserved;
+} kimkv_quant_plan;
+
+/* Plans one layer's decode attention of a batch of lanes of token_counts
+ * tokens each (pure host code, the same for every layer of a token step).
+ * compute_units is the device's (0: 256).  Fills entries[0 ..
+ * plan->entry_bytes) for upload; KIMKV_INVALID_ARGUMENT when capacity is too
+ * small (plan->entry_bytes then holds the size needed; entries may be NULL with
+ * capacity 0), for head_dim above 256, query heads that are no multiple of the
+ * KV heads, lanes of 2^31 tokens or more, or a batch of more work than one
+ * launch takes (2^24 workgroups). */
+kimkv_status kimkv_quant_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint32_t query_heads, uint32_t compute_units,
+                                     const uint32_t* token_counts, uint32_t lane_count, void* entries, uint64_t capacity,
+                                     kimkv_quant_plan* plan);
+
+/* kimkv_paged_decode_batch of the planned batch over a quantised storage: each
+ * query attends to its lane's codes times their scales, scores, softmax and
+ * sums in 32 bits, one rounding to fp16.  device_items: the lanes' items, whole
+ * tables and token counts as planned (their workspace is not used);
+ * device_entries: the plan's entries (made for the storage's heads and head
+ * dim); workspace: plan->workspace_bytes of device memory, contents ignored,
+ * not shared with a launch that may overlap this one.  A lane planned with no
+ * tokens is skipped, whatever its item holds (its output is not written); a
+ * lane whose item is invalid or not as planned sets KIMKV_FAULT_DECODE_ITEM and
+ * is skipped.  Tokens whose table entry names no page of the storage set the
+ * same bit and take no part, nor do tokens that the table does not cover; where
+ * none is left the output is 0.  A row of K that reads as NaN makes the outputs
+ * of its head NaN, and so does one of V that has a weight above 0.  Head dims
+ * of 64, 96 and 128 with up to 16 query heads a KV head run on the matrix
+ * cores, as long as the tables keep groups of 8 tokens whole (every entry
+ * begins at a multiple of 8); others take a slower path.  Results are the same
+ * for every run of one plan. */
+kimkv_status kimkv_quant_decode_batch(const kimkv_quant_storage* storage, const kimkv_decode_item* device_items,
+                                      const void* device_entries, const kimkv_quant_plan* plan, void* workspace,
+                                      kimkv_stream_t stream);
+
 /* New tokens handled by one prefill workgroup (per KV head) for this
  * storage's shape and query head count: items need
  * ceil(new_tokens / this) workgroups each.  0 for an invalid head count. */
@@ -811,6 +936,42 @@ size_t kimkv_logits_workspace_bytes(uint32_t rows, uint32_t vocabulary);
 kimkv_status kimkv_model_logits_adjust(const float* logits, uint32_t rows, uint32_t vocabulary,
                                        const kimkv_logits_rule* device_rules, float* out, uint32_t* device_tokens,
                                        void* workspace, kimkv_stream_t stream);
+/* How a row's next token is drawn.  With T the temperature, x(v) the logits
+ * and m the highest of them, token v weighs e^((x(v) - m) / T).  In the order
+ * of falling logits, the lower token first among equals, the kept tokens are
+ * the first top_k (0: all), of these the shortest run whose weight is at least
+ * top_p of theirs (1: all), and of these the ones that weigh at least min_p of
+ * the first (0: all).  T = 0 keeps the first alone. */
+typedef struct kimkv_sample_rule {
+    float temperature;   /* >= 0 and finite */
+    float top_p;         /* above 0, at most 1 */
+    float min_p;         /* 0 .. 1 */
+    uint32_t top_k;
+} kimkv_sample_rule;
+
+/* Workspace of kimkv_model_sample for up to `rows` rows of up to `vocabulary`
+ * tokens (0 for shapes that need none): what is enough for a batch is enough
+ * for every smaller one. */
+size_t kimkv_sample_workspace_bytes(uint32_t rows, uint32_t vocabulary);
+
+/* The token that row r of logits[rows][vocabulary] (fp32; as
+ * kimkv_model_logits_adjust leaves them) gives by device_rules[r] and the
+ * random number device_uniforms[r] in [0, 1): the first token, in the order of
+ * the vocabulary, at which the kept tokens' weight up to it exceeds that part
+ * of all kept tokens' weight; with probabilities (NULL: not wanted) its weight
+ * as a part of theirs.  Weights and their sums are held in 63 bits, to 2^-46 of
+ * the highest token's at 131072 tokens and to fewer bits in a larger
+ * vocabulary, whatever the order they are added in, so a row gives the same
+ * token in every batch.  Logits of -inf and NaN are never drawn; among
+ * logits of +inf, these alone share the weight.  A row with nothing to draw, an
+ * invalid rule or a random number outside [0, 1) gives KIMKV_NO_TOKEN and
+ * probability 0.  workspace: kimkv_sample_workspace_bytes of at least these
+ * rows and this vocabulary, in device memory, 16-byte aligned, contents
+ * ignored, not shared with a call that may overlap this one (NULL where that is
+ * 0).  No counterpart in the reference, whose runner is greedy. */
+kimkv_status kimkv_model_sample(const float* logits, uint32_t rows, uint32_t vocabulary,
+                                const kimkv_sample_rule* device_rules, const float* device_uniforms,
+                                uint32_t* device_tokens, float* probabilities, void* workspace, kimkv_stream_t stream);
 /* Seeded weights: out[i] = fp16(float(synth(seed, row0 + i / cols, i % cols)) * scale). */
 kimkv_status kimkv_fill_rows_scaled(uint16_t* device_out, uint64_t count, uint64_t seed, uint64_t row0, uint32_t cols,
                                     float scale, kimkv_stream_t stream);

@@ -1,0 +1,646 @@
+// quant_page_kernels.hip -- a cache in 8 bits: its storage, append (with fused
+// partial-tail copy-on-write), read-back and promotion.  Formats and layout:
+// quant_common.h.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <limits>
+#include <mutex>
+#include <new>
+
+#include "quant_common.h"
+#include "runtime_internal.h"
+
+namespace kimkv {
+namespace {
+
+constexpr unsigned kBlock = 256;
+constexpr uint32_t kTileTokens = kQuantMaxPage;
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+// Bytes (r, c) of four words, byte c of word r, as four words, byte r of word c.
+__device__ inline void transpose_bytes(uint32_t (&w)[4])
+{
+    uint32_t const t0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);
+    uint32_t const t1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    uint32_t const u0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+    uint32_t const u1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(u0, t0, 0x05040100u);
+    w[1] = __builtin_amdgcn_perm(u0, t0, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(u1, t1, 0x05040100u);
+    w[3] = __builtin_amdgcn_perm(u1, t1, 0x07060302u);
+}
+
+__device__ inline float half_value(uint16_t bits) { return __half2float(__ushort_as_half(bits)); }
+
+// Threads of a row, each with 8 dims: the power of two that covers D.
+inline uint32_t row_lanes_log2(uint32_t D)
+{
+    uint32_t log2 = 0;
+    while ((8u << log2) < D) ++log2;
+    return log2;
+}
+
+struct AppendGrid {
+    uint32_t heads;        // of a block
+    uint32_t lanes_log2;   // of a row
+};
+
+// ---------------------------------------------------------------------------
+// Append: block = (job, layer, some heads).
+// ---------------------------------------------------------------------------
+// Tokens [0, n) of one head of a page's block copied to another page, byte for
+// byte: the codes and the scales of each.  Only those tokens' bytes are stored:
+// others may be writing behind them.
+__device__ inline void copy_head(const uint8_t* src, const uint16_t* src_scales, uint32_t scap, uint8_t* dst, uint16_t* dst_scales,
+                                 uint32_t dcap, uint32_t D, uint32_t n)
+{
+    uint32_t const tid = threadIdx.x;
+    uint32_t const kw = quant_k_width(D);
+    uint32_t const run = n * kw;   // contiguous in both, for each column block
+    if (D % 8u == 0) {
+        for (uint32_t i = tid * 8; i < n * D; i += kBlock * 8) {
+            uint32_t const b = i / run;
+            uint32_t const o = i - b * run;
+            *reinterpret_cast<u32x2_t*>(dst + b * dcap * kw + o) = *reinterpret_cast<const u32x2_t*>(src + b * scap * kw + o);
+        }
+    } else {
+        for (uint32_t i = tid; i < run; i += kBlock) dst[i] = src[i];
+    }
+    uint32_t const groups = (n + 7) / 8;
+    for (uint32_t i = tid; i < groups * D; i += kBlock) {
+        uint32_t const d = i / groups;
+        uint32_t const t = (i - d * groups) * 8;
+        const uint8_t* from = src + quant_v_at(scap, D, t, d);
+        uint8_t* to = dst + quant_v_at(dcap, D, t, d);
+        u32x2_t const v = *reinterpret_cast<const u32x2_t*>(from);
+        if (n - t >= 8) {
+            *reinterpret_cast<u32x2_t*>(to) = v;
+        } else {
+            for (uint32_t j = 0; j < n - t; ++j) to[j] = static_cast<uint8_t>(v[j >> 2] >> (8 * (j & 3)));
+        }
+    }
+    for (uint32_t i = tid; i < n; i += kBlock) {
+        dst_scales[i] = src_scales[i];
+        dst_scales[dcap + i] = src_scales[scap + i];
+    }
+}
+
+// Dims [8 p, 8 p + 8) of a row of D, zeros past its end.
+__device__ inline u32x4_t load_piece(const uint16_t* row, uint32_t p, uint32_t D, bool aligned)
+{
+    u32x4_t w = {};
+    if (aligned && 8 * p + 8 <= D) {
+        w = *reinterpret_cast<const u32x4_t*>(row + 8 * p);
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            if (8 * p + j < D) w[j >> 1] |= static_cast<uint32_t>(row[8 * p + j]) << (16 * (j & 1));
+        }
+    }
+    return w;
+}
+
+// Codes of a piece, and the row's scale; the row's other pieces are in the
+// other threads of its group.
+template <uint32_t kFormat>
+__device__ inline u32x2_t quantise_piece(u32x4_t w, uint32_t lanes, uint16_t* scale)
+{
+    uint32_t most = 0;   // two fp16 numbers without sign, ordered as whole numbers
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        most = max(most, max(w[j] & 0x7FFFu, (w[j] >> 16) & 0x7FFFu));
+    }
+    for (uint32_t m = 1; m < lanes; m *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), static_cast<int>(m))));
+    *scale = row_scale<kFormat>(most);
+    RowQuant const r = row_quant(*scale);
+    u32x2_t codes;
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+        float const x[4] = {half_value(static_cast<uint16_t>(w[2 * j])), half_value(static_cast<uint16_t>(w[2 * j] >> 16)),
+                            half_value(static_cast<uint16_t>(w[2 * j + 1])), half_value(static_cast<uint16_t>(w[2 * j + 1] >> 16))};
+        codes[j] = row_codes<kFormat>(x, r);
+    }
+    return codes;
+}
+
+__device__ inline void store_key_piece(uint8_t* at, u32x2_t codes, uint32_t p, uint32_t D)
+{
+    if (D % 8u == 0) {
+        *reinterpret_cast<u32x2_t*>(at) = codes;
+    } else {
+        for (uint32_t j = 0; j < 8 && 8 * p + j < D; ++j) at[j] = static_cast<uint8_t>(codes[j >> 2] >> (8 * (j & 3)));
+    }
+}
+
+template <uint32_t kFormat>
+__global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const kimkv_append_job* jobs, AppendGrid g)
+{
+    __shared__ alignas(16) uint8_t tile[kTileTokens * (kQuantMaxDim + 4)];   // V codes of a head, rows of D + 4 bytes
+    kimkv_append_job const job = jobs[blockIdx.x];
+    if (blockIdx.y >= job.layer_count) return;   // a shorter job of a launch sized for the longest
+    uint32_t const layer = job.layer_begin + blockIdx.y;
+    uint32_t const D = P.dim;
+    uint32_t const n = job.token_count;
+    uint32_t const dcap = quant_page_tokens(P, job.dst_kind);
+    uint32_t const scap = quant_page_tokens(P, job.cow_kind);
+    uint8_t* const dst = quant_block(P, layer, job.dst_kind, job.dst_slot, dcap);
+    uint8_t* const src = job.cow_tokens != 0 ? quant_block(P, layer, job.cow_kind, job.cow_slot, scap) : nullptr;
+    if (job.layer_begin >= P.layers || layer >= P.layers || dst == nullptr || n > dcap || job.dst_token > dcap - n
+        || (n != 0 && (job.src_key == nullptr || job.src_value == nullptr))
+        || (job.cow_tokens != 0 && (src == nullptr || job.cow_tokens > scap || job.cow_tokens > job.dst_token))) {
+        report_fault(P, KIMKV_FAULT_APPEND_JOB);
+        return;
+    }
+    uint32_t const tid = threadIdx.x;
+    uint32_t const h0 = blockIdx.z * g.heads;
+    uint32_t const h1 = min(h0 + g.heads, P.heads);
+
+    // The copied positions lie below the written ones: neither waits for the other.
+    for (uint32_t h = h0; job.cow_tokens != 0 && h < h1; ++h) {
+        copy_head(quant_codes(src, P, scap, h), quant_scales(src, P, scap, h), scap, quant_codes(dst, P, dcap, h),
+                  quant_scales(dst, P, dcap, h), dcap, D, job.cow_tokens);
+    }
+    if (n == 0) return;
+
+    uint64_t const layer_off = static_cast<uint64_t>(blockIdx.y) * job.src_layer_stride;
+    const uint16_t* const sk = job.src_key + layer_off;
+    const uint16_t* const sv = job.src_value + layer_off;
+    uint64_t const stride = job.src_token_stride;
+    bool const aligned = ((D | stride) & 7u) == 0 && ((reinterpret_cast<uintptr_t>(sk) | reinterpret_cast<uintptr_t>(sv)) & 15u) == 0;
+    uint32_t const lanes = 1u << g.lanes_log2;
+    uint32_t const p = tid & (lanes - 1);          // piece of the row
+    uint32_t const first = tid >> g.lanes_log2;
+    uint32_t const step = kBlock >> g.lanes_log2;
+    bool const mine = 8 * p < D;
+    uint32_t const t0 = job.dst_token;
+
+    if (n < 8) {
+        // A token step: K and V rows of all heads at once, V byte by byte.
+        uint32_t const rows = 2 * n * (h1 - h0);
+        for (uint32_t base = 0; base < rows; base += step) {
+            uint32_t const i = base + first;
+            bool const there = i < rows && mine;
+            uint32_t const row = min(i, rows - 1);
+            uint32_t const h = h0 + row / (2 * n);
+            uint32_t const rem = row % (2 * n);
+            bool const value = rem >= n;
+            uint32_t const t = value ? rem - n : rem;
+            u32x4_t w = {};
+            if (there) w = load_piece((value ? sv : sk) + t * stride + static_cast<uint64_t>(h) * D, p, D, aligned);
+            uint16_t scale;
+            u32x2_t const codes = quantise_piece<kFormat>(w, lanes, &scale);
+            if (!there) continue;
+            uint8_t* const at = quant_codes(dst, P, dcap, h);
+            if (p == 0) quant_scales(dst, P, dcap, h)[(value ? dcap : 0) + t0 + t] = scale;
+            if (!value) {
+                store_key_piece(at + quant_k_at(dcap, D, t0 + t, 8 * p), codes, p, D);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    if (8 * p + j < D) at[quant_v_at(dcap, D, t0 + t, 8 * p + j)] = static_cast<uint8_t>(codes[j >> 2] >> (8 * (j & 3)));
+                }
+            }
+        }
+        return;
+    }
+
+    uint32_t const pitch = D + 4;
+    uint32_t const g0 = t0 / 8;                       // groups of 8 page tokens that the job touches
+    uint32_t const groups = (t0 + n + 7) / 8 - g0;
+    for (uint32_t h = h0; h < h1; ++h) {
+        uint8_t* const codes_at = quant_codes(dst, P, dcap, h);
+        uint16_t* const scales_at = quant_scales(dst, P, dcap, h);
+        for (uint32_t base = 0; base < 2 * n; base += step) {
+            uint32_t const i = base + first;
+            bool const there = i < 2 * n && mine;
+            bool const value = i >= n;
+            uint32_t const t = value ? i - n : i;
+            u32x4_t w = {};
+            if (there) w = load_piece((value ? sv : sk) + t * stride + static_cast<uint64_t>(h) * D, p, D, aligned);
+            uint16_t scale;
+            u32x2_t const codes = quantise_piece<kFormat>(w, lanes, &scale);
+            if (!there) continue;
+            if (p == 0) scales_at[(value ? dcap : 0) + t0 + t] = scale;
+            if (!value) {
+                store_key_piece(codes_at + quant_k_at(dcap, D, t0 + t, 8 * p), codes, p, D);
+            } else {
+                // Row t0 % 8 + t of the tile, so that its groups of 8 are the page's.
+                uint8_t* const row = tile + ((t0 & 7u) + t) * pitch + 8 * p;
+                if (D % 8u == 0) {
+                    reinterpret_cast<uint32_t*>(row)[0] = codes[0];
+                    reinterpret_cast<uint32_t*>(row)[1] = codes[1];
+                } else {
+                    store_key_piece(row, codes, p, D);
+                }
+            }
+        }
+        __syncthreads();
+        auto const row_of = [&](uint32_t gi, uint32_t j) { return tile + (8 * gi + j) * pitch; };
+        if (D % 8u == 0) {
+            for (uint32_t i = tid; i < groups * (D / 4); i += kBlock) {
+                uint32_t const q = i / groups;
+                uint32_t const gi = i - q * groups;
+                uint32_t const t = 8 * (g0 + gi);
+                uint32_t lo[4], hi[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    lo[j] = *reinterpret_cast<const uint32_t*>(row_of(gi, j) + 4 * q);
+                    hi[j] = *reinterpret_cast<const uint32_t*>(row_of(gi, j + 4) + 4 * q);
+                }
+                transpose_bytes(lo);
+                transpose_bytes(hi);
+                bool const whole = t >= t0 && t + 8 <= t0 + n;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    uint8_t* const at = codes_at + quant_v_at(dcap, D, t, 4 * q + k);
+                    if (whole) {
+                        *reinterpret_cast<u32x2_t*>(at) = u32x2_t{lo[k], hi[k]};
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 8; ++j) {
+                            uint32_t const word = j < 4 ? lo[k] : hi[k];
+                            if (t + j >= t0 && t + j < t0 + n) at[j] = static_cast<uint8_t>(word >> (8 * (j & 3)));
+                        }
+                    }
+                }
+            }
+        } else {
+            for (uint32_t i = tid; i < n * D; i += kBlock) {
+                uint32_t const d = i / n;
+                uint32_t const t = i - d * n;
+                codes_at[quant_v_at(dcap, D, t0 + t, d)] = tile[((t0 & 7u) + t) * pitch + d];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Read-back: block = (table entry, layer, some heads).
+// ---------------------------------------------------------------------------
+struct GatherArgs {
+    const kimkv_block_desc* descriptors;
+    uint16_t* out;
+    uint32_t first;        // token
+    uint32_t count;
+    uint32_t layer_begin;
+    uint32_t heads;        // of a block
+    bool wide;             // rows of 16-byte pieces
+};
+
+template <uint32_t kFormat>
+__global__ __launch_bounds__(kBlock) void quant_gather_kernel(QuantView P, GatherArgs a)
+{
+    __shared__ uint32_t tile[kQuantMaxDim * (kTileTokens / 4 + 1)];   // V codes of a head, rows of 17 words
+    kimkv_block_desc const e = a.descriptors[blockIdx.x];
+    uint64_t const begin = e.logical_token_begin;
+    uint64_t const last = static_cast<uint64_t>(a.first) + a.count;
+    if (begin >= last || begin + e.valid_tokens <= a.first) return;
+    uint32_t const cap = e.page_token_capacity;
+    uint32_t const layer = a.layer_begin + blockIdx.y;
+    uint8_t* const block = e.valid_tokens <= cap ? quant_block(P, layer, e.kind, e.slot, cap) : nullptr;
+    if (block == nullptr) {
+        report_fault(P, KIMKV_FAULT_GATHER_ENTRY);
+        return;
+    }
+    uint32_t const tid = threadIdx.x;
+    uint32_t const D = P.dim;
+    uint32_t const HD = P.heads * D;
+    // Page tokens [p0, p1), token p0 of which is row `to` of the output.
+    uint32_t const p0 = begin < a.first ? static_cast<uint32_t>(a.first - begin) : 0;
+    uint32_t const p1 = static_cast<uint32_t>(min<uint64_t>(e.valid_tokens, last - begin));
+    uint32_t const n = p1 - p0;
+    uint64_t const to = begin + p0 - a.first;
+    uint16_t* const key_out = a.out + (static_cast<uint64_t>(blockIdx.y) * 2 * a.count + to) * HD;
+    uint16_t* const value_out = key_out + static_cast<uint64_t>(a.count) * HD;
+    uint32_t const h0 = blockIdx.z * a.heads;
+    uint32_t const h1 = min(h0 + a.heads, P.heads);
+    for (uint32_t h = h0; h < h1; ++h) {
+        const uint8_t* const codes = quant_codes(block, P, cap, h);
+        const uint16_t* const scales = quant_scales(block, P, cap, h);
+        if (!a.wide) {
+            for (uint32_t i = tid; i < n * D; i += kBlock) {
+                uint32_t const t = i / D;
+                uint32_t const d = i - t * D;
+                uint64_t const o = static_cast<uint64_t>(t) * HD + h * D + d;
+                key_out[o] = read_back(code_value<kFormat>(codes[quant_k_at(cap, D, p0 + t, d)]), scale_value(scales[p0 + t]));
+                value_out[o] = read_back(code_value<kFormat>(codes[quant_v_at(cap, D, p0 + t, d)]), scale_value(scales[cap + p0 + t]));
+            }
+            continue;
+        }
+        uint32_t const words = cap / 4;   // of a row of V codes
+        for (uint32_t i = tid; i < D * cap / 8; i += kBlock) {
+            u32x2_t const v = *reinterpret_cast<const u32x2_t*>(codes + cap * D + 8 * i);
+            uint32_t const d = 2 * i / words;
+            uint32_t* const row = tile + d * (kTileTokens / 4 + 1) + (2 * i - d * words);
+            row[0] = v[0];
+            row[1] = v[1];
+        }
+        uint32_t const pieces = D / 8;
+        for (uint32_t i = tid; i < n * pieces; i += kBlock) {
+            uint32_t const t = i / pieces;
+            uint32_t const d = (i - t * pieces) * 8;
+            u32x2_t const w = *reinterpret_cast<const u32x2_t*>(codes + quant_k_at(cap, D, p0 + t, d));
+            float const s = scale_value(scales[p0 + t]);
+            u32x4_t o;
+#pragma unroll
+            for (uint32_t j = 0; j < 2; ++j) {
+                float x[4];
+                code_values<kFormat>(w[j], x);
+                o[2 * j] = read_back(x[0], s) | static_cast<uint32_t>(read_back(x[1], s)) << 16;
+                o[2 * j + 1] = read_back(x[2], s) | static_cast<uint32_t>(read_back(x[3], s)) << 16;
+            }
+            *reinterpret_cast<u32x4_t*>(key_out + static_cast<uint64_t>(t) * HD + h * D + d) = o;
+        }
+        __syncthreads();
+        // Four tokens by 8 dims a thread.
+        uint32_t const q0 = p0 / 4;
+        uint32_t const quads = (p1 + 3) / 4 - q0;
+        for (uint32_t i = tid; i < quads * pieces; i += kBlock) {
+            uint32_t const q = i / pieces;
+            uint32_t const d = (i - q * pieces) * 8;
+            uint32_t lo[4], hi[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                lo[j] = tile[(d + j) * (kTileTokens / 4 + 1) + q0 + q];
+                hi[j] = tile[(d + 4 + j) * (kTileTokens / 4 + 1) + q0 + q];
+            }
+            transpose_bytes(lo);
+            transpose_bytes(hi);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                uint32_t const t = 4 * (q0 + q) + k;
+                if (t < p0 || t >= p1) continue;
+                float const s = scale_value(scales[cap + t]);
+                float x[4], y[4];
+                code_values<kFormat>(lo[k], x);
+                code_values<kFormat>(hi[k], y);
+                u32x4_t const o = {read_back(x[0], s) | static_cast<uint32_t>(read_back(x[1], s)) << 16,
+                                   read_back(x[2], s) | static_cast<uint32_t>(read_back(x[3], s)) << 16,
+                                   read_back(y[0], s) | static_cast<uint32_t>(read_back(y[1], s)) << 16,
+                                   read_back(y[2], s) | static_cast<uint32_t>(read_back(y[3], s)) << 16};
+                *reinterpret_cast<u32x4_t*>(value_out + static_cast<uint64_t>(t - p0) * HD + h * D + d) = o;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Promotion: block = (job, layer, some heads).  Eight pages of 8 tokens into
+// one of 64: K in runs of 8 tokens of a column block, V and the scales in
+// pieces of 8 tokens.
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(kBlock) void quant_promote_kernel(QuantView P, const kimkv_promotion_job* jobs, uint32_t heads)
+{
+    __shared__ const uint8_t* source[8];
+    kimkv_promotion_job const& job = jobs[blockIdx.x];
+    uint32_t const layer = blockIdx.y;
+    uint32_t const tid = threadIdx.x;
+    uint8_t* const dst = quant_block(P, layer, KIMKV_PAGE_EXTENT, job.extent_slot, 64);
+    if (tid < 8) source[tid] = quant_block(P, layer, KIMKV_PAGE_MICRO, job.micro_slots[tid], 8);
+    __syncthreads();
+    bool good = dst != nullptr;
+    for (uint32_t m = 0; m < 8; ++m) good = good && source[m] != nullptr;
+    if (!good) {
+        report_fault(P, KIMKV_FAULT_PROMOTION_JOB);
+        return;
+    }
+    uint32_t const D = P.dim;
+    uint32_t const kw = quant_k_width(D);
+    uint32_t const run = 8 * kw;   // a micro page's column block
+    uint32_t const h0 = blockIdx.z * heads;
+    uint32_t const h1 = min(h0 + heads, P.heads);
+    for (uint32_t h = h0; h < h1; ++h) {
+        uint8_t* const to = quant_codes(dst, P, 64, h);
+        uint64_t const from = static_cast<uint64_t>(h) * 16 * D;
+        for (uint32_t i = tid; i < 8 * D; i += kBlock) {
+            uint32_t const piece = i / kw;             // 8-byte pieces: (column block, micro page)
+            uint32_t const o = (i - piece * kw) * 8;
+            uint32_t const m = piece & 7u;
+            uint32_t const b = piece >> 3;
+            *reinterpret_cast<u32x2_t*>(to + b * 8 * run + m * run + o) = *reinterpret_cast<const u32x2_t*>(source[m] + from + b * run + o);
+            uint32_t const vm = i & 7u;
+            uint32_t const d = i >> 3;
+            *reinterpret_cast<u32x2_t*>(to + 64 * D + d * 64 + vm * 8) = *reinterpret_cast<const u32x2_t*>(source[vm] + from + 8 * D + d * 8);
+        }
+        if (tid < 128) {
+            uint32_t const m = (tid >> 3) & 7u;
+            uint32_t const value = tid >> 6;
+            const uint16_t* const s = reinterpret_cast<const uint16_t*>(source[m] + static_cast<uint64_t>(P.heads) * 16 * D) + h * 16;
+            quant_scales(dst, P, 64, h)[tid] = s[value * 8 + (tid & 7u)];
+        }
+    }
+}
+
+// Moves the fault word to the mapped host word and clears it in one exchange.
+__global__ __launch_bounds__(64) void quant_take_faults_kernel(uint32_t* faults, uint32_t* host_word)
+{
+    if (threadIdx.x == 0) *host_word = atomicExch(faults, 0u);
+}
+
+// Heads a block takes: all of them where the rest of the grid fills the chip,
+// fewer where it does not.
+uint32_t heads_of_block(uint32_t heads, uint64_t blocks)
+{
+    uint32_t per = heads;
+    while (per > 1 && blocks * ceil_div(heads, per) < 1024) per = (per + 1) / 2;
+    return per;
+}
+
+bool on_device(const kimkv_quant_storage* s)
+{
+    int device = -1;
+    return hipGetDevice(&device) == hipSuccess && device == s->device;
+}
+
+constexpr uint32_t kGridRows = 65535;   // of a launch's second and third dimension
+constexpr uint32_t kGridBlocks = 0xFFFFFFu;   // times kBlock threads: fewer than 2^32
+
+}  // namespace
+}  // namespace kimkv
+
+using namespace kimkv;
+
+extern "C" {
+
+kimkv_status kimkv_quant_storage_create(kimkv_quant_storage** out, kimkv_layout layout, uint32_t format, uint32_t micro_capacity,
+                                        uint32_t extent_capacity, uint16_t micro_page_tokens, uint16_t extent_page_tokens)
+{
+    if (out == nullptr) return KIMKV_INVALID_ARGUMENT;
+    *out = nullptr;
+    auto const page = [](uint32_t tokens) { return tokens != 0 && tokens % 8 == 0 && tokens <= kQuantMaxPage; };
+    if (layout.layers == 0 || layout.layers > 0x7FFFu || layout.kv_heads == 0 || layout.kv_heads > kGridRows || layout.head_dim == 0
+        || layout.head_dim > kQuantMaxDim || (format != KIMKV_QUANT_INT8 && format != KIMKV_QUANT_E4M3) || !page(micro_page_tokens)
+        || !page(extent_page_tokens)) {
+        return KIMKV_INVALID_ARGUMENT;
+    }
+    // At most 2^15 layers x 2^32 pages x 2^16 heads x 2^15 bytes: 2^78.
+    uint64_t const layer_bytes_limit = std::numeric_limits<int64_t>::max() / layout.layers / 2;
+    uint64_t const micro_slot = quant_slot_bytes(layout, micro_page_tokens);
+    uint64_t const extent_slot = quant_slot_bytes(layout, extent_page_tokens);
+    if ((micro_capacity != 0 && micro_slot > layer_bytes_limit / micro_capacity)
+        || (extent_capacity != 0 && extent_slot > layer_bytes_limit / extent_capacity)) {
+        return KIMKV_INVALID_ARGUMENT;
+    }
+    int count = 0;
+    if (hipGetDeviceCount(&count) != hipSuccess || count == 0) return KIMKV_RUNTIME_UNAVAILABLE;
+    auto* s = new (std::nothrow) kimkv_quant_storage{};
+    if (s == nullptr) return KIMKV_ALLOCATION_FAILED;
+    s->layout = layout;
+    s->format = format;
+    s->micro_capacity = micro_capacity;
+    s->extent_capacity = extent_capacity;
+    s->micro_tokens = micro_page_tokens;
+    s->extent_tokens = extent_page_tokens;
+    uint64_t const bytes = (micro_slot * micro_capacity + extent_slot * extent_capacity) * layout.layers;
+    hipError_t e = hipGetDevice(&s->device);
+    if (e == hipSuccess) e = hipDeviceGetAttribute(&s->compute_units, hipDeviceAttributeMultiprocessorCount, s->device);
+    if (e == hipSuccess && bytes != 0) {
+        e = hipMalloc(reinterpret_cast<void**>(&s->pool), bytes);
+        if (e == hipSuccess) e = hipMemset(s->pool, 0, bytes);
+    }
+    if (e == hipSuccess) {
+        e = hipMalloc(reinterpret_cast<void**>(&s->faults), 256);
+        if (e == hipSuccess) e = hipMemset(s->faults, 0, 256);
+    }
+    if (e == hipSuccess) {
+        e = hipHostMalloc(reinterpret_cast<void**>(&s->fault_host), 256, hipHostMallocMapped | hipHostMallocCoherent);
+        if (e == hipSuccess) e = hipHostGetDevicePointer(reinterpret_cast<void**>(&s->fault_view), s->fault_host, 0);
+    }
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        record_error(e, KIMKV_ALLOCATION_FAILED);
+        if (s->pool) static_cast<void>(hipFree(s->pool));
+        if (s->faults) static_cast<void>(hipFree(s->faults));
+        if (s->fault_host) static_cast<void>(hipHostFree(s->fault_host));
+        delete s;
+        return KIMKV_ALLOCATION_FAILED;
+    }
+    *out = s;
+    return KIMKV_OK;
+}
+
+kimkv_status kimkv_quant_storage_destroy(kimkv_quant_storage* storage)
+{
+    if (storage == nullptr) return KIMKV_OK;
+    // In-flight work may still read the pools.
+    static_cast<void>(hipDeviceSynchronize());
+    if (storage->pool) static_cast<void>(hipFree(storage->pool));
+    if (storage->faults) static_cast<void>(hipFree(storage->faults));
+    if (storage->fault_host) static_cast<void>(hipHostFree(storage->fault_host));
+    delete storage;
+    return KIMKV_OK;
+}
+
+kimkv_status kimkv_quant_storage_query(const kimkv_quant_storage* s, kimkv_quant_storage_info* info)
+{
+    if (s == nullptr || info == nullptr) return KIMKV_INVALID_ARGUMENT;
+    *info = kimkv_quant_storage_info{};
+    info->layout = s->layout;
+    info->format = s->format;
+    info->micro_capacity = s->micro_capacity;
+    info->extent_capacity = s->extent_capacity;
+    info->micro_page_tokens = s->micro_tokens;
+    info->extent_page_tokens = s->extent_tokens;
+    info->micro_page_bytes = quant_slot_bytes(s->layout, s->micro_tokens) * s->layout.layers;
+    info->extent_page_bytes = quant_slot_bytes(s->layout, s->extent_tokens) * s->layout.layers;
+    info->reserved_bytes = info->micro_page_bytes * s->micro_capacity + info->extent_page_bytes * s->extent_capacity;
+    info->device = s->device;
+    info->compute_units = s->compute_units;
+    return KIMKV_OK;
+}
+
+kimkv_status kimkv_quant_storage_faults(kimkv_quant_storage* storage, kimkv_stream_t stream, uint32_t* faults)
+{
+    if (faults != nullptr) *faults = 0;
+    if (storage == nullptr || !on_device(storage)) return KIMKV_INVALID_ARGUMENT;
+    // One reader of the mapped word at a time.
+    static std::mutex mutex;
+    std::lock_guard<std::mutex> lock(mutex);
+    *reinterpret_cast<volatile uint32_t*>(storage->fault_host) = 0;
+    quant_take_faults_kernel<<<1, 64, 0, native(stream)>>>(storage->faults, storage->fault_view);
+    kimkv_status const launched = launch_status();
+    if (launched != KIMKV_OK) return launched;
+    kimkv_status const done = record_error(hipStreamSynchronize(native(stream)), KIMKV_EXECUTION_FAILED);
+    if (done != KIMKV_OK) return done;
+    uint32_t const bits = *reinterpret_cast<volatile uint32_t*>(storage->fault_host);
+    if (faults != nullptr) *faults = bits;
+    return bits != 0 ? KIMKV_INVALID_ARGUMENT : KIMKV_OK;
+}
+
+kimkv_status kimkv_quant_append_batch(const kimkv_quant_storage* storage, const kimkv_append_job* device_jobs, uint32_t job_count,
+                                      uint32_t max_layer_count, kimkv_stream_t stream)
+{
+    if (storage == nullptr || (job_count != 0 && device_jobs == nullptr) || max_layer_count > storage->layout.layers || !on_device(storage)) {
+        return KIMKV_INVALID_ARGUMENT;
+    }
+    if (job_count == 0 || max_layer_count == 0) return KIMKV_OK;
+    QuantView const view = quant_view(*storage);
+    uint32_t const heads = heads_of_block(view.heads, static_cast<uint64_t>(job_count) * max_layer_count);
+    uint32_t const z = ceil_div(view.heads, heads);
+    uint32_t const most = kGridBlocks / (max_layer_count * z) == 0 ? 1 : kGridBlocks / (max_layer_count * z);
+    auto const kernel = storage->format == KIMKV_QUANT_INT8 ? quant_append_kernel<KIMKV_QUANT_INT8> : quant_append_kernel<KIMKV_QUANT_E4M3>;
+    for (uint32_t first = 0; first < job_count;) {
+        uint32_t const jobs = job_count - first < most ? job_count - first : most;
+        kernel<<<dim3(jobs, max_layer_count, z), kBlock, 0, native(stream)>>>(view, device_jobs + first, AppendGrid{heads, row_lanes_log2(view.dim)});
+        kimkv_status const status = launch_status();
+        if (status != KIMKV_OK) return status;
+        first += jobs;
+    }
+    return KIMKV_OK;
+}
+
+kimkv_status kimkv_quant_gather(const kimkv_quant_storage* storage, const kimkv_block_desc* device_descriptors, uint32_t descriptor_count,
+                                uint32_t first_token, uint32_t token_count, uint32_t layer_begin, uint32_t layer_count,
+                                uint16_t* device_output, kimkv_stream_t stream)
+{
+    if (storage == nullptr || layer_begin > storage->layout.layers || layer_count > storage->layout.layers - layer_begin
+        || token_count > 0xFFFFFFFFu - first_token || !on_device(storage)) {
+        return KIMKV_INVALID_ARGUMENT;
+    }
+    if (token_count == 0 || layer_count == 0) return KIMKV_OK;
+    if (device_descriptors == nullptr || descriptor_count == 0 || device_output == nullptr) return KIMKV_INVALID_ARGUMENT;
+    QuantView const view = quant_view(*storage);
+    uint32_t const heads = heads_of_block(view.heads, static_cast<uint64_t>(descriptor_count) * layer_count);
+    uint32_t const z = ceil_div(view.heads, heads);
+    uint32_t const most = kGridBlocks / (layer_count * z) == 0 ? 1 : kGridBlocks / (layer_count * z);
+    bool const wide = view.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(device_output) & 15u) == 0;
+    auto const kernel = storage->format == KIMKV_QUANT_INT8 ? quant_gather_kernel<KIMKV_QUANT_INT8> : quant_gather_kernel<KIMKV_QUANT_E4M3>;
+    for (uint32_t first = 0; first < descriptor_count;) {
+        uint32_t const entries = descriptor_count - first < most ? descriptor_count - first : most;
+        GatherArgs const args{device_descriptors + first, device_output, first_token, token_count, layer_begin, heads, wide};
+        kernel<<<dim3(entries, layer_count, z), kBlock, 0, native(stream)>>>(view, args);
+        kimkv_status const status = launch_status();
+        if (status != KIMKV_OK) return status;
+        first += entries;
+    }
+    return KIMKV_OK;
+}
+
+kimkv_status kimkv_quant_promote_batch(const kimkv_quant_storage* storage, const kimkv_promotion_job* device_jobs, uint32_t job_count,
+                                       kimkv_stream_t stream)
+{
+    if (storage == nullptr || (job_count != 0 && device_jobs == nullptr) || storage->micro_tokens != 8 || storage->extent_tokens != 64
+        || !on_device(storage)) {
+        return KIMKV_INVALID_ARGUMENT;
+    }
+    if (job_count == 0) return KIMKV_OK;
+    QuantView const view = quant_view(*storage);
+    uint32_t const heads = heads_of_block(view.heads, static_cast<uint64_t>(job_count) * view.layers);
+    uint32_t const z = ceil_div(view.heads, heads);
+    uint32_t const most = kGridBlocks / (view.layers * z) == 0 ? 1 : kGridBlocks / (view.layers * z);
+    for (uint32_t first = 0; first < job_count;) {
+        uint32_t const jobs = job_count - first < most ? job_count - first : most;
+        quant_promote_kernel<<<dim3(jobs, view.layers, z), kBlock, 0, native(stream)>>>(view, device_jobs + first, heads);
+        kimkv_status const status = launch_status();
+        if (status != KIMKV_OK) return status;
+        first += jobs;
+    }
+    return KIMKV_OK;
+}
+
+}  // extern "C"

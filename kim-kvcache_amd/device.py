@@ -58,6 +58,7 @@ LOGITS_RULE = np.dtype({
     "itemsize": 56,
 })
 NO_TOKEN = 0xFFFFFFFF
+SAMPLE_RULE = np.dtype([("temperature", "<f4"), ("top_p", "<f4"), ("min_p", "<f4"), ("top_k", "<u4")])
 PREFILL_BLOCK = np.dtype([("item", "<u4"), ("head", "<u2"), ("block", "<u2")])
 DESCRIPTOR_PATCH = np.dtype({
     "names": ["table", "first", "count", "source"],
@@ -119,6 +120,14 @@ class SharedPlan(ctypes.Structure):
                 ("merge_split", ctypes.c_uint32), ("waves", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
 
 
+class QuantPlan(ctypes.Structure):
+    """kimkv_quant_plan: what a quantised decode's plan decided (entry and workspace sizes, counts)."""
+    _fields_ = [("entry_bytes", ctypes.c_uint64), ("workspace_bytes", ctypes.c_uint64), ("kv_heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("query_heads", ctypes.c_uint32), ("lane_count", ctypes.c_uint32),
+                ("unit_count", ctypes.c_uint32), ("slot_count", ctypes.c_uint32), ("merge_lanes", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
 # kimkv_decode_lane (48 bytes): one chunk of a batched decode with its lane's step-constant part.
 DECODE_LANE = np.dtype([("descriptors", np.uint64), ("descriptor_count", np.uint32), ("token_count", np.uint32),
                         ("dst_slot", np.uint32), ("cow_slot", np.uint32), ("dst_token", np.uint16),
@@ -135,6 +144,16 @@ class StorageInfo(ctypes.Structure):
         ("micro_page_elements", ctypes.c_uint64), ("extent_page_elements", ctypes.c_uint64),
         ("micro_reserved_bytes", ctypes.c_uint64), ("extent_reserved_bytes", ctypes.c_uint64),
         ("device", ctypes.c_int), ("compute_units", ctypes.c_int),
+    ]
+
+
+class QuantStorageInfo(ctypes.Structure):
+    _fields_ = [
+        ("layout", Layout), ("format", ctypes.c_uint32), ("micro_capacity", ctypes.c_uint32),
+        ("extent_capacity", ctypes.c_uint32), ("micro_page_tokens", ctypes.c_uint16),
+        ("extent_page_tokens", ctypes.c_uint16), ("reserved", ctypes.c_uint32), ("micro_page_bytes", ctypes.c_uint64),
+        ("extent_page_bytes", ctypes.c_uint64), ("reserved_bytes", ctypes.c_uint64), ("device", ctypes.c_int),
+        ("compute_units", ctypes.c_int),
     ]
 
 
@@ -183,6 +202,26 @@ _SIGNATURES = {
     "kimkv_logits_workspace_bytes": (ctypes.c_size_t, [ctypes.c_uint32, ctypes.c_uint32]),
     "kimkv_model_logits_adjust": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p,
                                                  ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "kimkv_sample_workspace_bytes": (ctypes.c_size_t, [ctypes.c_uint32, ctypes.c_uint32]),
+    "kimkv_model_sample": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                          ctypes.c_void_p]),
+    "kimkv_quant_storage_create": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), Layout, ctypes.c_uint32,
+                                                  ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint16, ctypes.c_uint16]),
+    "kimkv_quant_storage_destroy": (ctypes.c_int, [ctypes.c_void_p]),
+    "kimkv_quant_storage_query": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(QuantStorageInfo)]),
+    "kimkv_quant_storage_faults": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
+    "kimkv_quant_append_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32,
+                                                ctypes.c_void_p]),
+    "kimkv_quant_gather": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32,
+                                          ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p,
+                                          ctypes.c_void_p]),
+    "kimkv_quant_promote_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p]),
+    "kimkv_quant_decode_plan": (ctypes.c_int, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
+                                               ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_uint64,
+                                               ctypes.POINTER(QuantPlan)]),
+    "kimkv_quant_decode_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                                ctypes.POINTER(QuantPlan), ctypes.c_void_p, ctypes.c_void_p]),
     "kimkv_gather": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint32,
                                     ctypes.c_void_p, ctypes.c_void_p]),
     "kimkv_promote_batch": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p]),
@@ -572,6 +611,98 @@ class Storage:
             pass
 
 
+QUANT_INT8 = 1
+QUANT_E4M3 = 2
+
+
+class QuantStorage:
+    """Device page pools that hold K and V in 8 bits (kimkv_quant_storage); format QUANT_INT8 or QUANT_E4M3."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, micro_capacity: int, extent_capacity: int, format: int,
+                 micro_tokens: int = 8, extent_tokens: int = 64):
+        self.handle = None
+        handle = ctypes.c_void_p()
+        check(lib().kimkv_quant_storage_create(ctypes.byref(handle), Layout(layers, kv_heads, head_dim), format,
+                                               micro_capacity, extent_capacity, micro_tokens, extent_tokens),
+              "quant_storage_create")
+        self.handle = handle.value
+        self.layers, self.kv_heads, self.head_dim, self.format = layers, kv_heads, head_dim, format
+        self.micro_tokens, self.extent_tokens = micro_tokens, extent_tokens
+
+    def info(self) -> QuantStorageInfo:
+        info = QuantStorageInfo()
+        check(lib().kimkv_quant_storage_query(self.handle, ctypes.byref(info)), "quant_storage_query")
+        return info
+
+    def faults(self, stream: Optional[Stream] = None) -> tuple[int, int]:
+        """kimkv_quant_storage_faults: (status, FAULT_* bits) after waiting for `stream`; clears the word."""
+        bits = ctypes.c_uint32()
+        status = lib().kimkv_quant_storage_faults(self.handle, _sh(stream), ctypes.byref(bits))
+        return int(status), int(bits.value)
+
+    def append_launch(self, jobs_ptr: int, job_count: int, max_layers: int, stream: Optional[Stream] = None) -> None:
+        """kimkv_quant_append_batch: jobs (APPEND_JOB) in device memory; max_layers the largest layer_count among them."""
+        check(lib().kimkv_quant_append_batch(self.handle, jobs_ptr, job_count, max_layers, stream.handle if stream else None),
+              "quant_append_batch")
+
+    def gather_launch(self, descriptors_ptr: int, count: int, first_token: int, token_count: int, layer_begin: int,
+                      layer_count: int, out_ptr: int, stream: Optional[Stream] = None) -> None:
+        """kimkv_quant_gather: [layer_count][K/V][token_count][head][dim] fp16 rows of a table in device memory."""
+        check(lib().kimkv_quant_gather(self.handle, descriptors_ptr, count, first_token, token_count, layer_begin, layer_count,
+                                       out_ptr, stream.handle if stream else None), "quant_gather")
+
+    def promote_launch(self, jobs_ptr: int, job_count: int, stream: Optional[Stream] = None) -> None:
+        """kimkv_quant_promote_batch: jobs (PROMOTION_JOB) in device memory."""
+        check(lib().kimkv_quant_promote_batch(self.handle, jobs_ptr, job_count, stream.handle if stream else None),
+              "quant_promote_batch")
+
+    def append_batch(self, jobs: np.ndarray, stream: Optional[Stream] = None) -> None:
+        jobs = np.ascontiguousarray(jobs, dtype=APPEND_JOB)
+        if len(jobs) == 0:
+            return
+        dev = upload(jobs, stream)
+        self.append_launch(dev.ptr, len(jobs), int(jobs["layer_count"].max()), stream)
+        sync(stream)
+
+    def gather(self, descs: np.ndarray, total_tokens: int, first_token: int = 0, layer_begin: int = 0,
+               layer_count: Optional[int] = None, stream: Optional[Stream] = None) -> np.ndarray:
+        descs = np.ascontiguousarray(descs, dtype=BLOCK_DESC)
+        layers = self.layers - layer_begin if layer_count is None else layer_count
+        d = upload(descs, stream)
+        n = layers * 2 * total_tokens * self.kv_heads * self.head_dim
+        out = DeviceBuffer(max(n, 1) * 2)
+        self.gather_launch(d.ptr, len(descs), first_token, total_tokens, layer_begin, layers, out.ptr, stream)
+        return download(out.ptr, (n,), np.uint16, stream)
+
+    def promote_batch(self, jobs: np.ndarray, stream: Optional[Stream] = None) -> None:
+        jobs = np.ascontiguousarray(jobs, dtype=PROMOTION_JOB)
+        if len(jobs) == 0:
+            return
+        dev = upload(jobs, stream)
+        self.promote_launch(dev.ptr, len(jobs), stream)
+        sync(stream)
+
+    def decode_plan(self, token_counts, query_heads: int) -> tuple[np.ndarray, QuantPlan]:
+        return quant_decode_plan(self.kv_heads, self.head_dim, query_heads, self.info().compute_units, token_counts)
+
+    def decode_launch(self, items_ptr: int, entries_ptr: int, plan: QuantPlan, workspace_ptr: int,
+                      stream: Optional[Stream] = None) -> None:
+        """kimkv_quant_decode_batch: one layer of a planned batch (entries and workspace in device memory)."""
+        check(lib().kimkv_quant_decode_batch(self.handle, items_ptr, entries_ptr, plan, workspace_ptr,
+                                             stream.handle if stream else None), "quant_decode_batch")
+
+    def destroy(self) -> None:
+        if self.handle:
+            lib().kimkv_quant_storage_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
 def prefill_order(kv_heads: int, head_dim: int, query_heads: int, compute_units: int, token_counts, new_tokens):
     """kimkv_prefill_order: the workgroup placement of an ordered prefill launch."""
     tc = np.ascontiguousarray(token_counts, dtype=np.uint32)
@@ -598,6 +729,7 @@ FAULT_APPEND_JOB = 0x1
 FAULT_DECODE_ITEM = 0x2
 FAULT_PREFILL_ITEM = 0x4
 FAULT_PROMOTION_JOB = 0x8
+FAULT_GATHER_ENTRY = 0x10
 
 
 def decode_plan(storage_handle: int, token_counts, query_heads: int):
@@ -630,6 +762,22 @@ def shared_decode_plan(kv_heads: int, head_dim: int, query_heads: int, compute_u
         entries = np.empty(plan.entry_bytes, dtype=np.uint8)
         status = lib().kimkv_shared_decode_plan(*args, entries.ctypes.data_as(ctypes.c_void_p), len(entries), ctypes.byref(plan))
     check(status, "shared_decode_plan")
+    return entries[:plan.entry_bytes], plan
+
+
+def quant_decode_plan(kv_heads: int, head_dim: int, query_heads: int, compute_units: int,
+                      token_counts) -> tuple[np.ndarray, QuantPlan]:
+    """kimkv_quant_decode_plan: (entries to upload, plan) of a batch over a quantised storage."""
+    counts = np.ascontiguousarray(token_counts, dtype=np.uint32)
+    plan = QuantPlan()
+    args = (kv_heads, head_dim, query_heads, compute_units, counts.ctypes.data_as(ctypes.c_void_p), len(counts))
+    # Room for the usual plan: a few units for each lane's head and for each compute unit.
+    entries = np.empty(32 * (2 * kv_heads * len(counts) + 8 * (compute_units or 256)), dtype=np.uint8)
+    status = lib().kimkv_quant_decode_plan(*args, entries.ctypes.data_as(ctypes.c_void_p), len(entries), ctypes.byref(plan))
+    if status != OK and plan.entry_bytes > len(entries):
+        entries = np.empty(plan.entry_bytes, dtype=np.uint8)
+        status = lib().kimkv_quant_decode_plan(*args, entries.ctypes.data_as(ctypes.c_void_p), len(entries), ctypes.byref(plan))
+    check(status, "quant_decode_plan")
     return entries[:plan.entry_bytes], plan
 
 
@@ -687,6 +835,18 @@ def logits_adjust(logits_ptr: int, rows: int, vocabulary: int, rules_ptr: int, o
     adjusted rows to out_ptr, their greedy tokens to tokens_ptr (0: not wanted)."""
     check(lib().kimkv_model_logits_adjust(logits_ptr, rows, vocabulary, rules_ptr, out_ptr, tokens_ptr, workspace_ptr,
                                           stream.handle if stream else None), "model_logits_adjust")
+
+
+def sample_workspace_bytes(rows: int, vocabulary: int) -> int:
+    return int(lib().kimkv_sample_workspace_bytes(rows, vocabulary))
+
+
+def sample(logits_ptr: int, rows: int, vocabulary: int, rules_ptr: int, uniforms_ptr: int, tokens_ptr: int,
+           probabilities_ptr: int = 0, workspace_ptr: int = 0, stream: Optional[Stream] = None) -> None:
+    """kimkv_model_sample: the token of each row of fp32 logits by its SAMPLE_RULE and random number (device memory), to
+    tokens_ptr; its probability to probabilities_ptr (0: not wanted)."""
+    check(lib().kimkv_model_sample(logits_ptr, rows, vocabulary, rules_ptr, uniforms_ptr, tokens_ptr, probabilities_ptr,
+                                   workspace_ptr, stream.handle if stream else None), "model_sample")
 
 
 def decode_timing(enable, every: int = 1):
