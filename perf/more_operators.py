@@ -425,7 +425,11 @@ def _prepare_decode(case, seed):
         storage = _storage(device, case, micro, extent)
         _write_rows(device, storage, rows, [p for pages in lanes for p in pages])
         tables = [_table(device, pages) for pages in lanes]
-        flat = _on_gpu(np.concatenate(tables))
+        # Entries are of 20 bytes; numpy's concatenation would pack them.
+        flat = np.zeros(sum(len(t) for t in tables), dtype=device.BLOCK_DESC)
+        for t, end in zip(tables, np.cumsum([len(t) for t in tables])):
+            flat[end - len(t):end] = t
+        flat = _on_gpu(flat)
         out = torch.zeros_like(query)
         items = np.zeros(len(counts), dtype=device.DECODE_ITEM)
         lengths = np.array([len(t) for t in tables], dtype=np.int64)
