@@ -8,19 +8,23 @@
 // sum of a larger vocabulary within 64 bits.
 //
 // The kept tokens are a run of the order "falling logit, lower token first
-// among equals": all up to a last one, whose key (the logit's bits as an
-// ordered whole number) and token bound the set.  Block = row, which passes
-// over the row's logits, from the caches after the first time:
-//   1. the highest logit (and the lowest, which sets the bins);
-//   2. where top-k or top-p cut: counts and weights of 1024 bins of the logits,
-//      the bin that the cut falls into, its tokens sorted in LDS (bins of more
-//      tokens than LDS takes are cut into 1024 again, by their keys);
-//   3. the kept tokens' weights, summed by ranges of the vocabulary, the range
-//      that the random number falls into, and the token in it.
+// among equals".  Block = row, which passes over the row's logits, from the
+// caches after the first time:
+//   - The highest logit, and the maxima of 4096 parts of the row.
+//   - Short list (top_k of at most 1024): the top_k-th highest of the maxima is
+//     reached by at least top_k tokens, and by not many more: those are collected
+//     in LDS and sorted, and the cuts and the draw go on there.
+//   - Else, where top-k or top-p cut: counts and weights of 1024 bins of the
+//     logits, the bin that the cut falls into, its tokens sorted in LDS (bins of
+//     more tokens than LDS takes are cut into 1024 again, by their keys), which
+//     gives the last kept token.
+//   - The draw from a row: the kept tokens' weights summed by ranges of the
+//     vocabulary, the range that the random number falls into, the token in it.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "attention_common.h"
 #include "device_common.h"
@@ -32,17 +36,22 @@ namespace {
 constexpr unsigned kBlock = 1024;
 constexpr uint32_t kWaves = kBlock / kWave;
 constexpr uint32_t kRow = 4 * kBlock;        // tokens of one vector of each thread
+constexpr uint32_t kAhead = 4;               // vectors of a thread in flight
 constexpr uint32_t kBins = 1024;
-constexpr uint32_t kSorted = 2048;           // tokens that are sorted in LDS
-constexpr uint32_t kRanges = 32;
+constexpr uint32_t kListed = 2048;           // tokens that are sorted in LDS
+constexpr uint32_t kShortList = 1024;        // the largest top_k whose tokens are listed at once
+constexpr uint32_t kSmall = 128;             // tokens that are ranked by counting
+constexpr uint32_t kBucket = 32;             // tokens of a bucket that are ranked by counting
+constexpr uint32_t kRanges = 8;
 constexpr uint32_t kMostTokens = 1u << 20;
 constexpr uint32_t kMostRows = kMostTokens / kRow + 1;   // vectors of a thread
 constexpr uint32_t kPerRange = (kMostRows + kRanges - 1) / kRanges;
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// ---- whole-number sums over a wave -------------------------------------------
+// ---- sums and maxima over a wave and the block ---------------------------------
 
+// A lower lane's value, 0 where there is none.
 template <int kControl, int kRows>
 __device__ inline uint64_t dpp_u64(uint64_t v)
 {
@@ -51,26 +60,82 @@ __device__ inline uint64_t dpp_u64(uint64_t v)
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-// Each lane's sum of its own and all lower lanes' values.
-__device__ inline uint64_t wave_scan(uint64_t v)
+// Each lane's sum of its own and the lower lanes' values of its row of 16.
+__device__ inline uint64_t row_scan(uint64_t v)
 {
-    v += dpp_u64<0x111, 0xF>(v);   // rows of 16 shifted by 1, 2, 4, 8
+    v += dpp_u64<0x111, 0xF>(v);   // shifted by 1, 2, 4, 8
     v += dpp_u64<0x112, 0xF>(v);
     v += dpp_u64<0x114, 0xF>(v);
     v += dpp_u64<0x118, 0xF>(v);
+    return v;
+}
+
+// The same over the wave.
+__device__ inline uint64_t wave_scan(uint64_t v)
+{
+    v = row_scan(v);
     v += dpp_u64<0x142, 0xA>(v);   // the last lane of rows 0 and 2 to rows 1 and 3
     v += dpp_u64<0x143, 0xC>(v);   // lane 31 to rows 2 and 3
     return v;
 }
 
-__device__ inline uint64_t lane_u64(uint64_t v, int lane)
+__device__ inline uint64_t lane_u64(uint64_t v, uint32_t lane)
 {
-    auto const lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), lane));
-    auto const hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), lane));
+    auto const lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), static_cast<int>(lane)));
+    auto const hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), static_cast<int>(lane)));
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-__device__ inline uint64_t wave_total(uint64_t v) { return lane_u64(wave_scan(v), 63); }
+__device__ inline uint64_t wave_total(uint64_t v) { return lane_u64(wave_scan(v), kWave - 1); }
+
+// The highest of a row of 16, in each of its lanes.
+__device__ inline float row_max(float v)
+{
+    auto const turned = [&](auto control) {
+        return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)), decltype(control)::value, 0xF, 0xF, true)));
+    };
+    v = fmaxf(v, turned(std::integral_constant<int, 0x128>{}));   // rotated by 8, 4, 2, 1
+    v = fmaxf(v, turned(std::integral_constant<int, 0x124>{}));
+    v = fmaxf(v, turned(std::integral_constant<int, 0x122>{}));
+    v = fmaxf(v, turned(std::integral_constant<int, 0x121>{}));
+    return v;
+}
+
+struct SampleLds {
+    uint32_t count[4 * kBlock];      // of 4096 bins of keys, or of kBins
+    uint64_t mass[kBins];
+    uint64_t listed[kListed];        // key, then ~token, so that falling numbers are the order
+    uint64_t other[kListed];         // of a sort, and the listed tokens' weights
+    uint64_t range[kRanges * kWaves];
+    uint64_t row[kPerRange * kWaves];
+    uint64_t wave[kWaves];
+    uint64_t found;
+    uint64_t before;
+    float wave_f[kWaves];
+    uint32_t word[4];
+};
+
+// Sum of the lower threads' values, and of all in *total.
+__device__ inline uint64_t block_scan(uint64_t v, SampleLds& lds, uint64_t* total)
+{
+    uint32_t const wave = threadIdx.x / kWave;
+    uint64_t const upto = wave_scan(v);
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == kWave - 1) lds.wave[wave] = upto;
+    __syncthreads();
+    static_assert(kWaves == 16, "a row of lanes holds the waves' sums");
+    uint64_t const waves = row_scan(lds.wave[threadIdx.x & (kWaves - 1)]);
+    *total = lane_u64(waves, kWaves - 1);
+    uint64_t const before = wave == 0 ? 0 : lane_u64(waves, __builtin_amdgcn_readfirstlane(static_cast<int>(wave)) - 1u);
+    return before + upto - v;
+}
+
+__device__ inline uint64_t block_total(uint64_t v, SampleLds& lds)
+{
+    uint64_t total;
+    static_cast<void>(block_scan(v, lds, &total));
+    return total;
+}
 
 // floor(a b) of a float a in [0, 1] and a whole number, exactly; with `up` the
 // least whole number that is not below a b.
@@ -100,56 +165,46 @@ __device__ inline uint64_t part_of(float a, uint64_t b, bool up)
 
 // ---- keys and weights --------------------------------------------------------
 
-// An ordered whole number of a logit that is not NaN; 0 is below all of them.
+// An ordered whole number of a logit that is not NaN (-0 as 0); 0 is below all of them.
 __device__ inline uint32_t key_of(float x)
 {
-    uint32_t const b = __float_as_uint(x);
+    uint32_t const b = __float_as_uint(x + 0.0f);
     return (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
 }
 __device__ inline float logit_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) != 0 ? key & 0x7FFFFFFFu : ~key); }
+
+// Weights below 2^-48, of tokens this many T under the highest, are 0.
+constexpr float kWeightless = 33.5f;
 
 struct Weights {
     double highest;
     double rate;       // log2(e) / T
     uint32_t scale;    // S
 
-    // 2^t of t = (x - m) rate by the exponential's series on [-1/2, 1/2] ln 2: 13
-    // terms leave 2^-52 of it.
+    // 2^t of t = (x - m) rate = n + f, n whole: 1 + f q(f) on [-1/2, 1/2], q the
+    // polynomial of degree 9 through (2^f - 1) / f at the Chebyshev nodes, off by
+    // 2^-50.  Sums with 1.5 2^52 and 2^52 round to whole numbers, in their low
+    // bits.  0 for -inf and NaN.
     __device__ uint64_t of(float x) const
     {
         double const t = (static_cast<double>(x) - highest) * rate;
-        if (!(t > -64.0)) return 0;
-        double const n = rint(t);
-        double const y = (t - n) * 0.6931471805599453;
-        double s = 1.0 / 479001600.0;
-        s = fma(s, y, 1.0 / 39916800.0);
-        s = fma(s, y, 1.0 / 3628800.0);
-        s = fma(s, y, 1.0 / 362880.0);
-        s = fma(s, y, 1.0 / 40320.0);
-        s = fma(s, y, 1.0 / 5040.0);
-        s = fma(s, y, 1.0 / 720.0);
-        s = fma(s, y, 1.0 / 120.0);
-        s = fma(s, y, 1.0 / 24.0);
-        s = fma(s, y, 1.0 / 6.0);
-        s = fma(s, y, 0.5);
-        s = fma(s, y, 1.0);
-        s = fma(s, y, 1.0);
-        // The sum with 2^52 rounds to whole numbers, which are its low bits.
-        double const w = ldexp(s, static_cast<int>(n) + static_cast<int>(scale)) + 4503599627370496.0;
-        return static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
+        double const z = t + 6755399441055744.0;
+        double const f = t - (z - 6755399441055744.0);
+        double s = 7.070968007227213e-09;
+        s = fma(s, f, 1.0205905282567993e-07);
+        s = fma(s, f, 1.3215451685760035e-06);
+        s = fma(s, f, 1.5252672925515726e-05);
+        s = fma(s, f, 0.0001540353042468356);
+        s = fma(s, f, 0.001333355820079351);
+        s = fma(s, f, 0.009618129107618728);
+        s = fma(s, f, 0.05550410866465168);
+        s = fma(s, f, 0.24022650695910075);
+        s = fma(s, f, 0.6931471805599462);
+        s = fma(s, f, 1.0);
+        int64_t const n = static_cast<int32_t>(__double_as_longlong(z)) + static_cast<int32_t>(scale);
+        double const w = __longlong_as_double(__double_as_longlong(s) + (n << 52)) + 4503599627370496.0;
+        return t > -64.0 ? static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull : 0;
     }
-};
-
-struct SampleLds {
-    uint32_t count[kBins];
-    uint64_t mass[kBins];
-    uint64_t sorted[kSorted];        // key, then ~token, so that falling numbers are the order
-    uint64_t range[kRanges * kWaves];
-    uint64_t row[kPerRange * kWaves];
-    uint64_t wave[kWaves];
-    uint64_t found;
-    float wave_f[2][kWaves];
-    uint32_t word[4];
 };
 
 // The row as the block reads it: vector j of thread t is tokens
@@ -163,7 +218,7 @@ struct Row {
 
     __device__ uint32_t token(uint32_t j) const { return 4 * (j * kBlock + threadIdx.x) - shift; }
 
-    // Tokens past the row, and NaN, are -inf.
+    // -inf past the row.  With logits of +inf, these alone are there, all alike.
     __device__ f32x4_t load(uint32_t j) const
     {
         uint32_t const v = token(j);
@@ -174,181 +229,270 @@ struct Row {
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) x[i] = v + i < V ? from[v + i] : -INFINITY;
         }
+        return x;
+    }
+    __device__ f32x4_t as_counted(f32x4_t x) const
+    {
+        if (infinite) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) x[i] = x[i] != x[i] ? -INFINITY : x[i] + 0.0f;   // no -0
+            for (uint32_t i = 0; i < 4; ++i) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+        }
         return x;
     }
 
-    // With logits of +inf, these alone are there, all alike.
-    __device__ float value(float x) const { return infinite ? (x == INFINITY ? 0.0f : -INFINITY) : x; }
-
-    // f(token, logit) for every token of this thread that can be drawn.
+    // f(j, vector) for every vector, in order, the next ones on their way.  One
+    // vector an iteration: code that a row's block runs through once comes from
+    // memory at its own pace, and eight vectors held in registers and passed over
+    // in unrolled code took 43 us for 4 rows of 32000 drawn whole, a loop 26.
     template <typename F>
-    __device__ void each(F f) const
+    __device__ __attribute__((always_inline)) void vectors_do(F f) const
     {
+        f32x4_t ahead[kAhead];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) ahead[k] = load(k);
+#pragma nounroll
         for (uint32_t j = 0; j < vectors; ++j) {
-            f32x4_t const y = load(j);
+            f32x4_t const now = as_counted(ahead[0]);
+#pragma unroll
+            for (uint32_t k = 1; k < kAhead; ++k) ahead[k - 1] = ahead[k];
+            ahead[kAhead - 1] = load(j + kAhead);
+            f(j, now);
+        }
+    }
+
+    // f(token, logit) for every token of this thread with a logit in [low, high];
+    // vectors without one in any lane cost four comparisons.
+    template <typename F>
+    __device__ __attribute__((always_inline)) void each_within(float low, float high, F f) const
+    {
+        vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
+            bool in[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) in[i] = y[i] >= low && y[i] <= high;
+            if (!(in[0] || in[1] || in[2] || in[3])) return;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
-                float const x = value(y[i]);
-                if (x != -INFINITY) f(token(j) + i, x);
+                if (in[i]) f(token(j) + i, y[i]);
             }
-        }
+        });
     }
 };
 
-// Sum over the block, in every thread.
-__device__ inline uint64_t block_total(uint64_t v, SampleLds& lds)
-{
-    uint64_t const total = wave_total(v);
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) lds.wave[threadIdx.x / kWave] = total;
-    __syncthreads();
-    uint64_t sum = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) sum += lds.wave[w];
-    return sum;
-}
+__device__ inline float highest_of(f32x4_t const& y) { return fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])); }
 
-// Sum of the lower threads' values, and of all in *total.
-__device__ inline uint64_t block_scan(uint64_t v, SampleLds& lds, uint64_t* total)
-{
-    uint64_t const upto = wave_scan(v);
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == kWave - 1) lds.wave[threadIdx.x / kWave] = upto;
-    __syncthreads();
-    uint64_t before = 0, sum = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) {
-        if (w < threadIdx.x / kWave) before += lds.wave[w];
-        sum += lds.wave[w];
+// The last kept token: its logit and its number.  Kept are the higher logits,
+// and of its own the tokens up to it.
+struct Last {
+    float logit;
+    uint32_t token;
+    __device__ bool keeps(float x, uint32_t t) const { return x > logit || (x == logit && t <= token); }
+};
+
+// ---- the draw from a row -------------------------------------------------------
+
+// What a token weighs in a draw.
+struct Kept {
+    Weights weights;
+    Last last;
+    uint64_t least;   // weights below it are not kept
+    float floor;      // no logit below it is kept or weighs anything
+
+    __device__ __attribute__((always_inline)) uint64_t of(float x, uint32_t token) const
+    {
+        uint64_t const w = weights.of(x);
+        return last.keeps(x, token) && w >= least ? w : 0;
     }
-    *total = sum;
-    return before + upto - v;
-}
+};
 
-// The ranges' sums of weight(token, logit), and all of them.
-template <typename F>
-__device__ uint64_t sum_ranges(const Row& row, SampleLds& lds, uint32_t per, F weight)
+// One for each token of a logit.
+struct Same {
+    float floor;
+    __device__ uint64_t of(float x, uint32_t) const { return x == floor ? 1 : 0; }
+};
+
+// The sums of the tokens' weights by ranges of `per` vectors, and all of them.
+template <typename W>
+__device__ __attribute__((always_inline)) inline uint64_t sum_ranges(const Row& row, SampleLds& lds, uint32_t per, const W& weight)
 {
     uint32_t const wave = threadIdx.x / kWave;
     uint32_t const lane = threadIdx.x & (kWave - 1);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kRanges * kWaves; i += kBlock) lds.range[i] = 0;
+    if (threadIdx.x < kRanges * kWaves) lds.range[threadIdx.x] = 0;
     __syncthreads();
     uint64_t all = 0, sum = 0;
-    uint32_t at = 0;
-    auto const flush = [&] {
-        if (__ballot(sum != 0) != 0) {
-            uint64_t const total = wave_total(sum);
-            if (lane == 0) lds.range[at * kWaves + wave] = total;
-            all += total;
-        }
-        sum = 0;
-        ++at;
-    };
-    for (uint32_t j = 0; j < row.vectors; ++j) {
-        f32x4_t const y = row.load(j);
+    uint32_t at = 0, left = per;
+    row.vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
+        if (highest_of(y) >= weight.floor) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            float const x = row.value(y[i]);
-            if (x != -INFINITY) sum += weight(row.token(j) + i, x);
+            for (uint32_t i = 0; i < 4; ++i) sum += weight.of(y[i], row.token(j) + i);
         }
-        if ((j + 1) % per == 0 || j + 1 == row.vectors) flush();
-    }
-    if (lane == 0) lds.wave[wave] = all;
-    __syncthreads();
-    uint64_t total = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) total += lds.wave[w];
-    return total;
-}
-
-// Of sums by (part, wave), in order: the part that the target falls into, and
-// what lies before it.  Every thread reads them.
-__device__ inline uint32_t part_at(const uint64_t* sums, uint32_t parts, uint64_t target, uint64_t* before)
-{
-    uint64_t sum = 0;
-    for (uint32_t p = 0; p < parts; ++p) {
-        uint64_t part = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < kWaves; ++w) part += sums[p * kWaves + w];
-        if (target < sum + part) {
-            *before = sum;
-            return p;
+        if (--left == 0 || j + 1 == row.vectors) {
+            if (__ballot(sum != 0) != 0) {
+                uint64_t const total = wave_total(sum);
+                if (lane == 0) lds.range[at * kWaves + wave] = total;
+                all += total;
+            }
+            sum = 0;
+            ++at;
+            left = per;
         }
-        sum += part;
-    }
-    *before = sum;
-    return parts;   // only for a target that is no part of the sum
+    });
+    return block_total(lane == 0 ? all : 0, lds);
 }
 
 // The first token at which the running sum exceeds `target`, less than all of
 // it; the ranges' sums are in place.  Its weight in *its.
-template <typename F>
-__device__ uint32_t token_at(const Row& row, SampleLds& lds, uint32_t per, uint64_t target, F weight, uint64_t* its)
+template <typename W>
+__device__ uint32_t token_at(const Row& row, SampleLds& lds, uint32_t per, uint64_t target, const W& weight, uint64_t* its)
 {
     uint32_t const wave = threadIdx.x / kWave;
     uint32_t const lane = threadIdx.x & (kWave - 1);
-    uint64_t before;
-    uint32_t const range = part_at(lds.range, kRanges, target, &before);
-    uint32_t const j0 = range * per;
+    static_assert(kRanges * kWaves == 2 * kWave, "two a lane, eight lanes a range");
+    if (wave == 0) {
+        uint64_t const sum = lds.range[2 * lane] + lds.range[2 * lane + 1];
+        uint64_t const upto = wave_scan(sum);
+        // The lane in which the target lies; its range's first lane knows what lies before.
+        uint64_t const hit = __ballot(target >= upto - sum && target - (upto - sum) < sum);
+        uint32_t const at = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(hit)) - 1) & ~7u;
+        if (lane == at) {
+            lds.word[0] = at / 8;
+            lds.before = upto - sum;
+        }
+    }
+    __syncthreads();
+    uint32_t const j0 = lds.word[0] * per;
     uint32_t const j1 = min(j0 + per, row.vectors);
+    uint64_t at = lds.before;
+    uint64_t w4[4] = {};
+#pragma nounroll
     for (uint32_t j = j0; j < j1; ++j) {
-        f32x4_t const y = row.load(j);
+        f32x4_t const y = row.as_counted(row.load(j));
         uint64_t sum = 0;
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            float const x = row.value(y[i]);
-            if (x != -INFINITY) sum += weight(row.token(j) + i, x);
+            w4[i] = weight.of(y[i], row.token(j) + i);
+            sum += w4[i];
         }
-        uint64_t const total = __ballot(sum != 0) != 0 ? wave_total(sum) : 0;
+        uint64_t const total = wave_total(sum);
         if (lane == 0) lds.row[(j - j0) * kWaves + wave] = total;
     }
     __syncthreads();
-    uint64_t rows_before;
-    uint32_t const j = j0 + part_at(lds.row, j1 > j0 ? j1 - j0 : 0, target - before, &rows_before);
-    if (j < j1) {
-        uint64_t at = before + rows_before;
-        for (uint32_t w = 0; w < wave; ++w) at += lds.row[(j - j0) * kWaves + w];
-        uint64_t const mine = lds.row[(j - j0) * kWaves + wave];
-        if (target >= at && target - at < mine) {   // this wave's
-            f32x4_t const y = row.load(j);
-            uint64_t w4[4];
-            uint64_t sum = 0;
+#pragma nounroll
+    for (uint32_t j = j0; j < j1; ++j) {
+        uint64_t const part = lds.row[(j - j0) * kWaves + (lane & (kWaves - 1))];
+        uint64_t const upto = row_scan(part);
+        uint64_t const mine = lane_u64(part, __builtin_amdgcn_readfirstlane(static_cast<int>(wave)));
+        uint64_t before = at + lane_u64(upto, __builtin_amdgcn_readfirstlane(static_cast<int>(wave))) - mine;
+        at += lane_u64(upto, kWaves - 1);
+        if (target < before || target - before >= mine) continue;
+        // In this vector of this wave.
+        if (j + 1 != j1) {
+            f32x4_t const y = row.as_counted(row.load(j));
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                float const x = row.value(y[i]);
-                w4[i] = x != -INFINITY ? weight(row.token(j) + i, x) : 0;
-                sum += w4[i];
+            for (uint32_t i = 0; i < 4; ++i) w4[i] = weight.of(y[i], row.token(j) + i);
+        }
+        uint64_t const sum = w4[0] + w4[1] + w4[2] + w4[3];
+        before += wave_scan(sum) - sum;
+        if (target < before || target - before >= sum) continue;
+        bool found = false;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (!found && target - before < w4[i]) {
+                found = true;
+                lds.word[1] = row.token(j) + i;
+                lds.found = w4[i];
             }
-            at += wave_scan(sum) - sum;
-            if (target >= at && target - at < sum) {   // this thread's
-                bool found = false;
+            if (!found) before += w4[i];
+        }
+    }
+    __syncthreads();
+    *its = lds.found;
+    return lds.word[1];
+}
+
+// ---- sorting ---------------------------------------------------------------------
+
+// Sorts numbers[0, n), all different, into falling order; n at most kListed,
+// their upper words within low .. high.
+__device__ __attribute__((noinline)) void sort_falling(uint64_t* numbers, SampleLds& lds, uint32_t n, uint32_t low, uint32_t high)
+{
+    uint32_t const tid = threadIdx.x;
+    __syncthreads();
+    if (n <= kSmall) {
+        // Each goes to the place that the higher ones leave it: eight threads a number.
+        uint32_t const mine = tid / (kBlock / kSmall);
+        uint32_t const part = tid % (kBlock / kSmall);
+        uint64_t const x = mine < n ? numbers[mine] : 0;
+        uint32_t higher = 0;
+        for (uint32_t i = part; i < n; i += kBlock / kSmall) higher += numbers[i] > x ? 1u : 0u;
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    if (!found && target - at < w4[i]) {
-                        found = true;
-                        lds.word[0] = row.token(j) + i;
-                        lds.found = w4[i];
-                    }
-                    if (!found) at += w4[i];
+        for (uint32_t k = 1; k < kBlock / kSmall; k *= 2) higher += static_cast<uint32_t>(__shfl_xor(static_cast<int>(higher), static_cast<int>(k)));
+        __syncthreads();
+        if (mine < n && part == 0) numbers[higher] = x;
+        __syncthreads();
+        return;
+    }
+    // Buckets of the upper words, a thread each; then each number to its place in its bucket.
+    static_assert(kBins == kBlock && kListed == 2 * kBlock, "a bucket and two numbers a thread");
+    uint32_t shift = 0;
+    while (((high - low) >> shift) >= kBins) ++shift;
+    lds.count[tid] = 0;
+    __syncthreads();
+    uint64_t x[2];
+    uint32_t bucket[2], place[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        uint32_t const at = tid + i * kBlock;
+        if (at >= n) continue;
+        x[i] = numbers[at];
+        bucket[i] = (high - static_cast<uint32_t>(x[i] >> 32)) >> shift;
+        place[i] = atomicAdd(&lds.count[bucket[i]], 1u);
+    }
+    __syncthreads();
+    uint32_t const size = lds.count[tid];
+    uint64_t all;
+    uint64_t const start = block_scan(size, lds, &all);
+    lds.count[kBins + tid] = static_cast<uint32_t>(start);
+    if (__syncthreads_or(size > kBucket) == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            if (tid + i * kBlock < n) lds.other[lds.count[kBins + bucket[i]] + place[i]] = x[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            if (tid + i * kBlock >= n) continue;
+            uint32_t const first = lds.count[kBins + bucket[i]];
+            uint32_t const last = first + lds.count[bucket[i]];
+            uint32_t higher = 0;
+            for (uint32_t k = first; k < last; ++k) higher += lds.other[k] > x[i] ? 1u : 0u;
+            numbers[first + higher] = x[i];
+        }
+        __syncthreads();
+        return;
+    }
+    // Crowded buckets: pairs compared and exchanged.
+    uint32_t padded = 2 * kSmall;
+    while (padded < n) padded *= 2;
+    for (uint32_t i = n + tid; i < padded; i += kBlock) numbers[i] = 0;
+    for (uint32_t k = 2; k <= padded; k *= 2) {
+        for (uint32_t j = k / 2; j > 0; j /= 2) {
+            __syncthreads();
+            for (uint32_t p = tid; p < padded / 2; p += kBlock) {
+                uint32_t const i = 2 * p - (p & (j - 1));
+                uint64_t const a = numbers[i];
+                uint64_t const b = numbers[i + j];
+                if ((a < b) == ((i & k) == 0)) {
+                    numbers[i] = b;
+                    numbers[i + j] = a;
                 }
             }
         }
     }
     __syncthreads();
-    *its = lds.found;
-    return lds.word[0];
 }
 
-// The last kept token: its key and its number.  Kept are the higher keys, and
-// of its own the tokens up to it.
-struct Last {
-    uint32_t key;
-    uint32_t token;
-    __device__ bool keeps(uint32_t k, uint32_t t) const { return k > key || (k == key && t <= token); }
-};
+// ---- the cuts of a row -------------------------------------------------------------
 
 // What a cut looks for: the `amount`-th token (from 1) of the order, or the
 // first at which the weight reaches `amount`.
@@ -357,100 +501,71 @@ struct Cut {
     uint64_t amount;
 };
 
+// Bins of the logits from the highest down to where weights are 0; the last
+// one's tokens are not counted.  Half a logit, as the difference of two may be
+// past the largest number.
 struct Bins {
-    float highest;
-    float rate;      // bins for a unit of the logit
-    bool bounded;    // the last bin holds tokens of weight 0 and of any logit
-    __device__ uint32_t of(float x) const { return static_cast<uint32_t>(fminf((highest - x) * rate, static_cast<float>(kBins - 1))); }
+    float half;      // of the highest logit
+    float rate;      // bins for a unit of half a logit, finite
+    __device__ uint32_t of(float x) const { return static_cast<uint32_t>(fminf((half - 0.5f * x) * rate, static_cast<float>(kBins - 1))); }
 };
 
-// The bin of the counted ones that the cut falls into, what lies in the bins
-// before it, and how many tokens it holds.
+// The bin of the counted ones that the cut falls into, how many tokens it
+// holds, and what lies before it of what the cut counts.
 struct Place {
-    uint32_t bin;
+    uint32_t bin;     // kBins: the cut lies past all that is counted
     uint32_t count;
-    uint64_t before_count;
-    uint64_t before_mass;
+    uint64_t before;
 };
 
-__device__ inline Place place_of(SampleLds& lds, const Cut& cut, uint64_t before_count, uint64_t before_mass)
+__device__ inline Place place_of(SampleLds& lds, const Cut& cut, uint64_t before)
 {
     static_assert(kBins == kBlock, "a thread a bin");
     uint32_t const tid = threadIdx.x;
-    uint64_t all_count, all_mass;
-    uint64_t const count = lds.count[tid];
-    uint64_t const mass = lds.mass[tid];
-    uint64_t const counts = before_count + block_scan(count, lds, &all_count);
-    uint64_t const masses = before_mass + block_scan(mass, lds, &all_mass);
-    uint64_t const at = cut.by_mass ? masses : counts;
-    uint64_t const mine = cut.by_mass ? mass : count;
-    __syncthreads();
+    uint64_t all;
+    uint64_t const mine = cut.by_mass ? lds.mass[tid] : lds.count[tid];
+    uint64_t const at = before + block_scan(mine, lds, &all);
     if (tid == 0) lds.word[0] = kBins;
     __syncthreads();
     if (at < cut.amount && cut.amount - at <= mine) {   // one thread at most
         lds.word[0] = tid;
-        lds.word[1] = static_cast<uint32_t>(count);
-        lds.range[0] = counts;
-        lds.range[1] = masses;
+        lds.word[1] = lds.count[tid];
+        lds.before = at;
     }
     __syncthreads();
-    Place const p{lds.word[0], lds.word[1], lds.range[0], lds.range[1]};
+    Place const p{lds.word[0], lds.word[1], lds.before};
     __syncthreads();
     return p;
 }
 
-// Sorts lds.sorted[0, n) into falling order; n at most kSorted.
-__device__ inline void sort_falling(SampleLds& lds, uint32_t n)
-{
-    uint32_t size = 2;
-    while (size < n) size *= 2;
-    for (uint32_t i = n + threadIdx.x; i < size; i += kBlock) lds.sorted[i] = 0;
-    for (uint32_t k = 2; k <= size; k *= 2) {
-        for (uint32_t j = k / 2; j > 0; j /= 2) {
-            __syncthreads();
-            for (uint32_t p = threadIdx.x; p < size / 2; p += kBlock) {
-                uint32_t const i = 2 * p - (p & (j - 1));
-                uint64_t const a = lds.sorted[i];
-                uint64_t const b = lds.sorted[i + j];
-                if ((a < b) == ((i & k) == 0)) {
-                    lds.sorted[i] = b;
-                    lds.sorted[i + j] = a;
-                }
-            }
-        }
-    }
-    __syncthreads();
-}
-
-// Where the cut falls, and the weight up to and with its token in *upto.  Bins'
-// counts (and weights, where `weigh`) are in lds.
-__device__ Last find_cut(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, const Cut& cut, bool weigh,
-                         uint32_t per, uint64_t* upto)
+// Where the cut falls; everything is kept where it lies past what is counted.
+// The bins' counts and weights are in lds.
+__device__ __attribute__((noinline)) Last find_cut(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, const Cut& cut,
+                                                   uint32_t per)
 {
     uint32_t const tid = threadIdx.x;
-    Last const everything{0, 0xFFFFFFFFu};
-    Place place = place_of(lds, cut, 0, 0);
-    *upto = 0;
-    // Past the last token, or among tokens that weigh nothing.
-    if (place.bin == kBins || (bins.bounded && place.bin == kBins - 1)) return everything;
-    // The bin's tokens, and their highest and lowest keys.
+    Place place = place_of(lds, cut, 0);
+    if (place.bin == kBins) return Last{-INFINITY, 0xFFFFFFFFu};
     uint32_t const bin = place.bin;
+    // The bin's tokens, and their highest and lowest keys, of the logits that
+    // may be in it: its bounds with a part in 2^18 of the largest on the way.
+    auto const border = [&](uint32_t b) { return 2.0f * (bins.half - static_cast<float>(b) / bins.rate); };
+    float const slack = (fabsf(bins.half) + static_cast<float>(bin + 1) / bins.rate) * 0x1p-17f;
+    float const low_x = border(bin + 1) - slack;
+    float const high_x = border(bin) + slack;
     if (tid < 3) lds.word[tid] = tid == 2 ? 0xFFFFFFFFu : 0;
     __syncthreads();
-    row.each([&](uint32_t token, float x) {
+    row.each_within(low_x == low_x ? low_x : -INFINITY, high_x == high_x ? high_x : INFINITY, [&](uint32_t token, float x) __attribute__((always_inline)) {
         if (bins.of(x) != bin) return;
         uint32_t const key = key_of(x);
-        if (place.count <= kSorted) {
-            lds.sorted[atomicAdd(&lds.word[0], 1u)] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - token);
-        } else {
-            atomicMax(&lds.word[1], key);
-            atomicMin(&lds.word[2], key);
-        }
+        if (place.count <= kListed) lds.listed[atomicAdd(&lds.word[0], 1u)] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - token);
+        atomicMax(&lds.word[1], key);
+        atomicMin(&lds.word[2], key);
     });
     __syncthreads();
     uint32_t high = lds.word[1];
     uint32_t low = lds.word[2];
-    while (place.count > kSorted && high != low) {
+    while (place.count > kListed && high != low) {
         // The keys low .. high, cut into bins of 2^shift keys.
         uint32_t shift = 0;
         while (((high - low) >> shift) >= kBins) ++shift;
@@ -458,66 +573,124 @@ __device__ Last find_cut(const Row& row, SampleLds& lds, const Weights& weights,
         lds.count[tid] = 0;
         lds.mass[tid] = 0;
         __syncthreads();
-        row.each([&](uint32_t, float x) {
+        // The keys' own bounds count: that of -0 is no logit's, but compares as 0.
+        row.each_within(logit_of(low), logit_of(high), [&](uint32_t, float x) __attribute__((always_inline)) {
             uint32_t const key = key_of(x);
             if (key < low || key > high) return;
             uint32_t const b = (high - key) >> shift;
             atomicAdd(&lds.count[b], 1u);
-            if (weigh) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.mass[b]), static_cast<unsigned long long>(weights.of(x)));
+            if (cut.by_mass) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.mass[b]), static_cast<unsigned long long>(weights.of(x)));
         });
         __syncthreads();
-        place = place_of(lds, cut, place.before_count, place.before_mass);
+        place = place_of(lds, cut, place.before);
         high -= place.bin << shift;
         uint32_t const keys = 1u << shift;
         low = high - low >= keys ? high - keys + 1 : low;
-        if (place.count > kSorted) continue;
+        if (place.count > kListed) continue;
         if (tid == 0) lds.word[0] = 0;
         __syncthreads();
-        row.each([&](uint32_t token, float x) {
+        row.each_within(logit_of(low), logit_of(high), [&](uint32_t token, float x) __attribute__((always_inline)) {
             uint32_t const key = key_of(x);
-            if (key >= low && key <= high) lds.sorted[atomicAdd(&lds.word[0], 1u)] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - token);
+            if (key >= low && key <= high) lds.listed[atomicAdd(&lds.word[0], 1u)] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - token);
         });
         __syncthreads();
     }
-    uint64_t const left = cut.amount - (cut.by_mass ? place.before_mass : place.before_count);   // at least 1
-    if (place.count > kSorted) {
+    uint64_t const left = cut.amount - place.before;   // at least 1
+    if (place.count > kListed) {
         // One key: so many of its tokens, the lowest first.
-        uint64_t const weight = weights.of(logit_of(high));
-        uint64_t const tokens = cut.by_mass ? (left + weight - 1) / weight : left;
-        auto const same = [&](uint32_t, float x) { return key_of(x) == high ? uint64_t{1} : uint64_t{0}; };
+        uint64_t const weight = cut.by_mass ? weights.of(logit_of(high)) : 1;
+        Same const same{logit_of(high)};
         static_cast<void>(sum_ranges(row, lds, per, same));
         uint64_t one;
-        uint32_t const token = token_at(row, lds, per, tokens - 1, same, &one);
-        *upto = place.before_mass + tokens * weight;
-        return Last{high, token};
+        uint32_t const token = token_at(row, lds, per, (left - 1) / weight, same, &one);
+        return Last{logit_of(high), token};
     }
-    sort_falling(lds, place.count);
+    sort_falling(lds.listed, lds, place.count, low, high);
     // Two neighbours of the order a thread.
-    uint64_t w[2];
+    uint64_t w[2] = {};
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
         uint32_t const n = 2 * tid + i;
-        w[i] = n < place.count && weigh ? weights.of(logit_of(static_cast<uint32_t>(lds.sorted[n] >> 32))) : 0;
+        if (n < place.count) w[i] = cut.by_mass ? weights.of(logit_of(static_cast<uint32_t>(lds.listed[n] >> 32))) : 1;
     }
-    uint64_t total = 0;
-    uint64_t at = weigh ? block_scan(w[0] + w[1], lds, &total) : 0;
-    __syncthreads();
+    uint64_t total;
+    uint64_t at = block_scan(w[0] + w[1], lds, &total);
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
-        uint32_t const n = 2 * tid + i;
-        bool const here = n < place.count && (cut.by_mass ? at < left && left - at <= w[i] : n + 1 == left);
-        at += w[i];
-        if (here) {
-            lds.word[0] = static_cast<uint32_t>(lds.sorted[n] >> 32);
-            lds.word[1] = 0xFFFFFFFFu - static_cast<uint32_t>(lds.sorted[n]);
-            lds.found = at;
+        if (at < left && left - at <= w[i]) {
+            lds.word[0] = static_cast<uint32_t>(lds.listed[2 * tid + i] >> 32);
+            lds.word[1] = 0xFFFFFFFFu - static_cast<uint32_t>(lds.listed[2 * tid + i]);
         }
+        at += w[i];
     }
     __syncthreads();
-    *upto = place.before_mass + lds.found;
-    Last const last{lds.word[0], lds.word[1]};
+    Last const last{logit_of(lds.word[0]), lds.word[1]};
     __syncthreads();
     return last;
+}
+
+// ---- the draw from a short list -----------------------------------------------------
+
+struct Drawn {
+    uint32_t token;
+    uint64_t weight;
+    uint64_t total;
+};
+
+// From the list of the highest tokens, keys within low .. high, the first top_k
+// of which count.  Each thread has up to two neighbours of the list.
+__device__ inline Drawn draw_listed(SampleLds& lds, const Weights& weights, const kimkv_sample_rule& rule, uint32_t listed, uint32_t top_k,
+                                    uint32_t low, uint32_t high, float uniform, uint32_t V)
+{
+    uint32_t const tid = threadIdx.x;
+    sort_falling(lds.listed, lds, listed, low, high);
+    uint32_t const n = min(listed, top_k);
+    uint64_t const least = part_of(rule.min_p, uint64_t{1} << weights.scale, true);
+    uint64_t w[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) w[i] = 2 * tid + i < n ? weights.of(logit_of(static_cast<uint32_t>(lds.listed[2 * tid + i] >> 32))) : 0;
+    uint64_t total;
+    uint64_t at = block_scan(w[0] + w[1], lds, &total);
+    // What top-p keeps begins before its part of the weight is reached.
+    uint64_t const need = rule.top_p < 1.0f ? part_of(rule.top_p, total, true) : ~uint64_t{0};
+    uint32_t kept = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        if (2 * tid + i < n && at < need && w[i] >= least) {
+            kept += 1;
+            at += w[i];
+        } else {
+            at = ~uint64_t{0};   // nor what comes behind
+            w[i] = 0;
+        }
+    }
+    uint32_t const m = static_cast<uint32_t>(block_total(kept, lds));
+    // The kept ones in the vocabulary's order: ~token, then the place in the list.
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        uint32_t const p = 2 * tid + i;
+        if (p < m) lds.listed[p] = lds.listed[p] << 32 | p;
+    }
+    sort_falling(lds.listed, lds, m, 0xFFFFFFFFu - (V - 1), 0xFFFFFFFFu);
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        if (2 * tid + i < m) lds.other[2 * tid + i] = w[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) w[i] = 2 * tid + i < m ? lds.other[static_cast<uint32_t>(lds.listed[2 * tid + i])] : 0;
+    at = block_scan(w[0] + w[1], lds, &total);
+    uint64_t const target = part_of(uniform, total, false);
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        if (target >= at && target - at < w[i]) {
+            lds.word[0] = 0xFFFFFFFFu - static_cast<uint32_t>(lds.listed[2 * tid + i] >> 32);
+            lds.found = w[i];
+        }
+        at += w[i];
+    }
+    __syncthreads();
+    return Drawn{lds.word[0], lds.found, total};
 }
 
 struct SampleArgs {
@@ -553,59 +726,96 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
         answer(KIMKV_NO_TOKEN, 0.0f);
         return;
     }
+    auto const clear = [&] {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) lds.count[i * kBlock + tid] = 0;
+        lds.mass[tid] = 0;
+    };
+    clear();
 
-    // ---- the highest logit, and the lowest that is not -inf ----
-    float high = -INFINITY;
-    float low = INFINITY;
-    for (uint32_t j = 0; j < row.vectors; ++j) {
-        f32x4_t const y = row.load(j);
+    // ---- the highest logit, by place in a vector (NaN is left out) ----
+    f32x4_t high4 = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            high = fmaxf(high, y[i]);
-            low = fminf(low, y[i] == -INFINITY ? INFINITY : y[i]);
-        }
-    }
-    high = wave_max(high);
-    low = -wave_max(-low);
-    if (lane == 0) {
-        lds.wave_f[0][tid / kWave] = high;
-        lds.wave_f[1][tid / kWave] = low;
-    }
-    lds.count[tid] = 0;
-    lds.mass[tid] = 0;
+        for (uint32_t i = 0; i < 4; ++i) high4[i] = fmaxf(high4[i], y[i]);
+    });
+    float high = row_max(highest_of(high4));
+    high = fmaxf(high, xor16(high));
+    high = fmaxf(high, xor32(high));
+    if (lane == 0) lds.wave_f[tid / kWave] = high;
     __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) {
-        high = fmaxf(high, lds.wave_f[0][w]);
-        low = fminf(low, lds.wave_f[1][w]);
-    }
+    high = row_max(lds.wave_f[lane & (kWaves - 1)]);
     if (high == -INFINITY) {
         answer(KIMKV_NO_TOKEN, 0.0f);
         return;
     }
     row.infinite = high == INFINITY;
-    if (row.infinite) high = low = 0.0f;
+    high4 = row.as_counted(high4);
+    if (row.infinite) high = 0.0f;
 
     bool const greedy = rule.temperature == 0.0f;
+    float const temperature = greedy ? 1.0f : rule.temperature;
     uint32_t const top_k = greedy ? 1 : rule.top_k == 0 || rule.top_k >= a.V ? a.V : rule.top_k;
-    bool const cut_k = top_k < a.V;
+    bool const cut_k = top_k < a.V || greedy;
     bool const cut_p = !greedy && rule.top_p < 1.0f;
-    Weights const weights{high, greedy ? 1.0 : 1.4426950408889634 / static_cast<double>(rule.temperature), a.scale};
+    Weights const weights{high, 1.4426950408889634 / static_cast<double>(temperature), a.scale};
+
+    if (cut_k && top_k <= kShortList) {
+        // Bins of the maxima's keys, from the highest down; four of them a thread.
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (high4[i] != -INFINITY) atomicAdd(&lds.count[4095u - (key_of(high4[i]) >> 20)], 1u);
+        }
+        if (tid == 0) {
+            lds.word[0] = 0;       // listed tokens
+            lds.word[1] = 4095;    // the bound's bin: all, where there are fewer maxima
+        }
+        __syncthreads();
+        uint32_t of[4];
+        uint64_t sum = 0, all;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            of[i] = lds.count[4 * tid + i];
+            sum += of[i];
+        }
+        uint64_t at = block_scan(sum, lds, &all);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (at < top_k && at + of[i] >= top_k) lds.word[1] = 4 * tid + i;   // one thread at most
+            at += of[i];
+        }
+        __syncthreads();
+        uint32_t const bound = max((4095u - lds.word[1]) << 20, 0x00800000u);   // at least the lowest number's key
+        row.each_within(logit_of(bound), INFINITY, [&](uint32_t token, float x) __attribute__((always_inline)) {
+            uint32_t const at_list = atomicAdd(&lds.word[0], 1u);
+            if (at_list < kListed) lds.listed[at_list] = static_cast<uint64_t>(key_of(x)) << 32 | (0xFFFFFFFFu - token);
+        });
+        __syncthreads();
+        uint32_t const listed = lds.word[0];
+        if (listed <= kListed) {
+            Drawn const d = draw_listed(lds, weights, rule, listed, top_k, bound, key_of(high), uniform, a.V);
+            answer(d.token, static_cast<float>(static_cast<double>(d.weight) / static_cast<double>(d.total)));
+            return;
+        }
+        __syncthreads();
+        clear();
+        __syncthreads();
+    }
+
     // Ranges of `per` vectors.
     uint32_t const per = (row.vectors + kRanges - 1) / kRanges;
-    Last last{0, 0xFFFFFFFFu};
+    float const weightless = high - kWeightless * temperature;   // no logit below weighs anything; -inf past the largest number
+    Last last{-INFINITY, 0xFFFFFFFFu};
     if (cut_k || cut_p) {
-        // Tokens 64 T or more below the highest weigh nothing, whatever their order.
-        float const span = high - low;
-        float const most = greedy ? INFINITY : 64.0f * rule.temperature;
-        bool const bounded = span > most;
-        Bins const bins{high, span == 0.0f || most == 0.0f ? 0.0f : static_cast<float>(kBins - 1) / fminf(span, most), bounded};
-        row.each([&](uint32_t, float x) {
-            uint32_t const b = bins.of(x);
-            atomicAdd(&lds.count[b], 1u);
-            if (cut_p) {
-                uint64_t const w = weights.of(x);
-                if (w != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.mass[b]), static_cast<unsigned long long>(w));
+        Bins const bins{0.5f * high, fminf(2 * (kBins - 1) / (kWeightless * temperature), 3e38f)};
+        row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
+            if (bins.of(highest_of(y)) >= kBins - 1) return;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                uint32_t const b = bins.of(y[i]);
+                if (b >= kBins - 1) continue;
+                atomicAdd(&lds.count[b], 1u);
+                if (cut_p) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.mass[b]), static_cast<unsigned long long>(weights.of(y[i])));
             }
         });
         __syncthreads();
@@ -614,28 +824,27 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
         uint64_t total = 0;
         if (cut_p) total = block_total(mass, lds);
         if (cut_k) {
-            uint64_t upto;
-            last = find_cut(row, lds, weights, bins, Cut{false, top_k}, cut_p, per, &upto);
-            if (last.key != 0) total = upto;
+            last = find_cut(row, lds, weights, bins, Cut{false, top_k}, per);
+            if (cut_p && last.logit != -INFINITY) total = sum_ranges(row, lds, per, Kept{weights, last, 0, fmaxf(last.logit, weightless)});
         }
         if (cut_p) {
             __syncthreads();
             lds.count[tid] = count;
             lds.mass[tid] = mass;
             __syncthreads();
-            uint64_t upto;
-            Last const mine = find_cut(row, lds, weights, bins, Cut{true, part_of(rule.top_p, total, true)}, true, per, &upto);
-            if (mine.key > last.key || (mine.key == last.key && mine.token < last.token)) last = mine;
+            Last const mine = find_cut(row, lds, weights, bins, Cut{true, part_of(rule.top_p, total, true)}, per);
+            if (mine.logit > last.logit || (mine.logit == last.logit && mine.token < last.token)) last = mine;
         }
     }
 
     // ---- the draw ----
-    uint64_t const least = part_of(rule.min_p, uint64_t{1} << a.scale, true);
-    auto const kept = [&](uint32_t token, float x) -> uint64_t {
-        if (!last.keeps(key_of(x), token)) return 0;
-        uint64_t const w = weights.of(x);
-        return w >= least ? w : 0;
-    };
+    float floor = fmaxf(last.logit, weightless);
+    if (rule.min_p > 0.0f) {
+        // Below min-p's logit by more than what 32 bits lose on the way to it.
+        float const under = temperature * logf(rule.min_p);
+        floor = fmaxf(floor, high + under - (fabsf(high) - under) * 0x1p-18f);
+    }
+    Kept const kept{weights, last, part_of(rule.min_p, uint64_t{1} << a.scale, true), floor};
     uint64_t const total = sum_ranges(row, lds, per, kept);
     uint64_t its;
     uint32_t const token = token_at(row, lds, per, part_of(uniform, total, false), kept, &its);
