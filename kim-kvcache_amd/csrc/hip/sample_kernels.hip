@@ -14,9 +14,9 @@
 //   - Short list (top_k of at most 1024): the top_k-th highest of the maxima is
 //     reached by at least top_k tokens, and by not many more: those are collected
 //     in LDS and sorted, and the cuts and the draw go on there.
-//   - Else, where top-k or top-p cut: counts and weights of 1024 bins of the
+//   - Else, where top-k or top-p cut: counts and weights of 4096 bins of the
 //     logits, the bin that the cut falls into, its tokens sorted in LDS (bins of
-//     more tokens than LDS takes are cut into 1024 again, by their keys), which
+//     more tokens than LDS takes are cut into 4096 again, by their keys), which
 //     gives the last kept token.
 //   - The draw from a row: the kept tokens' weights summed by ranges of the
 //     vocabulary, the range that the random number falls into, the token in it.
@@ -35,17 +35,16 @@ namespace {
 
 constexpr unsigned kBlock = 1024;
 constexpr uint32_t kWaves = kBlock / kWave;
-constexpr uint32_t kRow = 4 * kBlock;        // tokens of one vector of each thread
+constexpr uint32_t kVector = 4 * kWave;      // tokens of one load of a wave
 constexpr uint32_t kAhead = 4;               // vectors of a thread in flight
-constexpr uint32_t kBins = 1024;
+constexpr uint32_t kBins = 4096;             // four a thread
 constexpr uint32_t kListed = 2048;           // tokens that are sorted in LDS
 constexpr uint32_t kShortList = 1024;        // the largest top_k whose tokens are listed at once
 constexpr uint32_t kSmall = 128;             // tokens that are ranked by counting
 constexpr uint32_t kBucket = 32;             // tokens of a bucket that are ranked by counting
-constexpr uint32_t kRanges = 8;
 constexpr uint32_t kMostTokens = 1u << 20;
-constexpr uint32_t kMostRows = kMostTokens / kRow + 1;   // vectors of a thread
-constexpr uint32_t kPerRange = (kMostRows + kRanges - 1) / kRanges;
+constexpr uint32_t kRange = 4 * kBlock;      // tokens of a range of a draw: four a thread
+constexpr uint32_t kRanges = kMostTokens / kRange + kWaves;   // of all waves, the last of each wave's a part
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
@@ -102,12 +101,11 @@ __device__ inline float row_max(float v)
 }
 
 struct SampleLds {
-    uint32_t count[4 * kBlock];      // of 4096 bins of keys, or of kBins
+    uint32_t count[kBins];
     uint64_t mass[kBins];
     uint64_t listed[kListed];        // key, then ~token, so that falling numbers are the order
     uint64_t other[kListed];         // of a sort, and the listed tokens' weights
-    uint64_t range[kRanges * kWaves];
-    uint64_t row[kPerRange * kWaves];
+    uint64_t range[kRanges];
     uint64_t wave[kWaves];
     uint64_t found;
     uint64_t before;
@@ -187,7 +185,7 @@ struct Weights {
     // bits.  0 for -inf and NaN.
     __device__ uint64_t of(float x) const
     {
-        double const t = (static_cast<double>(x) - highest) * rate;
+        double const t = fmax((static_cast<double>(x) - highest) * rate, -64.0);   // of NaN too
         double const z = t + 6755399441055744.0;
         double const f = t - (z - 6755399441055744.0);
         double s = 7.070968007227213e-09;
@@ -203,34 +201,36 @@ struct Weights {
         s = fma(s, f, 1.0);
         int64_t const n = static_cast<int32_t>(__double_as_longlong(z)) + static_cast<int32_t>(scale);
         double const w = __longlong_as_double(__double_as_longlong(s) + (n << 52)) + 4503599627370496.0;
-        return t > -64.0 ? static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull : 0;
+        return static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
     }
 };
 
-// The row as the block reads it: vector j of thread t is tokens
-// 4 (j kBlock + t) - shift + 0 .. 3, at a 16-byte address.
+// The row as the block reads it: each wave a run of whole vectors, of which
+// vector j of lane l is tokens first + kVector j + 4 l + 0 .. 3, at any address of
+// 4 bytes.  So the vocabulary's order is the waves', the vectors' and the lanes'.
 struct Row {
     const float* from;
     uint32_t V;
-    uint32_t shift;
-    uint32_t vectors;
+    uint32_t run;        // vectors of a wave
     bool infinite;       // the highest logit is +inf
 
-    __device__ uint32_t token(uint32_t j) const { return 4 * (j * kBlock + threadIdx.x) - shift; }
-
-    // -inf past the row.  With logits of +inf, these alone are there, all alike.
-    __device__ f32x4_t load(uint32_t j) const
+    __device__ uint32_t first() const { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave))) * run * kVector; }
+    __device__ uint32_t token(uint32_t j) const { return first() + j * kVector + 4 * (threadIdx.x & (kWave - 1)); }
+    __device__ uint32_t vectors() const
     {
-        uint32_t const v = token(j);
+        uint32_t const at = first();
+        return at < V ? min(run, (V - at + kVector - 1) / kVector) : 0;
+    }
+
+    // Four tokens, -inf past the row.
+    __device__ f32x4_t load(uint32_t v) const
+    {
         f32x4_t x;
-        if (v < V && V - v > 3) {
-            x = *reinterpret_cast<const f32x4_t*>(from + v);
-        } else {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) x[i] = v + i < V ? from[v + i] : -INFINITY;
-        }
+        for (uint32_t i = 0; i < 4; ++i) x[i] = v + i < V ? from[v + i] : -INFINITY;
         return x;
     }
+    // With logits of +inf, these alone are there, all alike.
     __device__ f32x4_t as_counted(f32x4_t x) const
     {
         if (infinite) {
@@ -240,45 +240,74 @@ struct Row {
         return x;
     }
 
-    // f(j, vector) for every vector, in order, the next ones on their way.  One
-    // vector an iteration: code that a row's block runs through once comes from
+    // f(j, vector) for every vector of the wave, in order, the next ones on their
+    // way: loads that the hardware bounds to the row, without a branch, behind
+    // which the compiler would wait for all of them, each to its own registers,
+    // as a copy would wait too; the last vector comes from a load of its own.  A
+    // loop of kAhead vectors: code that a row's block runs through once comes from
     // memory at its own pace, and eight vectors held in registers and passed over
-    // in unrolled code took 43 us for 4 rows of 32000 drawn whole, a loop 26.
+    // in unrolled code took 43 us for 4 rows of 32000 drawn whole.
     template <typename F>
     __device__ __attribute__((always_inline)) void vectors_do(F f) const
     {
+        uint32_t const n = vectors();
+        if (n == 0) return;
+        auto const bounded = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), 0, static_cast<int>(4 * V), 0x00027000);
+        uint32_t const at = 4 * token(0);
+        auto const ahead_of = [&](uint32_t j) {
+            return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(bounded, static_cast<int>(at + j * kVector * 4), 0, 0));
+        };
+        f32x4_t const last = load(token(n - 1));
         f32x4_t ahead[kAhead];
 #pragma unroll
-        for (uint32_t k = 0; k < kAhead; ++k) ahead[k] = load(k);
+        for (uint32_t k = 0; k < kAhead; ++k) ahead[k] = ahead_of(k);
 #pragma nounroll
-        for (uint32_t j = 0; j < vectors; ++j) {
-            f32x4_t const now = as_counted(ahead[0]);
+        for (uint32_t j = 0; j < n; j += kAhead) {
 #pragma unroll
-            for (uint32_t k = 1; k < kAhead; ++k) ahead[k - 1] = ahead[k];
-            ahead[kAhead - 1] = load(j + kAhead);
-            f(j, now);
-        }
-    }
-
-    // f(token, logit) for every token of this thread with a logit in [low, high];
-    // vectors without one in any lane cost four comparisons.
-    template <typename F>
-    __device__ __attribute__((always_inline)) void each_within(float low, float high, F f) const
-    {
-        vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
-            bool in[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) in[i] = y[i] >= low && y[i] <= high;
-            if (!(in[0] || in[1] || in[2] || in[3])) return;
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                if (in[i]) f(token(j) + i, y[i]);
+            for (uint32_t k = 0; k < kAhead; ++k) {
+                f32x4_t now = ahead[k];
+                if (j + k + 1 >= n) now = last;
+                now = as_counted(now);
+                ahead[k] = ahead_of(j + k + kAhead);
+                if (j + k < n) f(j + k, now);
             }
-        });
+        }
     }
 };
 
 __device__ inline float highest_of(f32x4_t const& y) { return fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])); }
+
+// Lists the tokens whose logits are in [low, high] and pass, as far as the list
+// goes; returns how many there are.  One atomic operation a wave and vector: a
+// token's is one of 64 at one address.
+template <typename F>
+__device__ __attribute__((always_inline)) inline uint32_t list_tokens(const Row& row, SampleLds& lds, float low, float high, F passes)
+{
+    __syncthreads();
+    if (threadIdx.x == 0) lds.word[0] = 0;
+    __syncthreads();
+    row.vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
+        bool any = false;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) any = any || (y[i] >= low && y[i] <= high);
+        if (__ballot(any) == 0) return;
+        uint64_t in[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) in[i] = __ballot(y[i] >= low && y[i] <= high && passes(y[i]));
+        uint32_t at = 0;
+        if ((threadIdx.x & (kWave - 1)) == 0) at = atomicAdd(&lds.word[0], static_cast<uint32_t>(__popcll(in[0]) + __popcll(in[1]) + __popcll(in[2]) + __popcll(in[3])));
+        at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            uint32_t const place = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in[i] >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in[i]), at));
+            bool const mine = (in[i] >> (threadIdx.x & (kWave - 1)) & 1u) != 0;
+            if (mine && place < kListed) lds.listed[place] = static_cast<uint64_t>(key_of(y[i])) << 32 | (0xFFFFFFFFu - (row.token(j) + i));
+            at += static_cast<uint32_t>(__popcll(in[i]));
+        }
+    });
+    __syncthreads();
+    return lds.word[0];
+}
 
 // The last kept token: its logit and its number.  Kept are the higher logits,
 // and of its own the tokens up to it.
@@ -296,11 +325,31 @@ struct Kept {
     Last last;
     uint64_t least;   // weights below it are not kept
     float floor;      // no logit below it is kept or weighs anything
+    float sure;       // every logit above it is kept
 
     __device__ __attribute__((always_inline)) uint64_t of(float x, uint32_t token) const
     {
         uint64_t const w = weights.of(x);
         return last.keeps(x, token) && w >= least ? w : 0;
+    }
+    __device__ __attribute__((always_inline)) uint64_t of(f32x4_t const& y, uint32_t token) const
+    {
+        uint64_t sum = 0;
+        bool border = false;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) border = border || (y[i] >= floor && y[i] <= sure);
+        if (__ballot(border) != 0) {
+#pragma nounroll
+            for (uint32_t i = 0; i < 4; ++i) sum += of(i < 2 ? (i == 0 ? y[0] : y[1]) : (i == 2 ? y[2] : y[3]), token + i);
+        } else {
+            // All four at once: a weight is a chain of dependent operations.
+            uint64_t w[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) w[i] = weights.of(y[i]);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) sum += y[i] > sure ? w[i] : 0;
+        }
+        return sum;
     }
 };
 
@@ -308,33 +357,47 @@ struct Kept {
 struct Same {
     float floor;
     __device__ uint64_t of(float x, uint32_t) const { return x == floor ? 1 : 0; }
+    __device__ uint64_t of(f32x4_t const& y, uint32_t) const { return of(y[0], 0) + of(y[1], 0) + of(y[2], 0) + of(y[3], 0); }
 };
 
-// The sums of the tokens' weights by ranges of `per` vectors, and all of them.
-template <typename W>
-__device__ __attribute__((always_inline)) inline uint64_t sum_ranges(const Row& row, SampleLds& lds, uint32_t per, const W& weight)
+// The kept tokens down to the last one of a cut, of those that weigh `least` or more.
+__device__ inline Kept kept_tokens(const Weights& weights, const Last& last, float temperature, float min_p)
 {
-    uint32_t const wave = threadIdx.x / kWave;
+    float const high = static_cast<float>(weights.highest);
+    Kept k{weights, last, part_of(min_p, uint64_t{1} << weights.scale, true), fmaxf(last.logit, high - kWeightless * temperature), last.logit};
+    if (min_p > 0.0f) {
+        // Min-p's logit, by more than what 32 bits lose on the way to it.
+        float const under = temperature * logf(min_p);
+        float const slack = (fabsf(high) - under) * 0x1p-18f;
+        k.floor = fmaxf(k.floor, high + under - slack);
+        k.sure = fmaxf(k.sure, high + under + slack);
+    }
+    return k;
+}
+
+// Ranges of a wave's run.
+__device__ inline uint32_t ranges_of(const Row& row) { return (row.run * kVector + kRange - 1) / kRange; }
+
+// The sums of the tokens' weights by ranges, and all of them.
+template <typename W>
+__device__ __attribute__((always_inline)) inline uint64_t sum_ranges(const Row& row, SampleLds& lds, const W& weight)
+{
     uint32_t const lane = threadIdx.x & (kWave - 1);
+    uint32_t const ranges = ranges_of(row);
+    uint32_t const mine = threadIdx.x / kWave * ranges;
     __syncthreads();
-    if (threadIdx.x < kRanges * kWaves) lds.range[threadIdx.x] = 0;
+    // Runs that end before the row's last range leave some of theirs empty.
+    for (uint32_t i = threadIdx.x; i < kRanges; i += kBlock) lds.range[i] = 0;
     __syncthreads();
     uint64_t all = 0, sum = 0;
-    uint32_t at = 0, left = per;
+    uint32_t const n = row.vectors();
     row.vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
-        if (highest_of(y) >= weight.floor) {
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) sum += weight.of(y[i], row.token(j) + i);
-        }
-        if (--left == 0 || j + 1 == row.vectors) {
-            if (__ballot(sum != 0) != 0) {
-                uint64_t const total = wave_total(sum);
-                if (lane == 0) lds.range[at * kWaves + wave] = total;
-                all += total;
-            }
+        if (highest_of(y) >= weight.floor) sum += weight.of(y, row.token(j));
+        if (j % (kRange / kVector) == kRange / kVector - 1 || j + 1 == n) {
+            uint64_t const total = wave_total(sum);
+            if (lane == 0) lds.range[mine + j / (kRange / kVector)] = total;
+            all += total;
             sum = 0;
-            ++at;
-            left = per;
         }
     });
     return block_total(lane == 0 ? all : 0, lds);
@@ -343,63 +406,39 @@ __device__ __attribute__((always_inline)) inline uint64_t sum_ranges(const Row& 
 // The first token at which the running sum exceeds `target`, less than all of
 // it; the ranges' sums are in place.  Its weight in *its.
 template <typename W>
-__device__ uint32_t token_at(const Row& row, SampleLds& lds, uint32_t per, uint64_t target, const W& weight, uint64_t* its)
+__device__ uint32_t token_at(const Row& row, SampleLds& lds, uint64_t target, const W& weight, uint64_t* its)
 {
-    uint32_t const wave = threadIdx.x / kWave;
-    uint32_t const lane = threadIdx.x & (kWave - 1);
-    static_assert(kRanges * kWaves == 2 * kWave, "two a lane, eight lanes a range");
-    if (wave == 0) {
-        uint64_t const sum = lds.range[2 * lane] + lds.range[2 * lane + 1];
-        uint64_t const upto = wave_scan(sum);
-        // The lane in which the target lies; its range's first lane knows what lies before.
-        uint64_t const hit = __ballot(target >= upto - sum && target - (upto - sum) < sum);
-        uint32_t const at = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(hit)) - 1) & ~7u;
-        if (lane == at) {
-            lds.word[0] = at / 8;
-            lds.before = upto - sum;
-        }
+    static_assert(kRanges <= kBlock, "a thread a range");
+    uint32_t const tid = threadIdx.x;
+    uint32_t const ranges = ranges_of(row);
+    uint64_t all;
+    uint64_t sum = tid < ranges * kWaves ? lds.range[tid] : 0;
+    uint64_t before = block_scan(sum, lds, &all);
+    if (target >= before && target - before < sum) {   // one thread
+        lds.word[0] = tid / ranges * row.run * kVector + tid % ranges * kRange;
+        lds.word[1] = min((tid / ranges + 1) * row.run * kVector, lds.word[0] + kRange);
+        lds.before = before;
     }
     __syncthreads();
-    uint32_t const j0 = lds.word[0] * per;
-    uint32_t const j1 = min(j0 + per, row.vectors);
-    uint64_t at = lds.before;
-    uint64_t w4[4] = {};
-#pragma nounroll
-    for (uint32_t j = j0; j < j1; ++j) {
-        f32x4_t const y = row.as_counted(row.load(j));
-        uint64_t sum = 0;
+    // Four tokens a thread, those of the range.
+    uint32_t const v = lds.word[0] + 4 * tid;
+    uint32_t const end = lds.word[1];
+    f32x4_t y = row.as_counted(row.load(v));
+    uint64_t w4[4];
+    sum = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            w4[i] = weight.of(y[i], row.token(j) + i);
-            sum += w4[i];
-        }
-        uint64_t const total = wave_total(sum);
-        if (lane == 0) lds.row[(j - j0) * kWaves + wave] = total;
+    for (uint32_t i = 0; i < 4; ++i) {
+        w4[i] = v + i < end ? weight.of(y[i], v + i) : 0;
+        sum += w4[i];
     }
-    __syncthreads();
-#pragma nounroll
-    for (uint32_t j = j0; j < j1; ++j) {
-        uint64_t const part = lds.row[(j - j0) * kWaves + (lane & (kWaves - 1))];
-        uint64_t const upto = row_scan(part);
-        uint64_t const mine = lane_u64(part, __builtin_amdgcn_readfirstlane(static_cast<int>(wave)));
-        uint64_t before = at + lane_u64(upto, __builtin_amdgcn_readfirstlane(static_cast<int>(wave))) - mine;
-        at += lane_u64(upto, kWaves - 1);
-        if (target < before || target - before >= mine) continue;
-        // In this vector of this wave.
-        if (j + 1 != j1) {
-            f32x4_t const y = row.as_counted(row.load(j));
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) w4[i] = weight.of(y[i], row.token(j) + i);
-        }
-        uint64_t const sum = w4[0] + w4[1] + w4[2] + w4[3];
-        before += wave_scan(sum) - sum;
-        if (target < before || target - before >= sum) continue;
+    before = lds.before + block_scan(sum, lds, &all);
+    if (target >= before && target - before < sum) {   // one thread
         bool found = false;
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
             if (!found && target - before < w4[i]) {
                 found = true;
-                lds.word[1] = row.token(j) + i;
+                lds.word[2] = v + i;
                 lds.found = w4[i];
             }
             if (!found) before += w4[i];
@@ -407,7 +446,7 @@ __device__ uint32_t token_at(const Row& row, SampleLds& lds, uint32_t per, uint6
     }
     __syncthreads();
     *its = lds.found;
-    return lds.word[1];
+    return lds.word[2];
 }
 
 // ---- sorting ---------------------------------------------------------------------
@@ -433,9 +472,9 @@ __device__ __attribute__((noinline)) void sort_falling(uint64_t* numbers, Sample
         return;
     }
     // Buckets of the upper words, a thread each; then each number to its place in its bucket.
-    static_assert(kBins == kBlock && kListed == 2 * kBlock, "a bucket and two numbers a thread");
+    static_assert(kListed == 2 * kBlock, "two numbers a thread");
     uint32_t shift = 0;
-    while (((high - low) >> shift) >= kBins) ++shift;
+    while (((high - low) >> shift) >= kBlock) ++shift;
     lds.count[tid] = 0;
     __syncthreads();
     uint64_t x[2];
@@ -452,17 +491,17 @@ __device__ __attribute__((noinline)) void sort_falling(uint64_t* numbers, Sample
     uint32_t const size = lds.count[tid];
     uint64_t all;
     uint64_t const start = block_scan(size, lds, &all);
-    lds.count[kBins + tid] = static_cast<uint32_t>(start);
+    lds.count[kBlock + tid] = static_cast<uint32_t>(start);
     if (__syncthreads_or(size > kBucket) == 0) {
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
-            if (tid + i * kBlock < n) lds.other[lds.count[kBins + bucket[i]] + place[i]] = x[i];
+            if (tid + i * kBlock < n) lds.other[lds.count[kBlock + bucket[i]] + place[i]] = x[i];
         }
         __syncthreads();
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
             if (tid + i * kBlock >= n) continue;
-            uint32_t const first = lds.count[kBins + bucket[i]];
+            uint32_t const first = lds.count[kBlock + bucket[i]];
             uint32_t const last = first + lds.count[bucket[i]];
             uint32_t higher = 0;
             for (uint32_t k = first; k < last; ++k) higher += lds.other[k] > x[i] ? 1u : 0u;
@@ -510,108 +549,137 @@ struct Bins {
     __device__ uint32_t of(float x) const { return static_cast<uint32_t>(fminf((half - 0.5f * x) * rate, static_cast<float>(kBins - 1))); }
 };
 
-// The bin of the counted ones that the cut falls into, how many tokens it
-// holds, and what lies before it of what the cut counts.
+// The bin that the cut falls into, and what lies before it of what the cut counts.
 struct Place {
     uint32_t bin;     // kBins: the cut lies past all that is counted
-    uint32_t count;
     uint64_t before;
 };
 
 __device__ inline Place place_of(SampleLds& lds, const Cut& cut, uint64_t before)
 {
-    static_assert(kBins == kBlock, "a thread a bin");
+    static_assert(kBins == 4 * kBlock, "four bins a thread");
     uint32_t const tid = threadIdx.x;
-    uint64_t all;
-    uint64_t const mine = cut.by_mass ? lds.mass[tid] : lds.count[tid];
-    uint64_t const at = before + block_scan(mine, lds, &all);
+    uint64_t of[4];
+    uint64_t sum = 0, all;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        of[i] = cut.by_mass ? lds.mass[4 * tid + i] : lds.count[4 * tid + i];
+        sum += of[i];
+    }
+    uint64_t at = before + block_scan(sum, lds, &all);
     if (tid == 0) lds.word[0] = kBins;
     __syncthreads();
-    if (at < cut.amount && cut.amount - at <= mine) {   // one thread at most
-        lds.word[0] = tid;
-        lds.word[1] = lds.count[tid];
-        lds.before = at;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        if (at < cut.amount && cut.amount - at <= of[i]) {   // one bin at most
+            lds.word[0] = 4 * tid + i;
+            lds.before = at;
+        }
+        at += of[i];
     }
     __syncthreads();
-    Place const p{lds.word[0], lds.word[1], lds.before};
+    Place const p{lds.word[0], lds.before};
     __syncthreads();
     return p;
 }
 
+__device__ inline void clear_bins(SampleLds& lds)
+{
+#pragma unroll
+    for (uint32_t i = 0; i < kBins / kBlock; ++i) {
+        lds.count[i * kBlock + threadIdx.x] = 0;
+        lds.mass[i * kBlock + threadIdx.x] = 0;
+    }
+}
+
 // Where the cut falls; everything is kept where it lies past what is counted.
-// The bins' counts and weights are in lds.
-__device__ __attribute__((noinline)) Last find_cut(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, const Cut& cut,
-                                                   uint32_t per)
+// The bins' counts (or weights, for a cut by them) are in lds.
+__device__ __attribute__((noinline)) Last find_cut(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, const Cut& cut)
 {
     uint32_t const tid = threadIdx.x;
     Place place = place_of(lds, cut, 0);
     if (place.bin == kBins) return Last{-INFINITY, 0xFFFFFFFFu};
     uint32_t const bin = place.bin;
-    // The bin's tokens, and their highest and lowest keys, of the logits that
-    // may be in it: its bounds with a part in 2^18 of the largest on the way.
+    // The bin's tokens; the keys that they can have, from the bin's bounds and a
+    // part in 2^17 of the largest number on the way.
     auto const border = [&](uint32_t b) { return 2.0f * (bins.half - static_cast<float>(b) / bins.rate); };
     float const slack = (fabsf(bins.half) + static_cast<float>(bin + 1) / bins.rate) * 0x1p-17f;
     float const low_x = border(bin + 1) - slack;
     float const high_x = border(bin) + slack;
-    if (tid < 3) lds.word[tid] = tid == 2 ? 0xFFFFFFFFu : 0;
-    __syncthreads();
-    row.each_within(low_x == low_x ? low_x : -INFINITY, high_x == high_x ? high_x : INFINITY, [&](uint32_t token, float x) __attribute__((always_inline)) {
-        if (bins.of(x) != bin) return;
+    uint32_t low = low_x > -3.4028234664e38f ? key_of(low_x) : 0x00800000u;
+    uint32_t high = high_x < 2.0f * bins.half ? key_of(high_x) : key_of(2.0f * bins.half);
+    uint32_t listed = list_tokens(row, lds, low_x == low_x ? low_x : -INFINITY, high_x == high_x ? high_x : INFINITY, [&](float x) { return bins.of(x) == bin; });
+    if (listed > kListed) {
+        // Too many: their highest and lowest keys, and bins of these.
+        if (tid == 0) {
+            lds.word[1] = 0;
+            lds.word[2] = 0xFFFFFFFFu;
+        }
+        __syncthreads();
+        uint32_t most = 0, least = 0xFFFFFFFFu;
+        row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                if (bins.of(y[i]) != bin) continue;
+                most = max(most, key_of(y[i]));
+                least = min(least, key_of(y[i]));
+            }
+        });
+        atomicMax(&lds.word[1], most);
+        atomicMin(&lds.word[2], least);
+        __syncthreads();
+        high = lds.word[1];
+        low = lds.word[2];
+    }
+    // A token of the keys low .. high: that of -0 is no logit's, but compares as 0.
+    auto const within = [&](float x) {
         uint32_t const key = key_of(x);
-        if (place.count <= kListed) lds.listed[atomicAdd(&lds.word[0], 1u)] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - token);
-        atomicMax(&lds.word[1], key);
-        atomicMin(&lds.word[2], key);
-    });
-    __syncthreads();
-    uint32_t high = lds.word[1];
-    uint32_t low = lds.word[2];
-    while (place.count > kListed && high != low) {
-        // The keys low .. high, cut into bins of 2^shift keys.
+        return key >= low && key <= high;
+    };
+    while (listed > kListed && high != low) {
+        // The keys, cut into bins of 2^shift of them.
         uint32_t shift = 0;
         while (((high - low) >> shift) >= kBins) ++shift;
         __syncthreads();
-        lds.count[tid] = 0;
-        lds.mass[tid] = 0;
+        clear_bins(lds);
         __syncthreads();
-        // The keys' own bounds count: that of -0 is no logit's, but compares as 0.
-        row.each_within(logit_of(low), logit_of(high), [&](uint32_t, float x) __attribute__((always_inline)) {
-            uint32_t const key = key_of(x);
-            if (key < low || key > high) return;
-            uint32_t const b = (high - key) >> shift;
-            atomicAdd(&lds.count[b], 1u);
-            if (cut.by_mass) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.mass[b]), static_cast<unsigned long long>(weights.of(x)));
+        row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
+#pragma nounroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                float const x = i < 2 ? (i == 0 ? y[0] : y[1]) : (i == 2 ? y[2] : y[3]);
+                if (x != x || !within(x)) continue;
+                uint32_t const b = (high - key_of(x)) >> shift;
+                if (cut.by_mass) {
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&lds.mass[b]), static_cast<unsigned long long>(weights.of(x)));
+                } else {
+                    atomicAdd(&lds.count[b], 1u);
+                }
+            }
         });
         __syncthreads();
         place = place_of(lds, cut, place.before);
         high -= place.bin << shift;
         uint32_t const keys = 1u << shift;
         low = high - low >= keys ? high - keys + 1 : low;
-        if (place.count > kListed) continue;
-        if (tid == 0) lds.word[0] = 0;
-        __syncthreads();
-        row.each_within(logit_of(low), logit_of(high), [&](uint32_t token, float x) __attribute__((always_inline)) {
-            uint32_t const key = key_of(x);
-            if (key >= low && key <= high) lds.listed[atomicAdd(&lds.word[0], 1u)] = static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - token);
-        });
-        __syncthreads();
+        listed = list_tokens(row, lds, logit_of(low), logit_of(high), within);
     }
     uint64_t const left = cut.amount - place.before;   // at least 1
-    if (place.count > kListed) {
+    if (listed > kListed) {
         // One key: so many of its tokens, the lowest first.
         uint64_t const weight = cut.by_mass ? weights.of(logit_of(high)) : 1;
         Same const same{logit_of(high)};
-        static_cast<void>(sum_ranges(row, lds, per, same));
+        static_cast<void>(sum_ranges(row, lds, same));
         uint64_t one;
-        uint32_t const token = token_at(row, lds, per, (left - 1) / weight, same, &one);
+        uint32_t const token = token_at(row, lds, (left - 1) / weight, same, &one);
         return Last{logit_of(high), token};
     }
-    sort_falling(lds.listed, lds, place.count, low, high);
+    sort_falling(lds.listed, lds, listed, low, high);
     // Two neighbours of the order a thread.
     uint64_t w[2] = {};
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
         uint32_t const n = 2 * tid + i;
-        if (n < place.count) w[i] = cut.by_mass ? weights.of(logit_of(static_cast<uint32_t>(lds.listed[n] >> 32))) : 1;
+        if (n < listed) w[i] = cut.by_mass ? weights.of(logit_of(static_cast<uint32_t>(lds.listed[n] >> 32))) : 1;
     }
     uint64_t total;
     uint64_t at = block_scan(w[0] + w[1], lds, &total);
@@ -711,8 +779,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     Row row;
     row.from = a.logits + static_cast<uint64_t>(blockIdx.x) * a.V;
     row.V = a.V;
-    row.shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row.from) >> 2) & 3u;
-    row.vectors = (a.V + row.shift + kRow - 1) / kRow;
+    row.run = (a.V + kWaves * kVector - 1) / (kWaves * kVector);
     row.infinite = false;
     kimkv_sample_rule const rule = a.rules[blockIdx.x];
     float const uniform = a.uniforms[blockIdx.x];
@@ -726,12 +793,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
         answer(KIMKV_NO_TOKEN, 0.0f);
         return;
     }
-    auto const clear = [&] {
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) lds.count[i * kBlock + tid] = 0;
-        lds.mass[tid] = 0;
-    };
-    clear();
+    clear_bins(lds);
 
     // ---- the highest logit, by place in a vector (NaN is left out) ----
     f32x4_t high4 = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -761,93 +823,81 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     Weights const weights{high, 1.4426950408889634 / static_cast<double>(temperature), a.scale};
 
     if (cut_k && top_k <= kShortList) {
-        // Bins of the maxima's keys, from the highest down; four of them a thread.
+        // Bins of the maxima's keys, from the highest down: 12 bits of 32.
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            if (high4[i] != -INFINITY) atomicAdd(&lds.count[4095u - (key_of(high4[i]) >> 20)], 1u);
-        }
-        if (tid == 0) {
-            lds.word[0] = 0;       // listed tokens
-            lds.word[1] = 4095;    // the bound's bin: all, where there are fewer maxima
+            if (high4[i] != -INFINITY) atomicAdd(&lds.count[kBins - 1 - (key_of(high4[i]) >> 20)], 1u);
         }
         __syncthreads();
-        uint32_t of[4];
-        uint64_t sum = 0, all;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            of[i] = lds.count[4 * tid + i];
-            sum += of[i];
-        }
-        uint64_t at = block_scan(sum, lds, &all);
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            if (at < top_k && at + of[i] >= top_k) lds.word[1] = 4 * tid + i;   // one thread at most
-            at += of[i];
-        }
-        __syncthreads();
-        uint32_t const bound = max((4095u - lds.word[1]) << 20, 0x00800000u);   // at least the lowest number's key
-        row.each_within(logit_of(bound), INFINITY, [&](uint32_t token, float x) __attribute__((always_inline)) {
-            uint32_t const at_list = atomicAdd(&lds.word[0], 1u);
-            if (at_list < kListed) lds.listed[at_list] = static_cast<uint64_t>(key_of(x)) << 32 | (0xFFFFFFFFu - token);
-        });
-        __syncthreads();
-        uint32_t const listed = lds.word[0];
+        // The bound's bin, or all where there are fewer maxima.
+        uint32_t const bin = min(place_of(lds, Cut{false, top_k}, 0).bin, kBins - 1);
+        uint32_t const bound = max((kBins - 1 - bin) << 20, 0x00800000u);   // at least the lowest number's key
+        float const bound_x = logit_of(bound);
+        uint32_t const listed = list_tokens(row, lds, bound_x, INFINITY, [](float) { return true; });
         if (listed <= kListed) {
             Drawn const d = draw_listed(lds, weights, rule, listed, top_k, bound, key_of(high), uniform, a.V);
             answer(d.token, static_cast<float>(static_cast<double>(d.weight) / static_cast<double>(d.total)));
             return;
         }
         __syncthreads();
-        clear();
+        clear_bins(lds);
         __syncthreads();
     }
 
-    // Ranges of `per` vectors.
-    uint32_t const per = (row.vectors + kRanges - 1) / kRanges;
-    float const weightless = high - kWeightless * temperature;   // no logit below weighs anything; -inf past the largest number
     Last last{-INFINITY, 0xFFFFFFFFu};
     if (cut_k || cut_p) {
         Bins const bins{0.5f * high, fminf(2 * (kBins - 1) / (kWeightless * temperature), 3e38f)};
         row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
             if (bins.of(highest_of(y)) >= kBins - 1) return;
+            uint32_t b[4];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                uint32_t const b = bins.of(y[i]);
-                if (b >= kBins - 1) continue;
-                atomicAdd(&lds.count[b], 1u);
-                if (cut_p) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.mass[b]), static_cast<unsigned long long>(weights.of(y[i])));
+            for (uint32_t i = 0; i < 4; ++i) b[i] = bins.of(y[i]);
+            if (cut_k) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    if (b[i] < kBins - 1) atomicAdd(&lds.count[b[i]], 1u);
+                }
+            }
+            if (cut_p) {
+                uint64_t w[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) w[i] = weights.of(y[i]);
+                // Here, and not each behind its condition.
+                asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    if (b[i] < kBins - 1) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.mass[b[i]]), static_cast<unsigned long long>(w[i]));
+                }
             }
         });
         __syncthreads();
-        uint32_t const count = lds.count[tid];
-        uint64_t const mass = lds.mass[tid];
+        uint64_t mass[kBins / kBlock];
         uint64_t total = 0;
-        if (cut_p) total = block_total(mass, lds);
+#pragma unroll
+        for (uint32_t i = 0; i < kBins / kBlock; ++i) {
+            mass[i] = lds.mass[i * kBlock + tid];
+            total += mass[i];
+        }
+        if (cut_p) total = block_total(total, lds);
         if (cut_k) {
-            last = find_cut(row, lds, weights, bins, Cut{false, top_k}, per);
-            if (cut_p && last.logit != -INFINITY) total = sum_ranges(row, lds, per, Kept{weights, last, 0, fmaxf(last.logit, weightless)});
+            last = find_cut(row, lds, weights, bins, Cut{false, top_k});
+            if (cut_p && last.logit != -INFINITY) total = sum_ranges(row, lds, kept_tokens(weights, last, temperature, 0.0f));
         }
         if (cut_p) {
             __syncthreads();
-            lds.count[tid] = count;
-            lds.mass[tid] = mass;
+#pragma unroll
+            for (uint32_t i = 0; i < kBins / kBlock; ++i) lds.mass[i * kBlock + tid] = mass[i];
             __syncthreads();
-            Last const mine = find_cut(row, lds, weights, bins, Cut{true, part_of(rule.top_p, total, true)}, per);
+            Last const mine = find_cut(row, lds, weights, bins, Cut{true, part_of(rule.top_p, total, true)});
             if (mine.logit > last.logit || (mine.logit == last.logit && mine.token < last.token)) last = mine;
         }
     }
 
     // ---- the draw ----
-    float floor = fmaxf(last.logit, weightless);
-    if (rule.min_p > 0.0f) {
-        // Below min-p's logit by more than what 32 bits lose on the way to it.
-        float const under = temperature * logf(rule.min_p);
-        floor = fmaxf(floor, high + under - (fabsf(high) - under) * 0x1p-18f);
-    }
-    Kept const kept{weights, last, part_of(rule.min_p, uint64_t{1} << a.scale, true), floor};
-    uint64_t const total = sum_ranges(row, lds, per, kept);
+    Kept const kept = kept_tokens(weights, last, temperature, rule.min_p);
+    uint64_t const total = sum_ranges(row, lds, kept);
     uint64_t its;
-    uint32_t const token = token_at(row, lds, per, part_of(uniform, total, false), kept, &its);
+    uint32_t const token = token_at(row, lds, part_of(uniform, total, false), kept, &its);
     answer(token, static_cast<float>(static_cast<double>(its) / static_cast<double>(total)));
 }
 
