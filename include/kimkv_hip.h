@@ -955,7 +955,7 @@ typedef struct kimkv_sample_rule {
 size_t kimkv_sample_workspace_bytes(uint32_t rows, uint32_t vocabulary);
 
 /* The token that row r of logits[rows][vocabulary] (fp32; as
- * kimkv_model_logits_adjust leaves them) gives by device_rules[r] and the
+ * kimkv_model_logits_adjust leaves them; at most 2^20 tokens) gives by device_rules[r] and the
  * random number device_uniforms[r] in [0, 1): the first token, in the order of
  * the vocabulary, at which the kept tokens' weight up to it exceeds that part
  * of all kept tokens' weight; with probabilities (NULL: not wanted) its weight

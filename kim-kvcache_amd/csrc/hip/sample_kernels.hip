@@ -10,16 +10,28 @@
 // The kept tokens are a run of the order "falling logit, lower token first
 // among equals".  Block = row, which passes over the row's logits, from the
 // caches after the first time:
-//   - The highest logit, and the maxima of 4096 parts of the row.
-//   - Short list (top_k of at most 1024): the top_k-th highest of the maxima is
-//     reached by at least top_k tokens, and by not many more: those are collected
-//     in LDS and sorted, and the cuts and the draw go on there.
+//   - The highest logit.  Where a list may do, for each of 4096 parts of the row
+//     (columns) the highest, its place and the second.
+//   - List (top_k of at most 1024; min-p alone): a bound that top_k columns reach,
+//     or min-p's logit.  The tokens from it up are known from the columns, but for
+//     those in which two reach it, so the row is not read again.  They are sorted
+//     in LDS, and the cuts and the draw go on there.
 //   - Else, where top-k or top-p cut: counts and weights of 4096 bins of the
 //     logits, the bin that the cut falls into, its tokens sorted in LDS (bins of
 //     more tokens than LDS takes are cut into 4096 again, by their keys), which
 //     gives the last kept token.
 //   - The draw from a row: the kept tokens' weights summed by ranges of the
 //     vocabulary, the range that the random number falls into, the token in it.
+//
+// Bound by the instructions of one block's waves: a weight is 26 of them, and a
+// pass of weights over 32000 tokens 7 us, where reading the row takes 1 us.  So a
+// list saves passes: 72 rows of 50255 with top_k 50 take 17 us (20 us where the
+// list came from a second pass over the row), 256 rows of 128000 36 us (58), which
+// is 3.6 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
+// and these took 17 and 42 us.  Drawn from all the row 28 and 77 us, top-p of 0.9
+// 62 and 160.  Tried and slower: a list for top-p, from the highest columns up
+// (256 flat rows of 128000 184 us, as it falls back there); the sums by ranges in
+// the pass that lists a bin's tokens (128 us for top_k 3000, as it was without).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -33,17 +45,23 @@
 namespace kimkv {
 namespace {
 
-constexpr unsigned kBlock = 1024;
+constexpr unsigned kBlock = 512;
 constexpr uint32_t kWaves = kBlock / kWave;
 constexpr uint32_t kVector = 4 * kWave;      // tokens of one load of a wave
 constexpr uint32_t kAhead = 4;               // vectors of a thread in flight
-constexpr uint32_t kBins = 4096;             // four a thread
+constexpr uint32_t kBins = 4096;
+constexpr uint32_t kBinsEach = kBins / kBlock;
 constexpr uint32_t kListed = 2048;           // tokens that are sorted in LDS
+constexpr uint32_t kListedEach = kListed / kBlock;
 constexpr uint32_t kShortList = 1024;        // the largest top_k whose tokens are listed at once
+constexpr uint32_t kCrowded = 32;            // columns that a wave reads again one by one (8: 72 rows of 50255, top_k 700, 31 us, not 25)
+constexpr uint32_t kSets = 2;                // of a thread's columns
 constexpr uint32_t kSmall = 128;             // tokens that are ranked by counting
+static_assert(2 * kListed <= kBins, "a sort's counts and starts");
 constexpr uint32_t kBucket = 32;             // tokens of a bucket that are ranked by counting
 constexpr uint32_t kMostTokens = 1u << 20;
-constexpr uint32_t kRange = 4 * kBlock;      // tokens of a range of a draw: four a thread
+constexpr uint32_t kRange = 4096;            // tokens of a range of a draw
+constexpr uint32_t kRangeEach = kRange / kBlock;
 constexpr uint32_t kRanges = kMostTokens / kRange + kWaves;   // of all waves, the last of each wave's a part
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -102,9 +120,11 @@ __device__ inline float row_max(float v)
 
 struct SampleLds {
     uint32_t count[kBins];
-    uint64_t mass[kBins];
+    union {
+        uint64_t mass[kBins];
+        uint64_t other[kListed];     // of a sort, and the listed tokens' weights
+    };
     uint64_t listed[kListed];        // key, then ~token, so that falling numbers are the order
-    uint64_t other[kListed];         // of a sort, and the listed tokens' weights
     uint64_t range[kRanges];
     uint64_t wave[kWaves];
     uint64_t found;
@@ -121,7 +141,7 @@ __device__ inline uint64_t block_scan(uint64_t v, SampleLds& lds, uint64_t* tota
     __syncthreads();
     if ((threadIdx.x & (kWave - 1)) == kWave - 1) lds.wave[wave] = upto;
     __syncthreads();
-    static_assert(kWaves == 16, "a row of lanes holds the waves' sums");
+    static_assert(kWaves <= 16, "a row of lanes holds the waves' sums");
     uint64_t const waves = row_scan(lds.wave[threadIdx.x & (kWaves - 1)]);
     *total = lane_u64(waves, kWaves - 1);
     uint64_t const before = wave == 0 ? 0 : lane_u64(waves, __builtin_amdgcn_readfirstlane(static_cast<int>(wave)) - 1u);
@@ -277,15 +297,49 @@ struct Row {
 
 __device__ inline float highest_of(f32x4_t const& y) { return fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])); }
 
-// Lists the tokens whose logits are in [low, high] and pass, as far as the list
-// goes; returns how many there are.  One atomic operation a wave and vector: a
-// token's is one of 64 at one address.
-template <typename F>
-__device__ __attribute__((always_inline)) inline uint32_t list_tokens(const Row& row, SampleLds& lds, float low, float high, F passes)
+// A token's number of the list: falling numbers are the order.
+__device__ inline uint64_t listing(float x, uint32_t token) { return static_cast<uint64_t>(key_of(x)) << 32 | (0xFFFFFFFFu - token); }
+
+// Lists the lanes' tokens that are in, as far as the list goes.  One atomic
+// operation a wave: a token's is one of 64 at one address.
+__device__ inline void list_lanes(SampleLds& lds, uint64_t in, float x, uint32_t token)
+{
+    uint32_t const lane = threadIdx.x & (kWave - 1);
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(&lds.word[0], static_cast<uint32_t>(__popcll(in)));
+    at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+    uint32_t const place = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in), at));
+    if ((in >> lane & 1u) != 0 && place < kListed) lds.listed[place] = listing(x, token);
+}
+
+// Lists the tokens of a vector that pass, a lane's bit in[i] for its i-th.
+__device__ inline void list_vector(SampleLds& lds, const uint64_t (&in)[4], f32x4_t const& y, uint32_t token)
+{
+    uint32_t const lane = threadIdx.x & (kWave - 1);
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(&lds.word[0], static_cast<uint32_t>(__popcll(in[0]) + __popcll(in[1]) + __popcll(in[2]) + __popcll(in[3])));
+    at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        uint32_t const place = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in[i] >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in[i]), at));
+        if ((in[i] >> lane & 1u) != 0 && place < kListed) lds.listed[place] = listing(y[i], token + i);
+        at += static_cast<uint32_t>(__popcll(in[i]));
+    }
+}
+
+__device__ inline void start_list(SampleLds& lds)
 {
     __syncthreads();
     if (threadIdx.x == 0) lds.word[0] = 0;
     __syncthreads();
+}
+
+// Lists the tokens whose logits are in [low, high] and pass; returns how many
+// there are.
+template <typename F>
+__device__ __attribute__((always_inline)) inline uint32_t list_tokens(const Row& row, SampleLds& lds, float low, float high, F passes)
+{
+    start_list(lds);
     row.vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
         bool any = false;
 #pragma unroll
@@ -294,17 +348,62 @@ __device__ __attribute__((always_inline)) inline uint32_t list_tokens(const Row&
         uint64_t in[4];
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) in[i] = __ballot(y[i] >= low && y[i] <= high && passes(y[i]));
-        uint32_t at = 0;
-        if ((threadIdx.x & (kWave - 1)) == 0) at = atomicAdd(&lds.word[0], static_cast<uint32_t>(__popcll(in[0]) + __popcll(in[1]) + __popcll(in[2]) + __popcll(in[3])));
-        at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+        list_vector(lds, in, y, row.token(j));
+    });
+    __syncthreads();
+    return lds.word[0];
+}
+
+// What a lane's i-th tokens of every kSets-th vector (a column) come to: the
+// highest, in which vector it is, and the second.
+struct Columns {
+    f32x4_t first;
+    f32x4_t second;
+    uint32_t vector[4];
+};
+
+// Lists the tokens from a bound up, and returns how many there are, or more than
+// the list takes.  Each is in a column whose highest has reached the bound: it is
+// that one where the second has not, else the column is read again, its tokens
+// side by side in the wave, or the row where a wave has many such columns.
+__device__ inline uint32_t list_columns(const Row& row, SampleLds& lds, const Columns (&columns)[kSets], float bound)
+{
+    uint32_t const lane = threadIdx.x & (kWave - 1);
+    uint32_t crowded = 0;
+#pragma unroll
+    for (uint32_t set = 0; set < kSets; ++set) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) crowded += static_cast<uint32_t>(__popcll(__ballot(columns[set].second[i] >= bound)));
+    }
+    if (__syncthreads_or(crowded > kListed / kWaves) != 0) return kListed + 1;
+    if (__syncthreads_or(crowded > kCrowded) != 0) return list_tokens(row, lds, bound, INFINITY, [](float) { return true; });
+    start_list(lds);
+    uint32_t const n = row.vectors();
+#pragma unroll
+    for (uint32_t set = 0; set < kSets; ++set) {
+        Columns const& c = columns[set];
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            uint32_t const place = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in[i] >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in[i]), at));
-            bool const mine = (in[i] >> (threadIdx.x & (kWave - 1)) & 1u) != 0;
-            if (mine && place < kListed) lds.listed[place] = static_cast<uint64_t>(key_of(y[i])) << 32 | (0xFFFFFFFFu - (row.token(j) + i));
-            at += static_cast<uint32_t>(__popcll(in[i]));
+            uint64_t const one = __ballot(c.first[i] >= bound && !(c.second[i] >= bound));
+            if (one != 0) list_lanes(lds, one, c.first[i], row.token(c.vector[i]) + i);
         }
-    });
+#pragma nounroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            float const second = i < 2 ? (i == 0 ? c.second[0] : c.second[1]) : (i == 2 ? c.second[2] : c.second[3]);
+#pragma nounroll
+            for (uint64_t more = __ballot(second >= bound); more != 0; more &= more - 1) {
+                uint32_t const column = 4 * (static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(more))) - 1) + i;
+                for (uint32_t first = set; first < n; first += kSets * kWave) {
+                    uint32_t const j = first + kSets * lane;
+                    uint32_t const token = row.first() + j * kVector + column;
+                    float x = j < n && token < row.V ? row.from[token] : -INFINITY;
+                    if (row.infinite) x = x == INFINITY ? 0.0f : -INFINITY;
+                    uint64_t const in = __ballot(x >= bound);
+                    if (in != 0) list_lanes(lds, in, x, token);
+                }
+            }
+        }
+    }
     __syncthreads();
     return lds.word[0];
 }
@@ -420,28 +519,32 @@ __device__ uint32_t token_at(const Row& row, SampleLds& lds, uint64_t target, co
         lds.before = before;
     }
     __syncthreads();
-    // Four tokens a thread, those of the range.
-    uint32_t const v = lds.word[0] + 4 * tid;
+    // The range's tokens, neighbours each thread.
+    uint32_t const v = lds.word[0] + kRangeEach * tid;
     uint32_t const end = lds.word[1];
-    f32x4_t y = row.as_counted(row.load(v));
-    uint64_t w4[4];
+    uint64_t w[kRangeEach];
     sum = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        w4[i] = v + i < end ? weight.of(y[i], v + i) : 0;
-        sum += w4[i];
+    for (uint32_t k = 0; k < kRangeEach; k += 4) {
+        f32x4_t const y = row.as_counted(row.load(v + k));
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            uint64_t const x = weight.of(y[i], v + k + i);
+            w[k + i] = v + k + i < end ? x : 0;
+            sum += w[k + i];
+        }
     }
     before = lds.before + block_scan(sum, lds, &all);
     if (target >= before && target - before < sum) {   // one thread
         bool found = false;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            if (!found && target - before < w4[i]) {
+        for (uint32_t k = 0; k < kRangeEach; ++k) {
+            if (!found && target - before < w[k]) {
                 found = true;
-                lds.word[2] = v + i;
-                lds.found = w4[i];
+                lds.word[2] = v + k;
+                lds.found = w[k];
             }
-            if (!found) before += w4[i];
+            if (!found) before += w[k];
         }
     }
     __syncthreads();
@@ -451,9 +554,10 @@ __device__ uint32_t token_at(const Row& row, SampleLds& lds, uint64_t target, co
 
 // ---- sorting ---------------------------------------------------------------------
 
-// Sorts numbers[0, n), all different, into falling order; n at most kListed,
-// their upper words within low .. high.
-__device__ __attribute__((noinline)) void sort_falling(uint64_t* numbers, SampleLds& lds, uint32_t n, uint32_t low, uint32_t high)
+// Sorts numbers[0, n), all different, into falling order; n at most kListed.
+// Their upper words are keys of logits, or ~tokens, which count as -token;
+// these are at most `highest`, and lie within about `width`.
+__device__ __attribute__((noinline)) void sort_falling(uint64_t* numbers, SampleLds& lds, uint32_t n, bool logits, float highest, float width)
 {
     uint32_t const tid = threadIdx.x;
     __syncthreads();
@@ -471,37 +575,49 @@ __device__ __attribute__((noinline)) void sort_falling(uint64_t* numbers, Sample
         __syncthreads();
         return;
     }
-    // Buckets of the upper words, a thread each; then each number to its place in its bucket.
-    static_assert(kListed == 2 * kBlock, "two numbers a thread");
-    uint32_t shift = 0;
-    while (((high - low) >> shift) >= kBlock) ++shift;
-    lds.count[tid] = 0;
-    __syncthreads();
-    uint64_t x[2];
-    uint32_t bucket[2], place[2];
+    // Buckets, as many as the list has places; then each number to its place in its bucket.
+    float const rate = static_cast<float>(kListed) / width;
+    uint32_t* const starts = lds.count + kListed;
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
+    for (uint32_t i = 0; i < kListedEach; ++i) lds.count[i * kBlock + tid] = 0;
+    __syncthreads();
+    uint64_t x[kListedEach];
+    uint32_t bucket[kListedEach], place[kListedEach];
+#pragma unroll
+    for (uint32_t i = 0; i < kListedEach; ++i) {
         uint32_t const at = tid + i * kBlock;
         if (at >= n) continue;
         x[i] = numbers[at];
-        bucket[i] = (high - static_cast<uint32_t>(x[i] >> 32)) >> shift;
+        uint32_t const word = static_cast<uint32_t>(x[i] >> 32);
+        float const value = logits ? logit_of(word) : -static_cast<float>(0xFFFFFFFFu - word);
+        bucket[i] = static_cast<uint32_t>(fminf((highest - value) * rate, static_cast<float>(kListed - 1)));   // of NaN the last
         place[i] = atomicAdd(&lds.count[bucket[i]], 1u);
     }
     __syncthreads();
-    uint32_t const size = lds.count[tid];
-    uint64_t all;
-    uint64_t const start = block_scan(size, lds, &all);
-    lds.count[kBlock + tid] = static_cast<uint32_t>(start);
-    if (__syncthreads_or(size > kBucket) == 0) {
+    uint32_t size[kListedEach], sum = 0, most = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) {
-            if (tid + i * kBlock < n) lds.other[lds.count[kBlock + bucket[i]] + place[i]] = x[i];
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        size[i] = lds.count[kListedEach * tid + i];
+        sum += size[i];
+        most = max(most, size[i]);
+    }
+    uint64_t all;
+    uint32_t start = static_cast<uint32_t>(block_scan(sum, lds, &all));
+#pragma unroll
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        starts[kListedEach * tid + i] = start;
+        start += size[i];
+    }
+    if (__syncthreads_or(most > kBucket) == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < kListedEach; ++i) {
+            if (tid + i * kBlock < n) lds.other[starts[bucket[i]] + place[i]] = x[i];
         }
         __syncthreads();
 #pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < kListedEach; ++i) {
             if (tid + i * kBlock >= n) continue;
-            uint32_t const first = lds.count[kBlock + bucket[i]];
+            uint32_t const first = starts[bucket[i]];
             uint32_t const last = first + lds.count[bucket[i]];
             uint32_t higher = 0;
             for (uint32_t k = first; k < last; ++k) higher += lds.other[k] > x[i] ? 1u : 0u;
@@ -547,6 +663,19 @@ struct Bins {
     float half;      // of the highest logit
     float rate;      // bins for a unit of half a logit, finite
     __device__ uint32_t of(float x) const { return static_cast<uint32_t>(fminf((half - 0.5f * x) * rate, static_cast<float>(kBins - 1))); }
+    // No logit of the bin is below under(b), and none above over(b): the borders,
+    // and what a part in 2^17 of the largest number on the way may take from them.
+    __device__ float slack(uint32_t b) const { return (fabsf(half) + static_cast<float>(b + 1) / rate) * 0x1p-17f; }
+    __device__ float under(uint32_t b) const
+    {
+        float const x = 2.0f * (half - static_cast<float>(b + 1) / rate) - slack(b);
+        return x == x ? x : -INFINITY;
+    }
+    __device__ float over(uint32_t b) const
+    {
+        float const x = 2.0f * (half - static_cast<float>(b) / rate) + slack(b);
+        return x == x ? x : INFINITY;
+    }
 };
 
 // The bin that the cut falls into, and what lies before it of what the cut counts.
@@ -557,22 +686,21 @@ struct Place {
 
 __device__ inline Place place_of(SampleLds& lds, const Cut& cut, uint64_t before)
 {
-    static_assert(kBins == 4 * kBlock, "four bins a thread");
     uint32_t const tid = threadIdx.x;
-    uint64_t of[4];
+    uint64_t of[kBinsEach];
     uint64_t sum = 0, all;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        of[i] = cut.by_mass ? lds.mass[4 * tid + i] : lds.count[4 * tid + i];
+    for (uint32_t i = 0; i < kBinsEach; ++i) {
+        of[i] = cut.by_mass ? lds.mass[kBinsEach * tid + i] : lds.count[kBinsEach * tid + i];
         sum += of[i];
     }
     uint64_t at = before + block_scan(sum, lds, &all);
     if (tid == 0) lds.word[0] = kBins;
     __syncthreads();
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
+    for (uint32_t i = 0; i < kBinsEach; ++i) {
         if (at < cut.amount && cut.amount - at <= of[i]) {   // one bin at most
-            lds.word[0] = 4 * tid + i;
+            lds.word[0] = kBinsEach * tid + i;
             lds.before = at;
         }
         at += of[i];
@@ -586,7 +714,7 @@ __device__ inline Place place_of(SampleLds& lds, const Cut& cut, uint64_t before
 __device__ inline void clear_bins(SampleLds& lds)
 {
 #pragma unroll
-    for (uint32_t i = 0; i < kBins / kBlock; ++i) {
+    for (uint32_t i = 0; i < kBinsEach; ++i) {
         lds.count[i * kBlock + threadIdx.x] = 0;
         lds.mass[i * kBlock + threadIdx.x] = 0;
     }
@@ -600,15 +728,12 @@ __device__ __attribute__((noinline)) Last find_cut(const Row& row, SampleLds& ld
     Place place = place_of(lds, cut, 0);
     if (place.bin == kBins) return Last{-INFINITY, 0xFFFFFFFFu};
     uint32_t const bin = place.bin;
-    // The bin's tokens; the keys that they can have, from the bin's bounds and a
-    // part in 2^17 of the largest number on the way.
-    auto const border = [&](uint32_t b) { return 2.0f * (bins.half - static_cast<float>(b) / bins.rate); };
-    float const slack = (fabsf(bins.half) + static_cast<float>(bin + 1) / bins.rate) * 0x1p-17f;
-    float const low_x = border(bin + 1) - slack;
-    float const high_x = border(bin) + slack;
-    uint32_t low = low_x > -3.4028234664e38f ? key_of(low_x) : 0x00800000u;
-    uint32_t high = high_x < 2.0f * bins.half ? key_of(high_x) : key_of(2.0f * bins.half);
-    uint32_t listed = list_tokens(row, lds, low_x == low_x ? low_x : -INFINITY, high_x == high_x ? high_x : INFINITY, [&](float x) { return bins.of(x) == bin; });
+    // The bin's tokens, and the keys that they can have.
+    float const low_x = bins.under(bin);
+    float const high_x = bins.over(bin);
+    uint32_t low = key_of(fmaxf(low_x, -3.4028234664e38f));
+    uint32_t high = key_of(fminf(high_x, 2.0f * bins.half));
+    uint32_t listed = list_tokens(row, lds, low_x, high_x, [&](float x) { return bins.of(x) == bin; });
     if (listed > kListed) {
         // Too many: their highest and lowest keys, and bins of these.
         if (tid == 0) {
@@ -616,17 +741,17 @@ __device__ __attribute__((noinline)) Last find_cut(const Row& row, SampleLds& ld
             lds.word[2] = 0xFFFFFFFFu;
         }
         __syncthreads();
-        uint32_t most = 0, least = 0xFFFFFFFFu;
+        uint32_t most = 0, fewest = 0xFFFFFFFFu;
         row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 if (bins.of(y[i]) != bin) continue;
                 most = max(most, key_of(y[i]));
-                least = min(least, key_of(y[i]));
+                fewest = min(fewest, key_of(y[i]));
             }
         });
         atomicMax(&lds.word[1], most);
-        atomicMin(&lds.word[2], least);
+        atomicMin(&lds.word[2], fewest);
         __syncthreads();
         high = lds.word[1];
         low = lds.word[2];
@@ -673,21 +798,23 @@ __device__ __attribute__((noinline)) Last find_cut(const Row& row, SampleLds& ld
         uint32_t const token = token_at(row, lds, (left - 1) / weight, same, &one);
         return Last{logit_of(high), token};
     }
-    sort_falling(lds.listed, lds, listed, low, high);
-    // Two neighbours of the order a thread.
-    uint64_t w[2] = {};
+    sort_falling(lds.listed, lds, listed, true, logit_of(high), logit_of(high) - logit_of(low));
+    // Neighbours of the order each thread.
+    uint64_t w[kListedEach] = {};
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        uint32_t const n = 2 * tid + i;
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        uint32_t const n = kListedEach * tid + i;
         if (n < listed) w[i] = cut.by_mass ? weights.of(logit_of(static_cast<uint32_t>(lds.listed[n] >> 32))) : 1;
     }
-    uint64_t total;
-    uint64_t at = block_scan(w[0] + w[1], lds, &total);
+    uint64_t total, sum = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
+    for (uint32_t i = 0; i < kListedEach; ++i) sum += w[i];
+    uint64_t at = block_scan(sum, lds, &total);
+#pragma unroll
+    for (uint32_t i = 0; i < kListedEach; ++i) {
         if (at < left && left - at <= w[i]) {
-            lds.word[0] = static_cast<uint32_t>(lds.listed[2 * tid + i] >> 32);
-            lds.word[1] = 0xFFFFFFFFu - static_cast<uint32_t>(lds.listed[2 * tid + i]);
+            lds.word[0] = static_cast<uint32_t>(lds.listed[kListedEach * tid + i] >> 32);
+            lds.word[1] = 0xFFFFFFFFu - static_cast<uint32_t>(lds.listed[kListedEach * tid + i]);
         }
         at += w[i];
     }
@@ -705,26 +832,31 @@ struct Drawn {
     uint64_t total;
 };
 
-// From the list of the highest tokens, keys within low .. high, the first top_k
-// of which count.  Each thread has up to two neighbours of the list.
+// From a list of the first top_k tokens and more, keys within low .. high.  Each
+// thread has neighbours of it.
 __device__ inline Drawn draw_listed(SampleLds& lds, const Weights& weights, const kimkv_sample_rule& rule, uint32_t listed, uint32_t top_k,
-                                    uint32_t low, uint32_t high, float uniform, uint32_t V)
+                                    float low, float high, float uniform, uint32_t V)
 {
     uint32_t const tid = threadIdx.x;
-    sort_falling(lds.listed, lds, listed, low, high);
+    sort_falling(lds.listed, lds, listed, true, high, high - low);
     uint32_t const n = min(listed, top_k);
     uint64_t const least = part_of(rule.min_p, uint64_t{1} << weights.scale, true);
-    uint64_t w[2];
+    uint64_t w[kListedEach];
+    uint64_t sum = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) w[i] = 2 * tid + i < n ? weights.of(logit_of(static_cast<uint32_t>(lds.listed[2 * tid + i] >> 32))) : 0;
-    uint64_t total;
-    uint64_t at = block_scan(w[0] + w[1], lds, &total);
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        uint32_t const p = kListedEach * tid + i;
+        w[i] = p < n ? weights.of(logit_of(static_cast<uint32_t>(lds.listed[p] >> 32))) : 0;
+        sum += w[i];
+    }
+    uint64_t all;
+    uint64_t at = block_scan(sum, lds, &all);
     // What top-p keeps begins before its part of the weight is reached.
-    uint64_t const need = rule.top_p < 1.0f ? part_of(rule.top_p, total, true) : ~uint64_t{0};
+    uint64_t const need = rule.top_p < 1.0f ? part_of(rule.top_p, all, true) : ~uint64_t{0};
     uint32_t kept = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        if (2 * tid + i < n && at < need && w[i] >= least) {
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        if (kListedEach * tid + i < n && at < need && w[i] >= least) {
             kept += 1;
             at += w[i];
         } else {
@@ -735,30 +867,34 @@ __device__ inline Drawn draw_listed(SampleLds& lds, const Weights& weights, cons
     uint32_t const m = static_cast<uint32_t>(block_total(kept, lds));
     // The kept ones in the vocabulary's order: ~token, then the place in the list.
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        uint32_t const p = 2 * tid + i;
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        uint32_t const p = kListedEach * tid + i;
         if (p < m) lds.listed[p] = lds.listed[p] << 32 | p;
     }
-    sort_falling(lds.listed, lds, m, 0xFFFFFFFFu - (V - 1), 0xFFFFFFFFu);
+    sort_falling(lds.listed, lds, m, false, 0.0f, static_cast<float>(V));
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        if (2 * tid + i < m) lds.other[2 * tid + i] = w[i];
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        if (kListedEach * tid + i < m) lds.other[kListedEach * tid + i] = w[i];
     }
     __syncthreads();
+    sum = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) w[i] = 2 * tid + i < m ? lds.other[static_cast<uint32_t>(lds.listed[2 * tid + i])] : 0;
-    at = block_scan(w[0] + w[1], lds, &total);
-    uint64_t const target = part_of(uniform, total, false);
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        w[i] = kListedEach * tid + i < m ? lds.other[static_cast<uint32_t>(lds.listed[kListedEach * tid + i])] : 0;
+        sum += w[i];
+    }
+    at = block_scan(sum, lds, &all);
+    uint64_t const target = part_of(uniform, all, false);
 #pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
+    for (uint32_t i = 0; i < kListedEach; ++i) {
         if (target >= at && target - at < w[i]) {
-            lds.word[0] = 0xFFFFFFFFu - static_cast<uint32_t>(lds.listed[2 * tid + i] >> 32);
+            lds.word[0] = 0xFFFFFFFFu - static_cast<uint32_t>(lds.listed[kListedEach * tid + i] >> 32);
             lds.found = w[i];
         }
         at += w[i];
     }
     __syncthreads();
-    return Drawn{lds.word[0], lds.found, total};
+    return Drawn{lds.word[0], lds.found, all};
 }
 
 struct SampleArgs {
@@ -795,13 +931,41 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     }
     clear_bins(lds);
 
-    // ---- the highest logit, by place in a vector (NaN is left out) ----
-    f32x4_t high4 = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
+    bool const greedy = rule.temperature == 0.0f;
+    float const temperature = greedy ? 1.0f : rule.temperature;
+    uint32_t const top_k = greedy ? 1 : rule.top_k == 0 || rule.top_k >= a.V ? a.V : rule.top_k;
+    bool const cut_k = top_k < a.V || greedy;
+    bool const short_k = cut_k && top_k <= kShortList;
+    bool const cut_p = !greedy && rule.top_p < 1.0f;
+    bool const list = short_k || (!cut_k && !cut_p && rule.min_p > 0.0f);
+
+    // ---- the columns' highest logits (NaN is left out) ----
+    constexpr f32x4_t kNone{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    static_assert(kAhead % kSets == 0, "a vector's set is known where the code is built");
+    Columns columns[kSets];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) high4[i] = fmaxf(high4[i], y[i]);
-    });
-    float high = row_max(highest_of(high4));
+    for (uint32_t set = 0; set < kSets; ++set) columns[set] = Columns{kNone, kNone, {0, 0, 0, 0}};
+    if (list) {
+        row.vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
+            Columns& c = columns[j % kSets];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                c.second[i] = fmaxf(c.second[i], fminf(c.first[i], y[i]));
+                c.vector[i] = y[i] > c.first[i] ? j : c.vector[i];
+                c.first[i] = fmaxf(c.first[i], y[i]);
+            }
+        });
+    } else {
+        row.vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
+            Columns& c = columns[j % kSets];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) c.first[i] = fmaxf(c.first[i], y[i]);
+        });
+    }
+    float high = -INFINITY;
+#pragma unroll
+    for (uint32_t set = 0; set < kSets; ++set) high = fmaxf(high, highest_of(columns[set].first));
+    high = row_max(high);
     high = fmaxf(high, xor16(high));
     high = fmaxf(high, xor32(high));
     if (lane == 0) lds.wave_f[tid / kWave] = high;
@@ -812,38 +976,51 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
         return;
     }
     row.infinite = high == INFINITY;
-    high4 = row.as_counted(high4);
     if (row.infinite) high = 0.0f;
-
-    bool const greedy = rule.temperature == 0.0f;
-    float const temperature = greedy ? 1.0f : rule.temperature;
-    uint32_t const top_k = greedy ? 1 : rule.top_k == 0 || rule.top_k >= a.V ? a.V : rule.top_k;
-    bool const cut_k = top_k < a.V || greedy;
-    bool const cut_p = !greedy && rule.top_p < 1.0f;
     Weights const weights{high, 1.4426950408889634 / static_cast<double>(temperature), a.scale};
+    Kept kept = kept_tokens(weights, Last{-INFINITY, 0xFFFFFFFFu}, temperature, rule.min_p);
 
-    if (cut_k && top_k <= kShortList) {
-        // Bins of the maxima's keys, from the highest down: 12 bits of 32.
+    // ---- from a list ----
+    if (list) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            if (high4[i] != -INFINITY) atomicAdd(&lds.count[kBins - 1 - (key_of(high4[i]) >> 20)], 1u);
+        for (uint32_t set = 0; set < kSets; ++set) {
+            columns[set].first = row.as_counted(columns[set].first);
+            columns[set].second = row.as_counted(columns[set].second);
         }
-        __syncthreads();
-        // The bound's bin, or all where there are fewer maxima.
-        uint32_t const bin = min(place_of(lds, Cut{false, top_k}, 0).bin, kBins - 1);
-        uint32_t const bound = max((kBins - 1 - bin) << 20, 0x00800000u);   // at least the lowest number's key
-        float const bound_x = logit_of(bound);
-        uint32_t const listed = list_tokens(row, lds, bound_x, INFINITY, [](float) { return true; });
+        // A bound that so many columns reach, to a part in 4096 of what is looked at;
+        // what lies below `none` weighs nothing.
+        float const none = fmaxf(high - kWeightless * temperature, -3.4028234664e38f);
+        float bound = none;
+        if (short_k) {
+            Bins const near{0.5f * high, fminf(2 * (kBins - 1) / fminf(kWeightless * temperature, 64.0f), 3e38f)};
+#pragma unroll
+            for (uint32_t set = 0; set < kSets; ++set) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    uint32_t const b = near.of(columns[set].first[i]);
+                    if (b < kBins - 1) atomicAdd(&lds.count[b], 1u);
+                }
+            }
+            __syncthreads();
+            uint32_t const bin = place_of(lds, Cut{false, top_k}, 0).bin;
+            if (bin < kBins) bound = fmaxf(near.under(bin), none);
+        }
+        // One that min-p leaves out counts where top-p takes its part of the list.
+        if (!cut_p) bound = fmaxf(bound, kept.floor);
+        uint32_t const listed = list_columns(row, lds, columns, bound);
         if (listed <= kListed) {
-            Drawn const d = draw_listed(lds, weights, rule, listed, top_k, bound, key_of(high), uniform, a.V);
+            Drawn const d = draw_listed(lds, weights, rule, listed, top_k, bound, high, uniform, a.V);
             answer(d.token, static_cast<float>(static_cast<double>(d.weight) / static_cast<double>(d.total)));
             return;
         }
-        __syncthreads();
-        clear_bins(lds);
-        __syncthreads();
+        if (short_k) {
+#pragma unroll
+            for (uint32_t i = 0; i < kBinsEach; ++i) lds.count[i * kBlock + tid] = 0;
+            __syncthreads();
+        }
     }
 
+    // ---- the cuts of the row ----
     Last last{-INFINITY, 0xFFFFFFFFu};
     if (cut_k || cut_p) {
         Bins const bins{0.5f * high, fminf(2 * (kBins - 1) / (kWeightless * temperature), 3e38f)};
@@ -871,34 +1048,37 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
             }
         });
         __syncthreads();
-        uint64_t mass[kBins / kBlock];
+        uint64_t mass[kBinsEach];
         uint64_t total = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kBins / kBlock; ++i) {
-            mass[i] = lds.mass[i * kBlock + tid];
-            total += mass[i];
-        }
-        if (cut_p) total = block_total(total, lds);
-        if (cut_k) {
-            last = find_cut(row, lds, weights, bins, Cut{false, top_k});
-            if (cut_p && last.logit != -INFINITY) total = sum_ranges(row, lds, kept_tokens(weights, last, temperature, 0.0f));
-        }
         if (cut_p) {
-            __syncthreads();
 #pragma unroll
-            for (uint32_t i = 0; i < kBins / kBlock; ++i) lds.mass[i * kBlock + tid] = mass[i];
-            __syncthreads();
-            Last const mine = find_cut(row, lds, weights, bins, Cut{true, part_of(rule.top_p, total, true)});
-            if (mine.logit > last.logit || (mine.logit == last.logit && mine.token < last.token)) last = mine;
+            for (uint32_t i = 0; i < kBinsEach; ++i) {
+                mass[i] = lds.mass[i * kBlock + tid];
+                total += mass[i];
+            }
+            total = block_total(total, lds);
+        }
+        // The top_k tokens' cut, then that of top-p's part of their weight.
+#pragma nounroll
+        for (uint32_t by_mass = cut_k ? 0 : 1; by_mass <= (cut_p ? 1 : 0); ++by_mass) {
+            if (by_mass != 0 && cut_k) {
+                if (last.logit != -INFINITY) total = sum_ranges(row, lds, kept_tokens(weights, last, temperature, 0.0f));
+                __syncthreads();
+#pragma unroll
+                for (uint32_t i = 0; i < kBinsEach; ++i) lds.mass[i * kBlock + tid] = mass[i];
+                __syncthreads();
+            }
+            Last const its = find_cut(row, lds, weights, bins, Cut{by_mass != 0, by_mass != 0 ? part_of(rule.top_p, total, true) : top_k});
+            if (its.logit > last.logit || (its.logit == last.logit && its.token < last.token)) last = its;
         }
     }
 
     // ---- the draw ----
-    Kept const kept = kept_tokens(weights, last, temperature, rule.min_p);
-    uint64_t const total = sum_ranges(row, lds, kept);
+    kept = kept_tokens(weights, last, temperature, rule.min_p);
+    uint64_t const sums = sum_ranges(row, lds, kept);
     uint64_t its;
-    uint32_t const token = token_at(row, lds, part_of(uniform, total, false), kept, &its);
-    answer(token, static_cast<float>(static_cast<double>(its) / static_cast<double>(total)));
+    uint32_t const token = token_at(row, lds, part_of(uniform, sums, false), kept, &its);
+    answer(token, static_cast<float>(static_cast<double>(its) / static_cast<double>(sums)));
 }
 
 }  // namespace
