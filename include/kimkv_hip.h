@@ -757,9 +757,8 @@ kimkv_status kimkv_quant_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint3
  * none is left the output is 0.  A row of K that reads as NaN makes the outputs
  * of its head NaN, and so does one of V that has a weight above 0.  Head dims
  * of 64, 96 and 128 with up to 16 query heads a KV head run on the matrix
- * cores, as long as the tables keep groups of 8 tokens whole (every entry
- * begins at a multiple of 8); others take a slower path.  Results are the same
- * for every run of one plan. */
+ * cores; others take a slower path.  Results are the same for every run of one
+ * plan. */
 kimkv_status kimkv_quant_decode_batch(const kimkv_quant_storage* storage, const kimkv_decode_item* device_items,
                                       const void* device_entries, const kimkv_quant_plan* plan, void* workspace,
                                       kimkv_stream_t stream);

@@ -10,15 +10,23 @@
 // Work: block = unit (a lane, a KV head, a range of its tokens), its four waves
 // a quarter of the range each, joined in LDS; a lane of one unit a head is
 // written at once, the others' parts are merged by a second launch.  A wave
-// reads 64 table entries at a time.  An entry that is a whole page of 64 tokens
-// is a tile; the groups of 8 of all others are collected eight to a tile: the
-// order of the tokens does not matter to the sums.  Per tile
+// takes the table entries that begin in its range, so no page is cut; it reads
+// 64 of them at a time.  An entry that is a whole page of 64 tokens is a tile;
+// the groups of 8 of all others are collected eight to a tile: the order of the
+// tokens does not matter to the sums.  Per tile
 //   S^T[token][q] = K[token][:] . Q[q][:]           D / 2 / 4 MFMA 16x16x32
 //   online softmax (base 2) on the 16 scores of a lane
 //   O^T[d][q]    += V^T[d][token] . (b P)[q][token]  D / 4 MFMA, weights in two fp16 parts
 // K rows and V^T rows go from memory to the operand registers in 16-byte loads
 // (8 for small pages); tokens are numbered so that the scores a lane holds are
 // the weights it needs.
+//
+// Bound by HBM where batches are large: 128 lanes of 32768 tokens, 4 heads of 64
+// (2.2 GB) take 350 us, 6.3 TB/s.  A tile's K registers take the next tile's K as
+// soon as the scores stand, and V's the next V behind the sums: two sets of
+// registers for a tile (128 dims: 108 of them spilled) made 64 ragged lanes of up
+// to 6000 tokens, 8 heads of 128, 55 us instead of 29.  There the launches, the
+// chain of loads to the first page and the last tiles bound: 103 MB take 15 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -113,6 +121,20 @@ typedef const __attribute__((address_space(1))) u32x2_t global_u32x2_t;
 __device__ inline u32x4_t stream16(const uint8_t* p) { return __builtin_nontemporal_load((global_u32x4_t*)(p)); }
 __device__ inline u32x2_t stream8(const uint8_t* p) { return __builtin_nontemporal_load((global_u32x2_t*)(p)); }
 __device__ inline u32x4_t load16(const uint8_t* p) { return *(global_u32x4_t*)(p); }
+constexpr int kStreamed = 2;
+
+// A page's bytes behind a pointer that is the same in all lanes, or none of
+// them: loads of it then read nothing and wait for nothing.
+struct PageBytes {
+    __amdgpu_buffer_rsrc_t bounded;
+    __device__ PageBytes(const uint8_t* p, uint32_t bytes)
+        : bounded(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, static_cast<int>(p != nullptr ? bytes : 0), 0x00027000))
+    {
+    }
+    __device__ u32x4_t stream16(uint32_t at) const { return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(bounded, static_cast<int>(at), 0, kStreamed)); }
+    __device__ u32x2_t stream8(uint32_t at) const { return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(bounded, static_cast<int>(at), 0, kStreamed)); }
+    __device__ u32x4_t load16(uint32_t at) const { return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(bounded, static_cast<int>(at), 0, 0)); }
+};
 
 __device__ inline uint64_t lane_value(uint64_t v, int lane)
 {
@@ -201,45 +223,45 @@ struct Decoder {
         }
     }
 
-    // The tile of a whole page of 64 tokens: `block` is uniform.
-    __device__ void load_page(Ops& o, const uint8_t* block, uint32_t codes_at, uint32_t scales_at) const
+    // The tile of a whole page of 64 tokens, its K and its V.
+    __device__ void load_page_k(Ops& o, const PageBytes& page, uint32_t codes_at, uint32_t scales_at) const
     {
-        const uint8_t* const codes = block + codes_at;
-        uint32_t const row = (16 * (r >> 2) + (r & 3u)) * kKw + g * (kWide ? 16 : 8);
+        uint32_t const row = codes_at + (16 * (r >> 2) + (r & 3u)) * kKw + g * (kWide ? 16 : 8);
 #pragma unroll
         for (uint32_t tau = 0; tau < 4; ++tau) {
             if (kWide) {
 #pragma unroll
                 for (uint32_t b = 0; b < kSteps / 2; ++b) {
-                    u32x4_t const w = stream16(codes + (row + 4 * tau * kKw + b * kTile * 64));
+                    u32x4_t const w = page.stream16(row + 4 * tau * kKw + b * kTile * 64);
                     o.k[tau][2 * b] = u32x2_t{w[0], w[1]};
                     o.k[tau][2 * b + 1] = u32x2_t{w[2], w[3]};
                 }
             } else {
 #pragma unroll
-                for (uint32_t j = 0; j < kSteps; ++j) o.k[tau][j] = stream8(codes + (row + 4 * tau * kKw + 32 * j));
+                for (uint32_t j = 0; j < kSteps; ++j) o.k[tau][j] = page.stream8(row + 4 * tau * kKw + 32 * j);
             }
         }
-        uint32_t const column = kTile * kDim + r * kTile + 16 * g;
 #pragma unroll
-        for (uint32_t db = 0; db < kDb; ++db) o.v[db] = stream16(codes + (column + db * 16 * kTile));
-        const uint8_t* const scales = block + scales_at;
+        for (uint32_t s = 0; s < 2; ++s) o.ks[s] = page.load16(scales_at + 32 * g + 16 * s);
+    }
+    __device__ void load_page_v(Ops& o, const PageBytes& page, uint32_t codes_at, uint32_t scales_at) const
+    {
 #pragma unroll
-        for (uint32_t s = 0; s < 2; ++s) {
-            o.ks[s] = load16(scales + (32 * g + 16 * s));
-            o.vs[s] = load16(scales + (2 * kTile + 32 * g + 16 * s));
-        }
+        for (uint32_t s = 0; s < 2; ++s) o.vs[s] = page.load16(scales_at + 2 * kTile + 32 * g + 16 * s);
+        uint32_t const column = codes_at + kTile * kDim + r * kTile + 16 * g;
+#pragma unroll
+        for (uint32_t db = 0; db < kDb; ++db) o.v[db] = page.stream16(column + db * 16 * kTile);
     }
 
     // A tile of 8 groups of pages of any kind; `count` (1 .. 8) are there.
-    __device__ void load_groups(Ops& o, const Group* groups, uint32_t count, uint32_t heads, uint32_t h, uint32_t (&valid)[2]) const
+    static __device__ const uint8_t* codes_of(const Group& x, uint32_t h) { return x.block + static_cast<uint64_t>(h) * 2 * x.cap * kDim; }
+    __device__ void load_groups_k(Ops& o, const Group* groups, uint32_t count, uint32_t heads, uint32_t h) const
     {
-        auto const codes_of = [&](const Group& x) { return x.block + static_cast<uint64_t>(h) * 2 * x.cap * kDim; };
 #pragma unroll
         for (uint32_t s = 0; s < 2; ++s) {
             uint32_t const n = 2 * (r >> 2) + s;
             Group const x = groups[min(n, count - 1)];
-            const uint8_t* const codes = codes_of(x);
+            const uint8_t* const codes = codes_of(x, h);
 #pragma unroll
             for (uint32_t u = 0; u < 2; ++u) {
                 const uint8_t* const row = codes + (x.first + 4 * u + (r & 3u)) * kKw + g * (kWide ? 16 : 8);
@@ -258,25 +280,32 @@ struct Decoder {
         }
 #pragma unroll
         for (uint32_t s = 0; s < 2; ++s) {
+            Group const x = groups[min(2 * g + s, count - 1)];
+            o.ks[s] = load16(x.block + static_cast<uint64_t>(heads) * 2 * x.cap * kDim + h * 4u * x.cap + 2 * x.first);
+        }
+    }
+    __device__ void load_groups_v(Ops& o, const Group* groups, uint32_t count, uint32_t heads, uint32_t h, uint32_t (&valid)[2]) const
+    {
+#pragma unroll
+        for (uint32_t s = 0; s < 2; ++s) {
             uint32_t const n = 2 * g + s;
             Group const x = groups[min(n, count - 1)];
             valid[s] = n < count ? x.valid : 0;
-            const uint8_t* const column = codes_of(x) + x.cap * kDim + r * x.cap + x.first;
+            const uint8_t* const column = codes_of(x, h) + x.cap * kDim + r * x.cap + x.first;
 #pragma unroll
             for (uint32_t db = 0; db < kDb; ++db) {
                 u32x2_t const w = stream8(column + db * 16 * x.cap);
                 o.v[db][2 * s] = w[0];
                 o.v[db][2 * s + 1] = w[1];
             }
-            const uint8_t* const scales = x.block + static_cast<uint64_t>(heads) * 2 * x.cap * kDim + h * 4u * x.cap + 2 * x.first;
-            o.ks[s] = load16(scales);
-            o.vs[s] = load16(scales + 2 * x.cap);
+            o.vs[s] = load16(x.block + static_cast<uint64_t>(heads) * 2 * x.cap * kDim + h * 4u * x.cap + 2 * x.first + 2 * x.cap);
         }
     }
 
     // kMasked: only the first valid[s] tokens of a lane's groups s are there.
-    template <bool kMasked>
-    __device__ void add(Ops& o, uint32_t (&valid)[2])
+    // next_k, next_v: the next tile's loads, into the registers that are done with.
+    template <bool kMasked, typename K, typename V>
+    __device__ __attribute__((always_inline)) void add(Ops& o, uint32_t (&valid)[2], K next_k, V next_v)
     {
         auto const scale_of = [](const u32x4_t& w, uint32_t t) {
             return __uint_as_float((t & 1u) != 0 ? w[t >> 1] & 0xFFFF0000u : w[t >> 1] << 16);
@@ -302,6 +331,9 @@ struct Decoder {
                 mx = fmaxf(mx, x);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        next_k();
+        __builtin_amdgcn_sched_barrier(0);
         mx = fmaxf(mx, xor16(mx));
         mx = fmaxf(mx, xor32(mx));
         float const m_new = fmaxf(m, mx);
@@ -378,6 +410,9 @@ struct Decoder {
                 acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[s], acc[db], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        next_v();
+        __builtin_amdgcn_sched_barrier(0);
     }
 
     __device__ WavePart<kDim> part() const
@@ -394,84 +429,77 @@ struct Decoder {
     }
 };
 
-// Bits of what a wave met in its tables.
-constexpr uint32_t kBadPage = 1;    // an entry names no page of the storage
-constexpr uint32_t kLoose = 2;      // groups of 8 tokens are not whole: the general path takes the unit
-
+// The entries that begin within [t0, t1), as far as the lane's tokens go; *bad
+// where one names no page of the storage.
 template <uint32_t kFormat, uint32_t kDim>
 __device__ WavePart<kDim> decode_wave(const QuantView& P, const kimkv_decode_item& item, uint32_t h, uint32_t G, uint32_t t0,
-                                      uint32_t t1, Group* groups, uint32_t* met)
+                                      uint32_t t1, uint32_t tokens, Group* groups, bool* bad)
 {
     uint32_t const lane = threadIdx.x & (kWave - 1);
     Decoder<kFormat, kDim> d(item, h, G);
-    uint32_t whole[2] = {8, 8};
-    uint32_t idx = t0 < t1 ? find_descriptor_wave(item.descriptors, item.descriptor_count, t0) : item.descriptor_count;
+    // A short table is read whole, without the search's own read of it.
+    uint32_t const count = item.descriptor_count;
+    uint32_t idx = t0 >= t1 ? count : count <= kWave ? 0 : find_descriptor_wave(item.descriptors, count, t0);
     uint32_t const codes_at = h * 2 * kTile * kDim;
     uint32_t const scales_at = P.heads * 2 * kTile * kDim + h * 4 * kTile;
-    while (idx < item.descriptor_count) {
+    uint32_t const page_bytes = P.heads * kTile * (2 * kDim + 4);
+    while (idx < count) {
         // This lane's entry.
-        bool const there = item.descriptor_count - idx > lane;
+        bool const there = count - idx > lane;
         kimkv_block_desc entry{};
         if (there) entry = item.descriptors[idx + lane];
         uint32_t const begin = entry.logical_token_begin;
-        uint32_t const end = begin + entry.valid_tokens;
-        uint32_t const lo = max(begin, t0);
-        uint32_t const hi = min(end, t1);
-        bool const covers = there && lo < hi;
         uint32_t const cap = entry.page_token_capacity;
+        bool const mine = there && begin >= t0 && begin < t1 && entry.valid_tokens != 0;
+        uint32_t const valid = mine ? min(static_cast<uint32_t>(entry.valid_tokens), tokens - begin) : 0;
         const uint8_t* block = nullptr;
-        if (covers && entry.valid_tokens <= cap) block = quant_block(P, item.layer, entry.kind, entry.slot, cap);
-        if (__ballot(covers && block == nullptr) != 0) *met |= kBadPage;
-        if (__ballot(covers && ((begin & 7u) != 0 || ((end & 7u) != 0 && end < t1))) != 0) {
-            *met |= kLoose;
-            break;
-        }
-        bool const page = block != nullptr && cap == kTile && hi - lo == kTile;
-        uint32_t const mine = block != nullptr && !page ? (hi - lo + 7) / 8 : 0;
-        uint32_t before = mine;   // groups of the lanes up to this one
+        if (mine && entry.valid_tokens <= cap) block = quant_block(P, item.layer, entry.kind, entry.slot, cap);
+        *bad = *bad || __ballot(mine && block == nullptr) != 0;
+        bool const page = block != nullptr && cap == kTile && valid == kTile;
+        uint32_t const parts = block != nullptr && !page ? (valid + 7) / 8 : 0;
+        uint32_t before = parts;   // groups of the lanes up to this one
 #pragma unroll
         for (uint32_t k = 1; k < kWave; k *= 2) {
             uint32_t const v = static_cast<uint32_t>(__shfl_up(static_cast<int>(before), k));
             if (lane >= k) before += v;
         }
         uint32_t const total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(before), 63));
-        for (uint32_t k = 0; k < mine; ++k) {
-            groups[before - mine + k] = Group{block, static_cast<uint16_t>(lo - begin + 8 * k), static_cast<uint16_t>(cap),
-                                              min(8u, hi - lo - 8 * k)};
+        for (uint32_t k = 0; k < parts; ++k) {
+            groups[before - parts + k] = Group{block, static_cast<uint16_t>(8 * k), static_cast<uint16_t>(cap), min(8u, valid - 8 * k)};
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 
-        // Whole pages, the next one's loads in flight behind the current one's work.
+        // Whole pages.
         uint64_t left = __ballot(page);
-        auto const next = [&] {
-            int const j = __ffsll(static_cast<unsigned long long>(left)) - 1;
-            left &= left - 1;
-            return reinterpret_cast<const uint8_t*>(lane_value(reinterpret_cast<uint64_t>(block), j));
-        };
         if (left != 0) {
-            typename Decoder<kFormat, kDim>::Ops a, b;
-            d.load_page(a, next(), codes_at, scales_at);
-            for (;;) {
-                if (left == 0) {
-                    d.template add<false>(a, whole);
-                    break;
-                }
-                d.load_page(b, next(), codes_at, scales_at);
-                d.template add<false>(a, whole);
-                if (left == 0) {
-                    d.template add<false>(b, whole);
-                    break;
-                }
-                d.load_page(a, next(), codes_at, scales_at);
-                d.template add<false>(b, whole);
-            }
+            typename Decoder<kFormat, kDim>::Ops o;
+            uint32_t whole[2] = {8, 8};
+            auto const next = [&] {
+                if (left == 0) return PageBytes(nullptr, 0);
+                int const j = __ffsll(static_cast<unsigned long long>(left)) - 1;
+                return PageBytes(reinterpret_cast<const uint8_t*>(lane_value(reinterpret_cast<uint64_t>(block), j)), page_bytes);
+            };
+            PageBytes p = next();
+            d.load_page_k(o, p, codes_at, scales_at);
+            d.load_page_v(o, p, codes_at, scales_at);
+            do {
+                left &= left - 1;
+                p = next();
+                d.template add<false>(o, whole, [&] { d.load_page_k(o, p, codes_at, scales_at); }, [&] { d.load_page_v(o, p, codes_at, scales_at); });
+            } while (left != 0);
         }
-        for (uint32_t k = 0; k < total; k += 8) {
-            typename Decoder<kFormat, kDim>::Ops a;
-            uint32_t valid[2];
-            d.load_groups(a, groups + k, min(8u, total - k), P.heads, h, valid);
-            d.template add<true>(a, valid);
+        if (total != 0) {
+            typename Decoder<kFormat, kDim>::Ops o;
+            uint32_t there_of[2];
+            d.load_groups_k(o, groups, min(8u, total), P.heads, h);
+            d.load_groups_v(o, groups, min(8u, total), P.heads, h, there_of);
+            for (uint32_t k = 0; k < total; k += 8) {
+                uint32_t const n = k + 8;
+                d.template add<true>(o, there_of,
+                    [&] { if (n < total) d.load_groups_k(o, groups + n, min(8u, total - n), P.heads, h); },
+                    [&] { if (n < total) d.load_groups_v(o, groups + n, min(8u, total - n), P.heads, h, there_of); });
+            }
         }
         // The last entry read decides whether there are more.
         uint32_t const last = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(there ? begin : 0xFFFFFFFFu), 63));
@@ -640,11 +668,11 @@ __global__ __launch_bounds__(kBlock, 2) void quant_decode_kernel(QuantView P, De
         uint32_t const end = unit.first + unit.count;
         uint32_t const per = ((unit.count + kTile - 1) / kTile + kWaves - 1) / kWaves * kTile;
         uint32_t const t0 = min(unit.first + wave * per, end);
-        uint32_t met = 0;
-        WavePart<kDim> const part = decode_wave<kFormat, kDim>(P, item, unit.head, G, t0, min(t0 + per, end), f.groups[wave], &met);
-        bool const loose = __syncthreads_or((met & kLoose) != 0) != 0;   // every wave is done with its groups
-        if (!loose) {
-            if (met != 0 && lane == 0 && P.faults != nullptr) atomicOr(P.faults, KIMKV_FAULT_DECODE_ITEM);
+        bool bad = false;
+        WavePart<kDim> const part = decode_wave<kFormat, kDim>(P, item, unit.head, G, t0, min(t0 + per, end), unit.tokens, f.groups[wave], &bad);
+        if (bad && lane == 0 && P.faults != nullptr) atomicOr(P.faults, KIMKV_FAULT_DECODE_ITEM);
+        __syncthreads();   // every wave is done with its groups
+        {
             uint32_t const g = lane >> 4;
             uint32_t const r = lane & 15u;
 #pragma unroll
@@ -682,35 +710,53 @@ __global__ __launch_bounds__(kBlock, 2) void quant_decode_kernel(QuantView P, De
                     }
                 }
             }
-            return;
         }
+    } else {
+        decode_general<kFormat>(P, item, unit, G, slot, *reinterpret_cast<GeneralLds*>(lds));
     }
-    decode_general<kFormat>(P, item, unit, G, slot, *reinterpret_cast<GeneralLds*>(lds));
 }
 
-// Block = (merged lane, KV head): the parts of its query heads.
+// Block = (merged lane, KV head, kBlock of its values): a thread a value, the
+// parts eight at a time in flight.
 __global__ __launch_bounds__(kBlock) void quant_merge_kernel(QuantView P, const kimkv_decode_item* items, const QuantMerge* merges,
-                                                         const float* work, uint32_t G)
+                                                             const float* work, uint32_t G)
 {
+    constexpr uint32_t kAtOnce = 8;
     QuantMerge const x = merges[blockIdx.x];
     kimkv_decode_item const item = items[x.lane];
-    if (!item_good(P, item, x.tokens)) return;   // reported by its units
     uint32_t const D = P.dim;
     uint32_t const h = blockIdx.y;
+    uint32_t const i = blockIdx.z * kBlock + threadIdx.x;
+    if (i >= G * D) return;
     uint64_t const size = slot_floats(G, D);
-    const float* const parts = work + (x.first_slot + static_cast<uint64_t>(h) * x.parts) * size;
-    for (uint32_t i = threadIdx.x; i < G * D; i += kBlock) {
-        const float* const ml = parts + static_cast<uint64_t>(G) * D + 2 * (i / D);
-        float top = -INFINITY;
-        for (uint32_t p = 0; p < x.parts; ++p) top = fmaxf(top, ml[p * size]);
-        float sum = 0.0f, total = 0.0f;
-        for (uint32_t p = 0; p < x.parts; ++p) {
-            float const f = part_weight(ml[p * size], top);
-            total += ml[p * size + 1] * f;
-            if (f != 0.0f) sum += parts[p * size + i] * f;
+    const float* const values = work + (x.first_slot + static_cast<uint64_t>(h) * x.parts) * size + i;
+    const float* const ml = values - i + static_cast<uint64_t>(G) * D + 2 * (i / D);
+    float m = -INFINITY, total = 0.0f, sum = 0.0f;
+    for (uint32_t p = 0; p < x.parts; p += kAtOnce) {
+        float top[kAtOnce], l[kAtOnce], v[kAtOnce];
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            uint64_t const at = min(p + k, x.parts - 1) * size;
+            top[k] = ml[at];
+            l[k] = ml[at + 1];
+            v[k] = values[at];
         }
-        item.output[static_cast<uint64_t>(h) * G * D + i] = quotient_half(sum, total);
+        float most = m;
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) most = fmaxf(most, top[k]);
+        float const f = part_weight(m, most);
+        sum = f != 0.0f ? sum * f : 0.0f;
+        total *= f;
+        m = most;
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            float const w = p + k < x.parts ? part_weight(top[k], most) : 0.0f;
+            total += l[k] * w;
+            if (w != 0.0f) sum += v[k] * w;
+        }
     }
+    // An item that is not as planned is reported by its units, which wrote no parts.
+    if (item_good(P, item, x.tokens)) item.output[static_cast<uint64_t>(h) * G * D + i] = quotient_half(sum, total);
 }
 
 // ---- plan ------------------------------------------------------------------------
@@ -748,7 +794,9 @@ kimkv_status kimkv_quant_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint3
         tiles += n;
         longest = n > longest ? n : longest;
     }
-    // The tiles of a unit: as many as make two units for each place, 16 at least.
+    // The tiles of a unit: as many as make two units for each place, which evens
+    // out lanes that do not divide (one a place, 128 equal lanes of 32768 tokens:
+    // 345 us, not 353), 16 at least (8, 64 lanes of up to 6000: 31 us, not 29).
     uint64_t most = tiles / (2 * slots) * kv_heads + tiles % (2 * slots) * kv_heads / (2 * slots);
     most = most < 16 ? 16 : most;
     most = most > longest && longest != 0 ? longest : most;
@@ -839,7 +887,7 @@ kimkv_status kimkv_quant_decode_batch(const kimkv_quant_storage* storage, const 
     kimkv_status const status = launch_status();
     kernel_timing_end(TimedKernel::Decode, native(stream), start);
     if (status != KIMKV_OK || plan->merge_lanes == 0) return status;
-    quant_merge_kernel<<<dim3(plan->merge_lanes, plan->kv_heads), kBlock, 0, native(stream)>>>(
+    quant_merge_kernel<<<dim3(plan->merge_lanes, plan->kv_heads, (G * view.dim + kBlock - 1) / kBlock), kBlock, 0, native(stream)>>>(
         view, device_items, reinterpret_cast<const QuantMerge*>(units + plan->unit_count), args.work, G);
     return launch_status();
 }
