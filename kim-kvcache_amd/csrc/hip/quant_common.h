@@ -139,13 +139,15 @@ __device__ inline float scale_value(uint16_t bits) { return __uint_as_float(stat
 
 constexpr uint16_t kScaleNan = 0x7FC0;
 
-// The scale of a row whose |x| are at most the fp16 of these bits.
+// The scale of a row whose |x| are at most the fp16 of these bits: a / Q, by a
+// product that is off by 3 steps of 32 bits at most, rounded up.  a / Q is a bf16
+// or 256 of these steps away from one, so 64 of them are no part of a larger one.
 template <uint32_t kFormat>
 __device__ inline uint16_t row_scale(uint32_t largest_bits)
 {
     if (largest_bits >= 0x7C00u) return kScaleNan;
-    float const q = __half2float(__ushort_as_half(static_cast<uint16_t>(largest_bits))) / quant_largest<kFormat>();
-    return static_cast<uint16_t>((__float_as_uint(q) + 0xFFFFu) >> 16);
+    float const q = __half2float(__ushort_as_half(static_cast<uint16_t>(largest_bits))) * (1.0f / quant_largest<kFormat>());
+    return static_cast<uint16_t>((__float_as_uint(q) + (0xFFFFu - 64u)) >> 16);
 }
 
 // What codes of a row are made with: 1 / s, and s; 0 where every code is 0.
@@ -172,13 +174,13 @@ __device__ inline float row_quotient(float x, RowQuant r)
 
 // Four codes of a row, one a byte.  A whole number is held with 128 added, so
 // that the byte under the bits of 1024 is an fp16 number, and read by one
-// subtraction.  Values that are not finite come with an inverse of 0.
+// subtraction.
 template <uint32_t kFormat>
 __device__ inline uint32_t row_codes(const float (&x)[4], RowQuant r)
 {
     float y[4];
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) y[i] = r.inverse == 0.0f ? 0.0f : row_quotient(x[i], r);
+    for (uint32_t i = 0; i < 4; ++i) y[i] = row_quotient(x[i], r);
     if (kFormat == KIMKV_QUANT_INT8) {
         // The sum's last bit is 1: it rounds to the whole number, ties to even.
         uint32_t u[4];
@@ -192,29 +194,45 @@ __device__ inline uint32_t row_codes(const float (&x)[4], RowQuant r)
     return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], static_cast<int>(lo), true));
 }
 
-// Four codes as 32-bit numbers.
+// Four codes of 0.
 template <uint32_t kFormat>
-__device__ inline void code_values(uint32_t codes, float (&x)[4])
+__device__ inline uint32_t no_codes()
 {
-    if (kFormat == KIMKV_QUANT_INT8) {
+    return kFormat == KIMKV_QUANT_INT8 ? 0x80808080u : 0u;
+}
+
+// Eight codes as fp16.  A whole number's byte u under the bits of 1024 is
+// 1024 + u, and 1152 less is the number, exactly.
+typedef uint32_t code_words_t __attribute__((ext_vector_type(2)));
+typedef _Float16 code_halves_t __attribute__((ext_vector_type(8)));
+template <uint32_t kFormat>
+__device__ inline code_halves_t code_halves(code_words_t w)
+{
+    typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+    code_halves_t out;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) x[i] = static_cast<float>((codes >> (8 * i)) & 0xFFu) - 128.0f;
-    } else {
-        auto const lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes), false);
-        auto const hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes), true);
-        x[0] = lo[0];
-        x[1] = lo[1];
-        x[2] = hi[0];
-        x[3] = hi[1];
+    for (uint32_t j = 0; j < 2; ++j) {
+        half2_t a, b;
+        if (kFormat == KIMKV_QUANT_INT8) {
+            half2_t const shift = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+            a = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[j], 0x04010400u)) + shift;
+            b = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[j], 0x04030402u)) + shift;
+        } else {
+            a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w[j]), 1.0f, false);
+            b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w[j]), 1.0f, true);
+        }
+        out[4 * j] = a[0];
+        out[4 * j + 1] = a[1];
+        out[4 * j + 2] = b[0];
+        out[4 * j + 3] = b[1];
     }
+    return out;
 }
 
 template <uint32_t kFormat>
 __device__ inline float code_value(uint8_t code)
 {
-    float x[4];
-    code_values<kFormat>(code, x);
-    return x[0];
+    return static_cast<float>(code_halves<kFormat>(code_words_t{code, 0})[0]);
 }
 
 // A code times its scale as fp16.  The product is exact in 32 bits; the
@@ -225,6 +243,20 @@ __device__ inline uint16_t read_back(float code, float scale)
     v = v > 65504.0f ? 65504.0f : v;
     v = v < -65504.0f ? -65504.0f : v;
     return __half_as_ushort(__float2half_rn(v));
+}
+// Eight codes of a row; a product past 65504 only with a scale whose largest one is.
+template <uint32_t kFormat>
+__device__ inline code_halves_t read_back(code_words_t w, float scale)
+{
+    code_halves_t const code = code_halves<kFormat>(w);
+    code_halves_t out;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) out[j] = static_cast<_Float16>(static_cast<float>(code[j]) * scale);
+    if (__ballot(scale * quant_largest<kFormat>() > 65504.0f) != 0) {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) out[j] = __builtin_bit_cast(_Float16, read_back(static_cast<float>(code[j]), scale));
+    }
+    return out;
 }
 
 }  // namespace kimkv

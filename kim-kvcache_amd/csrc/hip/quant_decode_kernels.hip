@@ -49,7 +49,6 @@ constexpr uint32_t kDirect = 0xFFFFFFFFu;
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 // Tokens [first, first + count) of a lane of `tokens`, for a KV head; its part
 // goes to `slot`, or to the output.
@@ -86,33 +85,6 @@ __device__ inline bool item_good(const QuantView& P, const kimkv_decode_item& it
 {
     return item.token_count == tokens && item.descriptors != nullptr && item.descriptor_count != 0 && item.layer < P.layers
         && item.query != nullptr && item.output != nullptr;
-}
-
-// ---- codes to fp16 -----------------------------------------------------------
-
-// Eight codes.  A whole number's byte u under the bits of 1024 is 1024 + u, and
-// 1152 less is the number, exactly.
-template <uint32_t kFormat>
-__device__ inline half8_t code_halves(u32x2_t w)
-{
-    half8_t out;
-#pragma unroll
-    for (uint32_t j = 0; j < 2; ++j) {
-        half2_t a, b;
-        if (kFormat == KIMKV_QUANT_INT8) {
-            half2_t const shift = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
-            a = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[j], 0x04010400u)) + shift;
-            b = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[j], 0x04030402u)) + shift;
-        } else {
-            a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w[j]), 1.0f, false);
-            b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w[j]), 1.0f, true);
-        }
-        out[4 * j] = a[0];
-        out[4 * j + 1] = a[1];
-        out[4 * j + 2] = b[0];
-        out[4 * j + 3] = b[1];
-    }
-    return out;
 }
 
 // Codes are read once a launch: streamed past the caches.

@@ -7,6 +7,7 @@
 #include <limits>
 #include <mutex>
 #include <new>
+#include <type_traits>
 
 #include "quant_common.h"
 #include "runtime_internal.h"
@@ -16,9 +17,12 @@ namespace {
 
 constexpr unsigned kBlock = 256;
 constexpr uint32_t kTileTokens = kQuantMaxPage;
+constexpr uint32_t kGatherAtOnce = 2;
+constexpr uint32_t kAtOnce = 4;   // loads of a thread in flight
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
 // Bytes (r, c) of four words, byte c of word r, as four words, byte r of word c.
 __device__ inline void transpose_bytes(uint32_t (&w)[4])
@@ -35,16 +39,16 @@ __device__ inline void transpose_bytes(uint32_t (&w)[4])
 
 __device__ inline float half_value(uint16_t bits) { return __half2float(__ushort_as_half(bits)); }
 
-// Threads of a row, each with 8 dims: the power of two that covers D.
-inline uint32_t row_lanes_log2(uint32_t D)
+// Of the power of two that covers n: threads of a row of n pieces, for one.
+inline uint32_t log2_of(uint32_t n)
 {
     uint32_t log2 = 0;
-    while ((8u << log2) < D) ++log2;
+    while ((1u << log2) < n) ++log2;
     return log2;
 }
 
 struct AppendGrid {
-    uint32_t heads;        // of a block
+    uint32_t heads_log2;   // of a block
     uint32_t lanes_log2;   // of a row
 };
 
@@ -103,18 +107,32 @@ __device__ inline u32x4_t load_piece(const uint16_t* row, uint32_t p, uint32_t D
     return w;
 }
 
+// The largest of the lanes of a row, 2^log2 neighbours.
+__device__ inline uint32_t row_largest(uint32_t v, uint32_t lanes)
+{
+    auto const turned = [&](auto control) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(control)::value, 0xF, 0xF, false));
+    };
+    if (lanes > 1) v = max(v, turned(std::integral_constant<int, 0xB1>{}));    // the neighbour
+    if (lanes > 2) v = max(v, turned(std::integral_constant<int, 0x4E>{}));    // the pair beside
+    if (lanes > 4) v = max(v, turned(std::integral_constant<int, 0x141>{}));   // eight, turned round
+    if (lanes > 8) v = max(v, turned(std::integral_constant<int, 0x140>{}));   // sixteen
+    if (lanes > 16) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)));
+    return v;
+}
+
 // Codes of a piece, and the row's scale; the row's other pieces are in the
 // other threads of its group.
 template <uint32_t kFormat>
 __device__ inline u32x2_t quantise_piece(u32x4_t w, uint32_t lanes, uint16_t* scale)
 {
-    uint32_t most = 0;   // two fp16 numbers without sign, ordered as whole numbers
+    u16x2_t top = {0, 0};   // two fp16 numbers without sign, ordered as whole numbers
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
-        most = max(most, max(w[j] & 0x7FFFu, (w[j] >> 16) & 0x7FFFu));
+        uint32_t const pair = w[j] & 0x7FFF7FFFu;
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, pair));
     }
-    for (uint32_t m = 1; m < lanes; m *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), static_cast<int>(m))));
-    *scale = row_scale<kFormat>(most);
+    *scale = row_scale<kFormat>(row_largest(top[0] > top[1] ? top[0] : top[1], lanes));
     RowQuant const r = row_quant(*scale);
     u32x2_t codes;
 #pragma unroll
@@ -123,6 +141,7 @@ __device__ inline u32x2_t quantise_piece(u32x4_t w, uint32_t lanes, uint16_t* sc
                             half_value(static_cast<uint16_t>(w[2 * j + 1])), half_value(static_cast<uint16_t>(w[2 * j + 1] >> 16))};
         codes[j] = row_codes<kFormat>(x, r);
     }
+    if (__ballot(*scale == kScaleNan) != 0 && *scale == kScaleNan) codes = u32x2_t{no_codes<kFormat>(), no_codes<kFormat>()};
     return codes;
 }
 
@@ -135,14 +154,15 @@ __device__ inline void store_key_piece(uint8_t* at, u32x2_t codes, uint32_t p, u
     }
 }
 
-template <uint32_t kFormat>
+// kDim 0: any head dim.
+template <uint32_t kFormat, uint32_t kDim>
 __global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const kimkv_append_job* jobs, AppendGrid g)
 {
-    __shared__ alignas(16) uint8_t tile[kTileTokens * (kQuantMaxDim + 4)];   // V codes of a head, rows of D + 4 bytes
+    __shared__ alignas(16) uint8_t tile[kTileTokens * (kQuantMaxDim + 4)];   // V codes of the heads' tokens
     kimkv_append_job const job = jobs[blockIdx.x];
     if (blockIdx.y >= job.layer_count) return;   // a shorter job of a launch sized for the longest
     uint32_t const layer = job.layer_begin + blockIdx.y;
-    uint32_t const D = P.dim;
+    uint32_t const D = kDim != 0 ? kDim : P.dim;
     uint32_t const n = job.token_count;
     uint32_t const dcap = quant_page_tokens(P, job.dst_kind);
     uint32_t const scap = quant_page_tokens(P, job.cow_kind);
@@ -155,8 +175,8 @@ __global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const
         return;
     }
     uint32_t const tid = threadIdx.x;
-    uint32_t const h0 = blockIdx.z * g.heads;
-    uint32_t const h1 = min(h0 + g.heads, P.heads);
+    uint32_t const h0 = blockIdx.z << g.heads_log2;
+    uint32_t const h1 = min(h0 + (1u << g.heads_log2), P.heads);
 
     // The copied positions lie below the written ones: neither waits for the other.
     for (uint32_t h = h0; job.cow_tokens != 0 && h < h1; ++h) {
@@ -170,14 +190,15 @@ __global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const
     const uint16_t* const sv = job.src_value + layer_off;
     uint64_t const stride = job.src_token_stride;
     bool const aligned = ((D | stride) & 7u) == 0 && ((reinterpret_cast<uintptr_t>(sk) | reinterpret_cast<uintptr_t>(sv)) & 15u) == 0;
-    uint32_t const lanes = 1u << g.lanes_log2;
+    uint32_t const lanes_log2 = kDim == 64 ? 3 : kDim == 128 ? 4 : g.lanes_log2;
+    uint32_t const lanes = 1u << lanes_log2;
     uint32_t const p = tid & (lanes - 1);          // piece of the row
-    uint32_t const first = tid >> g.lanes_log2;
-    uint32_t const step = kBlock >> g.lanes_log2;
+    uint32_t const first = tid >> lanes_log2;
+    uint32_t const step = kBlock >> lanes_log2;
     bool const mine = 8 * p < D;
     uint32_t const t0 = job.dst_token;
 
-    if (n < 8) {
+    if (n < 8 || (kDim != 0 && !aligned)) {
         // A token step: K and V rows of all heads at once, V byte by byte.
         uint32_t const rows = 2 * n * (h1 - h0);
         for (uint32_t base = 0; base < rows; base += step) {
@@ -207,28 +228,40 @@ __global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const
         return;
     }
 
-    uint32_t const pitch = D + 4;
+    // Rows of all the block's heads, a token's side by side as they are in the source.
+    uint32_t const heads = h1 - h0;
+    uint32_t const pitch = (D << g.heads_log2) + 4;   // heads of a block: at most kQuantMaxDim dims
     uint32_t const g0 = t0 / 8;                       // groups of 8 page tokens that the job touches
     uint32_t const groups = (t0 + n + 7) / 8 - g0;
-    for (uint32_t h = h0; h < h1; ++h) {
-        uint8_t* const codes_at = quant_codes(dst, P, dcap, h);
-        uint16_t* const scales_at = quant_scales(dst, P, dcap, h);
-        for (uint32_t base = 0; base < 2 * n; base += step) {
-            uint32_t const i = base + first;
-            bool const there = i < 2 * n && mine;
-            bool const value = i >= n;
-            uint32_t const t = value ? i - n : i;
-            u32x4_t w = {};
-            if (there) w = load_piece((value ? sv : sk) + t * stride + static_cast<uint64_t>(h) * D, p, D, aligned);
+    uint32_t const rows = (2 * n) << g.heads_log2;
+    for (uint32_t base = 0; base < rows; base += kAtOnce * step) {
+        u32x4_t w[kAtOnce];
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            uint32_t const i = base + first + k * step;
+            uint32_t const h = i & ((1u << g.heads_log2) - 1);
+            uint32_t const t = i >> g.heads_log2;
+            w[k] = u32x4_t{};
+            if (t >= 2 * n || h >= heads || !mine) continue;
+            const uint16_t* const row = (t >= n ? sv + (t - n) * stride : sk + t * stride) + (h0 + h) * D;
+            w[k] = kDim != 0 ? *reinterpret_cast<const u32x4_t*>(row + 8 * p) : load_piece(row, p, D, aligned);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            if (base + k * step >= rows) break;
+            uint32_t const i = base + first + k * step;
+            uint32_t const h = i & ((1u << g.heads_log2) - 1);
+            bool const value = i >> g.heads_log2 >= n;
+            uint32_t const t = (i >> g.heads_log2) - (value ? n : 0);
             uint16_t scale;
-            u32x2_t const codes = quantise_piece<kFormat>(w, lanes, &scale);
-            if (!there) continue;
-            if (p == 0) scales_at[(value ? dcap : 0) + t0 + t] = scale;
+            u32x2_t const codes = quantise_piece<kFormat>(w[k], lanes, &scale);
+            if (t >= n || h >= heads || !mine) continue;
+            if (p == 0) quant_scales(dst, P, dcap, h0 + h)[(value ? dcap : 0) + t0 + t] = scale;
             if (!value) {
-                store_key_piece(codes_at + quant_k_at(dcap, D, t0 + t, 8 * p), codes, p, D);
+                store_key_piece(quant_codes(dst, P, dcap, h0 + h) + quant_k_at(dcap, D, t0 + t, 8 * p), codes, p, D);
             } else {
                 // Row t0 % 8 + t of the tile, so that its groups of 8 are the page's.
-                uint8_t* const row = tile + ((t0 & 7u) + t) * pitch + 8 * p;
+                uint8_t* const row = tile + ((t0 & 7u) + t) * pitch + h * D + 8 * p;
                 if (D % 8u == 0) {
                     reinterpret_cast<uint32_t*>(row)[0] = codes[0];
                     reinterpret_cast<uint32_t*>(row)[1] = codes[1];
@@ -237,44 +270,46 @@ __global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const
                 }
             }
         }
-        __syncthreads();
-        auto const row_of = [&](uint32_t gi, uint32_t j) { return tile + (8 * gi + j) * pitch; };
-        if (D % 8u == 0) {
-            for (uint32_t i = tid; i < groups * (D / 4); i += kBlock) {
-                uint32_t const q = i / groups;
-                uint32_t const gi = i - q * groups;
-                uint32_t const t = 8 * (g0 + gi);
-                uint32_t lo[4], hi[4];
+    }
+    __syncthreads();
+    auto const row_of = [&](uint32_t gi, uint32_t j) { return tile + (8 * gi + j) * pitch; };
+    if (D % 8u == 0) {
+        for (uint32_t i = tid; i < groups * heads * (D / 4); i += kBlock) {
+            uint32_t const q = i / groups;
+            uint32_t const gi = i - q * groups;
+            uint32_t const h = 4 * q / D;
+            uint32_t const t = 8 * (g0 + gi);
+            uint32_t lo[4], hi[4];
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    lo[j] = *reinterpret_cast<const uint32_t*>(row_of(gi, j) + 4 * q);
-                    hi[j] = *reinterpret_cast<const uint32_t*>(row_of(gi, j + 4) + 4 * q);
-                }
-                transpose_bytes(lo);
-                transpose_bytes(hi);
-                bool const whole = t >= t0 && t + 8 <= t0 + n;
+            for (uint32_t j = 0; j < 4; ++j) {
+                lo[j] = *reinterpret_cast<const uint32_t*>(row_of(gi, j) + 4 * q);
+                hi[j] = *reinterpret_cast<const uint32_t*>(row_of(gi, j + 4) + 4 * q);
+            }
+            transpose_bytes(lo);
+            transpose_bytes(hi);
+            bool const whole = t >= t0 && t + 8 <= t0 + n;
+            uint8_t* const codes_at = quant_codes(dst, P, dcap, h0 + h) + quant_v_at(dcap, D, t, 4 * q - h * D);
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
-                    uint8_t* const at = codes_at + quant_v_at(dcap, D, t, 4 * q + k);
-                    if (whole) {
-                        *reinterpret_cast<u32x2_t*>(at) = u32x2_t{lo[k], hi[k]};
-                    } else {
+            for (uint32_t k = 0; k < 4; ++k) {
+                uint8_t* const at = codes_at + k * dcap;
+                if (whole) {
+                    *reinterpret_cast<u32x2_t*>(at) = u32x2_t{lo[k], hi[k]};
+                } else {
 #pragma unroll
-                        for (uint32_t j = 0; j < 8; ++j) {
-                            uint32_t const word = j < 4 ? lo[k] : hi[k];
-                            if (t + j >= t0 && t + j < t0 + n) at[j] = static_cast<uint8_t>(word >> (8 * (j & 3)));
-                        }
+                    for (uint32_t j = 0; j < 8; ++j) {
+                        uint32_t const word = j < 4 ? lo[k] : hi[k];
+                        if (t + j >= t0 && t + j < t0 + n) at[j] = static_cast<uint8_t>(word >> (8 * (j & 3)));
                     }
                 }
             }
-        } else {
-            for (uint32_t i = tid; i < n * D; i += kBlock) {
-                uint32_t const d = i / n;
-                uint32_t const t = i - d * n;
-                codes_at[quant_v_at(dcap, D, t0 + t, d)] = tile[((t0 & 7u) + t) * pitch + d];
-            }
         }
-        __syncthreads();
+    } else {
+        for (uint32_t i = tid; i < n * heads * D; i += kBlock) {
+            uint32_t const d = i / n;
+            uint32_t const t = i - d * n;
+            uint32_t const h = d / D;
+            quant_codes(dst, P, dcap, h0 + h)[quant_v_at(dcap, D, t0 + t, d - h * D)] = tile[((t0 & 7u) + t) * pitch + d];
+        }
     }
 }
 
@@ -287,14 +322,15 @@ struct GatherArgs {
     uint32_t first;        // token
     uint32_t count;
     uint32_t layer_begin;
-    uint32_t heads;        // of a block
+    uint32_t heads;        // of a block: at most kQuantMaxDim dims
     bool wide;             // rows of 16-byte pieces
 };
 
-template <uint32_t kFormat>
+// kDim 0: any head dim.
+template <uint32_t kFormat, uint32_t kDim>
 __global__ __launch_bounds__(kBlock) void quant_gather_kernel(QuantView P, GatherArgs a)
 {
-    __shared__ uint32_t tile[kQuantMaxDim * (kTileTokens / 4 + 1)];   // V codes of a head, rows of 17 words
+    __shared__ uint32_t tile[kQuantMaxDim * (kTileTokens / 4 + 1)];   // V codes of the heads' dims, rows of 17 words
     kimkv_block_desc const e = a.descriptors[blockIdx.x];
     uint64_t const begin = e.logical_token_begin;
     uint64_t const last = static_cast<uint64_t>(a.first) + a.count;
@@ -307,7 +343,7 @@ __global__ __launch_bounds__(kBlock) void quant_gather_kernel(QuantView P, Gathe
         return;
     }
     uint32_t const tid = threadIdx.x;
-    uint32_t const D = P.dim;
+    uint32_t const D = kDim != 0 ? kDim : P.dim;
     uint32_t const HD = P.heads * D;
     // Page tokens [p0, p1), token p0 of which is row `to` of the output.
     uint32_t const p0 = begin < a.first ? static_cast<uint32_t>(a.first - begin) : 0;
@@ -318,10 +354,10 @@ __global__ __launch_bounds__(kBlock) void quant_gather_kernel(QuantView P, Gathe
     uint16_t* const value_out = key_out + static_cast<uint64_t>(a.count) * HD;
     uint32_t const h0 = blockIdx.z * a.heads;
     uint32_t const h1 = min(h0 + a.heads, P.heads);
-    for (uint32_t h = h0; h < h1; ++h) {
-        const uint8_t* const codes = quant_codes(block, P, cap, h);
-        const uint16_t* const scales = quant_scales(block, P, cap, h);
-        if (!a.wide) {
+    if (!a.wide) {
+        for (uint32_t h = h0; h < h1; ++h) {
+            const uint8_t* const codes = quant_codes(block, P, cap, h);
+            const uint16_t* const scales = quant_scales(block, P, cap, h);
             for (uint32_t i = tid; i < n * D; i += kBlock) {
                 uint32_t const t = i / D;
                 uint32_t const d = i - t * D;
@@ -329,65 +365,79 @@ __global__ __launch_bounds__(kBlock) void quant_gather_kernel(QuantView P, Gathe
                 key_out[o] = read_back(code_value<kFormat>(codes[quant_k_at(cap, D, p0 + t, d)]), scale_value(scales[p0 + t]));
                 value_out[o] = read_back(code_value<kFormat>(codes[quant_v_at(cap, D, p0 + t, d)]), scale_value(scales[cap + p0 + t]));
             }
-            continue;
         }
-        uint32_t const words = cap / 4;   // of a row of V codes
-        for (uint32_t i = tid; i < D * cap / 8; i += kBlock) {
-            u32x2_t const v = *reinterpret_cast<const u32x2_t*>(codes + cap * D + 8 * i);
-            uint32_t const d = 2 * i / words;
-            uint32_t* const row = tile + d * (kTileTokens / 4 + 1) + (2 * i - d * words);
-            row[0] = v[0];
-            row[1] = v[1];
-        }
-        uint32_t const pieces = D / 8;
-        for (uint32_t i = tid; i < n * pieces; i += kBlock) {
-            uint32_t const t = i / pieces;
-            uint32_t const d = (i - t * pieces) * 8;
-            u32x2_t const w = *reinterpret_cast<const u32x2_t*>(codes + quant_k_at(cap, D, p0 + t, d));
-            float const s = scale_value(scales[p0 + t]);
-            u32x4_t o;
+        return;
+    }
+    // Tokens' rows of all the block's heads, side by side.  V codes into LDS, K in the meantime.
+    uint32_t const pieces = D / 8;
+    uint32_t const row = (h1 - h0) * pieces;
+    uint32_t const eights = D * cap / 8;   // 8 codes each, of a head's V
+    uint32_t const words = cap / 4;        // of a dim
+    for (uint32_t base = tid; base < (h1 - h0) * eights || base < n * row; base += kGatherAtOnce * kBlock) {
+        u32x2_t v[kGatherAtOnce], k[kGatherAtOnce];
+        uint16_t s[kGatherAtOnce];
 #pragma unroll
-            for (uint32_t j = 0; j < 2; ++j) {
-                float x[4];
-                code_values<kFormat>(w[j], x);
-                o[2 * j] = read_back(x[0], s) | static_cast<uint32_t>(read_back(x[1], s)) << 16;
-                o[2 * j + 1] = read_back(x[2], s) | static_cast<uint32_t>(read_back(x[3], s)) << 16;
-            }
-            *reinterpret_cast<u32x4_t*>(key_out + static_cast<uint64_t>(t) * HD + h * D + d) = o;
+        for (uint32_t j = 0; j < kGatherAtOnce; ++j) {
+            uint32_t const i = base + j * kBlock;
+            if (i >= (h1 - h0) * eights) continue;
+            uint32_t const h = i / eights;
+            v[j] = *reinterpret_cast<const u32x2_t*>(quant_codes(block, P, cap, h0 + h) + cap * D + 8 * (i - h * eights));
         }
-        __syncthreads();
-        // Four tokens by 8 dims a thread.
-        uint32_t const q0 = p0 / 4;
-        uint32_t const quads = (p1 + 3) / 4 - q0;
-        for (uint32_t i = tid; i < quads * pieces; i += kBlock) {
-            uint32_t const q = i / pieces;
-            uint32_t const d = (i - q * pieces) * 8;
-            uint32_t lo[4], hi[4];
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                lo[j] = tile[(d + j) * (kTileTokens / 4 + 1) + q0 + q];
-                hi[j] = tile[(d + 4 + j) * (kTileTokens / 4 + 1) + q0 + q];
-            }
-            transpose_bytes(lo);
-            transpose_bytes(hi);
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-                uint32_t const t = 4 * (q0 + q) + k;
-                if (t < p0 || t >= p1) continue;
-                float const s = scale_value(scales[cap + t]);
-                float x[4], y[4];
-                code_values<kFormat>(lo[k], x);
-                code_values<kFormat>(hi[k], y);
-                u32x4_t const o = {read_back(x[0], s) | static_cast<uint32_t>(read_back(x[1], s)) << 16,
-                                   read_back(x[2], s) | static_cast<uint32_t>(read_back(x[3], s)) << 16,
-                                   read_back(y[0], s) | static_cast<uint32_t>(read_back(y[1], s)) << 16,
-                                   read_back(y[2], s) | static_cast<uint32_t>(read_back(y[3], s)) << 16};
-                *reinterpret_cast<u32x4_t*>(value_out + static_cast<uint64_t>(t - p0) * HD + h * D + d) = o;
-            }
+        for (uint32_t j = 0; j < kGatherAtOnce; ++j) {
+            uint32_t const i = base + j * kBlock;
+            if (i >= n * row) continue;
+            uint32_t const t = i / row;
+            uint32_t const h = (i - t * row) / pieces;
+            uint32_t const piece = i - t * row - h * pieces;
+            k[j] = *reinterpret_cast<const u32x2_t*>(quant_codes(block, P, cap, h0 + h) + quant_k_at(cap, D, p0 + t, 8 * piece));
+            s[j] = quant_scales(block, P, cap, h0 + h)[p0 + t];
         }
-        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < kGatherAtOnce; ++j) {
+            uint32_t const i = base + j * kBlock;
+            if (i >= (h1 - h0) * eights) continue;
+            uint32_t const d = 2 * i / words;   // of all heads
+            uint32_t* const to_row = tile + d * (kTileTokens / 4 + 1) + (2 * i - d * words);
+            to_row[0] = v[j][0];
+            to_row[1] = v[j][1];
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kGatherAtOnce; ++j) {
+            uint32_t const i = base + j * kBlock;
+            if (i >= n * row) continue;
+            uint32_t const t = i / row;
+            *reinterpret_cast<code_halves_t*>(key_out + static_cast<uint64_t>(t) * HD + h0 * D + 8 * (i - t * row)) = read_back<kFormat>(k[j], scale_value(s[j]));
+        }
+    }
+    __syncthreads();
+    // Four tokens by 8 dims a thread.
+    uint32_t const q0 = p0 / 4;
+    uint32_t const quads = (p1 + 3) / 4 - q0;
+    for (uint32_t i = tid; i < quads * row; i += kBlock) {
+        uint32_t const q = i / row;
+        uint32_t const d = (i - q * row) * 8;   // of all heads
+        const uint16_t* const scales = quant_scales(block, P, cap, h0 + d / D) + cap;
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            lo[j] = tile[(d + j) * (kTileTokens / 4 + 1) + q0 + q];
+            hi[j] = tile[(d + 4 + j) * (kTileTokens / 4 + 1) + q0 + q];
+        }
+        transpose_bytes(lo);
+        transpose_bytes(hi);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            uint32_t const t = 4 * (q0 + q) + k;
+            if (t < p0 || t >= p1) continue;
+            *reinterpret_cast<code_halves_t*>(value_out + static_cast<uint64_t>(t - p0) * HD + h0 * D + d) = read_back<kFormat>(u32x2_t{lo[k], hi[k]}, scale_value(scales[t]));
+        }
     }
 }
+
+// Pages that are left and filled: streamed past the caches.
+__device__ inline u32x4_t load_once(const uint8_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
+__device__ inline void store_once(uint8_t* p, u32x4_t v) { *reinterpret_cast<u32x4_t*>(p) = v; }
 
 // ---------------------------------------------------------------------------
 // Promotion: block = (job, layer, some heads).  Eight pages of 8 tokens into
@@ -414,25 +464,74 @@ __global__ __launch_bounds__(kBlock) void quant_promote_kernel(QuantView P, cons
     uint32_t const run = 8 * kw;   // a micro page's column block
     uint32_t const h0 = blockIdx.z * heads;
     uint32_t const h1 = min(h0 + heads, P.heads);
-    for (uint32_t h = h0; h < h1; ++h) {
-        uint8_t* const to = quant_codes(dst, P, 64, h);
-        uint64_t const from = static_cast<uint64_t>(h) * 16 * D;
-        for (uint32_t i = tid; i < 8 * D; i += kBlock) {
-            uint32_t const piece = i / kw;             // 8-byte pieces: (column block, micro page)
-            uint32_t const o = (i - piece * kw) * 8;
-            uint32_t const m = piece & 7u;
-            uint32_t const b = piece >> 3;
-            *reinterpret_cast<u32x2_t*>(to + b * 8 * run + m * run + o) = *reinterpret_cast<const u32x2_t*>(source[m] + from + b * run + o);
-            uint32_t const vm = i & 7u;
-            uint32_t const d = i >> 3;
-            *reinterpret_cast<u32x2_t*>(to + 64 * D + d * 64 + vm * 8) = *reinterpret_cast<const u32x2_t*>(source[vm] + from + 8 * D + d * 8);
+    if (D % 2u == 0) {
+        // 16 bytes at a time: of K a run's; of V two dims of two pages, which are two dims' of the page.
+        uint32_t const pieces = D * 4;   // of a head's K; half as many of its V
+        for (uint32_t base = tid; base < (h1 - h0) * pieces; base += kAtOnce * kBlock) {
+            u32x4_t w[kAtOnce];
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k) {
+                uint32_t const i = base + k * kBlock;
+                if (i >= (h1 - h0) * pieces) continue;
+                uint32_t const h = i / pieces;
+                uint32_t const at = (i - h * pieces) * 16;
+                uint32_t const b = at / (8 * run);
+                uint32_t const m = at / run & 7u;
+                w[k] = load_once(source[m] + static_cast<uint64_t>(h0 + h) * 16 * D + b * run + (at - (8 * b + m) * run));
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k) {
+                uint32_t const i = base + k * kBlock;
+                if (i >= (h1 - h0) * pieces) continue;
+                uint32_t const h = i / pieces;
+                store_once(quant_codes(dst, P, 64, h0 + h) + (i - h * pieces) * 16, w[k]);
+            }
         }
-        if (tid < 128) {
-            uint32_t const m = (tid >> 3) & 7u;
-            uint32_t const value = tid >> 6;
-            const uint16_t* const s = reinterpret_cast<const uint16_t*>(source[m] + static_cast<uint64_t>(P.heads) * 16 * D) + h * 16;
-            quant_scales(dst, P, 64, h)[tid] = s[value * 8 + (tid & 7u)];
+        for (uint32_t base = tid; base < (h1 - h0) * pieces / 2; base += kAtOnce / 2 * kBlock) {
+            u32x4_t w[kAtOnce / 2][2];
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce / 2; ++k) {
+                uint32_t const i = base + k * kBlock;
+                if (i >= (h1 - h0) * pieces / 2) continue;
+                uint32_t const h = i / (pieces / 2);
+                uint32_t const m = 2 * (i & 3u);
+                uint32_t const d = (i - h * (pieces / 2)) / 4 * 2;
+                uint64_t const at = static_cast<uint64_t>(h0 + h) * 16 * D + 8 * D + d * 8;
+                w[k][0] = load_once(source[m] + at);
+                w[k][1] = load_once(source[m + 1] + at);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce / 2; ++k) {
+                uint32_t const i = base + k * kBlock;
+                if (i >= (h1 - h0) * pieces / 2) continue;
+                uint32_t const h = i / (pieces / 2);
+                uint32_t const d = (i - h * (pieces / 2)) / 4 * 2;
+                uint8_t* const to = quant_codes(dst, P, 64, h0 + h) + 64 * D + d * 64 + 16 * (i & 3u);
+                store_once(to, u32x4_t{w[k][0][0], w[k][0][1], w[k][1][0], w[k][1][1]});
+                store_once(to + 64, u32x4_t{w[k][0][2], w[k][0][3], w[k][1][2], w[k][1][3]});
+            }
         }
+    } else {
+        for (uint32_t h = h0; h < h1; ++h) {
+            uint8_t* const to = quant_codes(dst, P, 64, h);
+            uint64_t const from = static_cast<uint64_t>(h) * 16 * D;
+            for (uint32_t i = tid; i < 8 * D; i += kBlock) {   // of 8 bytes
+                uint32_t const m = i / D;
+                uint32_t const o = (i - m * D) * 8;
+                *reinterpret_cast<u32x2_t*>(to + m * run + o) = *reinterpret_cast<const u32x2_t*>(source[m] + from + o);
+                uint32_t const vm = i & 7u;
+                uint32_t const d = i >> 3;
+                *reinterpret_cast<u32x2_t*>(to + 64 * D + d * 64 + vm * 8) = *reinterpret_cast<const u32x2_t*>(source[vm] + from + 8 * D + d * 8);
+            }
+        }
+    }
+    // The scales: of a head, 8 of K and 8 of V a page.
+    for (uint32_t i = tid; i < (h1 - h0) * 128; i += kBlock) {
+        uint32_t const h = h0 + i / 128;
+        uint32_t const m = (i >> 3) & 7u;
+        uint32_t const value = (i >> 6) & 1u;
+        const uint16_t* const s = reinterpret_cast<const uint16_t*>(source[m] + static_cast<uint64_t>(P.heads) * 16 * D) + h * 16;
+        quant_scales(dst, P, 64, h)[i & 127u] = s[value * 8 + (i & 7u)];
     }
 }
 
@@ -442,13 +541,31 @@ __global__ __launch_bounds__(64) void quant_take_faults_kernel(uint32_t* faults,
     if (threadIdx.x == 0) *host_word = atomicExch(faults, 0u);
 }
 
-// Heads a block takes: all of them where the rest of the grid fills the chip,
-// fewer where it does not.
-uint32_t heads_of_block(uint32_t heads, uint64_t blocks)
+// Heads a block takes, a power of two: about kQuantMaxDim dims (8 heads of 128:
+// 12 layers of 16384 tokens appended and read back in 265 us, 2 of them 244),
+// fewer where the rest of the grid does not fill the chip.
+uint32_t heads_of_block(uint32_t heads, uint32_t dim, uint64_t blocks)
 {
-    uint32_t per = heads;
-    while (per > 1 && blocks * ceil_div(heads, per) < 1024) per = (per + 1) / 2;
+    uint32_t per = 1;
+    while (per < heads && 2 * per * dim <= kQuantMaxDim) per *= 2;
+    while (per > 1 && blocks * ceil_div(heads, per) < 1024) per /= 2;
     return per;
+}
+
+// f(format, head dim) of a storage; the dims whose index arithmetic is fixed
+// where the code is built, 0 for all others.
+template <typename F>
+auto with_format(const kimkv_quant_storage& s, F f)
+{
+    auto const with_dim = [&](auto format) {
+        switch (s.layout.head_dim) {
+        case 64: return f(format, std::integral_constant<uint32_t, 64>{});
+        case 128: return f(format, std::integral_constant<uint32_t, 128>{});
+        default: return f(format, std::integral_constant<uint32_t, 0>{});
+        }
+    };
+    return s.format == KIMKV_QUANT_INT8 ? with_dim(std::integral_constant<uint32_t, KIMKV_QUANT_INT8>{})
+                                        : with_dim(std::integral_constant<uint32_t, KIMKV_QUANT_E4M3>{});
 }
 
 bool on_device(const kimkv_quant_storage* s)
@@ -580,13 +697,13 @@ kimkv_status kimkv_quant_append_batch(const kimkv_quant_storage* storage, const 
     }
     if (job_count == 0 || max_layer_count == 0) return KIMKV_OK;
     QuantView const view = quant_view(*storage);
-    uint32_t const heads = heads_of_block(view.heads, static_cast<uint64_t>(job_count) * max_layer_count);
+    uint32_t const heads = heads_of_block(view.heads, view.dim, static_cast<uint64_t>(job_count) * max_layer_count);
     uint32_t const z = ceil_div(view.heads, heads);
     uint32_t const most = kGridBlocks / (max_layer_count * z) == 0 ? 1 : kGridBlocks / (max_layer_count * z);
-    auto const kernel = storage->format == KIMKV_QUANT_INT8 ? quant_append_kernel<KIMKV_QUANT_INT8> : quant_append_kernel<KIMKV_QUANT_E4M3>;
+    auto const kernel = with_format(*storage, [](auto format, auto dim) { return quant_append_kernel<format.value, dim.value>; });
     for (uint32_t first = 0; first < job_count;) {
         uint32_t const jobs = job_count - first < most ? job_count - first : most;
-        kernel<<<dim3(jobs, max_layer_count, z), kBlock, 0, native(stream)>>>(view, device_jobs + first, AppendGrid{heads, row_lanes_log2(view.dim)});
+        kernel<<<dim3(jobs, max_layer_count, z), kBlock, 0, native(stream)>>>(view, device_jobs + first, AppendGrid{log2_of(heads), log2_of(ceil_div(view.dim, 8))});
         kimkv_status const status = launch_status();
         if (status != KIMKV_OK) return status;
         first += jobs;
@@ -605,11 +722,11 @@ kimkv_status kimkv_quant_gather(const kimkv_quant_storage* storage, const kimkv_
     if (token_count == 0 || layer_count == 0) return KIMKV_OK;
     if (device_descriptors == nullptr || descriptor_count == 0 || device_output == nullptr) return KIMKV_INVALID_ARGUMENT;
     QuantView const view = quant_view(*storage);
-    uint32_t const heads = heads_of_block(view.heads, static_cast<uint64_t>(descriptor_count) * layer_count);
+    uint32_t const heads = heads_of_block(view.heads, view.dim, static_cast<uint64_t>(descriptor_count) * layer_count);
     uint32_t const z = ceil_div(view.heads, heads);
     uint32_t const most = kGridBlocks / (layer_count * z) == 0 ? 1 : kGridBlocks / (layer_count * z);
     bool const wide = view.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(device_output) & 15u) == 0;
-    auto const kernel = storage->format == KIMKV_QUANT_INT8 ? quant_gather_kernel<KIMKV_QUANT_INT8> : quant_gather_kernel<KIMKV_QUANT_E4M3>;
+    auto const kernel = with_format(*storage, [](auto format, auto dim) { return quant_gather_kernel<format.value, dim.value>; });
     for (uint32_t first = 0; first < descriptor_count;) {
         uint32_t const entries = descriptor_count - first < most ? descriptor_count - first : most;
         GatherArgs const args{device_descriptors + first, device_output, first_token, token_count, layer_begin, heads, wide};
@@ -630,7 +747,7 @@ kimkv_status kimkv_quant_promote_batch(const kimkv_quant_storage* storage, const
     }
     if (job_count == 0) return KIMKV_OK;
     QuantView const view = quant_view(*storage);
-    uint32_t const heads = heads_of_block(view.heads, static_cast<uint64_t>(job_count) * view.layers);
+    uint32_t const heads = heads_of_block(view.heads, view.dim, static_cast<uint64_t>(job_count) * view.layers);
     uint32_t const z = ceil_div(view.heads, heads);
     uint32_t const most = kGridBlocks / (view.layers * z) == 0 ? 1 : kGridBlocks / (view.layers * z);
     for (uint32_t first = 0; first < job_count;) {
