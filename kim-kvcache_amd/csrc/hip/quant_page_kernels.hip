@@ -53,7 +53,11 @@ struct AppendGrid {
 };
 
 // ---------------------------------------------------------------------------
-// Append: block = (job, layer, some heads).
+// Append: block = (job, layer, some heads).  A job of fewer than 8 tokens, or
+// of rows off 16 bytes, writes V byte by byte; others turn V's codes in LDS.
+// Bound by HBM where jobs are many, with operations close behind (113 a piece of
+// 8 values kept the units busy for 0.56 of 130 us), so divisions, fallbacks and
+// index arithmetic are kept out of the way; a step of 128 lanes is its launch.
 // ---------------------------------------------------------------------------
 // Tokens [0, n) of one head of a page's block copied to another page, byte for
 // byte: the codes and the scales of each.  Only those tokens' bytes are stored:
@@ -106,6 +110,12 @@ __device__ inline u32x4_t load_piece(const uint16_t* row, uint32_t p, uint32_t D
     }
     return w;
 }
+
+// Of what is read once, lines at a time: past the caches.  Appended rows and V's
+// codes so, and read-back rows written so: 6 layers of 4 x 4096 tokens, 8 heads of
+// 128, appended and read back in 186 us, 6.0 TB/s, not 246.  With K's codes so too,
+// 199: a wave reads them in pieces of 64 bytes.
+__device__ inline u32x4_t load_once(const void* p) { return __builtin_nontemporal_load(static_cast<const u32x4_t*>(p)); }
 
 // The largest of the lanes of a row, 2^log2 neighbours.
 __device__ inline uint32_t row_largest(uint32_t v, uint32_t lanes)
@@ -244,7 +254,7 @@ __global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const
             w[k] = u32x4_t{};
             if (t >= 2 * n || h >= heads || !mine) continue;
             const uint16_t* const row = (t >= n ? sv + (t - n) * stride : sk + t * stride) + (h0 + h) * D;
-            w[k] = kDim != 0 ? *reinterpret_cast<const u32x4_t*>(row + 8 * p) : load_piece(row, p, D, aligned);
+            w[k] = kDim != 0 ? load_once(row + 8 * p) : load_piece(row, p, D, aligned);
         }
 #pragma unroll
         for (uint32_t k = 0; k < kAtOnce; ++k) {
@@ -314,7 +324,10 @@ __global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const
 }
 
 // ---------------------------------------------------------------------------
-// Read-back: block = (table entry, layer, some heads).
+// Read-back: block = (table entry, layer, some heads).  V's codes are turned in
+// LDS, and rows of up to 256 dims written whole: head after head, 22 layers of
+// 16384 tokens of 4 heads of 64 took 123 us with rows through the caches and 137
+// a head at a time; 101 us now, 5.5 TB/s.
 // ---------------------------------------------------------------------------
 struct GatherArgs {
     const kimkv_block_desc* descriptors;
@@ -325,6 +338,9 @@ struct GatherArgs {
     uint32_t heads;        // of a block: at most kQuantMaxDim dims
     bool wide;             // rows of 16-byte pieces
 };
+
+// Rows that are written once and whole, past the caches.
+__device__ inline void store_row(uint16_t* at, code_halves_t v) { __builtin_nontemporal_store(v, reinterpret_cast<code_halves_t*>(at)); }
 
 // kDim 0: any head dim.
 template <uint32_t kFormat, uint32_t kDim>
@@ -381,7 +397,7 @@ __global__ __launch_bounds__(kBlock) void quant_gather_kernel(QuantView P, Gathe
             uint32_t const i = base + j * kBlock;
             if (i >= (h1 - h0) * eights) continue;
             uint32_t const h = i / eights;
-            v[j] = *reinterpret_cast<const u32x2_t*>(quant_codes(block, P, cap, h0 + h) + cap * D + 8 * (i - h * eights));
+            v[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(quant_codes(block, P, cap, h0 + h) + cap * D + 8 * (i - h * eights)));
         }
 #pragma unroll
         for (uint32_t j = 0; j < kGatherAtOnce; ++j) {
@@ -407,7 +423,7 @@ __global__ __launch_bounds__(kBlock) void quant_gather_kernel(QuantView P, Gathe
             uint32_t const i = base + j * kBlock;
             if (i >= n * row) continue;
             uint32_t const t = i / row;
-            *reinterpret_cast<code_halves_t*>(key_out + static_cast<uint64_t>(t) * HD + h0 * D + 8 * (i - t * row)) = read_back<kFormat>(k[j], scale_value(s[j]));
+            store_row(key_out + static_cast<uint64_t>(t) * HD + h0 * D + 8 * (i - t * row), read_back<kFormat>(k[j], scale_value(s[j])));
         }
     }
     __syncthreads();
@@ -430,19 +446,16 @@ __global__ __launch_bounds__(kBlock) void quant_gather_kernel(QuantView P, Gathe
         for (uint32_t k = 0; k < 4; ++k) {
             uint32_t const t = 4 * (q0 + q) + k;
             if (t < p0 || t >= p1) continue;
-            *reinterpret_cast<code_halves_t*>(value_out + static_cast<uint64_t>(t - p0) * HD + h0 * D + d) = read_back<kFormat>(u32x2_t{lo[k], hi[k]}, scale_value(scales[t]));
+            store_row(value_out + static_cast<uint64_t>(t - p0) * HD + h0 * D + d, read_back<kFormat>(u32x2_t{lo[k], hi[k]}, scale_value(scales[t])));
         }
     }
 }
 
-// Pages that are left and filled: streamed past the caches.
-__device__ inline u32x4_t load_once(const uint8_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
-__device__ inline void store_once(uint8_t* p, u32x4_t v) { *reinterpret_cast<u32x4_t*>(p) = v; }
-
 // ---------------------------------------------------------------------------
 // Promotion: block = (job, layer, some heads).  Eight pages of 8 tokens into
 // one of 64: K in runs of 8 tokens of a column block, V and the scales in
-// pieces of 8 tokens.
+// pieces of 8 tokens.  512 jobs in 22 layers (1.5 GB moved) and their read-back
+// (1.1 GB) take 336 us; in pieces of 8 bytes 391 with the read-back of then.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kBlock) void quant_promote_kernel(QuantView P, const kimkv_promotion_job* jobs, uint32_t heads)
 {
@@ -484,7 +497,7 @@ __global__ __launch_bounds__(kBlock) void quant_promote_kernel(QuantView P, cons
                 uint32_t const i = base + k * kBlock;
                 if (i >= (h1 - h0) * pieces) continue;
                 uint32_t const h = i / pieces;
-                store_once(quant_codes(dst, P, 64, h0 + h) + (i - h * pieces) * 16, w[k]);
+                *reinterpret_cast<u32x4_t*>(quant_codes(dst, P, 64, h0 + h) + (i - h * pieces) * 16) = w[k];
             }
         }
         for (uint32_t base = tid; base < (h1 - h0) * pieces / 2; base += kAtOnce / 2 * kBlock) {
@@ -507,8 +520,8 @@ __global__ __launch_bounds__(kBlock) void quant_promote_kernel(QuantView P, cons
                 uint32_t const h = i / (pieces / 2);
                 uint32_t const d = (i - h * (pieces / 2)) / 4 * 2;
                 uint8_t* const to = quant_codes(dst, P, 64, h0 + h) + 64 * D + d * 64 + 16 * (i & 3u);
-                store_once(to, u32x4_t{w[k][0][0], w[k][0][1], w[k][1][0], w[k][1][1]});
-                store_once(to + 64, u32x4_t{w[k][0][2], w[k][0][3], w[k][1][2], w[k][1][3]});
+                *reinterpret_cast<u32x4_t*>(to) = u32x4_t{w[k][0][0], w[k][0][1], w[k][1][0], w[k][1][1]};
+                *reinterpret_cast<u32x4_t*>(to + 64) = u32x4_t{w[k][0][2], w[k][0][3], w[k][1][2], w[k][1][3]};
             }
         }
     } else {
