@@ -24,14 +24,17 @@
 //     vocabulary, the range that the random number falls into, the token in it.
 //
 // Bound by the instructions of one block's waves: a weight is 26 of them, and a
-// pass of weights over 32000 tokens 7 us, where reading the row takes 1 us.  So a
-// list saves passes: 72 rows of 50255 with top_k 50 take 17 us (20 us where the
-// list came from a second pass over the row), 256 rows of 128000 36 us (58), which
-// is 3.6 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
-// and these took 17 and 42 us.  Drawn from all the row 28 and 77 us, top-p of 0.9
-// 62 and 160.  Tried and slower: a list for top-p, from the highest columns up
-// (256 flat rows of 128000 184 us, as it falls back there); the sums by ranges in
-// the pass that lists a bin's tokens (128 us for top_k 3000, as it was without).
+// pass of weights over 32000 tokens 11 us, where reading the row takes 2.  So a
+// list saves passes: 72 rows of 50255 with top_k 50 take 16 us (20 us where the
+// list came from a second pass over the row), 256 rows of 128000 34 us (58), which
+// is 3.9 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
+// and these took 17 and 42 us.  Drawn from all the row 28 and 76 us, top-p of 0.9
+// 58 and 140 (62 and 160 while the cut was a function of its own, to which the row
+// and the LDS were addresses of any kind).  Tried and slower for top-p: a list from
+// the highest columns up (256 flat rows of 128000 184 us, as it falls back there);
+// counts and mean places of the bins first, then one pass of weights that sums by
+// ranges and lists the tokens of the bins in question (215 us: a pass of 64-bit
+// additions to LDS takes as long as one with the weights).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -505,7 +508,7 @@ __device__ __attribute__((always_inline)) inline uint64_t sum_ranges(const Row& 
 // The first token at which the running sum exceeds `target`, less than all of
 // it; the ranges' sums are in place.  Its weight in *its.
 template <typename W>
-__device__ uint32_t token_at(const Row& row, SampleLds& lds, uint64_t target, const W& weight, uint64_t* its)
+__device__ __attribute__((always_inline)) inline uint32_t token_at(const Row& row, SampleLds& lds, uint64_t target, const W& weight, uint64_t* its)
 {
     static_assert(kRanges <= kBlock, "a thread a range");
     uint32_t const tid = threadIdx.x;
@@ -557,7 +560,7 @@ __device__ uint32_t token_at(const Row& row, SampleLds& lds, uint64_t target, co
 // Sorts numbers[0, n), all different, into falling order; n at most kListed.
 // Their upper words are keys of logits, or ~tokens, which count as -token;
 // these are at most `highest`, and lie within about `width`.
-__device__ __attribute__((noinline)) void sort_falling(uint64_t* numbers, SampleLds& lds, uint32_t n, bool logits, float highest, float width)
+__device__ __attribute__((always_inline)) inline void sort_falling(uint64_t* numbers, SampleLds& lds, uint32_t n, bool logits, float highest, float width)
 {
     uint32_t const tid = threadIdx.x;
     __syncthreads();
@@ -722,7 +725,7 @@ __device__ inline void clear_bins(SampleLds& lds)
 
 // Where the cut falls; everything is kept where it lies past what is counted.
 // The bins' counts (or weights, for a cut by them) are in lds.
-__device__ __attribute__((noinline)) Last find_cut(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, const Cut& cut)
+__device__ __attribute__((always_inline)) inline Last find_cut(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, const Cut& cut)
 {
     uint32_t const tid = threadIdx.x;
     Place place = place_of(lds, cut, 0);
