@@ -698,37 +698,37 @@ __global__ __launch_bounds__(kBlock) void quant_merge_kernel(QuantView P, const 
     kimkv_decode_item const item = items[x.lane];
     uint32_t const D = P.dim;
     uint32_t const h = blockIdx.y;
-    uint32_t const i = blockIdx.z * kBlock + threadIdx.x;
-    if (i >= G * D) return;
     uint64_t const size = slot_floats(G, D);
-    const float* const values = work + (x.first_slot + static_cast<uint64_t>(h) * x.parts) * size + i;
-    const float* const ml = values - i + static_cast<uint64_t>(G) * D + 2 * (i / D);
-    float m = -INFINITY, total = 0.0f, sum = 0.0f;
-    for (uint32_t p = 0; p < x.parts; p += kAtOnce) {
-        float top[kAtOnce], l[kAtOnce], v[kAtOnce];
+    for (uint32_t i = blockIdx.z * kBlock + threadIdx.x; i < G * D; i += gridDim.z * kBlock) {
+        const float* const values = work + (x.first_slot + static_cast<uint64_t>(h) * x.parts) * size + i;
+        const float* const ml = values - i + static_cast<uint64_t>(G) * D + 2 * (i / D);
+        float m = -INFINITY, total = 0.0f, sum = 0.0f;
+        for (uint32_t p = 0; p < x.parts; p += kAtOnce) {
+            float top[kAtOnce], l[kAtOnce], v[kAtOnce];
 #pragma unroll
-        for (uint32_t k = 0; k < kAtOnce; ++k) {
-            uint64_t const at = min(p + k, x.parts - 1) * size;
-            top[k] = ml[at];
-            l[k] = ml[at + 1];
-            v[k] = values[at];
+            for (uint32_t k = 0; k < kAtOnce; ++k) {
+                uint64_t const at = min(p + k, x.parts - 1) * size;
+                top[k] = ml[at];
+                l[k] = ml[at + 1];
+                v[k] = values[at];
+            }
+            float most = m;
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k) most = fmaxf(most, top[k]);
+            float const f = part_weight(m, most);
+            sum = f != 0.0f ? sum * f : 0.0f;
+            total *= f;
+            m = most;
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k) {
+                float const w = p + k < x.parts ? part_weight(top[k], most) : 0.0f;
+                total += l[k] * w;
+                if (w != 0.0f) sum += v[k] * w;
+            }
         }
-        float most = m;
-#pragma unroll
-        for (uint32_t k = 0; k < kAtOnce; ++k) most = fmaxf(most, top[k]);
-        float const f = part_weight(m, most);
-        sum = f != 0.0f ? sum * f : 0.0f;
-        total *= f;
-        m = most;
-#pragma unroll
-        for (uint32_t k = 0; k < kAtOnce; ++k) {
-            float const w = p + k < x.parts ? part_weight(top[k], most) : 0.0f;
-            total += l[k] * w;
-            if (w != 0.0f) sum += v[k] * w;
-        }
+        // An item that is not as planned is reported by its units, which wrote no parts.
+        if (item_good(P, item, x.tokens)) item.output[static_cast<uint64_t>(h) * G * D + i] = quotient_half(sum, total);
     }
-    // An item that is not as planned is reported by its units, which wrote no parts.
-    if (item_good(P, item, x.tokens)) item.output[static_cast<uint64_t>(h) * G * D + i] = quotient_half(sum, total);
 }
 
 // ---- plan ------------------------------------------------------------------------
@@ -736,6 +736,7 @@ __global__ __launch_bounds__(kBlock) void quant_merge_kernel(QuantView P, const 
 // Parts of a lane of `tiles` tiles when a unit takes at most `most` of them.
 inline uint32_t lane_parts(uint32_t tiles, uint32_t most) { return (tiles + most - 1) / most; }
 
+constexpr uint32_t kGridRows = 65535;       // of a launch's third dimension
 constexpr uint32_t kMostUnits = 0xFFFFFF;   // times kBlock threads: fewer than 2^32
 
 }  // namespace
@@ -859,7 +860,7 @@ kimkv_status kimkv_quant_decode_batch(const kimkv_quant_storage* storage, const 
     kimkv_status const status = launch_status();
     kernel_timing_end(TimedKernel::Decode, native(stream), start);
     if (status != KIMKV_OK || plan->merge_lanes == 0) return status;
-    quant_merge_kernel<<<dim3(plan->merge_lanes, plan->kv_heads, (G * view.dim + kBlock - 1) / kBlock), kBlock, 0, native(stream)>>>(
+    quant_merge_kernel<<<dim3(plan->merge_lanes, plan->kv_heads, std::min((G * view.dim + kBlock - 1) / kBlock, kGridRows)), kBlock, 0, native(stream)>>>(
         view, device_items, reinterpret_cast<const QuantMerge*>(units + plan->unit_count), args.work, G);
     return launch_status();
 }

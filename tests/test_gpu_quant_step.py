@@ -929,3 +929,95 @@ def test_promoted_and_read_back_for_a_prefill(dev):
         size = p @ np.abs(v)
         off = (np.abs(k) @ np.abs(q[j].astype(np.float64))).max() / math.sqrt(dim) * (FP16 + 70 * 2.0 ** -24)
         assert np.all(np.abs(a[j] - b[j]) <= 2 * (FP16 * np.abs(p @ v) + TINY) + size * (FP16 + 2 * off + 2.0 ** -12))
+
+
+# ---- launches and sizes at which kernels take other ways ------------------------
+
+
+@pytest.mark.parametrize("form,heads,dim", [("int8", 3, 64), ("e4m3", 5, 33), ("int8", 3, 96), ("e4m3", 20, 12), ("int8", 5, 40), ("e4m3", 3, 128)])
+def test_pages_of_many_layers(dev, form, heads, dim):
+    """Launches that fill the chip, whose workgroups take several heads, the last ones fewer; appended, read back whole and
+    in part."""
+    print(f"quant pages of many layers {form} H={heads} D={dim}", flush=True)
+    c = _Cache(dev, FORMS[form], heads, dim, layers=128, micro=14, extent=8)
+    kv = _fp16(np.random.default_rng(5), 128, 2, ROWS, heads, dim)
+    buf = dev.upload(_bits(kv))
+    c.storage.append_batch(c.jobs_of(buf.ptr, ROWS, RUNS, COWS))
+    c.expect(kv, RUNS, COWS)
+    c.check()
+    part = c.storage.gather(c.tables[1], 300, first_token=37).view(np.float16).reshape(128, 2, 300, heads, dim)
+    _same(part, read(c.pages[1][:, :, 37:337]))
+    assert c.storage.faults() == (0, 0)
+
+
+@pytest.mark.parametrize("form,heads,dim", [("int8", 3, 64), ("e4m3", 3, 33), ("int8", 5, 12)])
+def test_promote_many_layers(dev, form, heads, dim):
+    print(f"quant_promote many layers {form} H={heads} D={dim}", flush=True)
+    c = _Cache(dev, FORMS[form], heads, dim, layers=512, micro=16, extent=2)
+    jobs = np.zeros(2, dtype=dev.PROMOTION_JOB)
+    order = np.random.default_rng(3).permutation(16)
+    for i in range(2):
+        jobs[i] = (order[8 * i:8 * i + 8], 1 - i)
+        rows = np.concatenate([np.arange(8) + 8 * s for s in order[8 * i:8 * i + 8]])
+        c.pages[1][:, :, 64 * (1 - i):64 * (2 - i)] = c.pages[0][:, :, rows]
+    c.storage.promote_batch(jobs)
+    c.check()
+    assert c.storage.faults() == (0, 0)
+
+
+@pytest.mark.parametrize("form,dim", [("int8", 128), ("e4m3", 128)])
+def test_pages_past_32_bits(dev, form, dim):
+    """Pages that lie more than 2^32 bytes into the storage, small ones behind as many."""
+    print(f"quant pages past 32 bits {form} D={dim}", flush=True)
+    heads, group, micro, extent = 8, 2, 270000, 35000   # 4.5 and 4.6 GB
+    free = [[micro - 1, micro - 7], [extent - 1, 3, extent - 5]]
+    lanes = _Lanes(dev, FORMS[form], heads, dim, group, [_table(205, free)], micro, extent, layers=1, layer=0)
+    lanes.check()
+    rows = lanes.storage.gather(lanes.tables[0], 205).view(np.float16).reshape(2, 205, heads, dim)
+    _same(rows, read(lanes.kv))
+    assert lanes.storage.faults() == (0, 0)
+
+
+LONG_LISTS = [(1.0, 600, 1.0, 0.0), (0.7, 1000, 0.95, 0.0), (1.0, 1024, 0.5, 0.001), (3.0, 1024, 1.0, 0.0), (1.0, 1025, 0.9, 0.0), (0.3, 1000, 1.0, 0.0), (1.0, 0, 1.0, 0.001),
+              (1.0, 0, 1.0, 0.2), (1.5, 0, 1.0, 1e-6), (1.0, 0, 0.3, 0.0), (1.0, 0, 0.999, 0.01)]
+
+
+@pytest.mark.parametrize("vocab", [1500, 4096, 32000, 50255, 270001])
+@pytest.mark.parametrize("kind", ["normal", "falling", "rising", "one run", "blocks", "below zero", "not there"])
+def test_sample_long_lists(dev, vocab, kind):
+    """Lists of about as many tokens as are sorted at once; rows whose highest tokens lie beside each other, and in one
+    place of every 256, so that many share a part of the row."""
+    print(f"sample long lists V={vocab} {kind}", flush=True)
+    rng = np.random.default_rng(vocab + len(kind))
+    x = (2 * rng.standard_normal((len(LONG_LISTS), vocab))).astype(np.float32)
+    if kind in ("falling", "rising"):
+        x = np.sort(x, 1)[:, ::-1 if kind == "falling" else 1]
+    if kind == "one run":
+        x[:, vocab // 3:vocab // 3 + 1100] += 9
+    if kind == "blocks":
+        x[:, 77::256] += 9
+    if kind == "below zero":
+        x -= 300
+    if kind == "not there":
+        x[rng.random(x.shape) < 0.4] = np.nan
+        x[rng.random(x.shape) < 0.4] = -np.inf
+    _check_sample(dev, x, LONG_LISTS, rng.random(len(x)).astype(np.float32), offset=3)
+
+
+def test_sample_rows_past_32_bits(dev):
+    """The last of rows that together hold more than 2^32 logits; the others hold whatever the memory does."""
+    print("sample rows past 32 bits", flush=True)
+    vocab, rows = 1 << 17, (1 << 15) + 2
+    x = (2 * np.random.default_rng(8).standard_normal((2, vocab))).astype(np.float32)
+    buf = dev.DeviceBuffer(4 * rows * vocab)
+    dev.copy_to_device(buf.ptr + 4 * (rows - 2) * vocab, x)
+    table = np.zeros(rows, dtype=dev.SAMPLE_RULE)
+    table[:] = (1.0, 1.0, 0.0, 1)
+    table[-2:] = [(0.9, 0.95, 0.0, 50), (1.0, 0.9, 0.0, 0)]
+    u = np.full(rows, 0.625, np.float32)
+    r, d = dev.upload(table), dev.upload(u)
+    tokens = dev.upload(np.zeros(rows, np.uint32))
+    dev.sample(buf.ptr, rows, vocab, r.ptr, d.ptr, tokens.ptr)
+    dev.sync()
+    got = dev.download(tokens.ptr, (rows,), np.uint32)[-2:]
+    assert got.tolist() == [_draw(x[0], u[0], 0.9, 50, 0.95, 0.0)[0], _draw(x[1], u[0], 1.0, 0, 0.9, 0.0)[0]]
