@@ -54,6 +54,8 @@ constexpr uint32_t kVector = 4 * kWave;      // tokens of one load of a wave
 constexpr uint32_t kAhead = 4;               // vectors of a thread in flight
 constexpr uint32_t kBins = 4096;
 constexpr uint32_t kBinsEach = kBins / kBlock;
+constexpr uint32_t kWaveBins = 2048;         // of a wave's own
+constexpr uint32_t kWaveBinsEach = kWaveBins / kBlock;
 constexpr uint32_t kListed = 2048;           // tokens that are sorted in LDS
 constexpr uint32_t kListedEach = kListed / kBlock;
 constexpr uint32_t kShortList = 1024;        // the largest top_k whose tokens are listed at once
@@ -122,14 +124,20 @@ __device__ inline float row_max(float v)
 }
 
 struct SampleLds {
-    uint32_t count[kBins];
     union {
-        uint64_t mass[kBins];
-        uint64_t other[kListed];     // of a sort, and the listed tokens' weights
+        uint64_t of_wave[kWaves][kWaveBins];   // weights
+        struct {
+            uint32_t count[kBins];
+            union {
+                uint64_t mass[kBins];
+                uint64_t other[kListed];       // of a sort, and the listed tokens' weights
+            };
+        };
     };
     uint64_t listed[kListed];        // key, then ~token, so that falling numbers are the order
     uint64_t range[kRanges];
     uint64_t wave[kWaves];
+    uint64_t run[kWaves];            // what is kept of a wave's run
     uint64_t found;
     uint64_t before;
     float wave_f[kWaves];
@@ -236,9 +244,11 @@ struct Row {
     uint32_t V;
     uint32_t run;        // vectors of a wave
     bool infinite;       // the highest logit is +inf
+    uint32_t base;       // number of its first token
 
     __device__ uint32_t first() const { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave))) * run * kVector; }
-    __device__ uint32_t token(uint32_t j) const { return first() + j * kVector + 4 * (threadIdx.x & (kWave - 1)); }
+    __device__ uint32_t place(uint32_t j) const { return first() + j * kVector + 4 * (threadIdx.x & (kWave - 1)); }
+    __device__ uint32_t token(uint32_t j) const { return base + place(j); }
     __device__ uint32_t vectors() const
     {
         uint32_t const at = first();
@@ -276,11 +286,11 @@ struct Row {
         uint32_t const n = vectors();
         if (n == 0) return;
         auto const bounded = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), 0, static_cast<int>(4 * V), 0x00027000);
-        uint32_t const at = 4 * token(0);
+        uint32_t const at = 4 * place(0);
         auto const ahead_of = [&](uint32_t j) {
             return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(bounded, static_cast<int>(at + j * kVector * 4), 0, 0));
         };
-        f32x4_t const last = load(token(n - 1));
+        f32x4_t const last = load(place(n - 1));
         f32x4_t ahead[kAhead];
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; ++k) ahead[k] = ahead_of(k);
@@ -532,7 +542,7 @@ __device__ __attribute__((always_inline)) inline uint32_t token_at(const Row& ro
         f32x4_t const y = row.as_counted(row.load(v + k));
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            uint64_t const x = weight.of(y[i], v + k + i);
+            uint64_t const x = weight.of(y[i], row.base + v + k + i);
             w[k + i] = v + k + i < end ? x : 0;
             sum += w[k + i];
         }
@@ -552,7 +562,7 @@ __device__ __attribute__((always_inline)) inline uint32_t token_at(const Row& ro
     }
     __syncthreads();
     *its = lds.found;
-    return lds.word[2];
+    return row.base + lds.word[2];
 }
 
 // ---- sorting ---------------------------------------------------------------------
@@ -659,13 +669,18 @@ struct Cut {
     uint64_t amount;
 };
 
-// Bins of the logits from the highest down to where weights are 0; the last
-// one's tokens are not counted.  Half a logit, as the difference of two may be
+// Bins of the logits from the highest down over `width`; the last one's tokens
+// are not counted.  Half a logit, as the difference of two may be
 // past the largest number.
 struct Bins {
     float half;      // of the highest logit
     float rate;      // bins for a unit of half a logit, finite
-    __device__ uint32_t of(float x) const { return static_cast<uint32_t>(fminf((half - 0.5f * x) * rate, static_cast<float>(kBins - 1))); }
+    float last;      // bin
+    __device__ uint32_t of(float x) const { return static_cast<uint32_t>(fminf((half - 0.5f * x) * rate, last)); }
+    __device__ Bins(float high, float width, uint32_t n)
+        : half(0.5f * high), rate(fminf(2.0f * static_cast<float>(n - 1) / width, 3e38f)), last(static_cast<float>(n - 1))
+    {
+    }
     // No logit of the bin is below under(b), and none above over(b): the borders,
     // and what a part in 2^17 of the largest number on the way may take from them.
     __device__ float slack(uint32_t b) const { return (fabsf(half) + static_cast<float>(b + 1) / rate) * 0x1p-17f; }
@@ -827,6 +842,95 @@ __device__ __attribute__((always_inline)) inline Last find_cut(const Row& row, S
     return last;
 }
 
+// ---- top-p's cut, and what it keeps of each wave's run -------------------------------
+
+// The weights in bins of each wave's own give the bin that the cut falls into and
+// what every run holds in the bins before it; the bin's tokens, listed and sorted,
+// give the last kept one and the rest of the runs' sums, of tokens that weigh
+// `least` or more: lds.run.  False where the bin is too full for the list.
+__device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, float top_p,
+                                                                  uint64_t least, Last* last, uint32_t* at_bin)
+{
+    uint32_t const tid = threadIdx.x;
+    uint32_t const lane = tid & (kWave - 1);
+    uint32_t const wave = tid / kWave;
+    row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
+        if (bins.of(highest_of(y)) >= kWaveBins - 1) return;
+        uint32_t b[4];
+        uint64_t w[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            b[i] = bins.of(y[i]);
+            w[i] = weights.of(y[i]);
+        }
+        // Here, and not each behind its condition.
+        asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (b[i] < kWaveBins - 1) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.of_wave[wave][b[i]]), static_cast<unsigned long long>(w[i]));
+        }
+    });
+    __syncthreads();
+    uint64_t of[kWaveBinsEach];
+    uint64_t sum = 0, total;
+#pragma unroll
+    for (uint32_t i = 0; i < kWaveBinsEach; ++i) {
+        of[i] = 0;
+#pragma unroll
+        for (uint32_t v = 0; v < kWaves; ++v) of[i] += lds.of_wave[v][kWaveBinsEach * tid + i];
+        sum += of[i];
+    }
+    uint64_t at = block_scan(sum, lds, &total);
+    uint64_t const amount = part_of(top_p, total, true);   // at least 1, at most the total
+#pragma unroll
+    for (uint32_t i = 0; i < kWaveBinsEach; ++i) {
+        if (at < amount && amount - at <= of[i]) {   // one bin
+            lds.word[3] = kWaveBinsEach * tid + i;
+            lds.before = at;
+        }
+        at += of[i];
+    }
+    __syncthreads();
+    uint32_t const bin = lds.word[3];
+    uint64_t const left = amount - lds.before;   // at least 1
+    sum = 0;
+    for (uint32_t b = lane; b < bin; b += kWave) sum += lds.of_wave[wave][b];
+    sum = wave_total(sum);
+    if (lane == 0) lds.run[wave] = sum;
+    float const low = fmaxf(bins.under(bin), -3.4028234664e38f);
+    float const high = fminf(bins.over(bin), 2.0f * bins.half);
+    uint32_t const listed = list_tokens(row, lds, low, high, [&](float x) { return bins.of(x) == bin; });
+    if (listed > kListed) return false;
+    sort_falling(lds.listed, lds, listed, true, high, high - low);
+    // Neighbours of the order each thread.
+    uint64_t w[kListedEach];
+    sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        uint32_t const n = kListedEach * tid + i;
+        w[i] = n < listed ? weights.of(logit_of(static_cast<uint32_t>(lds.listed[n] >> 32))) : 0;
+        sum += w[i];
+    }
+    at = block_scan(sum, lds, &total);
+#pragma unroll
+    for (uint32_t i = 0; i < kListedEach; ++i) {
+        uint32_t const n = kListedEach * tid + i;
+        if (n < listed && at < left) {
+            uint32_t const token = 0xFFFFFFFFu - static_cast<uint32_t>(lds.listed[n]);
+            if (left - at <= w[i]) {
+                lds.word[0] = static_cast<uint32_t>(lds.listed[n] >> 32);
+                lds.word[1] = token;
+            }
+            if (w[i] >= least) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.run[token / (row.run * kVector)]), static_cast<unsigned long long>(w[i]));
+        }
+        at += w[i];
+    }
+    __syncthreads();
+    *last = Last{logit_of(lds.word[0]), lds.word[1]};
+    *at_bin = bin;
+    return true;
+}
+
 // ---- the draw from a short list -----------------------------------------------------
 
 struct Drawn {
@@ -920,6 +1024,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     row.V = a.V;
     row.run = (a.V + kWaves * kVector - 1) / (kWaves * kVector);
     row.infinite = false;
+    row.base = 0;
     kimkv_sample_rule const rule = a.rules[blockIdx.x];
     float const uniform = a.uniforms[blockIdx.x];
     auto const answer = [&](uint32_t token, float probability) {
@@ -932,7 +1037,6 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
         answer(KIMKV_NO_TOKEN, 0.0f);
         return;
     }
-    clear_bins(lds);
 
     bool const greedy = rule.temperature == 0.0f;
     float const temperature = greedy ? 1.0f : rule.temperature;
@@ -941,6 +1045,12 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     bool const short_k = cut_k && top_k <= kShortList;
     bool const cut_p = !greedy && rule.top_p < 1.0f;
     bool const list = short_k || (!cut_k && !cut_p && rule.min_p > 0.0f);
+
+    if (cut_p && !cut_k) {
+        for (uint32_t b = lane; b < kWaveBins; b += kWave) lds.of_wave[tid / kWave][b] = 0;
+    } else {
+        clear_bins(lds);
+    }
 
     // ---- the columns' highest logits (NaN is left out) ----
     constexpr f32x4_t kNone{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -995,7 +1105,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
         float const none = fmaxf(high - kWeightless * temperature, -3.4028234664e38f);
         float bound = none;
         if (short_k) {
-            Bins const near{0.5f * high, fminf(2 * (kBins - 1) / fminf(kWeightless * temperature, 64.0f), 3e38f)};
+            Bins const near(high, fminf(kWeightless * temperature, 64.0f), kBins);
 #pragma unroll
             for (uint32_t set = 0; set < kSets; ++set) {
 #pragma unroll
@@ -1025,8 +1135,34 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
 
     // ---- the cuts of the row ----
     Last last{-INFINITY, 0xFFFFFFFFu};
-    if (cut_k || cut_p) {
-        Bins const bins{0.5f * high, fminf(2 * (kBins - 1) / (kWeightless * temperature), 3e38f)};
+    Row drawn = row;           // the part of the row that the draw falls into
+    uint64_t sums = 0;         // of all that is kept, where known
+    uint64_t before = 0;       // of it before that part
+    bool cut = !cut_k && !cut_p;
+    if (cut_p && !cut_k) {
+        Bins const bins(high, kWeightless * temperature, kWaveBins);
+        uint32_t bin = 0;
+        cut = cut_of_runs(row, lds, weights, bins, rule.top_p, kept.least, &last, &bin);
+        if (cut && (rule.min_p == 0.0f || bin == 0 || bins.under(bin - 1) > kept.sure)) {   // no bin before it holds what min-p leaves out
+            uint64_t const target_run = lds.run[lane & (kWaves - 1)];
+            uint64_t const upto = row_scan(target_run);
+            sums = lane_u64(upto, kWaves - 1);
+            uint64_t const target = part_of(uniform, sums, false);
+            uint32_t const wave = static_cast<uint32_t>(__popcll(__ballot(lane < kWaves && upto <= target)));
+            before = wave == 0 ? 0 : lane_u64(upto, wave - 1);
+            drawn.base = wave * row.run * kVector;
+            drawn.from = row.from + drawn.base;
+            drawn.V = min(row.V - drawn.base, row.run * kVector);
+            drawn.run = (drawn.V + kWaves * kVector - 1) / (kWaves * kVector);
+        }
+        if (!cut) {
+            __syncthreads();
+            clear_bins(lds);
+            __syncthreads();
+        }
+    }
+    if (!cut) {
+        Bins const bins(high, kWeightless * temperature, kBins);
         row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
             if (bins.of(highest_of(y)) >= kBins - 1) return;
             uint32_t b[4];
@@ -1078,9 +1214,10 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
 
     // ---- the draw ----
     kept = kept_tokens(weights, last, temperature, rule.min_p);
-    uint64_t const sums = sum_ranges(row, lds, kept);
+    uint64_t const found = sum_ranges(drawn, lds, kept);
+    if (sums == 0) sums = found;
     uint64_t its;
-    uint32_t const token = token_at(row, lds, part_of(uniform, sums, false), kept, &its);
+    uint32_t const token = token_at(drawn, lds, part_of(uniform, sums, false) - before, kept, &its);
     answer(token, static_cast<float>(static_cast<double>(its) / static_cast<double>(sums)));
 }
 
