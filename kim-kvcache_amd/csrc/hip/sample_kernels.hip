@@ -12,29 +12,31 @@
 // caches after the first time:
 //   - The highest logit.  Where a list may do, for each of 4096 parts of the row
 //     (columns) the highest, its place and the second.
-//   - List (top_k of at most 1024; min-p alone): a bound that top_k columns reach,
-//     or min-p's logit.  The tokens from it up are known from the columns, but for
-//     those in which two reach it, so the row is not read again.  They are sorted
-//     in LDS, and the cuts and the draw go on there.
-//   - Else, where top-k or top-p cut: counts and weights of 4096 bins of the
-//     logits, the bin that the cut falls into, its tokens sorted in LDS (bins of
-//     more tokens than LDS takes are cut into 4096 again, by their keys), which
-//     gives the last kept token.
-//   - The draw from a row: the kept tokens' weights summed by ranges of the
-//     vocabulary, the range that the random number falls into, the token in it.
+//   - List (top_k of at most 1024; few tokens that min-p keeps): a bound that
+//     top_k columns reach, or min-p's logit.  The tokens from it up are known from
+//     the columns, but for those in which two reach it, so the row is not read
+//     again.  They are sorted in LDS, and the cuts and the draw go on there.
+//   - Else, for top-p: weights of 2048 bins of the logits for each wave's run of
+//     the row, the bins that the cut and min-p's border fall into, their tokens
+//     sorted in LDS, which gives the last kept token and what is kept of each run.
+//   - With a longer top_k, or where the bins hold more tokens than LDS takes: counts
+//     (and weights) of 4096 bins, the bin of the cut, its tokens sorted, or cut into
+//     4096 again by their keys.
+//   - The draw from a row or a run: the kept tokens' weights summed by ranges of
+//     the vocabulary, the range that the random number falls into, the token in it.
 //
 // Bound by the instructions of one block's waves: a weight is 26 of them, and a
 // pass of weights over 32000 tokens 11 us, where reading the row takes 2.  So a
 // list saves passes: 72 rows of 50255 with top_k 50 take 16 us (20 us where the
-// list came from a second pass over the row), 256 rows of 128000 34 us (58), which
-// is 3.9 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
-// and these took 17 and 42 us.  Drawn from all the row 28 and 76 us, top-p of 0.9
-// 58 and 140 (62 and 160 while the cut was a function of its own, to which the row
-// and the LDS were addresses of any kind).  Tried and slower for top-p: a list from
-// the highest columns up (256 flat rows of 128000 184 us, as it falls back there);
-// counts and mean places of the bins first, then one pass of weights that sums by
-// ranges and lists the tokens of the bins in question (215 us: a pass of 64-bit
-// additions to LDS takes as long as one with the weights).
+// list came from a second pass over the row), 256 rows of 128000 35 us (58), which
+// is 3.8 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
+// and these took 17 and 42 us.  Drawn from all the row 28 and 77 us; top-p of 0.9
+// 49 and 113, of which one pass of weights (without the runs' own bins a second one
+// for the draw: 58 and 140), with min-p 47 and 103.  Tried and slower for top-p: a
+// list from the highest columns up (256 flat rows of 128000 184 us, as it falls back
+// there); counts and mean places of the bins first, then one pass of weights that
+// sums by ranges and lists the tokens of the bins in question (215 us: a pass of
+// 64-bit additions to LDS takes as long as one with the weights).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -376,19 +378,22 @@ struct Columns {
 };
 
 // Lists the tokens from a bound up, and returns how many there are, or more than
-// the list takes.  Each is in a column whose highest has reached the bound: it is
+// the list takes where they are more than `most`.  Each is in a column whose highest has reached the bound: it is
 // that one where the second has not, else the column is read again, its tokens
 // side by side in the wave, or the row where a wave has many such columns.
-__device__ inline uint32_t list_columns(const Row& row, SampleLds& lds, const Columns (&columns)[kSets], float bound)
+__device__ inline uint32_t list_columns(const Row& row, SampleLds& lds, const Columns (&columns)[kSets], float bound, uint32_t most)
 {
     uint32_t const lane = threadIdx.x & (kWave - 1);
-    uint32_t crowded = 0;
+    uint32_t least = 0, crowded = 0;
 #pragma unroll
     for (uint32_t set = 0; set < kSets; ++set) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) crowded += static_cast<uint32_t>(__popcll(__ballot(columns[set].second[i] >= bound)));
+        for (uint32_t i = 0; i < 4; ++i) {
+            least += static_cast<uint32_t>(__popcll(__ballot(columns[set].first[i] >= bound)));
+            crowded += static_cast<uint32_t>(__popcll(__ballot(columns[set].second[i] >= bound)));
+        }
     }
-    if (__syncthreads_or(crowded > kListed / kWaves) != 0) return kListed + 1;
+    if (block_total(lane == 0 ? least + crowded : 0, lds) > most) return kListed + 1;
     if (__syncthreads_or(crowded > kCrowded) != 0) return list_tokens(row, lds, bound, INFINITY, [](float) { return true; });
     start_list(lds);
     uint32_t const n = row.vectors();
@@ -844,12 +849,12 @@ __device__ __attribute__((always_inline)) inline Last find_cut(const Row& row, S
 
 // ---- top-p's cut, and what it keeps of each wave's run -------------------------------
 
-// The weights in bins of each wave's own give the bin that the cut falls into and
-// what every run holds in the bins before it; the bin's tokens, listed and sorted,
-// give the last kept one and the rest of the runs' sums, of tokens that weigh
-// `least` or more: lds.run.  False where the bin is too full for the list.
+// The weights in bins of each wave's own give the bin that the cut falls into, and
+// those that min-p's border can lie in; the tokens of the first of these, listed
+// and sorted, give the last kept one, and with the bins before them what is kept of
+// every run: lds.run.  False where they are too many for the list.
 __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, float top_p,
-                                                                  uint64_t least, Last* last, uint32_t* at_bin)
+                                                                  const Kept& kept, Last* last)
 {
     uint32_t const tid = threadIdx.x;
     uint32_t const lane = tid & (kWave - 1);
@@ -880,26 +885,37 @@ __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row
         for (uint32_t v = 0; v < kWaves; ++v) of[i] += lds.of_wave[v][kWaveBinsEach * tid + i];
         sum += of[i];
     }
-    uint64_t at = block_scan(sum, lds, &total);
+    uint64_t const first = block_scan(sum, lds, &total);
     uint64_t const amount = part_of(top_p, total, true);   // at least 1, at most the total
+    uint64_t at = first;
 #pragma unroll
     for (uint32_t i = 0; i < kWaveBinsEach; ++i) {
-        if (at < amount && amount - at <= of[i]) {   // one bin
-            lds.word[3] = kWaveBinsEach * tid + i;
-            lds.before = at;
-        }
+        if (at < amount && amount - at <= of[i]) lds.word[3] = kWaveBinsEach * tid + i;   // one bin
         at += of[i];
     }
     __syncthreads();
     uint32_t const bin = lds.word[3];
-    uint64_t const left = amount - lds.before;   // at least 1
+    uint32_t const from = kept.least != 0 ? min(bins.of(fminf(kept.sure, 2.0f * bins.half)), bin) : bin;
+    uint32_t const to = kept.least != 0 ? min(bins.of(kept.floor), bin) : bin;
+    at = first;
+#pragma unroll
+    for (uint32_t i = 0; i < kWaveBinsEach; ++i) {
+        if (kWaveBinsEach * tid + i == from) lds.before = at;
+        at += of[i];
+    }
     sum = 0;
-    for (uint32_t b = lane; b < bin; b += kWave) sum += lds.of_wave[wave][b];
+    for (uint32_t b = lane; b < from; b += kWave) sum += lds.of_wave[wave][b];
     sum = wave_total(sum);
     if (lane == 0) lds.run[wave] = sum;
-    float const low = fmaxf(bins.under(bin), -3.4028234664e38f);
-    float const high = fminf(bins.over(bin), 2.0f * bins.half);
-    uint32_t const listed = list_tokens(row, lds, low, high, [&](float x) { return bins.of(x) == bin; });
+    if (tid == 0) {
+        lds.word[1] = 0xFFFFFFFFu;   // the last token, where the list holds it
+        lds.word[2] = key_of(-INFINITY);
+    }
+    __syncthreads();
+    uint64_t const left = amount - lds.before;   // at least 1
+    float const low = fmaxf(bins.under(to), -3.4028234664e38f);
+    float const high = fminf(bins.over(from), 2.0f * bins.half);
+    uint32_t const listed = list_tokens(row, lds, low, high, [&](float x) { return bins.of(x) >= from && bins.of(x) <= to; });
     if (listed > kListed) return false;
     sort_falling(lds.listed, lds, listed, true, high, high - low);
     // Neighbours of the order each thread.
@@ -918,16 +934,15 @@ __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row
         if (n < listed && at < left) {
             uint32_t const token = 0xFFFFFFFFu - static_cast<uint32_t>(lds.listed[n]);
             if (left - at <= w[i]) {
-                lds.word[0] = static_cast<uint32_t>(lds.listed[n] >> 32);
+                lds.word[2] = static_cast<uint32_t>(lds.listed[n] >> 32);
                 lds.word[1] = token;
             }
-            if (w[i] >= least) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.run[token / (row.run * kVector)]), static_cast<unsigned long long>(w[i]));
+            if (w[i] >= kept.least) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.run[token / (row.run * kVector)]), static_cast<unsigned long long>(w[i]));
         }
         at += w[i];
     }
     __syncthreads();
-    *last = Last{logit_of(lds.word[0]), lds.word[1]};
-    *at_bin = bin;
+    *last = Last{logit_of(lds.word[2]), lds.word[1]};
     return true;
 }
 
@@ -939,10 +954,11 @@ struct Drawn {
     uint64_t total;
 };
 
-// From a list of the first top_k tokens and more, keys within low .. high.  Each
-// thread has neighbours of it.
+// From a list of the first top_k tokens and more, or of all that min-p keeps,
+// logits within low .. high; top-p's part is of `total`, or where that is 0 of the
+// first top_k's weight.  Each thread has neighbours of the list.
 __device__ inline Drawn draw_listed(SampleLds& lds, const Weights& weights, const kimkv_sample_rule& rule, uint32_t listed, uint32_t top_k,
-                                    float low, float high, float uniform, uint32_t V)
+                                    uint64_t total, float low, float high, float uniform, uint32_t V)
 {
     uint32_t const tid = threadIdx.x;
     sort_falling(lds.listed, lds, listed, true, high, high - low);
@@ -959,7 +975,7 @@ __device__ inline Drawn draw_listed(SampleLds& lds, const Weights& weights, cons
     uint64_t all;
     uint64_t at = block_scan(sum, lds, &all);
     // What top-p keeps begins before its part of the weight is reached.
-    uint64_t const need = rule.top_p < 1.0f ? part_of(rule.top_p, all, true) : ~uint64_t{0};
+    uint64_t const need = rule.top_p < 1.0f ? part_of(rule.top_p, total != 0 ? total : all, true) : ~uint64_t{0};
     uint32_t kept = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kListedEach; ++i) {
@@ -1044,7 +1060,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     bool const cut_k = top_k < a.V || greedy;
     bool const short_k = cut_k && top_k <= kShortList;
     bool const cut_p = !greedy && rule.top_p < 1.0f;
-    bool const list = short_k || (!cut_k && !cut_p && rule.min_p > 0.0f);
+    bool const list = short_k || (!cut_k && rule.min_p > 0.0f);
 
     if (cut_p && !cut_k) {
         for (uint32_t b = lane; b < kWaveBins; b += kWave) lds.of_wave[tid / kWave][b] = 0;
@@ -1119,10 +1135,21 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
             if (bin < kBins) bound = fmaxf(near.under(bin), none);
         }
         // One that min-p leaves out counts where top-p takes its part of the list.
-        if (!cut_p) bound = fmaxf(bound, kept.floor);
-        uint32_t const listed = list_columns(row, lds, columns, bound);
+        if (!short_k || !cut_p) bound = fmaxf(bound, kept.floor);
+        // A longer list of min-p's does not pay beside top-p, whose pass of weights comes
+        // on top (72 rows of 50255, some 1300 tokens: 50 us, without the list 47).
+        uint32_t const listed = list_columns(row, lds, columns, bound, short_k || !cut_p ? kListed : kShortList);
         if (listed <= kListed) {
-            Drawn const d = draw_listed(lds, weights, rule, listed, top_k, bound, high, uniform, a.V);
+            // Min-p leaves the list, and top-p keeps a part of the row.
+            uint64_t total = 0;
+            if (!short_k && cut_p) {
+                row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) total += weights.of(y[i]);
+                });
+                total = block_total(total, lds);
+            }
+            Drawn const d = draw_listed(lds, weights, rule, listed, top_k, total, bound, high, uniform, a.V);
             answer(d.token, static_cast<float>(static_cast<double>(d.weight) / static_cast<double>(d.total)));
             return;
         }
@@ -1141,11 +1168,9 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     bool cut = !cut_k && !cut_p;
     if (cut_p && !cut_k) {
         Bins const bins(high, kWeightless * temperature, kWaveBins);
-        uint32_t bin = 0;
-        cut = cut_of_runs(row, lds, weights, bins, rule.top_p, kept.least, &last, &bin);
-        if (cut && (rule.min_p == 0.0f || bin == 0 || bins.under(bin - 1) > kept.sure)) {   // no bin before it holds what min-p leaves out
-            uint64_t const target_run = lds.run[lane & (kWaves - 1)];
-            uint64_t const upto = row_scan(target_run);
+        cut = cut_of_runs(row, lds, weights, bins, rule.top_p, kept, &last);
+        if (cut) {
+            uint64_t const upto = row_scan(lds.run[lane & (kWaves - 1)]);
             sums = lane_u64(upto, kWaves - 1);
             uint64_t const target = part_of(uniform, sums, false);
             uint32_t const wave = static_cast<uint32_t>(__popcll(__ballot(lane < kWaves && upto <= target)));
@@ -1154,8 +1179,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
             drawn.from = row.from + drawn.base;
             drawn.V = min(row.V - drawn.base, row.run * kVector);
             drawn.run = (drawn.V + kWaves * kVector - 1) / (kWaves * kVector);
-        }
-        if (!cut) {
+        } else {
             __syncthreads();
             clear_bins(lds);
             __syncthreads();
