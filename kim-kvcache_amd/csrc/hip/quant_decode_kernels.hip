@@ -32,6 +32,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "attention_common.h"
 #include "quant_common.h"
@@ -608,21 +609,22 @@ __device__ void decode_general(const QuantView& P, const kimkv_decode_item& item
     }
 }
 
-// kDim 0: the general path alone.
-template <uint32_t kDim>
+template <uint32_t kDim, uint32_t kOf>
 struct FastLds {
     union {
-        Group groups[kWaves][kMaxGroups];
-        float sum[kWaves][kColumns][kDim + 4];
+        Group groups[kOf][kMaxGroups];
+        float sum[kOf][kColumns][kDim + 4];
     };
-    float m[kWaves][kColumns];
-    float l[kWaves][kColumns];
+    float m[kOf][kColumns];
+    float l[kOf][kColumns];
 };
 
-template <uint32_t kFormat, uint32_t kDim>
-__global__ __launch_bounds__(kBlock, 2) void quant_decode_kernel(QuantView P, DecodeArgs a)
+// kDim 0: the general path alone.  kOf: waves of a block.
+template <uint32_t kFormat, uint32_t kDim, uint32_t kOf>
+__global__ __launch_bounds__(kOf * kWave, 2 * kWaves / kOf) void quant_decode_kernel(QuantView P, DecodeArgs a)
 {
-    constexpr size_t kFast = kDim != 0 ? sizeof(FastLds<kDim == 0 ? 64 : kDim>) : 0;
+    static_assert(kDim != 0 || kOf == kWaves, "the general path's LDS is for kWaves");
+    constexpr size_t kFast = kDim != 0 ? sizeof(FastLds<kDim == 0 ? 64 : kDim, kOf>) : 0;
     __shared__ alignas(16) unsigned char lds[kFast > sizeof(GeneralLds) ? kFast : sizeof(GeneralLds)];
     QuantUnit const unit = a.units[blockIdx.x];
     kimkv_decode_item const item = a.items[unit.lane];
@@ -633,12 +635,12 @@ __global__ __launch_bounds__(kBlock, 2) void quant_decode_kernel(QuantView P, De
     uint32_t const G = a.G;
     float* const slot = unit.slot == kDirect ? nullptr : a.work + unit.slot * slot_floats(G, P.dim);
     if constexpr (kDim != 0) {
-        auto& f = *reinterpret_cast<FastLds<kDim>*>(lds);
+        auto& f = *reinterpret_cast<FastLds<kDim, kOf>*>(lds);
         uint32_t const tid = threadIdx.x;
         uint32_t const lane = tid & (kWave - 1);
         uint32_t const wave = tid / kWave;
         uint32_t const end = unit.first + unit.count;
-        uint32_t const per = ((unit.count + kTile - 1) / kTile + kWaves - 1) / kWaves * kTile;
+        uint32_t const per = ((unit.count + kTile - 1) / kTile + kOf - 1) / kOf * kTile;
         uint32_t const t0 = min(unit.first + wave * per, end);
         bool bad = false;
         WavePart<kDim> const part = decode_wave<kFormat, kDim>(P, item, unit.head, G, t0, min(t0 + per, end), unit.tokens, f.groups[wave], &bad);
@@ -654,16 +656,16 @@ __global__ __launch_bounds__(kBlock, 2) void quant_decode_kernel(QuantView P, De
                 f.l[wave][r] = part.l;
             }
             __syncthreads();
-            for (uint32_t i = tid; i < G * (kDim / 4); i += kBlock) {
+            for (uint32_t i = tid; i < G * (kDim / 4); i += kOf * kWave) {
                 uint32_t const j = i / (kDim / 4);
                 uint32_t const d = (i - j * (kDim / 4)) * 4;
                 float top = -INFINITY;
 #pragma unroll
-                for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, f.m[w][j]);
+                for (uint32_t w = 0; w < kOf; ++w) top = fmaxf(top, f.m[w][j]);
                 float4_t sum = {};
                 float total = 0.0f;
 #pragma unroll
-                for (uint32_t w = 0; w < kWaves; ++w) {
+                for (uint32_t w = 0; w < kOf; ++w) {
                     float const x = part_weight(f.m[w][j], top);
                     total += f.l[w][j] * x;
                     if (x != 0.0f) sum += *reinterpret_cast<const float4_t*>(&f.sum[w][j][d]) * x;
@@ -846,16 +848,30 @@ kimkv_status kimkv_quant_decode_batch(const kimkv_quant_storage* storage, const 
     QuantView const view = quant_view(*storage);
     auto const* const units = static_cast<const QuantUnit*>(device_entries);
     DecodeArgs const args{device_items, units, static_cast<float*>(workspace), plan->query_heads, G};
-    auto const launch = [&](auto kernel) { kernel<<<plan->unit_count, kBlock, 0, native(stream)>>>(view, args); };
-    uint32_t const dim = fast_dim(view.dim) && G <= kColumns ? view.dim : 0;
+    // A unit for a compute unit or less: twice the waves, which are there anyway.
+    bool const few = plan->unit_count <= static_cast<uint32_t>(storage->compute_units);
+    auto const launch = [&](auto kernel, uint32_t waves) { kernel<<<plan->unit_count, waves * kWave, 0, native(stream)>>>(view, args); };
+    auto const launch_dim = [&](auto format, auto dim) {
+        if (few) {
+            launch(quant_decode_kernel<format.value, dim.value, 2 * kWaves>, 2 * kWaves);
+        } else {
+            launch(quant_decode_kernel<format.value, dim.value, kWaves>, kWaves);
+        }
+    };
+    auto const launch_format = [&](auto format) {
+        switch (fast_dim(view.dim) && G <= kColumns ? view.dim : 0) {
+        case 64: launch_dim(format, std::integral_constant<uint32_t, 64>{}); break;
+        case 96: launch_dim(format, std::integral_constant<uint32_t, 96>{}); break;
+        case 128: launch_dim(format, std::integral_constant<uint32_t, 128>{}); break;
+        default: launch(quant_decode_kernel<format.value, 0, kWaves>, kWaves); break;
+        }
+    };
     void* start = nullptr;
     kernel_timing_begin(TimedKernel::Decode, native(stream), &start);
     if (storage->format == KIMKV_QUANT_INT8) {
-        dim == 64 ? launch(quant_decode_kernel<KIMKV_QUANT_INT8, 64>) : dim == 96 ? launch(quant_decode_kernel<KIMKV_QUANT_INT8, 96>)
-            : dim == 128 ? launch(quant_decode_kernel<KIMKV_QUANT_INT8, 128>) : launch(quant_decode_kernel<KIMKV_QUANT_INT8, 0>);
+        launch_format(std::integral_constant<uint32_t, KIMKV_QUANT_INT8>{});
     } else {
-        dim == 64 ? launch(quant_decode_kernel<KIMKV_QUANT_E4M3, 64>) : dim == 96 ? launch(quant_decode_kernel<KIMKV_QUANT_E4M3, 96>)
-            : dim == 128 ? launch(quant_decode_kernel<KIMKV_QUANT_E4M3, 128>) : launch(quant_decode_kernel<KIMKV_QUANT_E4M3, 0>);
+        launch_format(std::integral_constant<uint32_t, KIMKV_QUANT_E4M3>{});
     }
     kimkv_status const status = launch_status();
     kernel_timing_end(TimedKernel::Decode, native(stream), start);
