@@ -7,9 +7,9 @@
 // matrix cores and the scales stay outside of them, in 32 bits: a_j at the
 // score, b_j at the weight.
 //
-// Work: block = unit (a lane, a KV head, a range of its tokens), its four waves
-// a quarter of the range each, joined in LDS; a lane of one unit a head is
-// written at once, the others' parts are merged by a second launch.  A wave
+// Work: block = unit (a lane, a KV head, a range of its tokens), its waves, four
+// or for few units eight, a part of it each, joined in LDS; a lane of one unit a
+// head is written at once, the others' parts are merged by a second launch.  A wave
 // takes the table entries that begin in its range, so no page is cut; it reads
 // 64 of them at a time.  An entry that is a whole page of 64 tokens is a tile;
 // the groups of 8 of all others are collected eight to a tile: the order of the
@@ -25,8 +25,9 @@
 // (2.2 GB) take 350 us, 6.3 TB/s.  A tile's K registers take the next tile's K as
 // soon as the scores stand, and V's the next V behind the sums: two sets of
 // registers for a tile (128 dims: 108 of them spilled) made 64 ragged lanes of up
-// to 6000 tokens, 8 heads of 128, 55 us instead of 29.  There the launches, the
-// chain of loads to the first page and the last tiles bound: 103 MB take 15 us.
+// to 6000 tokens, 8 heads of 128, 55 us instead of 27.  Beside the 17 us that
+// their 103 MB take from HBM there are the chain of loads to a unit's first page
+// and the merge's launch (4.5 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -848,7 +849,8 @@ kimkv_status kimkv_quant_decode_batch(const kimkv_quant_storage* storage, const 
     QuantView const view = quant_view(*storage);
     auto const* const units = static_cast<const QuantUnit*>(device_entries);
     DecodeArgs const args{device_items, units, static_cast<float*>(workspace), plan->query_heads, G};
-    // A unit for a compute unit or less: twice the waves, which are there anyway.
+    // A unit for a compute unit or less: twice the waves, as there is room for them
+    // (16 lanes of 1000 tokens, 4 heads of 64: 10.5 us, not 12.1).
     bool const few = plan->unit_count <= static_cast<uint32_t>(storage->compute_units);
     auto const launch = [&](auto kernel, uint32_t waves) { kernel<<<plan->unit_count, waves * kWave, 0, native(stream)>>>(view, args); };
     auto const launch_dim = [&](auto format, auto dim) {
