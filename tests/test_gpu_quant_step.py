@@ -1021,3 +1021,22 @@ def test_sample_rows_past_32_bits(dev):
     dev.sync()
     got = dev.download(tokens.ptr, (rows,), np.uint32)[-2:]
     assert got.tolist() == [_draw(x[0], u[0], 0.9, 50, 0.95, 0.0)[0], _draw(x[1], u[0], 1.0, 0, 0.9, 0.0)[0]]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim,group", [(64, 2), (96, 3), (128, 2), (64, 16)])
+def test_decode_many_lanes(dev, form, dim, group):
+    """More units than compute units, of lanes in one part and in several; pages of all kinds, a lane of none."""
+    print(f"quant_decode many lanes {form} D={dim} G={group}", flush=True)
+    rng = np.random.default_rng(12)
+    counts = [int(n) for n in np.exp(rng.uniform(0, math.log(1500), 110))] + [0, 2900, 4100]
+    free = _pool(1400, 500)
+    tables = [_table(n, free, lead=i % 4 if i % 3 == 0 else 0, small=i % 17 == 5 and n < 300) for i, n in enumerate(counts)]
+    lanes = _Lanes(dev, FORMS[form], 3, dim, group, tables, 1400, 500)
+    _, plan = lanes.storage.decode_plan(lanes.counts, 3 * group)
+    assert plan.unit_count > lanes.storage.info().compute_units and plan.merge_lanes > 0
+    lanes.check()
+    # Query rows at an odd address.
+    lanes = _Lanes(dev, FORMS[form], 3, dim, group, tables, 1400, 500, offset=3, seed=5)
+    lanes.check()
+    assert lanes.storage.faults() == (0, 0)
