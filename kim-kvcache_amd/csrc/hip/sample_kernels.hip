@@ -28,8 +28,8 @@
 // Bound by the instructions of one block's waves: a weight is 26 of them, and a
 // pass of weights over 32000 tokens 11 us, where reading the row takes 2.  So a
 // list saves passes: 72 rows of 50255 with top_k 50 take 16 us (20 us where the
-// list came from a second pass over the row), 256 rows of 128000 35 us (58), which
-// is 3.8 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
+// list came from a second pass over the row), 256 rows of 128000 34 us (58), which
+// is 3.9 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
 // and these took 17 and 42 us.  Drawn from all the row 28 and 77 us; top-p of 0.9
 // 49 and 113, of which one pass of weights (without the runs' own bins a second one
 // for the draw: 58 and 140), with min-p 47 and 103.  Tried and slower for top-p: a
@@ -61,7 +61,8 @@ constexpr uint32_t kWaveBinsEach = kWaveBins / kBlock;
 constexpr uint32_t kListed = 2048;           // tokens that are sorted in LDS
 constexpr uint32_t kListedEach = kListed / kBlock;
 constexpr uint32_t kShortList = 1024;        // the largest top_k whose tokens are listed at once
-constexpr uint32_t kCrowded = 32;            // columns that a wave reads again one by one (8: 72 rows of 50255, top_k 700, 31 us, not 25)
+constexpr uint32_t kCrowded = 96;            // columns that a wave reads again (8, one by one: 72 rows of 50255, top_k 700, 31 us, not 22)
+constexpr uint32_t kAgain = 4;               // of these at once
 constexpr uint32_t kSets = 2;                // of a thread's columns
 constexpr uint32_t kSmall = 128;             // tokens that are ranked by counting
 static_assert(2 * kListed <= kBins, "a sort's counts and starts");
@@ -140,6 +141,7 @@ struct SampleLds {
     uint64_t range[kRanges];
     uint64_t wave[kWaves];
     uint64_t run[kWaves];            // what is kept of a wave's run
+    uint32_t again[kWaves][kCrowded];   // columns that a wave reads again
     uint64_t found;
     uint64_t before;
     float wave_f[kWaves];
@@ -315,31 +317,31 @@ __device__ inline float highest_of(f32x4_t const& y) { return fmaxf(fmaxf(y[0], 
 // A token's number of the list: falling numbers are the order.
 __device__ inline uint64_t listing(float x, uint32_t token) { return static_cast<uint64_t>(key_of(x)) << 32 | (0xFFFFFFFFu - token); }
 
-// Lists the lanes' tokens that are in, as far as the list goes.  One atomic
-// operation a wave: a token's is one of 64 at one address.
-__device__ inline void list_lanes(SampleLds& lds, uint64_t in, float x, uint32_t token)
+__device__ inline uint32_t lanes_below(uint64_t in) { return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in), 0)); }
+
+// Places of the list for a wave's tokens, the first of them: one atomic operation
+// for all, as the wave waits for it.
+__device__ inline uint32_t list_places(SampleLds& lds, uint32_t count)
 {
-    uint32_t const lane = threadIdx.x & (kWave - 1);
     uint32_t at = 0;
-    if (lane == 0) at = atomicAdd(&lds.word[0], static_cast<uint32_t>(__popcll(in)));
-    at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
-    uint32_t const place = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in), at));
-    if ((in >> lane & 1u) != 0 && place < kListed) lds.listed[place] = listing(x, token);
+    if (count != 0 && (threadIdx.x & (kWave - 1)) == 0) at = atomicAdd(&lds.word[0], count);
+    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+}
+
+// Lists the lanes' tokens that are in from place *at on, as far as the list goes.
+__device__ inline void list_lanes(SampleLds& lds, uint64_t in, float x, uint32_t token, uint32_t* at)
+{
+    uint32_t const place = *at + lanes_below(in);
+    if ((in >> (threadIdx.x & (kWave - 1)) & 1u) != 0 && place < kListed) lds.listed[place] = listing(x, token);
+    *at += static_cast<uint32_t>(__popcll(in));
 }
 
 // Lists the tokens of a vector that pass, a lane's bit in[i] for its i-th.
 __device__ inline void list_vector(SampleLds& lds, const uint64_t (&in)[4], f32x4_t const& y, uint32_t token)
 {
-    uint32_t const lane = threadIdx.x & (kWave - 1);
-    uint32_t at = 0;
-    if (lane == 0) at = atomicAdd(&lds.word[0], static_cast<uint32_t>(__popcll(in[0]) + __popcll(in[1]) + __popcll(in[2]) + __popcll(in[3])));
-    at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+    uint32_t at = list_places(lds, static_cast<uint32_t>(__popcll(in[0]) + __popcll(in[1]) + __popcll(in[2]) + __popcll(in[3])));
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        uint32_t const place = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in[i] >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in[i]), at));
-        if ((in[i] >> lane & 1u) != 0 && place < kListed) lds.listed[place] = listing(y[i], token + i);
-        at += static_cast<uint32_t>(__popcll(in[i]));
-    }
+    for (uint32_t i = 0; i < 4; ++i) list_lanes(lds, in[i], y[i], token + i, &at);
 }
 
 __device__ inline void start_list(SampleLds& lds)
@@ -396,30 +398,52 @@ __device__ inline uint32_t list_columns(const Row& row, SampleLds& lds, const Co
     if (block_total(lane == 0 ? least + crowded : 0, lds) > most) return kListed + 1;
     if (__syncthreads_or(crowded > kCrowded) != 0) return list_tokens(row, lds, bound, INFINITY, [](float) { return true; });
     start_list(lds);
+    uint32_t const wave = threadIdx.x / kWave;
+    uint64_t one[4 * kSets];
+    uint32_t alone = 0, again = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4 * kSets; ++k) {
+        Columns const& c = columns[k / 4];
+        one[k] = __ballot(c.first[k % 4] >= bound && !(c.second[k % 4] >= bound));
+        alone += static_cast<uint32_t>(__popcll(one[k]));
+        // The numbers of the columns to be read again.
+        uint64_t const more = __ballot(c.second[k % 4] >= bound);
+        if ((more >> lane & 1u) != 0) lds.again[wave][again + lanes_below(more)] = k / 4 * kVector + 4 * lane + k % 4;
+        again += static_cast<uint32_t>(__popcll(more));
+    }
+    uint32_t at = list_places(lds, alone);
+#pragma unroll
+    for (uint32_t k = 0; k < 4 * kSets; ++k) {
+        Columns const& c = columns[k / 4];
+        list_lanes(lds, one[k], c.first[k % 4], row.token(c.vector[k % 4]) + k % 4, &at);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     uint32_t const n = row.vectors();
-#pragma unroll
-    for (uint32_t set = 0; set < kSets; ++set) {
-        Columns const& c = columns[set];
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            uint64_t const one = __ballot(c.first[i] >= bound && !(c.second[i] >= bound));
-            if (one != 0) list_lanes(lds, one, c.first[i], row.token(c.vector[i]) + i);
-        }
 #pragma nounroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            float const second = i < 2 ? (i == 0 ? c.second[0] : c.second[1]) : (i == 2 ? c.second[2] : c.second[3]);
-#pragma nounroll
-            for (uint64_t more = __ballot(second >= bound); more != 0; more &= more - 1) {
-                uint32_t const column = 4 * (static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(more))) - 1) + i;
-                for (uint32_t first = set; first < n; first += kSets * kWave) {
-                    uint32_t const j = first + kSets * lane;
-                    uint32_t const token = row.first() + j * kVector + column;
-                    float x = j < n && token < row.V ? row.from[token] : -INFINITY;
-                    if (row.infinite) x = x == INFINITY ? 0.0f : -INFINITY;
-                    uint64_t const in = __ballot(x >= bound);
-                    if (in != 0) list_lanes(lds, in, x, token);
-                }
+    for (uint32_t k = 0; k < again; k += kAgain) {
+        for (uint32_t first = 0; first < n; first += kSets * kWave) {
+            uint32_t token[kAgain];
+            float x[kAgain];
+            uint64_t in[kAgain];
+            uint32_t count = 0;
+#pragma unroll
+            for (uint32_t e = 0; e < kAgain; ++e) {
+                uint32_t const number = lds.again[wave][min(k + e, again - 1)];
+                uint32_t const j = first + number / kVector + kSets * lane;
+                uint32_t const v = row.first() + j * kVector + number % kVector;
+                token[e] = row.base + v;
+                x[e] = k + e < again && j < n && v < row.V ? row.from[v] : -INFINITY;
             }
+#pragma unroll
+            for (uint32_t e = 0; e < kAgain; ++e) {
+                if (row.infinite) x[e] = x[e] == INFINITY ? 0.0f : -INFINITY;
+                in[e] = __ballot(x[e] >= bound);
+                count += static_cast<uint32_t>(__popcll(in[e]));
+            }
+            at = list_places(lds, count);
+#pragma unroll
+            for (uint32_t e = 0; e < kAgain; ++e) list_lanes(lds, in[e], x[e], token[e], &at);
         }
     }
     __syncthreads();
@@ -1136,9 +1160,10 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
         }
         // One that min-p leaves out counts where top-p takes its part of the list.
         if (!short_k || !cut_p) bound = fmaxf(bound, kept.floor);
-        // A longer list of min-p's does not pay beside top-p, whose pass of weights comes
-        // on top (72 rows of 50255, some 1300 tokens: 50 us, without the list 47).
-        uint32_t const listed = list_columns(row, lds, columns, bound, short_k || !cut_p ? kListed : kShortList);
+        // A list of min-p's pays while it is a small part of the row: 256 rows of 128000,
+        // some 1300 tokens, 42 us, drawn from the row 74; 72 rows of 50255, some 1500
+        // tokens, 38, from the row 28 (with top-p 50 and 47).
+        uint32_t const listed = list_columns(row, lds, columns, bound, short_k ? kListed : min(kListed, a.V / 48));
         if (listed <= kListed) {
             // Min-p leaves the list, and top-p keeps a part of the row.
             uint64_t total = 0;
