@@ -1040,3 +1040,22 @@ def test_decode_many_lanes(dev, form, dim, group):
     lanes = _Lanes(dev, FORMS[form], 3, dim, group, tables, 1400, 500, offset=3, seed=5)
     lanes.check()
     assert lanes.storage.faults() == (0, 0)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [8, 64])
+def test_append_every_scale(dev, form, dim):
+    """Rows whose largest value is each finite number above 0, in long runs and, the last ones, as single tokens."""
+    print(f"quant_append every scale {form} D={dim}", flush=True)
+    c = _Cache(dev, FORMS[form], 1, dim, layers=1, micro=1, extent=496)
+    rng = np.random.default_rng(2)
+    largest = np.arange(31744, dtype=np.uint16).view(np.float16)
+    kv = (largest[None, None, :, None, None].astype(np.float64) * rng.uniform(-1, 1, (1, 2, 31744, 1, dim))).astype(np.float16)
+    kv[0, 0, :, 0, dim - 1] = largest
+    kv[0, 1, :, 0, 3] = -largest
+    runs = [(64 * i, 64, 1, i, 0) for i in range(490)] + [(31360 + i, 1, 1, 490 + i // 64, i % 64) for i in range(384)]
+    buf = dev.upload(_bits(kv))
+    c.storage.append_batch(c.jobs_of(buf.ptr, 31744, runs))
+    c.expect(kv, runs)
+    c.check()
+    assert c.storage.faults() == (0, 0)
