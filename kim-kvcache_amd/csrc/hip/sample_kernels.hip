@@ -31,8 +31,8 @@
 // list came from a second pass over the row), 256 rows of 128000 34 us (58), which
 // is 3.9 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
 // and these took 17 and 42 us.  Drawn from all the row 28 and 77 us; top-p of 0.9
-// 49 and 113, of which one pass of weights (without the runs' own bins a second one
-// for the draw: 58 and 140), with min-p 47 and 103.  Tried and slower for top-p: a
+// 47 and 105, of which one pass of weights (without the runs' own bins a second one
+// for the draw: 58 and 140), with min-p 46 and 99.  Tried and slower for top-p: a
 // list from the highest columns up (256 flat rows of 128000 184 us, as it falls back
 // there); counts and mean places of the bins first, then one pass of weights that
 // sums by ranges and lists the tokens of the bins in question (215 us: a pass of
@@ -60,6 +60,7 @@ constexpr uint32_t kWaveBins = 2048;         // of a wave's own
 constexpr uint32_t kWaveBinsEach = kWaveBins / kBlock;
 constexpr uint32_t kListed = 2048;           // tokens that are sorted in LDS
 constexpr uint32_t kListedEach = kListed / kBlock;
+constexpr uint32_t kListedOfWave = kListed / kWaves;
 constexpr uint32_t kShortList = 1024;        // the largest top_k whose tokens are listed at once
 constexpr uint32_t kCrowded = 96;            // columns that a wave reads again (8, one by one: 72 rows of 50255, top_k 700, 31 us, not 22)
 constexpr uint32_t kAgain = 4;               // of these at once
@@ -141,6 +142,7 @@ struct SampleLds {
     uint64_t range[kRanges];
     uint64_t wave[kWaves];
     uint64_t run[kWaves];            // what is kept of a wave's run
+    uint32_t count_of[kWaves];       // what a wave has listed
     uint32_t again[kWaves][kCrowded];   // columns that a wave reads again
     uint64_t found;
     uint64_t before;
@@ -352,23 +354,63 @@ __device__ inline void start_list(SampleLds& lds)
 }
 
 // Lists the tokens whose logits are in [low, high] and pass; returns how many
-// there are.
+// there are.  A wave keeps its own in a part of the list, without waiting for
+// places (with that, top-p of 0.9 took 49 and 112 us at the shapes above); where one
+// has more, they go into the whole list.
 template <typename F>
 __device__ __attribute__((always_inline)) inline uint32_t list_tokens(const Row& row, SampleLds& lds, float low, float high, F passes)
 {
+    uint32_t const lane = threadIdx.x & (kWave - 1);
+    uint32_t const wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave)));
+    uint64_t* const mine = lds.listed + wave * kListedOfWave;
+    auto const each = [&](auto list) __attribute__((always_inline)) {
+        row.vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
+            bool any = false;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) any = any || (y[i] >= low && y[i] <= high);
+            if (__ballot(any) == 0) return;
+            uint64_t in[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) in[i] = __ballot(y[i] >= low && y[i] <= high && passes(y[i]));
+            list(in, y, row.token(j));
+        });
+    };
     start_list(lds);
-    row.vectors_do([&](uint32_t j, f32x4_t const& y) __attribute__((always_inline)) {
-        bool any = false;
+    uint32_t count = 0;
+    each([&](const uint64_t (&in)[4], f32x4_t const& y, uint32_t token) __attribute__((always_inline)) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) any = any || (y[i] >= low && y[i] <= high);
-        if (__ballot(any) == 0) return;
-        uint64_t in[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) in[i] = __ballot(y[i] >= low && y[i] <= high && passes(y[i]));
-        list_vector(lds, in, y, row.token(j));
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (in[i] == 0) continue;
+            uint32_t const place = count + lanes_below(in[i]);
+            if ((in[i] >> lane & 1u) != 0 && place < kListedOfWave) mine[place] = listing(y[i], token + i);
+            count += static_cast<uint32_t>(__popcll(in[i]));
+        }
     });
+    if (lane == 0) lds.count_of[wave] = count;
     __syncthreads();
-    return lds.word[0];
+    uint32_t before = 0, all = 0, most = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        uint32_t const n = lds.count_of[w];
+        before += w < wave ? n : 0;
+        all += n;
+        most = max(most, n);
+    }
+    if (most > kListedOfWave) {
+        each([&](const uint64_t (&in)[4], f32x4_t const& y, uint32_t token) __attribute__((always_inline)) { list_vector(lds, in, y, token); });
+        __syncthreads();
+        return all;
+    }
+    uint64_t x[kListedOfWave / kWave];
+#pragma unroll
+    for (uint32_t i = 0; i < kListedOfWave / kWave; ++i) x[i] = mine[i * kWave + lane];
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kListedOfWave / kWave; ++i) {
+        if (i * kWave + lane < count) lds.listed[before + i * kWave + lane] = x[i];
+    }
+    __syncthreads();
+    return all;
 }
 
 // What a lane's i-th tokens of every kSets-th vector (a column) come to: the
