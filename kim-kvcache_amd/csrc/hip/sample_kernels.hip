@@ -17,11 +17,12 @@
 //     the columns, but for those in which two reach it, so the row is not read
 //     again.  They are sorted in LDS, and the cuts and the draw go on there.
 //   - Else, for top-p: weights of 2048 bins of the logits for each wave's run of
-//     the row, the bins that the cut and min-p's border fall into, their tokens
-//     sorted in LDS, which gives the last kept token and what is kept of each run.
-//   - With a longer top_k, or where the bins hold more tokens than LDS takes: counts
-//     (and weights) of 4096 bins, the bin of the cut, its tokens sorted, or cut into
-//     4096 again by their keys.
+//     the row, with a longer top_k their counts; the bins that the cuts and min-p's
+//     border fall into, their tokens sorted in LDS, which gives the last kept token
+//     and what is kept of each run.
+//   - With a longer top_k alone, or where the bins hold more tokens than LDS takes:
+//     counts (and weights) of 4096 bins, the bin of the cut, its tokens sorted, or
+//     cut into 4096 again by their keys.
 //   - The draw from a row or a run: the kept tokens' weights summed by ranges of
 //     the vocabulary, the range that the random number falls into, the token in it.
 //
@@ -32,7 +33,7 @@
 // is 3.9 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
 // and these took 17 and 42 us.  Drawn from all the row 28 and 77 us; top-p of 0.9
 // 47 and 105, of which one pass of weights (without the runs' own bins a second one
-// for the draw: 58 and 140), with min-p 46 and 99.  Tried and slower for top-p: a
+// for the draw: 58 and 140), with min-p 46 and 99, with top_k 3000 57 and 127.  Tried and slower for top-p: a
 // list from the highest columns up (256 flat rows of 128000 184 us, as it falls back
 // there); counts and mean places of the bins first, then one pass of weights that
 // sums by ranges and lists the tokens of the bins in question (215 us: a pass of
@@ -918,13 +919,23 @@ __device__ __attribute__((always_inline)) inline Last find_cut(const Row& row, S
 // The weights in bins of each wave's own give the bin that the cut falls into, and
 // those that min-p's border can lie in; the tokens of the first of these, listed
 // and sorted, give the last kept one, and with the bins before them what is kept of
-// every run: lds.run.  False where they are too many for the list.
+// every run: lds.run.  Top-p's part is of the first top_k tokens' weight (V: of
+// all): counts of the bins give the one of the last of them, whose tokens are
+// listed and sorted for their weight.  False where a list is too long.
 __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, float top_p,
-                                                                  const Kept& kept, Last* last)
+                                                                  uint32_t top_k, const Kept& kept, Last* last)
 {
     uint32_t const tid = threadIdx.x;
     uint32_t const lane = tid & (kWave - 1);
     uint32_t const wave = tid / kWave;
+    auto* const counts = reinterpret_cast<uint32_t*>(lds.listed);   // until there is a list
+    static_assert(kWaveBins * sizeof(uint32_t) <= sizeof(lds.listed), "the bins' counts");
+    bool const cut_k = top_k < row.V;
+    if (cut_k) {
+#pragma unroll
+        for (uint32_t i = 0; i < kWaveBinsEach; ++i) counts[i * kBlock + tid] = 0;
+        __syncthreads();
+    }
     row.vectors_do([&](uint32_t, f32x4_t const& y) __attribute__((always_inline)) {
         if (bins.of(highest_of(y)) >= kWaveBins - 1) return;
         uint32_t b[4];
@@ -940,6 +951,12 @@ __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row
         for (uint32_t i = 0; i < 4; ++i) {
             if (b[i] < kWaveBins - 1) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.of_wave[wave][b[i]]), static_cast<unsigned long long>(w[i]));
         }
+        if (cut_k) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                if (b[i] < kWaveBins - 1) atomicAdd(&counts[b[i]], 1u);
+            }
+        }
     });
     __syncthreads();
     uint64_t of[kWaveBinsEach];
@@ -952,8 +969,61 @@ __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row
         sum += of[i];
     }
     uint64_t const first = block_scan(sum, lds, &total);
-    uint64_t const amount = part_of(top_p, total, true);   // at least 1, at most the total
     uint64_t at = first;
+    if (cut_k) {
+        uint32_t n[kWaveBinsEach];
+        sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kWaveBinsEach; ++i) {
+            n[i] = counts[kWaveBinsEach * tid + i];
+            sum += n[i];
+        }
+        uint64_t all;
+        uint64_t tokens = block_scan(sum, lds, &all);
+        if (tid == 0) lds.word[3] = kWaveBins;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kWaveBinsEach; ++i) {
+            if (tokens < top_k && top_k - tokens <= n[i]) {   // one bin, or none where fewer weigh anything
+                lds.word[3] = kWaveBinsEach * tid + i;
+                lds.word[2] = top_k - static_cast<uint32_t>(tokens);
+                lds.before = at;
+            }
+            tokens += n[i];
+            at += of[i];
+        }
+        __syncthreads();
+        uint32_t const bin = lds.word[3];
+        uint32_t const its = lds.word[2];
+        uint64_t const before = lds.before;
+        __syncthreads();
+        if (bin < kWaveBins) {
+            float const low = fmaxf(bins.under(bin), -3.4028234664e38f);
+            float const high = fminf(bins.over(bin), 2.0f * bins.half);
+            uint32_t const listed = list_tokens(row, lds, low, high, [&](float x) { return bins.of(x) == bin; });
+            if (listed > kListed) return false;
+            // What lies where the sort works.
+            constexpr uint32_t kSaved = (sizeof(lds.count) + sizeof(lds.other)) / sizeof(uint64_t) / kBlock;
+            uint64_t* const there = lds.of_wave[0];
+            uint64_t saved[kSaved];
+#pragma unroll
+            for (uint32_t i = 0; i < kSaved; ++i) saved[i] = there[i * kBlock + tid];
+            sort_falling(lds.listed, lds, listed, true, high, high - low);
+            sum = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kListedEach; ++i) {
+                uint32_t const p = i * kBlock + tid;
+                if (p < min(its, listed)) sum += weights.of(logit_of(static_cast<uint32_t>(lds.listed[p] >> 32)));
+            }
+            total = before + block_total(sum, lds);
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < kSaved; ++i) there[i * kBlock + tid] = saved[i];
+            __syncthreads();
+        }
+        at = first;
+    }
+    uint64_t const amount = part_of(top_p, total, true);   // at least 1, at most the total
 #pragma unroll
     for (uint32_t i = 0; i < kWaveBinsEach; ++i) {
         if (at < amount && amount - at <= of[i]) lds.word[3] = kWaveBinsEach * tid + i;   // one bin
@@ -1128,7 +1198,8 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     bool const cut_p = !greedy && rule.top_p < 1.0f;
     bool const list = short_k || (!cut_k && rule.min_p > 0.0f);
 
-    if (cut_p && !cut_k) {
+    bool const runs = cut_p && !short_k;
+    if (runs) {
         for (uint32_t b = lane; b < kWaveBins; b += kWave) lds.of_wave[tid / kWave][b] = 0;
     } else {
         clear_bins(lds);
@@ -1234,9 +1305,9 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     uint64_t sums = 0;         // of all that is kept, where known
     uint64_t before = 0;       // of it before that part
     bool cut = !cut_k && !cut_p;
-    if (cut_p && !cut_k) {
+    if (runs) {
         Bins const bins(high, kWeightless * temperature, kWaveBins);
-        cut = cut_of_runs(row, lds, weights, bins, rule.top_p, kept, &last);
+        cut = cut_of_runs(row, lds, weights, bins, rule.top_p, top_k, kept, &last);
         if (cut) {
             uint64_t const upto = row_scan(lds.run[lane & (kWaves - 1)]);
             sums = lane_u64(upto, kWaves - 1);

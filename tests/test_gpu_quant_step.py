@@ -1059,3 +1059,27 @@ def test_append_every_scale(dev, form, dim):
     c.expect(kv, runs)
     c.check()
     assert c.storage.faults() == (0, 0)
+
+
+MANY_OF_TOP_K = [(1.0, 3000, 0.9, 0.0), (1.0, 3000, 0.9, 0.01), (0.01, 2000, 0.9, 0.0), (0.05, 3000, 0.5, 0.1), (2.0, 20000, 0.99, 1e-5), (1.0, 1100, 0.999999, 0.0),
+                 (30.0, 4000, 0.5, 0.0), (1.0, 31999, 0.7, 0.0), (0.7, 1500, 0.01, 0.0)]
+
+
+@pytest.mark.parametrize("vocab", [3001, 32000, 140001])
+@pytest.mark.parametrize("kind", ["normal", "falling", "peaks", "few values", "not there"])
+def test_sample_top_p_of_many(dev, vocab, kind):
+    """Top-p of more tokens than are listed at once; of fewer that weigh anything than top_k; of many equal ones."""
+    print(f"sample top-p of many V={vocab} {kind}", flush=True)
+    rng = np.random.default_rng(vocab + len(kind))
+    x = (2 * rng.standard_normal((len(MANY_OF_TOP_K), vocab))).astype(np.float32)
+    if kind == "falling":
+        x = np.sort(x, 1)[:, ::-1]
+    if kind == "peaks":
+        x[:, rng.integers(0, vocab, 9)] += 12
+    if kind == "few values":
+        x = np.rint(2 * x) / 2
+    if kind == "not there":
+        x[rng.random(x.shape) < 0.5] = -np.inf
+        x[rng.random(x.shape) < 0.1] = np.nan
+    for u in (0.0, 0.3, 1 - 2.0 ** -24):
+        _check_sample(dev, x, MANY_OF_TOP_K, np.full(len(x), u, np.float32), offset=1)
