@@ -507,14 +507,14 @@ struct Last {
 struct Kept {
     Weights weights;
     Last last;
-    uint64_t least;   // weights below it are not kept
+    float border;     // min-p keeps the logits from it up
     float floor;      // no logit below it is kept or weighs anything
     float sure;       // every logit above it is kept
 
     __device__ __attribute__((always_inline)) uint64_t of(float x, uint32_t token) const
     {
         uint64_t const w = weights.of(x);
-        return last.keeps(x, token) && w >= least ? w : 0;
+        return last.keeps(x, token) && x >= border ? w : 0;
     }
     __device__ __attribute__((always_inline)) uint64_t of(f32x4_t const& y, uint32_t token) const
     {
@@ -544,19 +544,21 @@ struct Same {
     __device__ uint64_t of(f32x4_t const& y, uint32_t) const { return of(y[0], 0) + of(y[1], 0) + of(y[2], 0) + of(y[3], 0); }
 };
 
-// The kept tokens down to the last one of a cut, of those that weigh `least` or more.
-__device__ inline Kept kept_tokens(const Weights& weights, const Last& last, float temperature, float min_p)
+// The lowest logit that min-p keeps: the least number of 32 bits at or above
+// m + T log min_p, in 64 bits, as that may lie past the largest of 32.
+__device__ inline float min_p_border(double highest, float temperature, float min_p)
+{
+    if (min_p == 0.0f) return -INFINITY;
+    double const at = highest + static_cast<double>(temperature) * log(static_cast<double>(min_p));
+    float const near = static_cast<float>(at);
+    return static_cast<double>(near) < at ? nextafterf(near, INFINITY) : near;
+}
+
+// The kept tokens down to the last one of a cut, of those that min-p keeps.
+__device__ inline Kept kept_tokens(const Weights& weights, const Last& last, float temperature, float border)
 {
     float const high = static_cast<float>(weights.highest);
-    Kept k{weights, last, part_of(min_p, uint64_t{1} << weights.scale, true), fmaxf(last.logit, high - kWeightless * temperature), last.logit};
-    if (min_p > 0.0f) {
-        // Min-p's logit, by more than what 32 bits lose on the way to it.
-        float const under = temperature * logf(min_p);
-        float const slack = (fabsf(high) - under) * 0x1p-18f;
-        k.floor = fmaxf(k.floor, high + under - slack);
-        k.sure = fmaxf(k.sure, high + under + slack);
-    }
-    return k;
+    return Kept{weights, last, border, fmaxf(fmaxf(last.logit, high - kWeightless * temperature), border), fmaxf(last.logit, nextafterf(border, -INFINITY))};
 }
 
 // Ranges of a wave's run.
@@ -916,10 +918,10 @@ __device__ __attribute__((always_inline)) inline Last find_cut(const Row& row, S
 
 // ---- top-p's cut, and what it keeps of each wave's run -------------------------------
 
-// The weights in bins of each wave's own give the bin that the cut falls into, and
-// those that min-p's border can lie in; the tokens of the first of these, listed
-// and sorted, give the last kept one, and with the bins before them what is kept of
-// every run: lds.run.  Top-p's part is of the first top_k tokens' weight (V: of
+// The weights in bins of each wave's own give the bin that the cut falls into; the
+// tokens of that or of min-p's border's, whichever is first, listed and sorted,
+// give the last kept one, and with the bins before it what is kept of every run:
+// lds.run.  Top-p's part is of the first top_k tokens' weight (V: of
 // all): counts of the bins give the one of the last of them, whose tokens are
 // listed and sorted for their weight.  False where a list is too long.
 __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row, SampleLds& lds, const Weights& weights, const Bins& bins, float top_p,
@@ -1031,16 +1033,15 @@ __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row
     }
     __syncthreads();
     uint32_t const bin = lds.word[3];
-    uint32_t const from = kept.least != 0 ? min(bins.of(fminf(kept.sure, 2.0f * bins.half)), bin) : bin;
-    uint32_t const to = kept.least != 0 ? min(bins.of(kept.floor), bin) : bin;
+    uint32_t const end = min(bins.of(kept.floor), bin);
     at = first;
 #pragma unroll
     for (uint32_t i = 0; i < kWaveBinsEach; ++i) {
-        if (kWaveBinsEach * tid + i == from) lds.before = at;
+        if (kWaveBinsEach * tid + i == end) lds.before = at;
         at += of[i];
     }
     sum = 0;
-    for (uint32_t b = lane; b < from; b += kWave) sum += lds.of_wave[wave][b];
+    for (uint32_t b = lane; b < end; b += kWave) sum += lds.of_wave[wave][b];
     sum = wave_total(sum);
     if (lane == 0) lds.run[wave] = sum;
     if (tid == 0) {
@@ -1049,9 +1050,9 @@ __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row
     }
     __syncthreads();
     uint64_t const left = amount - lds.before;   // at least 1
-    float const low = fmaxf(bins.under(to), -3.4028234664e38f);
-    float const high = fminf(bins.over(from), 2.0f * bins.half);
-    uint32_t const listed = list_tokens(row, lds, low, high, [&](float x) { return bins.of(x) >= from && bins.of(x) <= to; });
+    float const low = fmaxf(bins.under(end), -3.4028234664e38f);
+    float const high = fminf(bins.over(end), 2.0f * bins.half);
+    uint32_t const listed = list_tokens(row, lds, low, high, [&](float x) { return bins.of(x) == end; });
     if (listed > kListed) return false;
     sort_falling(lds.listed, lds, listed, true, high, high - low);
     // Neighbours of the order each thread.
@@ -1068,12 +1069,13 @@ __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row
     for (uint32_t i = 0; i < kListedEach; ++i) {
         uint32_t const n = kListedEach * tid + i;
         if (n < listed && at < left) {
+            uint32_t const key = static_cast<uint32_t>(lds.listed[n] >> 32);
             uint32_t const token = 0xFFFFFFFFu - static_cast<uint32_t>(lds.listed[n]);
             if (left - at <= w[i]) {
-                lds.word[2] = static_cast<uint32_t>(lds.listed[n] >> 32);
+                lds.word[2] = key;
                 lds.word[1] = token;
             }
-            if (w[i] >= kept.least) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.run[token / (row.run * kVector)]), static_cast<unsigned long long>(w[i]));
+            if (logit_of(key) >= kept.border) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.run[token / (row.run * kVector)]), static_cast<unsigned long long>(w[i]));
         }
         at += w[i];
     }
@@ -1093,29 +1095,31 @@ struct Drawn {
 // From a list of the first top_k tokens and more, or of all that min-p keeps,
 // logits within low .. high; top-p's part is of `total`, or where that is 0 of the
 // first top_k's weight.  Each thread has neighbours of the list.
-__device__ inline Drawn draw_listed(SampleLds& lds, const Weights& weights, const kimkv_sample_rule& rule, uint32_t listed, uint32_t top_k,
-                                    uint64_t total, float low, float high, float uniform, uint32_t V)
+__device__ inline Drawn draw_listed(SampleLds& lds, const Kept& of, float top_p, uint32_t listed, uint32_t top_k, uint64_t total, float low,
+                                    float high, float uniform, uint32_t V)
 {
     uint32_t const tid = threadIdx.x;
     sort_falling(lds.listed, lds, listed, true, high, high - low);
     uint32_t const n = min(listed, top_k);
-    uint64_t const least = part_of(rule.min_p, uint64_t{1} << weights.scale, true);
     uint64_t w[kListedEach];
+    bool good[kListedEach];   // as far as min-p goes
     uint64_t sum = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kListedEach; ++i) {
         uint32_t const p = kListedEach * tid + i;
-        w[i] = p < n ? weights.of(logit_of(static_cast<uint32_t>(lds.listed[p] >> 32))) : 0;
+        float const x = p < n ? logit_of(static_cast<uint32_t>(lds.listed[p] >> 32)) : -INFINITY;
+        w[i] = of.weights.of(x);
+        good[i] = p < n && x >= of.border;
         sum += w[i];
     }
     uint64_t all;
     uint64_t at = block_scan(sum, lds, &all);
     // What top-p keeps begins before its part of the weight is reached.
-    uint64_t const need = rule.top_p < 1.0f ? part_of(rule.top_p, total != 0 ? total : all, true) : ~uint64_t{0};
+    uint64_t const need = top_p < 1.0f ? part_of(top_p, total != 0 ? total : all, true) : ~uint64_t{0};
     uint32_t kept = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kListedEach; ++i) {
-        if (kListedEach * tid + i < n && at < need && w[i] >= least) {
+        if (good[i] && at < need) {
             kept += 1;
             at += w[i];
         } else {
@@ -1244,7 +1248,8 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     row.infinite = high == INFINITY;
     if (row.infinite) high = 0.0f;
     Weights const weights{high, 1.4426950408889634 / static_cast<double>(temperature), a.scale};
-    Kept kept = kept_tokens(weights, Last{-INFINITY, 0xFFFFFFFFu}, temperature, rule.min_p);
+    float const border = min_p_border(high, temperature, rule.min_p);
+    Kept kept = kept_tokens(weights, Last{-INFINITY, 0xFFFFFFFFu}, temperature, border);
 
     // ---- from a list ----
     if (list) {
@@ -1288,7 +1293,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
                 });
                 total = block_total(total, lds);
             }
-            Drawn const d = draw_listed(lds, weights, rule, listed, top_k, total, bound, high, uniform, a.V);
+            Drawn const d = draw_listed(lds, kept, rule.top_p, listed, top_k, total, bound, high, uniform, a.V);
             answer(d.token, static_cast<float>(static_cast<double>(d.weight) / static_cast<double>(d.total)));
             return;
         }
@@ -1364,7 +1369,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
 #pragma nounroll
         for (uint32_t by_mass = cut_k ? 0 : 1; by_mass <= (cut_p ? 1 : 0); ++by_mass) {
             if (by_mass != 0 && cut_k) {
-                if (last.logit != -INFINITY) total = sum_ranges(row, lds, kept_tokens(weights, last, temperature, 0.0f));
+                if (last.logit != -INFINITY) total = sum_ranges(row, lds, kept_tokens(weights, last, temperature, -INFINITY));
                 __syncthreads();
 #pragma unroll
                 for (uint32_t i = 0; i < kBinsEach; ++i) lds.mass[i * kBlock + tid] = mass[i];
@@ -1376,7 +1381,7 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
     }
 
     // ---- the draw ----
-    kept = kept_tokens(weights, last, temperature, rule.min_p);
+    kept = kept_tokens(weights, last, temperature, border);
     uint64_t const found = sum_ranges(drawn, lds, kept);
     if (sums == 0) sums = found;
     uint64_t its;

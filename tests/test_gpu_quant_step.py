@@ -1083,3 +1083,46 @@ def test_sample_top_p_of_many(dev, vocab, kind):
         x[rng.random(x.shape) < 0.1] = np.nan
     for u in (0.0, 0.3, 1 - 2.0 ** -24):
         _check_sample(dev, x, MANY_OF_TOP_K, np.full(len(x), u, np.float32), offset=1)
+
+
+@pytest.mark.parametrize("vocab", [3001, 6000, 40000])
+def test_sample_min_p_of_far_logits(dev, vocab):
+    """Temperatures at which T log min_p is past the largest number of 32 bits, of logits as far apart, so that min-p still
+    leaves tokens out; alone, beside top-p, beside a long top_k and both."""
+    print(f"sample min-p of far logits V={vocab}", flush=True)
+    rng = np.random.default_rng(vocab)
+    rows, rules = [], []
+    for temperature in (2e37, 1e38, 3e38):
+        for min_p in (0.5, 0.2, 0.02, 1e-4):
+            for top_k, top_p in ((0, 1.0), (0, 0.9), (2500, 1.0), (2500, 0.9)):
+                x = rng.uniform(-3.3e38, 3.3e38, vocab)
+                if top_k == 0 and top_p == 1.0:   # a half that min-p leaves out, in front
+                    x = np.where(np.arange(vocab) < vocab // 2, -3e38, 3e38)
+                rows.append(x.astype(np.float32))
+                rules.append((temperature, top_k, top_p, min_p))
+    uniforms = rng.random(len(rows)).astype(np.float32)
+    uniforms[::3] = 0
+    _check_sample(dev, np.array(rows), rules, uniforms)
+
+
+def test_sample_min_p_beside_the_last_bits_of_weights(dev):
+    """Tokens just above and just below a min_p of a few units of 2^-46, drawn by a random number of 0 and by others: the
+    first that is kept, wherever the weights' last bit puts it.  Ordinary rows go before, whose answers are not these rows'."""
+    print("sample min-p beside the last bits", flush=True)
+    vocab = 20000
+    rng = np.random.default_rng(21)
+    ordinary = (2 * rng.standard_normal(vocab)).astype(np.float32)
+    border = np.full(vocab, -60, np.float32)
+    border[:4096] = np.log(0.97e-13)
+    border[4096:8192] = np.log(1.03e-13)
+    border[15000] = 0
+    rows = np.array([ordinary] * 600 + [border] * 600)
+    rules = [(1.0, 0, 1.0, 0.0)] * 600 + [(1.0, 0, 1.0, 1e-13), (2.0, 0, 1.0, 1e-13), (1.0, 9000, 1.0, 1e-13)] * 200
+    rows[601::3] *= 2
+    uniforms = rng.random(1200).astype(np.float32)
+    uniforms[600:900] = 0
+    uniforms[900:] = 0.25 + 0.5 * uniforms[900:]
+    tokens, chance = _sample(dev, rows, rules, uniforms)
+    assert set(tokens[600:900].tolist()) == {4096} and set(tokens[900:].tolist()) == {15000}
+    # A token's weight is off by half a unit at most.
+    assert np.all(np.abs(chance[600:900] - 1.03e-13) <= 2.0 ** -47 + 2.0 ** -24 * 1.03e-13) and np.all(chance[900:] > 0.999)
