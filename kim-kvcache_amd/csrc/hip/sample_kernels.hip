@@ -747,12 +747,13 @@ struct Cut {
 // are not counted.  Half a logit, as the difference of two may be
 // past the largest number.
 struct Bins {
-    float half;      // of the highest logit
+    float high;      // the highest logit
+    float half;      // of it: rounded, where it is below the normal numbers
     float rate;      // bins for a unit of half a logit, finite
     float last;      // bin
     __device__ uint32_t of(float x) const { return static_cast<uint32_t>(fminf((half - 0.5f * x) * rate, last)); }
     __device__ Bins(float high, float width, uint32_t n)
-        : half(0.5f * high), rate(fminf(2.0f * static_cast<float>(n - 1) / width, 3e38f)), last(static_cast<float>(n - 1))
+        : high(high), half(0.5f * high), rate(fminf(2.0f * static_cast<float>(n - 1) / width, 3e38f)), last(static_cast<float>(n - 1))
     {
     }
     // No logit of the bin is below under(b), and none above over(b): the borders,
@@ -824,7 +825,7 @@ __device__ __attribute__((always_inline)) inline Last find_cut(const Row& row, S
     float const low_x = bins.under(bin);
     float const high_x = bins.over(bin);
     uint32_t low = key_of(fmaxf(low_x, -3.4028234664e38f));
-    uint32_t high = key_of(fminf(high_x, 2.0f * bins.half));
+    uint32_t high = key_of(fminf(high_x, bins.high));
     uint32_t listed = list_tokens(row, lds, low_x, high_x, [&](float x) { return bins.of(x) == bin; });
     if (listed > kListed) {
         // Too many: their highest and lowest keys, and bins of these.
@@ -1001,7 +1002,7 @@ __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row
         __syncthreads();
         if (bin < kWaveBins) {
             float const low = fmaxf(bins.under(bin), -3.4028234664e38f);
-            float const high = fminf(bins.over(bin), 2.0f * bins.half);
+            float const high = fminf(bins.over(bin), bins.high);
             uint32_t const listed = list_tokens(row, lds, low, high, [&](float x) { return bins.of(x) == bin; });
             if (listed > kListed) return false;
             // What lies where the sort works.
@@ -1051,7 +1052,7 @@ __device__ __attribute__((always_inline)) inline bool cut_of_runs(const Row& row
     __syncthreads();
     uint64_t const left = amount - lds.before;   // at least 1
     float const low = fmaxf(bins.under(end), -3.4028234664e38f);
-    float const high = fminf(bins.over(end), 2.0f * bins.half);
+    float const high = fminf(bins.over(end), bins.high);
     uint32_t const listed = list_tokens(row, lds, low, high, [&](float x) { return bins.of(x) == end; });
     if (listed > kListed) return false;
     sort_falling(lds.listed, lds, listed, true, high, high - low);

@@ -1126,3 +1126,17 @@ def test_sample_min_p_beside_the_last_bits_of_weights(dev):
     assert set(tokens[600:900].tolist()) == {4096} and set(tokens[900:].tolist()) == {15000}
     # A token's weight is off by half a unit at most.
     assert np.all(np.abs(chance[600:900] - 1.03e-13) <= 2.0 ** -47 + 2.0 ** -24 * 1.03e-13) and np.all(chance[900:] > 0.999)
+
+
+@pytest.mark.parametrize("vocab", [1500, 5000])
+def test_sample_logits_below_the_normal_numbers(dev, vocab):
+    """The highest logit an odd multiple of 2^-149, of which half is no number, above and below 0."""
+    print(f"sample below the normal numbers V={vocab}", flush=True)
+    rng = np.random.default_rng(vocab)
+    rules = [(1.0, 0, 0.5, 0.0), (1.0, 0, 0.9, 0.5), (1.0, 1200, 1.0, 0.0), (1.0, 1200, 0.3, 0.0), (1.0, 7, 1.0, 0.0), (2.0 ** -149, 0, 0.9, 0.0), (2.0 ** -149, 1300, 0.5, 0.0),
+             (2.0 ** -149, 0, 1.0, 0.1), (2.0 ** -147, 0, 0.7, 0.01), (0.0, 0, 1.0, 0.0), (1e-44, 0, 1.0, 0.0)]
+    for highest, low in ((3, -2), (1, -40), (-1, -6), (5, 4)):
+        x = rng.integers(low, highest, (len(rules), vocab)) * 2.0 ** -149
+        x[:, vocab - 7] = highest * 2.0 ** -149
+        for u in (0.0, 0.4, 1 - 2.0 ** -24):
+            _check_sample(dev, x, rules, np.full(len(rules), u, np.float32))
