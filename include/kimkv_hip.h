@@ -687,11 +687,11 @@ kimkv_status kimkv_quant_storage_faults(kimkv_quant_storage* storage, kimkv_stre
  * copies page tokens that another one writes; any number may copy from one
  * page, while another writes on behind what they copy.  Page tokens that no
  * job names stay as they are.  A job that names no page of the storage, tokens
- * past the page, layers past the storage's, no source, or copies more tokens
- * than the page has or than lie below dst_token sets KIMKV_FAULT_APPEND_JOB and
- * is skipped.  Vector accesses where head_dim and the token stride are
- * multiples of 8 and the sources 16-byte aligned in every layer; anything else
- * goes element by element. */
+ * past the page, layers past the storage's or more than max_layer_count, no
+ * source, or copies more tokens than the page has or than lie below dst_token
+ * sets KIMKV_FAULT_APPEND_JOB and is skipped, in every layer.  Vector accesses
+ * where head_dim and the token stride are multiples of 8 and the sources
+ * 16-byte aligned in every layer; anything else goes element by element. */
 kimkv_status kimkv_quant_append_batch(const kimkv_quant_storage* storage, const kimkv_append_job* device_jobs,
                                       uint32_t job_count, uint32_t max_layer_count, kimkv_stream_t stream);
 

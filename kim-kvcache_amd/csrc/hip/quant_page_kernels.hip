@@ -178,7 +178,9 @@ __global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const
     uint32_t const scap = quant_page_tokens(P, job.cow_kind);
     uint8_t* const dst = quant_block(P, layer, job.dst_kind, job.dst_slot, dcap);
     uint8_t* const src = job.cow_tokens != 0 ? quant_block(P, layer, job.cow_kind, job.cow_slot, scap) : nullptr;
-    if (job.layer_begin >= P.layers || layer >= P.layers || dst == nullptr || n > dcap || job.dst_token > dcap - n
+    // Each block judges the job's whole range of layers, so that a bad one is skipped in all of them.
+    if (job.layer_begin >= P.layers || job.layer_count > P.layers - job.layer_begin || job.layer_count > gridDim.y || dst == nullptr
+        || n > dcap || job.dst_token > dcap - n
         || (n != 0 && (job.src_key == nullptr || job.src_value == nullptr))
         || (job.cow_tokens != 0 && (src == nullptr || job.cow_tokens > scap || job.cow_tokens > job.dst_token))) {
         report_fault(P, KIMKV_FAULT_APPEND_JOB);

@@ -1140,3 +1140,32 @@ def test_sample_logits_below_the_normal_numbers(dev, vocab):
         x[:, vocab - 7] = highest * 2.0 ** -149
         for u in (0.0, 0.4, 1 - 2.0 ** -24):
             _check_sample(dev, x, rules, np.full(len(rules), u, np.float32))
+
+
+@pytest.mark.parametrize("form,heads,dim", [("int8", 2, 64), ("e4m3", 2, 12)])
+def test_append_jobs_of_too_many_layers(dev, form, heads, dim):
+    """A job that begins within the storage's layers and ends past them, or is of more layers than the launch, is skipped in
+    every layer, its copy too; a job of no layers is none."""
+    c = _Cache(dev, FORMS[form], heads, dim, layers=3)
+    kv = _fp16(np.random.default_rng(14), 3, 2, 64, heads, dim)
+    buf = dev.upload(_bits(kv))
+    good = [(0, 1, 0, 0, 0), (1, 20, 1, 0, 3)]
+    for name, change, most in (("one past", dict(layer_begin=1, layer_count=3), 3), ("many past", dict(layer_begin=2, layer_count=2), 3),
+                               ("all but wrapped", dict(layer_begin=1, layer_count=0xFFFFFFFF), 3), ("more than the launch", dict(layer_count=3), 2)):
+        print(f"quant_append layers {name}", flush=True)
+        for bad in ((21, 1, 0, 2, 4), (22, 12, 1, 2, 9)):
+            jobs = c.jobs_of(buf.ptr, 64, good + [bad], {2: (0, 5, 4)}, layer_count=most)
+            for field, value in change.items():
+                jobs[2][field] = value
+            held_jobs = dev.upload(jobs)
+            c.storage.append_launch(held_jobs.ptr, len(jobs), most)
+            dev.sync()
+            assert c.storage.faults() == (dev.INVALID_ARGUMENT, dev.FAULT_APPEND_JOB), name
+        c.expect(kv[:most], good)
+        c.check()
+    jobs = c.jobs_of(buf.ptr, 64, good + [(21, 1, 0, 2, 4)])
+    jobs[2]["layer_begin"], jobs[2]["layer_count"] = 0xFFFFFFFF, 0
+    c.storage.append_batch(jobs)
+    c.expect(kv, good)
+    c.check()
+    assert c.storage.faults() == (0, 0)
