@@ -117,6 +117,16 @@ __device__ inline uint64_t lane_value(uint64_t v, int lane)
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
+// The highest of the four lanes of a query column: a swap with itself leaves a
+// lane its own value and its partner's.
+__device__ inline float column_max(float v)
+{
+    auto const rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
+    auto const halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
+
 // ---------------------------------------------------------------------------
 // Matrix-core path of one wave.
 // ---------------------------------------------------------------------------
@@ -141,11 +151,18 @@ constexpr uint32_t kMaxGroups = kWave * kGroupsOfEntry;
 
 constexpr bool fast_dim(uint32_t dim) { return dim == 64 || dim == 96 || dim == 128; }
 
-// The weights' reference for V's scales: weights enter the product as
-// p b 2^15 / c with c a power of two above every scale b so far, so they stay
-// below 2^15 and, in two fp16 parts, keep 20 bits down to 2^-24 of that.
-constexpr uint32_t kScaleTop = 136;     // exponent bits of the largest scale (516)
-constexpr uint32_t kScaleLow = 64;
+// A query column's weights enter the product as p b 2^15 / c, with c a power of
+// two above 2^7 times every p b of the column so far, all to its running max, and
+// above the tile's: they stay below 2^15, and two fp16 parts are off by 2^-22 of a
+// weight or by 2^-31 of the column's largest (a step of the lower part is 2^-24),
+// whichever is more.  So a row of V costs the others bits only as far as it is
+// attended to: with c above the scales b, whatever their p, one row of 65504 that
+// weighed nothing left rows of 2^-12 off by 2^-7 of themselves.  The 2^7 are room
+// for the scales of later tiles, so that c need not follow each: 128 lanes of
+// 32768 tokens, 4 heads of 64, take 348.6 us (346.0 with c above the scales);
+// without the room 349.8, with c found anew for every tile 352.0.
+constexpr uint32_t kWeightRoom = 7;
+constexpr uint32_t kWeightLow = 64;     // exponent bits of c's least, 2^-62
 __device__ inline float weight_factor(uint32_t e) { return __uint_as_float((127u + 15u + 126u - e) << 23); }    // 2^15 / c, c = 2^(e - 126)
 __device__ inline float weight_unit(uint32_t e) { return __uint_as_float((e - 126u + 127u - 15u) << 23); }      // c / 2^15
 
@@ -168,7 +185,8 @@ struct Decoder {
     float m = -INFINITY;
     float l = 0.0f;              // of this lane's tokens
     float scale2;
-    uint32_t e = kScaleLow;      // exponent bits of the weights' reference, uniform
+    float most = 0.0f;           // of the column's p b
+    uint32_t e = kWeightLow;     // c = 2^(e - 126)
     uint32_t g;
     uint32_t r;
 
@@ -308,15 +326,13 @@ struct Decoder {
         __builtin_amdgcn_sched_barrier(0);
         next_k();
         __builtin_amdgcn_sched_barrier(0);
-        mx = fmaxf(mx, xor16(mx));
-        mx = fmaxf(mx, xor32(mx));
-        float const m_new = fmaxf(m, mx);
+        float const m_new = fmaxf(m, column_max(mx));
         // While every score is -inf the reference is 0, so the weights are zeros and not NaN.
         float const m_top = m_new == -INFINITY ? 0.0f : m_new;
         float alpha = __builtin_amdgcn_exp2f(m - m_top);
         m = m_new;
 
-        // ---- V's scales: their largest, and whether one is NaN ----
+        // ---- V's scales: whether one is NaN ----
         if (kMasked) {
 #pragma unroll
             for (uint32_t s = 0; s < 2; ++s) {
@@ -335,22 +351,10 @@ struct Decoder {
                 top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, pair));
             }
         }
-        float most = __uint_as_float(static_cast<uint32_t>(top[0] > top[1] ? top[0] : top[1]));
-        auto const larger = [](float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); };
-        most = larger(most, xor16(most));
-        most = larger(most, xor32(most));
-        uint32_t const bits = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(__float_as_uint(most))));
-        bool const has_nan = bits >= 0x7F80u;
-        uint32_t const e_tile = min(bits >> 7, kScaleTop);
-        float change = 1.0f;
-        if (e_tile > e) {
-            change = __uint_as_float((127u + e - e_tile) << 23);
-            e = e_tile;
-        }
-        float const factor = weight_factor(e);
+        uint32_t const lane_top = top[0] > top[1] ? top[0] : top[1];   // of the lane's tokens
+        bool const has_nan = __ballot(lane_top >= 0x7F80u) != 0;
 
         // ---- weights ----
-        half8_t hi[2], lo[2];
         float sum = 0.0f;
 #pragma unroll
         for (uint32_t tau = 0; tau < 4; ++tau) {
@@ -359,20 +363,41 @@ struct Decoder {
                 uint32_t const t = 4 * (tau & 1) + i;
                 float const p = __builtin_amdgcn_exp2f(score[tau][i] - m_top);
                 sum += p;
-                float w = p * (scale_of(o.vs[tau >> 1], t) * factor);
+                float w = p * scale_of(o.vs[tau >> 1], t);
                 if (has_nan && p == 0.0f) w = 0.0f;   // a value that weighs nothing is left out, whatever it is
-                _Float16 const part = static_cast<_Float16>(w);
-                hi[tau >> 1][t] = part;
-                lo[tau >> 1][t] = static_cast<_Float16>(w - static_cast<float>(part));
+                score[tau][i] = w;
             }
         }
         l = l * alpha + sum;
-        alpha *= change;
-        if (__ballot(alpha != 1.0f) != 0) {
+        // c stays while no running max rises and no scale passes it.
+        if (__ballot(alpha != 1.0f || lane_top >> 7 > e) != 0) {
+            float tile_most = 0.0f;   // NaN is left out
+#pragma unroll
+            for (uint32_t tau = 0; tau < 4; ++tau) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) tile_most = fmaxf(tile_most, score[tau][i]);
+            }
+            most = fmaxf(most * alpha, column_max(tile_most));
+            uint32_t const e_new = max((__float_as_uint(most) >> 23) + kWeightRoom, kWeightLow);
+            alpha *= __uint_as_float((127u + e - e_new) << 23);
+            e = e_new;
 #pragma unroll
             for (uint32_t db = 0; db < kDb; ++db) {
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) acc[db][i] = alpha == 0.0f ? 0.0f : acc[db][i] * alpha;
+            }
+        }
+        float const factor = weight_factor(e);
+        half8_t hi[2], lo[2];
+#pragma unroll
+        for (uint32_t tau = 0; tau < 4; ++tau) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                uint32_t const t = 4 * (tau & 1) + i;
+                float const w = score[tau][i] * factor;
+                _Float16 const part = static_cast<_Float16>(w);
+                hi[tau >> 1][t] = part;
+                lo[tau >> 1][t] = static_cast<_Float16>(w - static_cast<float>(part));
             }
         }
 #pragma unroll

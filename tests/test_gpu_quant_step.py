@@ -1169,3 +1169,28 @@ def test_append_jobs_of_too_many_layers(dev, form, heads, dim):
     c.expect(kv, good)
     c.check()
     assert c.storage.faults() == (0, 0)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [64, 96, 128, 40])
+@pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** -17])
+@pytest.mark.parametrize("kind", ["one row", "rows in all places", "overtaken"])
+def test_decode_far_values_without_weight(dev, form, dim, size, kind):
+    """Rows of V of up to 65504 that weigh nothing cost the others, far smaller, no bits: their keys lie far below, or later
+    keys overtake them."""
+    print(f"quant_decode far values {form} D={dim} {size} {kind}", flush=True)
+    free = _pool(60, 100)
+    tables = [_table(n, free, lead=n % 3) for n in (600, 1500, 70)]
+    total = 600 + 1500 + 70
+    far = np.zeros(total, bool)
+    far[{"one row": [3, 603, 2103], "rows in all places": range(5, total, 13), "overtaken": [*range(20), *range(600, 640), *range(2100, 2110)]}[kind]] = True
+
+    def keys(k):
+        if kind == "overtaken":
+            return np.where(far[:, None, None], 0, 3 + 0.1 * k.astype(np.float32)).astype(np.float16)
+        return np.where(far[:, None, None], np.float16(-3), k)
+
+    def values(v):
+        return np.where(far[:, None, None], np.clip(30000 * v.astype(np.float32), -65504, 65504), size * v.astype(np.float32)).astype(np.float16)
+
+    _Lanes(dev, FORMS[form], 2, dim, 4, tables, 60, 100, keys=keys, values=values, query=np.abs).check()
