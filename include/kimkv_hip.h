@@ -861,9 +861,11 @@ kimkv_status kimkv_linear(const uint16_t* x, uint32_t rows, uint32_t in_features
  * times the two call after call.  The stream is synchronized, and y is
  * overwritten or accumulated into several times, so pass scratch contents.
  * The winner is the one kimkv_linear uses for the problem on this stream.
- * Successive timed products cycle through the weight_count weight matrices
- * (e.g. every layer's), so the weights are read from HBM as in a forward
- * pass, not from a warm cache.  No counterpart in the reference (cuBLAS picks
+ * Each candidate reads the matrices itself before it is timed on them, so that
+ * its time does not depend on the others.  Successive timed products cycle
+ * through the weight_count weight matrices (e.g. every layer's), or through as
+ * many as are more than 256 MB, so the weights are read as in a forward pass,
+ * not from a warm L2.  No counterpart in the reference (cuBLAS picks
  * its own algorithm). */
 kimkv_status kimkv_linear_tune(const uint16_t* x, uint32_t rows, uint32_t in_features,
                                const uint16_t* const* weights, uint32_t weight_count, uint32_t out_features, void* y,

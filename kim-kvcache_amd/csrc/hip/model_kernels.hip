@@ -687,6 +687,8 @@ kimkv_status kimkv_linear_tune(const uint16_t* x, uint32_t rows, uint32_t in_fea
     // Of candidates this near each other the first is taken: the best rounds
     // of one differ by up to 1.5% between processes.
     constexpr float kTie = 1.02f;
+    constexpr float kNear = 1.1f;   // of the short timing's fastest
+    constexpr uint64_t kCached = uint64_t{256} << 20;   // the memory-side cache
     if (weights == nullptr || weight_count == 0) return KIMKV_INVALID_ARGUMENT;
     for (uint32_t i = 0; i < weight_count; ++i) {
         if (!lt_args_ok(x, in_features, weights[i], out_features, y, rows)) return KIMKV_INVALID_ARGUMENT;
@@ -722,8 +724,8 @@ kimkv_status kimkv_linear_tune(const uint16_t* x, uint32_t rows, uint32_t in_fea
         usable[n] = launch_status() == KIMKV_OK;
     }
     // Time per product of `reps` of candidate a, or INFINITY on an error.  The
-    // matrices are taken in turn over all timings, so each was last read
-    // weight_count products ago, whoever read it.  wait: the products are
+    // matrices are taken in turn over all timings, all of them or as many as
+    // are more than the memory-side cache holds.  wait: the products are
     // queued behind a wait, so that the events bracket the GPU's work alone;
     // one too short for the host is doubled, for this and the candidates
     // after it, and the products are timed again (a busy host may need the
@@ -732,6 +734,8 @@ kimkv_status kimkv_linear_tune(const uint16_t* x, uint32_t rows, uint32_t in_fea
     constexpr uint32_t kMostTicks = 10000;
     constexpr int kAttempts = 8;
     uint32_t turn = 0;
+    uint64_t const uncached = kCached / (uint64_t{2} * in_features * out_features) + 1;
+    auto const cycle = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(uncached, kReps), weight_count));
     auto timed = [&](int a, int reps, bool wait) {
         float ms = 0.0f;
         bool ok = true;
@@ -740,7 +744,7 @@ kimkv_status kimkv_linear_tune(const uint16_t* x, uint32_t rows, uint32_t in_fea
             if (wait) wait_kernel<<<1, 64, 0, s>>>(ticks * static_cast<uint32_t>(reps));
             ok = hipEventRecord(e0, s) == hipSuccess;
             for (int i = 0; i < reps && ok; ++i) {
-                const uint16_t* w = weights[turn++ % weight_count];
+                const uint16_t* w = weights[turn++ % cycle];
                 if (a == n) {
                     linear_launch(x, rows, in_features, w, out_features, y, y_f32 != 0, beta, s);
                     ok = launch_status() == KIMKV_OK;
@@ -760,29 +764,28 @@ kimkv_status kimkv_linear_tune(const uint16_t* x, uint32_t rows, uint32_t in_fea
     // Of the library's candidates, by the GPU's work: a call of the library's
     // takes 10 us of host work, as long as a product of 128 rows, and times
     // of that decided between candidates 5% apart one way in one process and
-    // the other way in the next.  A short round finds the contenders, after
-    // each candidate's code and every matrix's translations have been loaded.
-    float limit = INFINITY;
-    for (int a = 0; a < n; ++a) {
-        for (uint32_t i = 0; usable[a] && i < 1 + weight_count / static_cast<uint32_t>(n); ++i) {
-            usable[a] = lt_run(st, *ctx, p, cand[a].algo, x, weights[turn++ % weight_count], y, beta, s) == HIPBLAS_STATUS_SUCCESS;
+    // the other way in the next.  Each candidate reads the matrices itself
+    // before it is timed, which loads its code too: some leave them in the
+    // memory-side cache and some do not, and with another's reads before its
+    // own, one candidate's products took 7.4 us or 8.7, as the number of
+    // candidates had it.  A short timing finds those near the fastest.
+    float least = INFINITY;
+    auto measure = [&](int a, int reps) {
+        for (uint32_t i = 0; usable[a] && i < cycle; ++i) {
+            usable[a] = lt_run(st, *ctx, p, cand[a].algo, x, weights[turn++ % cycle], y, beta, s) == HIPBLAS_STATUS_SUCCESS;
         }
-    }
+        for (int round = 0; usable[a] && round < kRounds; ++round) time_ms[a] = std::min(time_ms[a], timed(a, reps, true));
+        least = std::min(least, time_ms[a]);
+    };
+    std::fill(time_ms, time_ms + n, INFINITY);
+    for (int a = 0; a < n; ++a) measure(a, 2);
+    float const near = least * kNear;
+    least = INFINITY;
     for (int a = 0; a < n; ++a) {
-        time_ms[a] = usable[a] ? timed(a, 2, true) : INFINITY;
-        limit = std::min(limit, 1.25f * time_ms[a]);
-    }
-    for (int a = 0; a < n; ++a) {
-        usable[a] = usable[a] && time_ms[a] <= limit;
+        usable[a] = usable[a] && time_ms[a] <= near;
         time_ms[a] = INFINITY;
     }
-    float least = INFINITY;
-    for (int round = 0; round < kRounds; ++round) {
-        for (int a = 0; a < n; ++a) {
-            if (usable[a]) time_ms[a] = std::min(time_ms[a], timed(a, kReps, true));
-            least = std::min(least, time_ms[a]);
-        }
-    }
+    for (int a = 0; a < n; ++a) measure(a, kReps);
     int library = -1;
     for (int a = 0; a < n && library < 0; ++a) {
         if (time_ms[a] < INFINITY && time_ms[a] <= least * kTie) library = a;
