@@ -641,8 +641,9 @@ kimkv_status kimkv_shared_decode_batch(const kimkv_storage* storage, const kimkv
 
 /* ---- cache in 8 bits -------------------------------------------------------
  * The same micro and extent pages, tables and jobs over a storage that holds K
- * and V in 8 bits: about half the bytes of kimkv_storage, and half the time of
- * what reads them.  No counterpart in the reference.
+ * and V in 8 bits: about half the bytes of kimkv_storage, and from some 20 MB of
+ * fp16 a layer on about half the time of what reads them.  No counterpart in
+ * the reference.
  *
  * A row is the D values of one token's K or V of one head.  It is held as D
  * codes and one scale s: with a the largest |x| of the row, s is the smallest
@@ -745,7 +746,8 @@ kimkv_status kimkv_quant_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint3
 
 /* kimkv_paged_decode_batch of the planned batch over a quantised storage: each
  * query attends to its lane's codes times their scales, scores, softmax and
- * sums in 32 bits, one rounding to fp16.  device_items: the lanes' items, whole
+ * sums in 32 bits (a weight p b, of V's scale b, in two fp16 parts, off by 2^-22
+ * of itself or 2^-31 of the query's largest), one rounding to fp16.  device_items: the lanes' items, whole
  * tables and token counts as planned (their workspace is not used);
  * device_entries: the plan's entries (made for the storage's heads and head
  * dim); workspace: plan->workspace_bytes of device memory, contents ignored,
@@ -757,8 +759,8 @@ kimkv_status kimkv_quant_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint3
  * none is left the output is 0.  A row of K that reads as NaN makes the outputs
  * of its head NaN, and so does one of V that has a weight above 0.  Head dims
  * of 64, 96 and 128 with up to 16 query heads a KV head run on the matrix
- * cores; others take a slower path.  Results are the same for every run of one
- * plan. */
+ * cores; others take a path that is some hundred times slower for large
+ * batches.  Results are the same for every run of one plan. */
 kimkv_status kimkv_quant_decode_batch(const kimkv_quant_storage* storage, const kimkv_decode_item* device_items,
                                       const void* device_entries, const kimkv_quant_plan* plan, void* workspace,
                                       kimkv_stream_t stream);

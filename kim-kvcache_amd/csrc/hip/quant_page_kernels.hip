@@ -113,8 +113,9 @@ __device__ inline u32x4_t load_piece(const uint16_t* row, uint32_t p, uint32_t D
 
 // Of what is read once, lines at a time: past the caches.  Appended rows and V's
 // codes so, and read-back rows written so: 6 layers of 4 x 4096 tokens, 8 heads of
-// 128, appended and read back in 186 us, 6.0 TB/s, not 246.  With K's codes so too,
-// 199: a wave reads them in pieces of 64 bytes.
+// 128, appended and read back in 186 us, not 246, the same tensors every time (212
+// with others each time, 5.3 TB/s).  With K's codes so too, 199: a wave reads them
+// in pieces of 64 bytes.
 __device__ inline u32x4_t load_once(const void* p) { return __builtin_nontemporal_load(static_cast<const u32x4_t*>(p)); }
 
 // The largest of the lanes of a row, 2^log2 neighbours.
@@ -329,7 +330,8 @@ __global__ __launch_bounds__(kBlock) void quant_append_kernel(QuantView P, const
 // Read-back: block = (table entry, layer, some heads).  V's codes are turned in
 // LDS, and rows of up to 256 dims written whole: head after head, 22 layers of
 // 16384 tokens of 4 heads of 64 took 123 us with rows through the caches and 137
-// a head at a time; 101 us now, 5.5 TB/s.
+// a head at a time; 100 us now, all of the same pages every time, and 107 of
+// others each time, 5.2 TB/s.
 // ---------------------------------------------------------------------------
 struct GatherArgs {
     const kimkv_block_desc* descriptors;
@@ -456,8 +458,9 @@ __global__ __launch_bounds__(kBlock) void quant_gather_kernel(QuantView P, Gathe
 // ---------------------------------------------------------------------------
 // Promotion: block = (job, layer, some heads).  Eight pages of 8 tokens into
 // one of 64: K in runs of 8 tokens of a column block, V and the scales in
-// pieces of 8 tokens.  512 jobs in 22 layers (1.5 GB moved) and their read-back
-// (1.1 GB) take 336 us; in pieces of 8 bytes 391 with the read-back of then.
+// pieces of 8 tokens.  512 jobs in 22 layers (0.8 GB moved) and their read-back
+// (1.1 GB) take 331 us, the same pages every time, and 349 other ones; in pieces of
+// 8 bytes 391 with the read-back of then.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kBlock) void quant_promote_kernel(QuantView P, const kimkv_promotion_job* jobs, uint32_t heads)
 {

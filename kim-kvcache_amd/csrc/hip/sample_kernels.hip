@@ -26,18 +26,24 @@
 //   - The draw from a row or a run: the kept tokens' weights summed by ranges of
 //     the vocabulary, the range that the random number falls into, the token in it.
 //
-// Bound by the instructions of one block's waves: a weight is 26 of them, and a
-// pass of weights over 32000 tokens 11 us, where reading the row takes 2.  So a
-// list saves passes: 72 rows of 50255 with top_k 50 take 16 us (20 us where the
-// list came from a second pass over the row), 256 rows of 128000 34 us (58), which
-// is 3.9 TB/s.  8 waves a block: 16 left 128 registers a thread, which spilled,
-// and these took 17 and 42 us.  Drawn from all the row 28 and 77 us; top-p of 0.9
-// 47 and 105, of which one pass of weights (without the runs' own bins a second one
-// for the draw: 58 and 140), with min-p 46 and 99, with top_k 3000 57 and 127.  Tried and slower for top-p: a
-// list from the highest columns up (256 flat rows of 128000 184 us, as it falls back
-// there); counts and mean places of the bins first, then one pass of weights that
-// sums by ranges and lists the tokens of the bins in question (215 us: a pass of
-// 64-bit additions to LDS takes as long as one with the weights).
+// Bound by the one block of a row, 8 waves, two a SIMD: there is no room for more,
+// as the bins take 128 KB of LDS and a thread 185 registers, in rows too that end in
+// a list and need neither.  While the block runs, its SIMDs' vector units issue for
+// 0.47 of the time in rows from a list, for 0.51 to 0.57 in rows by weights; for the
+// rest both waves wait, for loads and for their own chains (256 rows of 128000: 15
+// vector instructions for 64 tokens with T = 0, 43 drawn from the row, a weight 26 of
+// them, 60 with top-p).  A pass of weights over 32000 tokens takes 11 us, where
+// reading the row takes 2.  So a list saves passes: 72 rows of 50255 with top_k 50
+// take 16 us (20 us where the list came from a second pass over the row), 256 rows of
+// 128000 34 us (58), which is 3.9 TB/s.  16 waves a block left 128 registers a thread,
+// which spilled, and these took 17 and 42 us.  Drawn from all the row 28 and 75 us;
+// top-p of 0.9 46 and 103, of which one pass of weights (without the runs' own bins a
+// second one for the draw: 58 and 140), with min-p 45 and 100, with top_k 3000 56 and
+// 125.  Tried and slower for top-p: a list from the highest columns up (256 flat rows
+// of 128000 184 us, as it falls back there); counts and mean places of the bins first,
+// then one pass of weights that sums by ranges and lists the tokens of the bins in
+// question (215 us: a pass of 64-bit additions to LDS takes as long as one with the
+// weights).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -63,7 +69,7 @@ constexpr uint32_t kListed = 2048;           // tokens that are sorted in LDS
 constexpr uint32_t kListedEach = kListed / kBlock;
 constexpr uint32_t kListedOfWave = kListed / kWaves;
 constexpr uint32_t kShortList = 1024;        // the largest top_k whose tokens are listed at once
-constexpr uint32_t kCrowded = 96;            // columns that a wave reads again (8, one by one: 72 rows of 50255, top_k 700, 31 us, not 22)
+constexpr uint32_t kCrowded = 96;            // columns that a wave reads again (8, one by one: 72 rows of 50255, top_k 700, 31 us, not 22; no other shape measured)
 constexpr uint32_t kAgain = 4;               // of these at once
 constexpr uint32_t kSets = 2;                // of a thread's columns
 constexpr uint32_t kSmall = 128;             // tokens that are ranked by counting
@@ -649,7 +655,7 @@ __device__ __attribute__((always_inline)) inline void sort_falling(uint64_t* num
     uint32_t const tid = threadIdx.x;
     __syncthreads();
     if (n <= kSmall) {
-        // Each goes to the place that the higher ones leave it: eight threads a number.
+        // Each goes to the place that the higher ones leave it: four threads a number.
         uint32_t const mine = tid / (kBlock / kSmall);
         uint32_t const part = tid % (kBlock / kSmall);
         uint64_t const x = mine < n ? numbers[mine] : 0;
@@ -1282,7 +1288,8 @@ __global__ __launch_bounds__(kBlock) void sample_kernel(SampleArgs a)
         // A list of min-p's pays while it is a small part of the row: 256 rows of 128000,
         // some 1300 tokens, 42 us, drawn from the row 74; 72 rows of 50255, some 1500
         // tokens, 38, from the row 28; beside top-p, whose pass of weights comes on top,
-        // 256 rows of 128000, up to 2000 tokens, 114, without the list 103.
+        // 256 rows of 128000, up to 2000 tokens, 114, without the list 103.  The 48th part
+        // lies between these; no other shape was measured.
         uint32_t const listed = list_columns(row, lds, columns, bound, short_k ? kListed : min(cut_p ? kShortList : kListed, a.V / 48));
         if (listed <= kListed) {
             // Min-p leaves the list, and top-p keeps a part of the row.
