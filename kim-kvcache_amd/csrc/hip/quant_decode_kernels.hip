@@ -151,16 +151,16 @@ constexpr uint32_t kMaxGroups = kWave * kGroupsOfEntry;
 constexpr bool fast_dim(uint32_t dim) { return dim == 64 || dim == 96 || dim == 128; }
 
 // A query column's weights enter the product as p b 2^15 / c, with c a power of
-// two above 2^7 times every p b of the column so far, all to its running max, and
+// two above 2^3 times every p b of the column so far, all to its running max, and
 // above the tile's: they stay below 2^15, and two fp16 parts are off by 2^-22 of a
-// weight or by 2^-31 of the column's largest (a step of the lower part is 2^-24),
-// whichever is more.  So a row of V costs the others bits only as far as it is
-// attended to: with c above the scales b, whatever their p, one row of 65504 that
-// weighed nothing left rows of 2^-12 off by 2^-7 of themselves.  The 2^7 are room
-// for the scales of later tiles, so that c need not follow each: 128 lanes of
-// 32768 tokens, 4 heads of 64, take 348.6 us (346.0 with c above the scales);
-// without the room 349.8, with c found anew for every tile 352.0.
-constexpr uint32_t kWeightRoom = 7;
+// weight or by 2^-36 of the column's largest (a step of the lower part is 2^-24, and
+// c at most 2^4 times that), whichever is more.  So a row of V costs the others bits
+// only as far as it is attended to: with c above the scales b, whatever their p, one
+// row of 65504 that weighed nothing left rows of 2^-12 off by 2^-7 of themselves.  The
+// 2^3 are room for the scales of later tiles, so that c need not follow each: 128
+// lanes of 32768 tokens, 4 heads of 64, take 356.6 us (353.1 with c above the scales);
+// without the room 357.4.
+constexpr uint32_t kWeightRoom = 3;
 constexpr uint32_t kWeightLow = 64;     // exponent bits of c's least, 2^-62
 __device__ inline float weight_factor(uint32_t e) { return __uint_as_float((127u + 15u + 126u - e) << 23); }    // 2^15 / c, c = 2^(e - 126)
 __device__ inline float weight_unit(uint32_t e) { return __uint_as_float((e - 126u + 127u - 15u) << 23); }      // c / 2^15
