@@ -747,7 +747,8 @@ kimkv_status kimkv_quant_decode_plan(uint32_t kv_heads, uint32_t head_dim, uint3
 /* kimkv_paged_decode_batch of the planned batch over a quantised storage: each
  * query attends to its lane's codes times their scales, scores, softmax and
  * sums in 32 bits (a weight p b, of V's scale b, in two fp16 parts, off by 2^-22
- * of itself or 2^-36 of the query's largest), one rounding to fp16.  device_items: the lanes' items, whole
+ * of itself or 2^-36 of the query's largest), one rounding to fp16, kept to
+ * +-65504.  device_items: the lanes' items, whole
  * tables and token counts as planned (their workspace is not used);
  * device_entries: the plan's entries (made for the storage's heads and head
  * dim); workspace: plan->workspace_bytes of device memory, contents ignored,

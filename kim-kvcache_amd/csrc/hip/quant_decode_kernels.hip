@@ -513,8 +513,16 @@ __device__ WavePart<kDim> decode_wave(const QuantView& P, const kimkv_decode_ite
 // What part (m, l) weighs beside the highest reference.
 __device__ inline float part_weight(float m, float top) { return __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top)); }
 
-// sum / l as fp16; 0 where no token had a weight.
-__device__ inline uint16_t quotient_half(float sum, float l) { return __half_as_ushort(__float2half_rn(l == 0.0f ? 0.0f : sum / l)); }
+// sum / l as fp16; 0 where no token had a weight.  A row's largest code times its
+// scale can be past fp16's largest number (read_back), and so can this: it stays
+// there, and NaN stays NaN.
+__device__ inline uint16_t quotient_half(float sum, float l)
+{
+    float v = l == 0.0f ? 0.0f : sum / l;
+    v = v > 65504.0f ? 65504.0f : v;
+    v = v < -65504.0f ? -65504.0f : v;
+    return __half_as_ushort(__float2half_rn(v));
+}
 
 // ---------------------------------------------------------------------------
 // General path: any head dim, any group, any table.  One query head at a time;

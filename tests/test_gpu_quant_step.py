@@ -1194,3 +1194,24 @@ def test_decode_far_values_without_weight(dev, form, dim, size, kind):
         return np.where(far[:, None, None], np.clip(30000 * v.astype(np.float32), -65504, 65504), size * v.astype(np.float32)).astype(np.float16)
 
     _Lanes(dev, FORMS[form], 2, dim, 4, tables, 60, 100, keys=keys, values=values, query=np.abs).check()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [64, 96, 128, 40])
+def test_decode_largest_values(dev, form, dim):
+    """Rows of V about the largest numbers of fp16, which their codes and scales can be past: finite outputs, as what is read
+    back; in one part and merged."""
+    print(f"quant_decode largest {form} D={dim}", flush=True)
+    free = _pool(60, 100)
+    tables = [_table(n, free, lead=n % 3) for n in (1, 600, 2500, 70)]
+
+    def values(v):
+        big = np.where(np.random.default_rng(3).random(v.shape) < 0.9, 65504, 65000) * np.where(np.arange(dim) % 2, 1, -1)
+        return big.astype(np.float16)
+
+    lanes = _Lanes(dev, FORMS[form], 2, dim, 4, tables, 60, 100, values=values)
+    want, bound = lanes.want()
+    assert np.abs(want).max() > 65504
+    for units in (256, 2):
+        got = lanes.run(compute_units=units).view(np.float16).astype(np.float64)
+        assert np.isfinite(got).all() and np.all(np.abs(got - np.clip(want, -65504, 65504)) <= bound)
